@@ -1,4 +1,6 @@
 // extern "C" boundary (include/speculate_hip.h) over Model / Decoder.
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -8,6 +10,7 @@
 #include "sd_common.hpp"
 #include "sd_draft.hpp"
 #include "sd_gguf.hpp"
+#include "sd_kvpool.hpp"
 #include "sd_qcodes.hpp"
 #include "sd_tiles.hpp"
 
@@ -25,6 +28,13 @@ struct sd_draft2 {
 };
 struct sd_draft3 {
     std::unique_ptr<sd::Draft3> d;
+};
+
+struct sd_kvpool {
+    std::unique_ptr<sd::KvPool> p;
+};
+struct sd_sampler {
+    std::unique_ptr<sd::Sampler> s;
 };
 
 static thread_local std::string g_err;
@@ -60,6 +70,25 @@ static void need(const sd_model *m) {
 static void need_weights(const sd_model *m) {
     need(m);
     if (!m->model->weights_ready()) throw sd::ArgError("model weights are not fully set");
+}
+static void need(const sd_kvpool *c) {
+    if (!c || !c->p) throw sd::ArgError("null pool handle");
+}
+// elements of a row: the caller's stride, or a dense row's
+static int64_t row_stride(size_t ld, int64_t dense, const char *what) {
+    if (ld == 0) return dense;
+    if (ld > ((size_t)1 << 40) || (int64_t)ld < dense) throw sd::ArgError(std::string(what) + ": rows overlap");
+    return (int64_t)ld;
+}
+static void need_aligned(const void *p, int64_t row_bytes, int align, const char *what) {
+    if ((uintptr_t)p % align || row_bytes % align)
+        throw sd::ArgError(std::string(what) + ": rows must start at multiples of " + std::to_string(align) + " bytes");
+}
+static sd::KvqRows kv_rows(const sd_kv_rows *r) {
+    if (!r || !r->slot || !r->table) throw sd::ArgError("null argument");
+    if (r->n > ((size_t)1 << 24)) throw sd::ArgError("at most 2^24 rows");
+    if (r->n_seqs < 1 || r->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
+    return sd::KvqRows{(int)r->n, r->seq, r->slot, 0, r->table, r->n_seqs, r->table_ld};
 }
 static void setdev(sd_model *m) { SD_HIP_CHECK(hipSetDevice(m->model->cfg.device)); }
 
@@ -857,6 +886,169 @@ sd_status sd_draft2_round(sd_draft2 *d, sd_model *m, const float *target_hidden,
         if (depth < 1 || depth > (size_t)sd::kDraftMaxSteps) throw sd::ArgError("draft depth out of range");
         setdev(m);
         d->d->round(*m->model, *m->dec, target_hidden, (int)depth, top_k, ids, log_probs);
+    });
+}
+
+sd_status sd_kvpool_create(const sd_kvpool_config *cfg, sd_kvpool **out) {
+    return guard([&] {
+        if (!cfg || !out) throw sd::ArgError("null argument");
+        *out = nullptr;
+        sd::KvPoolCfg c;
+        c.n_layers = cfg->n_layers;
+        c.n_heads = cfg->n_heads;
+        c.n_kv_heads = cfg->n_kv_heads;
+        c.head_dim = cfg->head_dim;
+        c.n_pages = cfg->n_pages;
+        c.page_tokens = cfg->page_tokens;
+        c.max_pos = cfg->max_pos;
+        c.interleaved = cfg->interleaved != 0;
+        c.rope_theta = cfg->rope_theta;
+        c.device = cfg->device;
+        if (c.max_pos < 1) throw sd::ArgError("kvpool: max_pos must be positive");
+        auto h = std::make_unique<sd_kvpool>();
+        h->p = std::make_unique<sd::KvPool>(c);
+        *out = h.release();
+    });
+}
+void sd_kvpool_destroy(sd_kvpool *c) { delete c; }
+size_t sd_kvpool_page_bytes(const sd_kvpool *c) { return c && c->p ? (size_t)c->p->layer(0).page_bytes : 0; }
+
+sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, int32_t fmt, const void *q, size_t q_ld,
+                           const void *k, size_t k_ld, const void *v, size_t v_ld, const int32_t *pos, uint16_t *q_out,
+                           void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        sd::KvqAppend a{};
+        a.rows = kv_rows(rows);
+        if (fmt != SD_F16 && fmt != SD_F32) throw sd::UnsupportedError("append: rows must be F16 or F32");
+        if (!k || !v || (q && !q_out)) throw sd::ArgError("null argument");
+        const int size = fmt == SD_F32 ? 4 : 2, hd = P.cfg.head_dim;
+        a.L = P.layer(layer);
+        a.pos = pos;
+        a.cos_t = P.cos_t;
+        a.sin_t = P.sin_t;
+        a.max_pos = P.cfg.max_pos;
+        a.interleaved = P.cfg.interleaved;
+        a.n_heads = P.cfg.n_heads;
+        a.f32 = fmt == SD_F32;
+        a.q = q;
+        a.k = k;
+        a.v = v;
+        a.q_ld = row_stride(q_ld, (int64_t)P.cfg.n_heads * hd, "q");
+        a.k_ld = row_stride(k_ld, (int64_t)P.cfg.n_kv_heads * hd, "k");
+        a.v_ld = row_stride(v_ld, (int64_t)P.cfg.n_kv_heads * hd, "v");
+        a.q_out = q_out;
+        a.q_out_row = (int64_t)P.cfg.n_heads * hd;
+        a.q_out_head = hd;
+        if (q) need_aligned(q, a.q_ld * size, 16, "q");
+        need_aligned(k, a.k_ld * size, 16, "k");
+        need_aligned(v, a.v_ld * size, 16, "v");
+        if (q) need_aligned(q_out, 16, 16, "q_out");
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kvq_append(a, (hipStream_t)stream);
+    });
+}
+
+sd_status sd_kvpool_read(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, uint16_t *k_out, uint16_t *v_out,
+                         void *stream) {
+    return guard([&] {
+        need(c);
+        c->p->check_layer(layer);
+        const sd::KvqRows r = kv_rows(rows);
+        need_aligned(k_out, 16, 16, "k_out");
+        need_aligned(v_out, 16, 16, "v_out");
+        if (!k_out && !v_out) return;
+        sd::DeviceScope dev(c->p->cfg.device);
+        sd::launch_kvq_read(c->p->layer(layer), r, k_out, v_out, (hipStream_t)stream);
+    });
+}
+
+size_t sd_kvpool_attend_workspace(const sd_kvpool *c, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len) {
+    size_t bytes = 0;
+    guard([&] {
+        need(c);
+        const size_t most = (size_t)1 << 40;
+        bytes = c->p->plan((int64_t)std::min(rows, most), (int64_t)std::min(n_seqs, most),
+                           (int64_t)std::min(max_rows, most), (int64_t)std::min(max_len, most)).ws_bytes;
+    });
+    return bytes;
+}
+
+sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *qy, void *ws, size_t ws_bytes, void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        if (!qy) throw sd::ArgError("null argument");
+        if (qy->rows == 0) return;
+        if (!qy->q || !qy->out || !qy->row_start || !qy->kv_len || !qy->table) throw sd::ArgError("null argument");
+        if (qy->n_seqs < 1 || qy->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
+        if (qy->mask && qy->mask_words < 1) throw sd::ArgError("mask_words must be positive");
+        const size_t most = (size_t)1 << 40;
+        const sd::KvqPlan plan = P.plan((int64_t)std::min(qy->rows, most), qy->n_seqs, (int64_t)std::min(qy->max_rows, most),
+                                        (int64_t)std::min(qy->max_len, most));
+        if (plan.ws_bytes && (!ws || ws_bytes < plan.ws_bytes))
+            throw sd::ArgError("attend: the workspace needs " + std::to_string(plan.ws_bytes) + " bytes");
+        need_aligned(ws, 16, 16, "workspace");
+        if (!std::isfinite(qy->scale)) throw sd::ArgError("scale must be finite");
+        const int hd = P.cfg.head_dim;
+        sd::KvqAttn a{};
+        a.L = P.layer(layer);
+        a.q = qy->q;
+        a.q_row = row_stride(qy->q_ld, (int64_t)P.cfg.n_heads * hd, "q");
+        a.q_head = hd;
+        a.out = qy->out;
+        a.out_ld = row_stride(qy->out_ld, (int64_t)P.cfg.n_heads * hd, "out");
+        need_aligned(a.q, a.q_row * 2, 16, "q");
+        need_aligned(a.out, a.out_ld * 2, 8, "out");
+        a.rows = (int)qy->rows;
+        a.n_seqs = qy->n_seqs;
+        a.row_start = qy->row_start;
+        a.kv_len = qy->kv_len;
+        a.table = qy->table;
+        a.table_ld = qy->table_ld;
+        a.mask = qy->mask;
+        a.mask_words = qy->mask_words;
+        a.max_rows = (int)qy->max_rows;
+        a.n_heads = P.cfg.n_heads;
+        a.n_rep = P.cfg.n_heads / P.cfg.n_kv_heads;
+        a.scale = qy->scale == 0.f ? (float)(1.0 / std::sqrt((double)hd)) : qy->scale;
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kvq_attention(a, plan, ws, (hipStream_t)stream);
+    });
+}
+
+sd_status sd_sampler_create(int32_t vocab, int32_t max_rows, int32_t device, sd_sampler **out) {
+    return guard([&] {
+        if (!out) throw sd::ArgError("null argument");
+        *out = nullptr;
+        auto h = std::make_unique<sd_sampler>();
+        h->s = std::make_unique<sd::Sampler>(vocab, max_rows, device);
+        *out = h.release();
+    });
+}
+void sd_sampler_destroy(sd_sampler *s) { delete s; }
+
+sd_status sd_sampler_run(sd_sampler *s, const float *logits, size_t ld, size_t rows, const sd_sampling *params,
+                         const float *uniforms, int32_t *tokens, float *probs, void *stream) {
+    return guard([&] {
+        if (!s || !s->s) throw sd::ArgError("null sampler handle");
+        if (!params) throw sd::ArgError("null argument");
+        if (rows > 65535 || ld > ((size_t)1 << 40)) throw sd::ArgError("sampler: rows or ld out of range");
+        sd::SampleParams p{};
+        p.logits = logits;
+        p.ld = (int64_t)ld;
+        p.rows = (int)rows;
+        p.temperature = params->temperature;
+        p.top_k = params->top_k;
+        p.top_p = params->top_p;
+        p.min_p = params->min_p;
+        p.u = uniforms;
+        p.tokens = tokens;
+        p.probs = probs;
+        s->s->run(p, (hipStream_t)stream);
     });
 }
 

@@ -34,6 +34,7 @@ LIB_PATH = os.environ.get("SPECULATE_HIP_LIB") or os.path.join(HERE, "libspecula
 SD_OK, SD_ERR_SAMPLING, SD_ERR_ROLLBACK, SD_ERR_BACKEND, SD_ERR_ARG, SD_ERR_UNSUPPORTED = range(6)
 # formats (GGML type ids)
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
+F16 = 1  # rows of the operators on device memory
 # tensor kinds
 (TOK_EMBD, OUTPUT, OUTPUT_NORM, ATTN_Q, ATTN_K, ATTN_V, ATTN_OUTPUT, FFN_GATE, FFN_UP, FFN_DOWN,
  ATTN_NORM, FFN_NORM, ATTN_Q_BIAS, ATTN_K_BIAS, ATTN_V_BIAS) = range(15)
@@ -113,6 +114,35 @@ class Draft2Config(ctypes.Structure):
     _fields_ = [("hidden", ctypes.c_int32), ("n_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
                 ("ffn", ctypes.c_int32), ("vocab", ctypes.c_int32), ("rms_eps", ctypes.c_float),
                 ("rope_theta", ctypes.c_float), ("max_pos", ctypes.c_int32), ("device", ctypes.c_int32)]
+
+
+class KvPoolConfig(ctypes.Structure):
+    """sd_kvpool_config"""
+    _fields_ = [("n_layers", ctypes.c_int32), ("n_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("page_tokens", ctypes.c_int32),
+                ("max_pos", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("rope_theta", ctypes.c_float),
+                ("device", ctypes.c_int32)]
+
+
+class KvRows(ctypes.Structure):
+    """sd_kv_rows"""
+    _fields_ = [("n", ctypes.c_size_t), ("seq", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int32), ("table_ld", ctypes.c_int32)]
+
+
+class KvQuery(ctypes.Structure):
+    """sd_kv_query"""
+    _fields_ = [("q", ctypes.c_void_p), ("q_ld", ctypes.c_size_t), ("out", ctypes.c_void_p),
+                ("out_ld", ctypes.c_size_t), ("rows", ctypes.c_size_t), ("row_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p), ("n_seqs", ctypes.c_int32),
+                ("table_ld", ctypes.c_int32), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int32),
+                ("max_rows", ctypes.c_size_t), ("max_len", ctypes.c_size_t), ("scale", ctypes.c_float)]
+
+
+class Sampling(ctypes.Structure):
+    """sd_sampling"""
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
 
 
 # tensor kinds of sd_draft2_set_tensor (eagle.rs:126-131, 279-286, 349-361)
@@ -205,6 +235,16 @@ def load_library(path: str = LIB_PATH):
         "sd_draft2_reset": ([P], I32),
         "sd_draft2_forward": ([P, P, SZ, ctypes.c_uint32, SZ, P], I32),
         "sd_draft2_round": ([P, P, P, SZ, P, P, P], I32),
+        "sd_kvpool_create": ([ctypes.POINTER(KvPoolConfig), ctypes.POINTER(P)], I32),
+        "sd_kvpool_destroy": ([P], None),
+        "sd_kvpool_page_bytes": ([P], SZ),
+        "sd_kvpool_append": ([P, I32, ctypes.POINTER(KvRows), I32, P, SZ, P, SZ, P, SZ, P, P, P], I32),
+        "sd_kvpool_read": ([P, I32, ctypes.POINTER(KvRows), P, P, P], I32),
+        "sd_kvpool_attend_workspace": ([P, SZ, SZ, SZ, SZ], SZ),
+        "sd_kvpool_attend": ([P, I32, ctypes.POINTER(KvQuery), P, SZ, P], I32),
+        "sd_sampler_create": ([I32, I32, I32, ctypes.POINTER(P)], I32),
+        "sd_sampler_destroy": ([P], None),
+        "sd_sampler_run": ([P, P, SZ, SZ, ctypes.POINTER(Sampling), P, P, P, P], I32),
         "sd_draft3_create": ([ctypes.POINTER(Draft3Config), ctypes.POINTER(P)], I32),
         "sd_draft3_destroy": ([P], None),
         "sd_draft3_tensor_bytes": ([P, I32], SZ),
@@ -1066,6 +1106,91 @@ class HipEagle3Draft:
         return ([[int(v) for v in ids[s, :ks[s]]] for s in range(depth)],
                 [[float(v) for v in lps[s, :ks[s]]] for s in range(depth)],
                 [[int(v) for v in dids[s, :ks[s]]] for s in range(depth)])
+
+
+class HipKvPool:
+    """A paged KV cache in 4 bits on one GPU and the attention over it
+    (sd_kvpool_*).  Arguments that are arrays are device addresses (int; 0 for
+    an optional one that is absent) of memory on the pool's GPU, `stream` a
+    hipStream_t (0: the default stream); calls enqueue and return."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_pages: int, page_tokens: int = 64,
+                 max_pos: int = 8192, rope_theta: float = 10000.0, interleaved: bool = True, device: int = 0):
+        load_library()
+        c = KvPoolConfig(n_layers, n_heads, n_kv_heads, head_dim, n_pages, page_tokens, max_pos, int(interleaved),
+                         rope_theta, device)
+        self._h = ctypes.c_void_p()
+        _check(_lib.sd_kvpool_create(ctypes.byref(c), ctypes.byref(self._h)))
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value:
+            _lib.sd_kvpool_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def page_bytes(self) -> int:
+        """Bytes of one page of one layer."""
+        return int(_lib.sd_kvpool_page_bytes(self._h))
+
+    def append(self, layer: int, n: int, k: int, v: int, slots: int, table: int, n_seqs: int, table_ld: int,
+               dtype: int = F16, seqs: int = 0, pos: int = 0, q: int = 0, q_out: int = 0, q_ld: int = 0, k_ld: int = 0,
+               v_ld: int = 0, stream: int = 0):
+        """Rows k, v [n][n_kv_heads][head_dim] (dtype F16 or F32) rotated,
+        quantised and written to their slots; the rotated q rows go to q_out (fp16)."""
+        r = KvRows(n, seqs, slots, table, n_seqs, table_ld)
+        _check(_lib.sd_kvpool_append(self._h, layer, ctypes.byref(r), dtype, q, q_ld, k, k_ld, v, v_ld, pos, q_out,
+                                     stream))
+
+    def read(self, layer: int, n: int, slots: int, table: int, n_seqs: int, table_ld: int, k_out: int, v_out: int,
+             seqs: int = 0, stream: int = 0):
+        """The rows' keys and values as fp16 [n][n_kv_heads][head_dim]."""
+        r = KvRows(n, seqs, slots, table, n_seqs, table_ld)
+        _check(_lib.sd_kvpool_read(self._h, layer, ctypes.byref(r), k_out, v_out, stream))
+
+    def attend_workspace(self, rows: int, n_seqs: int, max_rows: int, max_len: int) -> int:
+        """Bytes of zeroed device memory attend() needs for these sizes."""
+        return int(_lib.sd_kvpool_attend_workspace(self._h, rows, n_seqs, max_rows, max_len))
+
+    def attend(self, layer: int, q: int, out: int, row_start: int, kv_len: int, table: int, n_seqs: int, table_ld: int,
+               rows: int, max_rows: int, max_len: int, ws: int = 0, ws_bytes: int = 0, mask: int = 0,
+               mask_words: int = 0, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0, stream: int = 0):
+        """Attention of the sequences' last rows over their positions (sd_kv_query)."""
+        a = KvQuery(q, q_ld, out, out_ld, rows, row_start, kv_len, table, n_seqs, table_ld, mask, mask_words, max_rows,
+                    max_len, scale)
+        _check(_lib.sd_kvpool_attend(self._h, layer, ctypes.byref(a), ws, ws_bytes, stream))
+
+
+class HipSampler:
+    """Token sampling with temperature, top-k, top-p and min-p from given
+    random numbers on one GPU (sd_sampler_*); arrays are device addresses."""
+
+    def __init__(self, vocab: int, max_rows: int, device: int = 0):
+        load_library()
+        self._h = ctypes.c_void_p()
+        _check(_lib.sd_sampler_create(vocab, max_rows, device, ctypes.byref(self._h)))
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value:
+            _lib.sd_sampler_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def sample(self, logits: int, rows: int, uniforms: int, tokens: int, temperature: float = 1.0, top_k: int = 0,
+               top_p: float = 1.0, min_p: float = 0.0, probs: int = 0, ld: int = 0, stream: int = 0):
+        """tokens[r] drawn from row r of f32 logits by uniforms[r]; -1 for a row
+        without a distribution.  probs: the filtered distributions [rows][vocab]."""
+        s = Sampling(temperature, top_k, top_p, min_p)
+        _check(_lib.sd_sampler_run(self._h, logits, ld, rows, ctypes.byref(s), uniforms, tokens, probs, stream))
 
 
 def tree_cartesian(root: int, head_top_k: Sequence[Sequence[int]]) -> Tuple[np.ndarray, np.ndarray]:

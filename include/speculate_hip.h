@@ -43,6 +43,8 @@ typedef enum sd_status {
 
 /* Tensor formats: the GGML type ids of the GGUF blocks. */
 enum { SD_F32 = 0, SD_Q8_0 = 8, SD_Q4_K = 12, SD_Q5_K = 13, SD_Q6_K = 14 };
+/* fp16: a row format of the operators on device memory, not a tensor format */
+enum { SD_F16 = 1 };
 
 /* Tensor kinds.  The GGUF names follow quantized_llama_local.rs:242-281 and
  * quantized_qwen2_local.rs:232-275 ("blk.{i}." prefix for per-layer tensors). */
@@ -374,6 +376,138 @@ sd_status sd_gguf_tensor_info(const sd_gguf *g, const char *name, int32_t *type,
  * upload; the model must have been created from this file's config (ctx_len,
  * max_batch and device aside), else SD_ERR_ARG. */
 sd_status sd_model_load_gguf(sd_model *m, const sd_gguf *g);
+
+/* ---- a paged KV cache in 4 bits and the attention over it (device memory) ------- */
+/* The cache of sequences that are decoded at long contexts, in pages that the
+ * caller gives out.  No counterpart in the reference (its caches are tensors
+ * in the compute type).  32 channels of one position and KV head share one
+ * fp16 step d: with A the largest magnitude, |d| = fp16(fp32(A / 8)), negative
+ * when that magnitude is a positive number's alone; channel x is stored as
+ * clamp(round(x / d), -8, 7) (halves to even) and stands for fp16(d * code).
+ * A group with a value that is not finite or above 65504 stands for NaN.
+ * 4.5 bits a value: 144 bytes per position and KV head of 128 channels, for
+ * keys and values together.
+ *
+ * All pointers of these calls are device memory of the pool's GPU, complete
+ * before the call on `stream` (a hipStream_t; NULL is the default stream);
+ * the calls enqueue and return, allocate nothing and can be captured into a
+ * graph.  The current device is left as it was.  Calls that touch the same
+ * pages, or use the same workspace, must be ordered by the caller (one
+ * stream, or events); a pool has no other state that calls change. */
+typedef struct sd_kvpool sd_kvpool;
+typedef struct sd_kvpool_config {
+    int32_t n_layers, n_heads, n_kv_heads;
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t n_pages;      /* pages of each layer */
+    int32_t page_tokens;  /* positions of a page: a power of two, 32 to 4096 */
+    int32_t max_pos;      /* rotation positions [0, max_pos) */
+    int32_t interleaved;  /* 1: pairs (2i, 2i + 1) (Llama GGUF), 0: pairs (i, i + head_dim / 2) (Qwen2) */
+    float rope_theta;
+    int32_t device;
+} sd_kvpool_config;
+/* Pages are zeroed.  The angles pos * theta^(-2i/head_dim) are computed in 64
+ * bits, their cos and sin kept in 32. */
+sd_status sd_kvpool_create(const sd_kvpool_config *cfg, sd_kvpool **out);
+void sd_kvpool_destroy(sd_kvpool *c);
+/* bytes of one page of one layer */
+size_t sd_kvpool_page_bytes(const sd_kvpool *c);
+
+/* Rows of a call.  Row r is position slot[r] of sequence seq[r] (sequence 0
+ * with seq NULL); that position lives in page
+ * table[seq * table_ld + slot / page_tokens].  A row whose sequence is outside
+ * [0, n_seqs), whose slot is negative or past the table, or whose page id is
+ * outside the pool is padding: nothing is read or written for it.  No two rows
+ * of an append may be the same position of the same page (its content is then
+ * a mixture of the two). */
+typedef struct sd_kv_rows {
+    size_t n;
+    const int32_t *seq;
+    const int32_t *slot;
+    const int32_t *table;
+    int32_t n_seqs, table_ld;
+} sd_kv_rows;
+/* Appends k and v [n][n_kv_heads][head_dim] (fmt SD_F16 or SD_F32, row strides
+ * k_ld and v_ld elements, 0: dense) to a layer: k rotated to pos[r] (slot[r]
+ * with pos NULL), both quantised.  With q [n][n_heads][head_dim], the rotated
+ * queries go to q_out [n][n_heads][head_dim] fp16; q NULL: keys and values
+ * only.  Rows at a rotation position outside [0, max_pos) are padding.  Rows
+ * must start at multiples of 16 bytes. */
+sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, int32_t fmt, const void *q, size_t q_ld,
+                           const void *k, size_t k_ld, const void *v, size_t v_ld, const int32_t *pos, uint16_t *q_out,
+                           void *stream);
+/* The rows' keys (rotated) and values as fp16 [n][n_kv_heads][head_dim];
+ * either output may be NULL.  Padding rows' outputs are left as they were. */
+sd_status sd_kvpool_read(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, uint16_t *k_out, uint16_t *v_out,
+                         void *stream);
+
+/* Attention of query rows over a layer, softmax(scale q K^T) V with query head
+ * h reading KV head h / (n_heads / n_kv_heads).  Rows row_start[s] ..
+ * row_start[s + 1) are the last positions of sequence s, which holds kv_len[s]
+ * positions, these among them (append first): row i of n sees the positions up
+ * to kv_len - n + i, or with a mask all positions below kv_len - n and, of the
+ * sequence's own rows, row j where bit j of mask[row][mask_words] is set (a
+ * tree's ancestor bits).  A row that sees no position gives zeros, one whose
+ * scores are all -inf too.  What is masked has no influence, NaN included.
+ * Sequences may have no rows; rows outside every sequence, and those past
+ * max_rows of one, are left as they were.  Positions past the table, and
+ * pages whose id is outside the pool, hold nothing and are not seen. */
+typedef struct sd_kv_query {
+    const uint16_t *q;          /* fp16 [rows][n_heads][head_dim], row stride q_ld (0: dense), 16-byte aligned rows */
+    size_t q_ld;
+    uint16_t *out;              /* fp16 [rows][n_heads][head_dim], row stride out_ld (0: dense), 8-byte aligned rows */
+    size_t out_ld;
+    size_t rows;
+    const int32_t *row_start;   /* [n_seqs + 1] */
+    const int32_t *kv_len;      /* [n_seqs] */
+    const int32_t *table;       /* [n_seqs][table_ld] */
+    int32_t n_seqs, table_ld;
+    const uint64_t *mask;       /* [rows][mask_words] or NULL: causal */
+    int32_t mask_words;
+    size_t max_rows;            /* most rows of one sequence (host bound of row_start) */
+    size_t max_len;             /* most positions of one sequence: plans the work, larger kv_len stay correct */
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+} sd_kv_query;
+/* Bytes of workspace sd_kvpool_attend needs for these sizes (0 for a bad handle or bad sizes, or where none is needed). */
+size_t sd_kvpool_attend_workspace(const sd_kvpool *c, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len);
+/* ws: device memory of at least that many bytes, zeroed before its first use
+ * (calls leave zeros where they need them), 16-byte aligned; each call in
+ * flight needs its own, and two graphs that may run at once must not share one. */
+sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *query, void *ws, size_t ws_bytes,
+                           void *stream);
+
+/* ---- sampling (device memory) ----------------------------------------------------- */
+/* One token per row of logits from a given random number, with the filters
+ * applied in this order (softmax_with_temperature, top_p_filter and
+ * sample_from_distribution, sampling/tokens.rs:15-120, with top-k and min-p
+ * beside them and in 64 bits):
+ *   w_i = exp((l_i - max) / temperature); temperature 0: the first maximum
+ *   top-k  the k largest, of equal ones the first (0: off)
+ *   top-p  the shortest run of the rest, largest first (of equal ones the
+ *          first), whose weights reach top_p of the rest's sum (1: off)
+ *   min-p  of those the ones with w_i >= min_p (0: off)
+ *   token  the first kept i whose running sum, by index, exceeds u times the
+ *          kept sum
+ * A row with a NaN or +inf, or of -inf only, has no distribution: token -1,
+ * its probabilities zeros. */
+typedef struct sd_sampling {
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+} sd_sampling;
+typedef struct sd_sampler sd_sampler;
+/* A workspace for up to max_rows rows of vocab (<= 262144) logits.  Calls on
+ * one handle, replays of graphs that captured them among these, must be
+ * ordered by the caller. */
+sd_status sd_sampler_create(int32_t vocab, int32_t max_rows, int32_t device, sd_sampler **out);
+void sd_sampler_destroy(sd_sampler *s);
+/* logits f32 [rows] of stride ld (0: vocab), uniforms f32 [rows] in [0, 1),
+ * tokens int32 [rows], probs f32 [rows][vocab] (the filtered distributions,
+ * e.g. the draft rows of sd_verify_rejection_*_device_q) or NULL: device
+ * memory of the handle's GPU.  Enqueues on `stream` (NULL: the default
+ * stream); allocates nothing and can be captured.  SD_ERR_SAMPLING for
+ * filters out of range. */
+sd_status sd_sampler_run(sd_sampler *s, const float *logits, size_t ld, size_t rows, const sd_sampling *params,
+                         const float *uniforms, int32_t *tokens, float *probs, void *stream);
 
 /* ---- draft-tree builders (host only; no GPU needed) ---------------------------- */
 /* build_cartesian_tree (methods/medusa.rs:172-193): step d has branching[d]

@@ -1,0 +1,458 @@
+"""The 4-bit paged KV cache and the attention over it (sd_kvpool_*) against a
+64-bit restatement: stored values bit for bit, attention within the rounding of
+its fp16 weights, at the lengths, masks, strides and pages where it can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+import _kvq
+
+pytestmark = pytest.mark.gpu
+
+MAX_POS = 5000
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def host(t):
+    torch.cuda.synchronize()
+    return t.cpu().numpy()
+
+
+def ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+class Pool:
+    """A pool with the sequences' pages at random places and the oracle's copy of what they hold."""
+
+    def __init__(self, hip, seed, H, KV, hd, lens, page=64, layers=1, interleaved=True, theta=10000.0):
+        self.hip, self.H, self.KV, self.hd, self.page, self.lens = hip, H, KV, hd, page, list(lens)
+        self.inter, self.rng = interleaved, np.random.default_rng(seed)
+        need = [max(1, -(-n // page)) for n in lens]
+        self.n_pages = sum(need) + 2
+        ids = self.rng.permutation(self.n_pages).tolist()
+        self.table = np.full((len(lens), max(need)), -1, np.int32)
+        for s, n in enumerate(need):
+            self.table[s, :n] = [ids.pop() for _ in range(n)]
+        self.pool = hip.HipKvPool(n_layers=layers, n_heads=H, n_kv_heads=KV, head_dim=hd, n_pages=self.n_pages,
+                                  page_tokens=page, max_pos=MAX_POS, rope_theta=theta, interleaved=interleaved)
+        self.cos, self.sin = _kvq.tables(MAX_POS, hd, theta)
+        self.dtable = dev(self.table)
+
+    def rows(self, n, heads, dt=np.float16):
+        return (self.rng.standard_normal((n, heads, self.hd)) * (1 + 5 * (self.rng.random((1, heads, self.hd)) > .95))).astype(dt)
+
+    def append(self, k, v, seq, slot, layer=0, pos=None, q=None, stream=0):
+        dt = self.hip.F32 if k.dtype == np.float32 else self.hip.F16
+        dk, dv, ds, dl = dev(k), dev(v), dev(np.asarray(seq, np.int32)), dev(np.asarray(slot, np.int32))
+        dp = None if pos is None else dev(np.asarray(pos, np.int32))
+        dq = None if q is None else dev(q)
+        qo = None if q is None else torch.full((len(k), self.H, self.hd), 77.0, dtype=torch.float16, device="cuda")
+        torch.cuda.synchronize()
+        self.pool.append(layer, len(k), ptr(dk), ptr(dv), ptr(dl), ptr(self.dtable), *self.table.shape, dtype=dt,
+                         seqs=ptr(ds), pos=ptr(dp), q=ptr(dq), q_out=ptr(qo), stream=stream)
+        torch.cuda.synchronize()
+        return None if q is None else host(qo)
+
+    def read(self, seq, slot, layer=0, fill=5.0):
+        n = len(slot)
+        ds, dl = dev(np.asarray(seq, np.int32)), dev(np.asarray(slot, np.int32))
+        ko, vo = (torch.full((n, self.KV, self.hd), fill, dtype=torch.float16, device="cuda") for _ in range(2))
+        self.pool.read(layer, n, ptr(dl), ptr(self.dtable), *self.table.shape, ptr(ko), ptr(vo), seqs=ptr(ds))
+        return host(ko), host(vo)
+
+    def fill(self, layer=0, edit=None):
+        """all positions of all sequences; returns the values they stand for, a (k, v) pair per sequence"""
+        out = []
+        for s, n in enumerate(self.lens):
+            k, v = self.rows(n, self.KV), self.rows(n, self.KV)
+            if edit:
+                edit(s, k, v)
+            if n:
+                self.append(k, v, [s] * n, range(n), layer)
+            with np.errstate(invalid="ignore"):
+                out.append((_kvq.store(_kvq.rotate(k.astype(np.float64), np.arange(n), self.cos, self.sin, self.inter)),
+                            _kvq.store(v.astype(np.float64))))
+        return out
+
+    def attend(self, q, counts, lens=None, layer=0, mask=None, scale=0.0, max_len=None, out=None, q_ld=0, out_ld=0,
+               max_rows=None, table=None, stream=0, ws=None):
+        lens = self.lens if lens is None else lens
+        rows = int(sum(counts))
+        start = dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+        dl, dq, dm = dev(np.asarray(lens, np.int32)), dev(q), None if mask is None else dev(mask.view(np.int64))
+        if out is None:
+            out = torch.full((rows, self.H, self.hd), 9.0, dtype=torch.float16, device="cuda")
+        table = self.dtable if table is None else table
+        max_rows = max(counts) if max_rows is None else max_rows
+        max_len = max(lens) if max_len is None else max_len
+        if ws is None:
+            ws = torch.zeros(self.pool.attend_workspace(rows, len(counts), max_rows, max_len), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        self.pool.attend(layer, ptr(dq), ptr(out), ptr(start), ptr(dl), ptr(table), *table.shape, rows=rows,
+                         max_rows=max_rows, max_len=max_len, ws=ptr(ws) if ws.numel() else 0, ws_bytes=ws.numel(),
+                         mask=ptr(dm), mask_words=0 if mask is None else mask.shape[1], scale=scale, q_ld=q_ld,
+                         out_ld=out_ld, stream=stream)
+        return host(out)
+
+
+def causal(n, T):
+    return np.arange(T)[None] <= np.arange(n)[:, None] + (T - n)
+
+
+def check_rows(got, q, kv, visible, scale):
+    """Within the roundings: fp16 weights (2^-11 of each, and 2^-25 where they are subnormal), the fp16 result, fp32 scores
+    (hd products and sums of 2^-24) inside the exponential."""
+    k, v = kv
+    want, mag, smax = _kvq.attend(q, k, v, visible, scale)
+    hd, T = q.shape[-1], len(k)
+    vmax = float(np.max(np.abs(v.astype(np.float64)))) if T else 0.0
+    score = 2 * hd * 2.0 ** -24 * smax + 2.0 ** -20
+    tol = 2.0 ** -11 * (np.abs(want) + mag) * 1.01 + 2 * score * mag + T * 2.0 ** -25 * vmax + 2.0 ** -25
+    err = np.abs(got.astype(np.float64) - want)
+    assert not np.isnan(err).any()
+    bad = err > tol
+    assert not bad.any(), (float(np.max(err - tol)), np.argwhere(bad)[:4].tolist())
+
+
+# ---- append and read -------------------------------------------------------------
+@pytest.mark.parametrize("hd,KV,H", [(128, 8, 32), (64, 8, 8), (128, 1, 7), (64, 3, 6)])
+@pytest.mark.parametrize("dt", [np.float16, np.float32])
+@pytest.mark.parametrize("inter", [True, False])
+def test_append_and_read(hip, hd, KV, H, dt, inter):
+    p = Pool(hip, hd + KV, H, KV, hd, [130, 1, 33, 64], page=32, interleaved=inter, theta=500000.0)
+    seq = np.concatenate([[s] * n for s, n in enumerate(p.lens)])
+    slot = np.concatenate([np.arange(n) for n in p.lens])
+    order = p.rng.permutation(len(seq))  # any order
+    seq, slot = seq[order], slot[order]
+    pos = (slot * 13 + seq * 1000) % MAX_POS
+    k, v, q = p.rows(len(seq), KV, dt), p.rows(len(seq), KV, dt), p.rows(len(seq), H, dt)
+    k[3, 0, :32] = 0.0  # a group of zeros
+    v[5] *= np.asarray(1e-7, dt)  # steps that are subnormal or 0
+    qo = p.append(k, v, seq, slot, pos=pos, q=q)
+    gk, gv = p.read(seq, slot)
+    turned = _kvq.rotate(k.astype(np.float64), pos, p.cos, p.sin, inter)
+    assert np.array_equal(gk, _kvq.store(turned))
+    assert np.array_equal(gv, _kvq.store(v.astype(np.float64)))
+    want = _kvq.rotate(q.astype(np.float64), pos, p.cos, p.sin, inter)
+    # an fp16 rounding and two fp32 ones of terms up to the pair's magnitude
+    assert np.all(np.abs(qo.astype(np.float64) - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * np.abs(q).max() + 2.0 ** -25)
+
+
+def test_append_extremes_and_ties(hip):
+    """V rows chosen at the borders: halves, +A beside -A, the fp16 maximum, values that are not finite."""
+    p = Pool(hip, 3, 4, 2, 64, [40], page=32)
+    n = 40
+    v = np.zeros((n, 2, 64), np.float32)
+    k = p.rows(n, 2, np.float32)
+    for i in range(n):
+        v[i] = p.rng.integers(-16, 17, (2, 64)) * 0.5 * 2.0 ** p.rng.integers(-10, 8)  # many exact halves
+    v[0, 0, :32] = 0.0
+    v[0, 0, 3], v[0, 0, 9] = 4.0, -4.0
+    v[1, 0, 5] = 65504.0
+    v[1, 1, 5] = -65504.0
+    v[2, 0, 7] = 65505.0
+    v[2, 1, 40] = np.nan
+    v[3, 0, 1] = np.inf
+    v[3, 1, 33] = -np.inf
+    v[4] = 1e-30
+    k[6, 0, 2] = np.nan
+    k[6, 1, 50] = np.inf
+    k[7] *= 1e5
+    p.append(k, v, [0] * n, range(n))
+    gk, gv = p.read([0] * n, range(n))
+    with np.errstate(invalid="ignore"):
+        wk = _kvq.store(_kvq.rotate(k.astype(np.float64), np.arange(n), p.cos, p.sin, True))
+    assert np.array_equal(gv, _kvq.store(v.astype(np.float64)), equal_nan=True)
+    assert np.array_equal(gk, wk, equal_nan=True)
+    assert np.isnan(gv[2, 0, :32]).all() and not np.isnan(gv[2, 0, 32:]).any()
+
+
+def test_padding_rows_and_bad_pages_are_left_out(hip):
+    """Sequences, slots, positions and pages outside leave memory and outputs as they were."""
+    p = Pool(hip, 4, 4, 2, 128, [64, 64], page=32, layers=2)
+    p.table[1, 1] = p.n_pages  # outside the pool
+    p.dtable = dev(p.table)
+    base = p.rows(96, 2), p.rows(96, 2)
+    seq, slot = [0] * 64 + [1] * 32, list(range(64)) + list(range(32))
+    p.append(*base, seq, slot)
+    before = p.read(seq, slot)
+    bad_seq = [-1, 2, 0, 0, 1, 0, -2147483648, 0]
+    bad_slot = [3, 3, -1, 64, 40, 2147483647, 0, 5]
+    bad_pos = [0, 0, 0, 0, 0, 0, 0, MAX_POS]
+    k, v, q = p.rows(8, 2), p.rows(8, 2), p.rows(8, 4)
+    qo = p.append(k, v, bad_seq, bad_slot, pos=bad_pos, q=q)
+    assert (qo == 77.0).all()
+    p.append(k, v, bad_seq, bad_slot, layer=1, pos=bad_pos)
+    after = p.read(seq, slot)
+    assert np.array_equal(before[0], after[0]) and np.array_equal(before[1], after[1])
+    rk, rv = p.read(bad_seq[:7], bad_slot[:7], fill=5.0)
+    assert (rk == 5.0).all() and (rv == 5.0).all()
+    lk, lv = p.read(seq, slot, layer=1)  # the other layer holds zeros
+    assert not lk.any() and not lv.any()
+
+
+def test_strided_rows(hip):
+    """q, k and v as column ranges of one product's rows, as the decoder has them."""
+    p = Pool(hip, 5, 4, 2, 64, [50], page=64, interleaved=False)
+    n, w = 50, 8 * 64
+    x = p.rng.standard_normal((n, w)).astype(np.float32)
+    dx, ds = dev(x), dev(np.arange(n, dtype=np.int32))
+    qo = torch.zeros((n, 4, 64), dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    p.pool.append(0, n, ptr(dx) + 4 * 256, ptr(dx) + 4 * 384, ptr(ds), ptr(p.dtable), 1, 1, dtype=hip.F32, q=ptr(dx),
+                  q_out=ptr(qo), q_ld=w, k_ld=w, v_ld=w)
+    gk, gv = p.read([0] * n, range(n))
+    k = x[:, 256:384].reshape(n, 2, 64).astype(np.float64)
+    assert np.array_equal(gk, _kvq.store(_kvq.rotate(k, np.arange(n), p.cos, p.sin, False)))
+    assert np.array_equal(gv, _kvq.store(x[:, 384:].reshape(n, 2, 64)))
+    want = _kvq.rotate(x[:, :256].reshape(n, 4, 64).astype(np.float64), np.arange(n), p.cos, p.sin, False)
+    assert np.all(np.abs(host(qo) - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * np.abs(x).max())
+
+
+# ---- attention -------------------------------------------------------------------
+@pytest.mark.parametrize("hd,KV,H,page", [(128, 2, 8, 64), (64, 4, 4, 32), (128, 1, 7, 128), (64, 2, 16, 256), (128, 2, 2, 32)])
+@pytest.mark.parametrize("rows,T", [(1, 1), (1, 2), (1, 31), (1, 32), (1, 33), (1, 777), (1, 3000), (2, 2), (5, 5), (5, 64), (5, 1025),
+                                    (17, 17), (33, 100), (70, 200), (300, 301), (129, 129)])
+def test_attention_causal(hip, hd, KV, H, page, rows, T):
+    p = Pool(hip, rows * 7 + T, H, KV, hd, [T], page=page)
+    (kv,) = p.fill()
+    q = p.rows(rows, H)
+    got = p.attend(q, [rows])
+    check_rows(got, q, kv, causal(rows, T), hd ** -0.5)
+
+
+@pytest.mark.parametrize("hd,KV,H", [(128, 2, 8), (64, 4, 4), (128, 1, 7)])
+def test_attention_ragged_batch(hip, hd, KV, H):
+    lens = [0, 1, 700, 33, 64, 5, 2000, 31]
+    counts = [0, 1, 3, 0, 64, 5, 1, 2]
+    p = Pool(hip, 11, H, KV, hd, lens, page=64)
+    kvs = p.fill()
+    q = p.rows(sum(counts), H)
+    got = p.attend(q, counts)
+    at = 0
+    for s, n in enumerate(counts):
+        if n:
+            check_rows(got[at:at + n], q[at:at + n], kvs[s], causal(n, lens[s]), hd ** -0.5)
+        at += n
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,T", [(1, 1), (7, 7), (60, 500), (64, 96), (65, 65), (128, 1000), (100, 131)])
+def test_attention_tree_masks(hip, hd, rows, T):
+    """Random masks, among them rows that see only the prefix, or (without one) nothing at all."""
+    p = Pool(hip, rows + T, 4, 2, hd, [T], page=32)
+    (kv,) = p.fill()
+    bits = p.rng.random((rows, rows)) < 0.2
+    bits[::5] = False
+    words = -(-rows // 64)
+    mask = np.zeros((rows, words), np.uint64)
+    for i, j in np.argwhere(bits):
+        mask[i, j // 64] |= np.uint64(1) << np.uint64(j % 64)
+    mask[:, -1] |= np.uint64(1) << np.uint64(63) if rows % 64 else np.uint64(0)  # a bit past the rows means nothing
+    visible = np.concatenate([np.ones((rows, T - rows), bool), bits], 1)
+    q = p.rows(rows, 4)
+    got = p.attend(q, [rows], mask=mask)
+    check_rows(got, q, kv, visible, hd ** -0.5)
+    if T == rows:
+        assert not got[::5].any()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_nan_and_inf_behind_masks(hip, hd):
+    """NaN keys and values of positions that a row does not see leave it alone; a row that sees them is NaN there."""
+    T, rows = 70, 6
+
+    def edit(s, k, v):
+        v[67, 0, 40] = np.nan  # the second group of KV head 0
+        k[66, 1, 3] = np.inf  # a key of KV head 1
+        v[69, 1, 0] = np.inf
+    p = Pool(hip, 8, 4, 2, hd, [T], page=32)
+    kv = p.fill(edit=edit)[0]
+    q = p.rows(rows, 4)
+    bits = np.tril(np.ones((rows, rows), bool))
+    bits[4, 3] = False  # row 4 does not see position 67
+    bits[5] = [1, 0, 0, 0, 0, 1]
+    mask = np.zeros((rows, 1), np.uint64)
+    for i, j in np.argwhere(bits):
+        mask[i, 0] |= np.uint64(1) << np.uint64(j)
+    got = p.attend(q, [rows], mask=mask)
+    clean = [np.where(np.isnan(x), 0, x) for x in kv]
+    visible = np.concatenate([np.ones((rows, T - rows), bool), bits], 1)
+    for h in range(4):
+        kvh = h // 2
+        for r in range(rows):
+            hole = np.zeros(hd, bool)
+            for t in np.nonzero(visible[r])[0]:
+                if np.isnan(kv[0][t, kvh]).any():
+                    hole[:] = True
+                hole |= np.isnan(kv[1][t, kvh])
+            assert np.array_equal(np.isnan(got[r, h]), hole), (r, h)
+            if not hole.any():
+                one = [x[:, kvh:kvh + 1] for x in clean]
+                check_rows(got[r:r + 1, h:h + 1], q[r:r + 1, h:h + 1], one, visible[r:r + 1], hd ** -0.5)
+    # the same behind a causal mask and past the end
+    got = p.attend(q[:3], [3], lens=[66 + 1])
+    check_rows(got[:2], q[:2], [x[:66] for x in clean], causal(2, 66), hd ** -0.5)
+
+
+@pytest.mark.parametrize("value", [1.0, 60.0, -60.0])
+def test_attention_sharp_and_flat_scores(hip, value):
+    """Scores of some hundreds, one above the rest by far, and all alike."""
+    p = Pool(hip, 21, 4, 2, 128, [300], page=64)
+    (kv,) = p.fill()
+    q = (p.rows(2, 4).astype(np.float32) * value).astype(np.float16)
+    check_rows(p.attend(q, [2]), q, kv, causal(2, 300), 128 ** -0.5)
+    q[:] = 0
+    check_rows(p.attend(q, [2]), q, kv, causal(2, 300), 128 ** -0.5)
+
+
+def test_attention_infinite_scores(hip):
+    """A query of infinities: rows whose scores are all -inf weigh nothing, +inf gives NaN as the formula does."""
+    p = Pool(hip, 22, 2, 1, 64, [5], page=32)
+    n = 5
+    k, v = np.ones((n, 1, 64), np.float16), p.rows(n, 1)
+    p.append(k, v, [0] * n, range(n), pos=[0] * n)
+    q = np.zeros((1, 2, 64), np.float16)
+    q[0, 0, 0], q[0, 1, 0] = -np.inf, np.inf
+    got = p.attend(q, [1])
+    assert not got[0, 0].any() and np.isnan(got[0, 1]).all()
+
+
+def test_attention_strides_scale_and_untouched_rows(hip):
+    p = Pool(hip, 31, 4, 2, 64, [200, 90], page=64)
+    kvs = p.fill()
+    wide = np.zeros((9, 4 * 64 + 24), np.float16)
+    q = p.rows(9, 4)
+    wide[:, :256] = q.reshape(9, 256)
+    out = torch.full((9, 4 * 64 + 12), 3.0, dtype=torch.float16, device="cuda")
+    # rows 0-2 of the first sequence, 3-5 of the second; max_rows 2 leaves each one's third; 6-8 belong to nobody
+    start, lens, dq = dev(np.array([0, 3, 6], np.int32)), dev(np.array([200, 90], np.int32)), dev(wide)
+    ws = torch.zeros(max(16, p.pool.attend_workspace(9, 2, 2, 200)), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    p.pool.attend(0, ptr(dq), ptr(out), ptr(start), ptr(lens), ptr(p.dtable), *p.table.shape, rows=9, max_rows=2, max_len=200,
+                  ws=ptr(ws), ws_bytes=ws.numel(), scale=0.3, q_ld=280, out_ld=268)
+    got = host(out)
+    assert (got[:, 256:] == 3.0).all() and (got[[2, 5, 6, 7, 8]] == 3.0).all()
+    for s, T in ((0, 200), (1, 90)):
+        vis = causal(3, T)[:2]
+        check_rows(got[3 * s:3 * s + 2, :256].reshape(2, 4, 64), q[3 * s:3 * s + 2], kvs[s], vis, np.float32(0.3))
+
+
+def test_attention_absent_pages(hip):
+    """Page ids outside the pool and tables shorter than the length hold nothing."""
+    p = Pool(hip, 33, 4, 2, 128, [256], page=64)
+    (kv,) = p.fill()
+    q = p.rows(1, 4)
+    t = p.table.copy()
+    t[0, 1], t[0, 2] = -1, p.n_pages + 7
+    vis = np.ones((1, 256), bool)
+    vis[:, 64:192] = False
+    check_rows(p.attend(q, [1], table=dev(t)), q, kv, vis, 128 ** -0.5)
+    vis[:, 192:] = False
+    check_rows(p.attend(q, [1], table=dev(t[:, :1])), q, kv, vis, 128 ** -0.5)
+    assert not p.attend(q, [1], table=dev(np.full((1, 4), -1, np.int32))).any()
+
+
+def test_attention_fewer_positions_than_rows(hip):
+    """Rows before the first position see nothing."""
+    p = Pool(hip, 34, 2, 1, 64, [40], page=32)
+    (kv,) = p.fill()
+    q = p.rows(6, 2)
+    got = p.attend(q, [6], lens=[2])
+    assert not got[:4].any()
+    check_rows(got[4:], q[4:], [x[:2] for x in kv], causal(2, 2), 64 ** -0.5)
+    assert not p.attend(q, [6], lens=[0]).any()
+    # a length past max_len costs time, not correctness
+    check_rows(p.attend(q, [6], lens=[40], max_len=1), q, kv, causal(6, 40), 64 ** -0.5)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_captured_and_replayed(hip, rows):
+    """append and attend recorded into a graph, replayed on new inputs with eager calls between."""
+    T = 500
+    p = Pool(hip, 41, 8, 2, 128, [T], page=64)
+    (kv,) = p.fill()
+    ks, vs = kv[0].copy(), kv[1].copy()
+    slots = dev(np.arange(T - rows, T, dtype=np.int32))
+    q, k, v = (torch.zeros((rows, h, 128), dtype=torch.float16, device="cuda") for h in (8, 2, 2))
+    qo = torch.zeros_like(q)
+    out = torch.zeros((rows, 8, 128), dtype=torch.float16, device="cuda")
+    start, lens = dev(np.array([0, rows], np.int32)), dev(np.array([T], np.int32))
+    ws = torch.zeros(max(16, p.pool.attend_workspace(rows, 1, rows, T)), dtype=torch.uint8, device="cuda")
+
+    def step():
+        st = torch.cuda.current_stream().cuda_stream
+        p.pool.append(0, rows, ptr(k), ptr(v), ptr(slots), ptr(p.dtable), *p.table.shape, q=ptr(q), q_out=ptr(qo), stream=st)
+        p.pool.attend(0, ptr(qo), ptr(out), ptr(start), ptr(lens), ptr(p.dtable), *p.table.shape, rows=rows, max_rows=rows,
+                      max_len=T, ws=ptr(ws), ws_bytes=ws.numel(), stream=st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        nq, nk, nv = p.rows(rows, 8), p.rows(rows, 2), p.rows(rows, 2)
+        for t, a in ((q, nq), (k, nk), (v, nv)):
+            t.copy_(torch.from_numpy(a))
+        out.zero_()
+        graph.replay()
+        got, turned = host(out), host(qo)
+        pos = np.arange(T - rows, T)
+        ks[T - rows:] = _kvq.store(_kvq.rotate(nk.astype(np.float64), pos, p.cos, p.sin, True))
+        vs[T - rows:] = _kvq.store(nv.astype(np.float64))
+        check_rows(got, turned, (ks, vs), causal(rows, T), 128 ** -0.5)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            out.zero_()
+            step()
+        assert np.array_equal(host(out), got), i
+
+
+def test_repeated_calls_agree_bit_for_bit(hip):
+    p = Pool(hip, 51, 8, 2, 128, [3000, 40, 1500], page=64)
+    p.fill()
+    q = p.rows(9, 8)
+    first = p.attend(q, [3, 3, 3])
+    for _ in range(3):
+        assert np.array_equal(p.attend(q, [3, 3, 3]), first)
+
+
+# ---- refusals ---------------------------------------------------------------------
+def test_refusals(hip):
+    p = Pool(hip, 61, 4, 2, 64, [10], page=32, layers=2)
+    buf = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    b, P = ptr(buf), p.pool
+    ok = dict(n=1, k=b, v=b, slots=b, table=b, n_seqs=1, table_ld=1)
+    for bad in (dict(k=0), dict(v=0), dict(slots=0), dict(table=0), dict(n_seqs=0), dict(table_ld=0), dict(k=b + 2),
+                dict(q=b), dict(q=b, q_out=b + 8), dict(k_ld=64), dict(v_ld=100), dict(k_ld=132), dict(n=1 << 25)):
+        with pytest.raises(hip.ArgError):
+            P.append(0, **dict(ok, **bad))
+    with pytest.raises(hip.UnsupportedMethod):
+        P.append(0, **dict(ok, dtype=hip.Q8_0))
+    for layer in (-1, 2):
+        with pytest.raises(hip.ArgError):
+            P.append(layer, **ok)
+        with pytest.raises(hip.ArgError):
+            P.read(layer, 1, b, b, 1, 1, b, b)
+    with pytest.raises(hip.ArgError):
+        P.read(0, 1, b, b, 1, 1, b + 2, b)
+    need = P.attend_workspace(2, 1, 1, 100000)
+    assert need > 0 and P.attend_workspace(2, 1, 3, 10) == 0 and P.attend_workspace(0, 1, 1, 10) == 0
+    at = dict(q=b, out=b, row_start=b, kv_len=b, table=b, n_seqs=1, table_ld=1, rows=2, max_rows=1, max_len=100000, ws=b,
+              ws_bytes=need)
+    for bad in (dict(q=0), dict(out=0), dict(row_start=0), dict(kv_len=0), dict(table=0), dict(n_seqs=0), dict(table_ld=0),
+                dict(max_rows=0), dict(max_rows=3), dict(ws=0), dict(ws_bytes=need - 1), dict(ws=b + 8), dict(q=b + 8),
+                dict(out=b + 4), dict(mask=b), dict(scale=float("nan")), dict(q_ld=128), dict(out_ld=255), dict(out_ld=258),
+                dict(n_seqs=70000), dict(max_len=1 << 40)):
+        with pytest.raises(hip.ArgError):
+            P.attend(0, **dict(at, **bad))
+    P.append(0, **dict(ok, n=0))
+    P.read(0, 0, b, b, 1, 1, b, b)
+    P.attend(0, **dict(at, rows=0))
+    assert P.page_bytes() == 2 * 36 * 64
+    P.close()
+    with pytest.raises(hip.ArgError):
+        P.append(0, **ok)

@@ -1,0 +1,174 @@
+"""Filtered sampling (sd_sampler_*) against a 64-bit restatement: tokens equal, distributions to an fp32 rounding."""
+import numpy as np
+import pytest
+import torch
+
+import _kvq
+
+pytestmark = pytest.mark.gpu
+
+
+def draw(hip, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probs=True, ld=0, sampler=None, V=None):
+    x = np.ascontiguousarray(x, np.float32)
+    rows, V = x.shape[0], V or x.shape[1]
+    s = sampler or hip.HipSampler(V, rows)
+    dx, du = torch.from_numpy(x).cuda(), torch.from_numpy(np.ascontiguousarray(u, np.float32)).cuda()
+    tok = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    pr = torch.full((rows, V), 5.0, device="cuda") if probs else None
+    torch.cuda.synchronize()
+    s.sample(dx.data_ptr(), rows, du.data_ptr(), tok.data_ptr(), temperature, top_k, top_p, min_p,
+             probs=pr.data_ptr() if probs else 0, ld=ld)
+    torch.cuda.synchronize()
+    return tok.cpu().numpy(), pr.cpu().numpy() if probs else None
+
+
+def check(hip, x, u, **kw):
+    tok, pr = draw(hip, x, u, **kw)
+    args = {k: kw.get(k, d) for k, d in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))}
+    for r in range(len(x)):
+        want, p = _kvq.sample(x[r], u[r], **args)
+        assert tok[r] == want, (r, tok[r], want, args)
+        # an fp32 rounding of a value known to 1e-10
+        assert np.all(np.abs(pr[r] - p) <= 2.0 ** -24 * p * 1.01 + 2.0 ** -150), (r, args)
+        assert np.array_equal(pr[r] > 0, p.astype(np.float32) > 0) or np.abs(p[(pr[r] > 0) != (p > 0)]).max() < 2.0 ** -149
+
+
+FILTERS = [dict(), dict(top_k=1), dict(top_k=40), dict(top_k=700), dict(top_p=0.9), dict(top_p=0.3), dict(min_p=0.05), dict(top_k=50, top_p=0.8),
+           dict(top_k=5000, top_p=0.99, min_p=0.001), dict(top_p=0.0), dict(top_p=0.999, min_p=1.0), dict(temperature=0.0),
+           dict(temperature=0.1, top_p=0.9), dict(temperature=8.0, top_p=0.95), dict(temperature=8.0, top_k=4000),
+           dict(temperature=30.0), dict(temperature=1e-30, top_k=3), dict(temperature=1e30, top_p=0.5)]
+
+
+@pytest.mark.parametrize("V", [1, 2, 63, 1000, 8191, 8193, 32000])
+@pytest.mark.parametrize("f", range(len(FILTERS)))
+def test_filters(hip, V, f):
+    rng = np.random.default_rng(V * 100 + f)
+    x = rng.standard_normal((4, V)) * np.array([[0.2], [1.0], [2.5], [6.0]])
+    if V > 20:
+        x[:, 5::17] = -np.inf
+    check(hip, x.astype(np.float32), rng.random(4), **FILTERS[f])
+
+
+@pytest.mark.parametrize("V", [128256, 152064, 262144])
+@pytest.mark.parametrize("f", [0, 2, 3, 4, 6, 7, 8, 13])
+def test_filters_large_vocabularies(hip, V, f):
+    rng = np.random.default_rng(V + f)
+    x = rng.standard_normal((2, V)) * np.array([[1.0], [2.5]])
+    x[:, 1::1009] += 3.0
+    check(hip, x.astype(np.float32), rng.random(2), **FILTERS[f])
+
+
+@pytest.mark.parametrize("f", range(len(FILTERS)))
+def test_ties(hip, f):
+    """Few distinct values, so that every bound falls inside a run of equal ones; uniforms on exact borders; all equal."""
+    rng = np.random.default_rng(f)
+    V = 20011
+    x = rng.integers(-3, 4, (4, V)).astype(np.float32)
+    x[1] = 0.0
+    x[2, ::2], x[2, 1::2] = -0.0, 0.0
+    x[3, 7:] = -np.inf
+    check(hip, x, [0.5, 0.25, 0.75, 0.0], **FILTERS[f])
+
+
+def test_two_near_values(hip):
+    """A bin full of values that differ in their last bits only."""
+    rng = np.random.default_rng(1)
+    x = (np.float32(3.0) + rng.integers(0, 60, (2, 30000)).astype(np.float32) * np.float32(2.0 ** -22)).astype(np.float32)
+    for kw in (dict(top_k=9000), dict(top_p=0.37), dict(top_k=25000, top_p=0.5)):
+        check(hip, x, rng.random(2), **kw)
+
+
+def test_uniform_ends(hip):
+    x = np.zeros((4, 1000), np.float32)
+    u = np.array([0.0, np.nextafter(np.float32(1), np.float32(0)), 0.5, 0.999], np.float32)
+    check(hip, x, u)
+    check(hip, x, u, top_p=0.5)
+    tok, _ = draw(hip, x, np.array([1.0, 2.0, -1.0, np.nan], np.float32))  # outside [0, 1): still a token
+    assert ((tok >= 0) & (tok < 1000)).all()
+
+
+def test_rows_without_a_distribution(hip):
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((6, 9000)).astype(np.float32)
+    x[0, 8999] = np.nan
+    x[1, 17] = np.inf
+    x[2] = -np.inf
+    x[3, :8500] = -np.inf
+    x[4, 1:] = -np.inf
+    for kw in (dict(), dict(top_k=10), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=0.0)):
+        check(hip, x, rng.random(6), **kw)
+
+
+def test_stride_fewer_rows_and_untouched_outputs(hip):
+    rng = np.random.default_rng(3)
+    V, ld = 5000, 5013
+    wide = rng.standard_normal((5, ld)).astype(np.float32)
+    u = rng.random(5)
+    s = hip.HipSampler(V, 9)
+    tok, pr = draw(hip, wide, u, top_k=20, ld=ld, sampler=s, V=V)
+    for r in range(5):
+        want, p = _kvq.sample(wide[r, :V], u[r], 1.0, top_k=20)
+        assert tok[r] == want and np.all(np.abs(pr[r] - p) <= 2.0 ** -24 * p * 1.01)
+    # a smaller call after a larger one on the same handle
+    tok, _ = draw(hip, wide[:1], u[:1], top_p=0.5, ld=ld, sampler=s, V=V, probs=False)
+    assert tok[0] == _kvq.sample(wide[0, :V], u[0], 1.0, top_p=0.5)[0]
+
+
+def test_distribution_of_draws(hip):
+    """The draws over a grid of uniforms have the distribution's frequencies."""
+    rng = np.random.default_rng(4)
+    x = np.tile(rng.standard_normal(50).astype(np.float32) * 2, (4096, 1))
+    u = (np.arange(4096) + 0.5) / 4096
+    tok, pr = draw(hip, x, u, top_p=0.95)
+    freq = np.bincount(tok, minlength=50) / 4096
+    assert np.all(np.abs(freq - pr[0]) <= 1.0 / 4096 + 1e-6)  # a grid counts each interval to within one
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=40, top_p=0.9), dict(), dict(top_p=0.9)])
+def test_captured_and_replayed(hip, kw):
+    rng = np.random.default_rng(5)
+    V, rows = 33333, 3
+    s = hip.HipSampler(V, rows)
+    x, u = torch.zeros((rows, V), device="cuda"), torch.zeros(rows, device="cuda")
+    tok, pr = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros((rows, V), device="cuda")
+
+    def step():
+        s.sample(x.data_ptr(), rows, u.data_ptr(), tok.data_ptr(), probs=pr.data_ptr(),
+                 stream=torch.cuda.current_stream().cuda_stream, **kw)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for i in range(3):
+        a, b = (rng.standard_normal((rows, V)) * 2).astype(np.float32), rng.random(rows).astype(np.float32)
+        x.copy_(torch.from_numpy(a))
+        u.copy_(torch.from_numpy(b))
+        g.replay()
+        torch.cuda.synchronize()
+        got, dist = tok.cpu().numpy(), pr.cpu().numpy()
+        for r in range(rows):
+            want, p = _kvq.sample(a[r], b[r], 1.0, **kw)
+            assert got[r] == want and np.all(np.abs(dist[r] - p) <= 2.0 ** -24 * p * 1.01 + 2.0 ** -150)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            tok.fill_(-9)
+            step()
+        torch.cuda.synchronize()
+        assert np.array_equal(tok.cpu().numpy(), got)
+
+
+def test_refusals(hip):
+    s = hip.HipSampler(100, 4)
+    b = torch.zeros(4096, device="cuda").data_ptr()
+    for kw in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_k=-1),
+               dict(top_p=-0.1), dict(top_p=1.1), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=2.0)):
+        with pytest.raises(hip.SamplingError):
+            s.sample(b, 1, b, b, **kw)
+    for args, kw in (((0, 1, b, b), {}), ((b, 1, 0, b), {}), ((b, 1, b, 0), {}), ((b, 5, b, b), {}), ((b, 1, b, b), dict(ld=99)),
+                     ((b, 1 << 20, b, b), {})):
+        with pytest.raises(hip.ArgError):
+            s.sample(*args, **kw)
+    s.sample(b, 0, b, b)
+    s.close()
+    with pytest.raises(hip.ArgError):
+        s.sample(b, 1, b, b)
