@@ -542,6 +542,45 @@ sd_status sd_last_argmax(sd_model *m, int32_t *out, size_t n) {
     });
 }
 
+static sd::SampleParams filters_of(const sd_sampling *f) {
+    if (!f) throw sd::ArgError("null argument");
+    sd::SampleParams p{};
+    p.temperature = f->temperature;
+    p.top_k = f->top_k;
+    p.top_p = f->top_p;
+    p.min_p = f->min_p;
+    return p;
+}
+
+sd_status sd_sample_next(sd_model *m, const sd_sampling *params, float uniform, int32_t *token) {
+    return guard([&] {
+        need_weights(m);
+        if (!token) throw sd::ArgError("null output");
+        const sd::SampleParams f = filters_of(params);
+        setdev(m);
+        m->dec->sample_next(f, uniform, token);
+    });
+}
+
+sd_status sd_sample_rows(sd_model *m, const sd_sampling *params, const float *uniforms, size_t n, int32_t *tokens) {
+    return guard([&] {
+        need(m);
+        if (!uniforms || !tokens) throw sd::ArgError("null argument");
+        const sd::SampleParams f = filters_of(params);
+        setdev(m);
+        m->dec->sample_rows(f, uniforms, n, tokens);
+    });
+}
+
+sd_status sd_model_set_kv_format(sd_model *m, int32_t format) {
+    return guard([&] {
+        need(m);
+        if (m->dec->cache_len || !m->dec->history.empty()) throw sd::ArgError("the cache must be empty (reset first)");
+        setdev(m);
+        m->model->set_kv_format(format);
+    });
+}
+
 sd_status sd_prime_synthetic(sd_model *m, const uint32_t *ids, size_t n, uint64_t kv_seed) {
     return guard([&] {
         need(m);
@@ -593,21 +632,7 @@ sd_status sd_read_kv_rows(sd_model *m, int32_t layer, int32_t which, int32_t hea
         if (!out) throw sd::ArgError("null output");
         if (layer < 0 || layer >= c.n_layers || which < 0 || which > 1 || head < 0 || head >= c.n_kv_heads)
             throw sd::ArgError("kv row selector out of range");
-        if (pos0 + n > (size_t)m->model->cap) throw sd::ArgError("kv rows out of range");
-        setdev(m);
-        const uint16_t *base = m->model->kv + (((int64_t)layer * 2 + which) * c.n_kv_heads + head) * m->model->cap *
-                                                  c.head_dim;
-        // copy the whole 32-position blocks covering the rows, then gather the
-        // rows out of the blocked layout (sd_common.hpp: kv_k_off / kv_v_off)
-        const int64_t b0 = (int64_t)pos0 / 32, b1 = ((int64_t)(pos0 + n) + 31) / 32;
-        std::vector<uint16_t> blk((size_t)(b1 - b0) * 32 * c.head_dim);
-        m->model->sync();
-        if (!blk.empty())
-            SD_HIP_CHECK(hipMemcpy(blk.data(), base + b0 * 32 * c.head_dim, blk.size() * 2, hipMemcpyDeviceToHost));
-        const int64_t off0 = b0 * 32 * c.head_dim;
-        for (size_t j = 0; j < n; j++)
-            for (int d = 0; d < c.head_dim; d++)
-                out[j * c.head_dim + d] = blk[sd::kv_off(which, (int64_t)(pos0 + j), d, c.head_dim) - off0];
+        m->model->read_kv_rows(layer, which, head, pos0, n, out);
     });
 }
 

@@ -80,7 +80,8 @@ Model::~Model() {
                     (void *)acc_m, (void *)acc_s, (void *)acc_q, (void *)acc_am, (void *)acc_tree,
                     (void *)acc_out, (void *)t2d_inv, (void *)qg_part, (void *)aux_h, (void *)aux_x, (void *)aux_y,
                     (void *)aux_ids, (void *)ssq, (void *)split_cnt, (void *)acc_part, (void *)acc_cnt,
-                    (void *)acc_prob, (void *)acc_lin, (void *)qa_flags, (void *)d_prompt})
+                    (void *)acc_prob, (void *)acc_lin, (void *)qa_flags, (void *)d_prompt, (void *)kvq_table, kvq_ws,
+                    (void *)smp_u, (void *)smp_tok})
         F(p);
     if (qa_status) hipHostFree(qa_status);
     if (h_stage) hipHostFree(h_stage);
@@ -384,10 +385,129 @@ void Model::synthesize(int mix, uint64_t seed, float stdv) {
     SD_HIP_CHECK(hipStreamSynchronize(st));
 }
 
+void Model::set_kv_format(int fmt) {
+    if (fmt != KV_F16 && fmt != KV_Q4) throw UnsupportedError("kv format must be F16 or Q4");
+    if ((fmt == KV_Q4) == (kvq != nullptr)) return;
+    SD_HIP_CHECK(hipSetDevice(cfg.device));
+    sync();
+    if (fmt == KV_F16) {
+        kv = dalloc<uint16_t>((size_t)cfg.n_layers * 2 * cfg.n_kv_heads * cap * cfg.head_dim);
+        kvq.reset();
+    } else {
+        KvPoolCfg c;
+        c.n_layers = cfg.n_layers;
+        c.n_heads = cfg.n_heads;
+        c.n_kv_heads = cfg.n_kv_heads;
+        c.head_dim = cfg.head_dim;
+        c.page_tokens = kKvqPage;
+        c.n_pages = (int)((cap + kKvqPage - 1) / kKvqPage);
+        c.interleaved = cfg.arch == 0;
+        c.device = cfg.device;
+        auto pool = std::make_unique<KvPool>(c);
+        if (!kvq_table) {
+            std::vector<int> ids(c.n_pages);
+            for (int i = 0; i < c.n_pages; i++) ids[i] = i;
+            kvq_table = dalloc<int>(ids.size());
+            SD_HIP_CHECK(hipMemcpy(kvq_table, ids.data(), ids.size() * sizeof(int), hipMemcpyHostToDevice));
+        }
+        if (!kvq_ws) {
+            size_t most = 16;
+            for (int M = 1; M <= prompt_rows; M++) most = std::max(most, pool->plan(M, 1, M, cfg.ctx_len).ws_bytes);
+            kvq_ws = dalloc<uint8_t>(most);
+        }
+        SD_HIP_CHECK(hipFree(kv));
+        kv = nullptr;
+        kvq = std::move(pool);
+    }
+    fwd_count++;
+}
+
+void Model::read_kv_rows(int layer, int which, int head, size_t pos0, size_t n, uint16_t *out) {
+    if (pos0 + n > (size_t)cap) throw ArgError("kv rows out of range");
+    if (n == 0) return;
+    SD_HIP_CHECK(hipSetDevice(cfg.device));
+    const int hd = cfg.head_dim;
+    sync();
+    if (kvq) {
+        std::vector<uint16_t> all(n * cfg.n_kv_heads * hd);
+        std::unique_ptr<uint16_t, void (*)(uint16_t *)> rows(dalloc<uint16_t>(all.size()), [](uint16_t *p) { (void)hipFree(p); });
+        const KvqRows r{(int)n, nullptr, nullptr, (int)pos0, kvq_table, 1, kvq->cfg.n_pages};
+        launch_kvq_read(kvq->layer(layer), r, which ? nullptr : rows.get(), which ? rows.get() : nullptr, st);
+        SD_HIP_CHECK(hipMemcpyAsync(all.data(), rows.get(), all.size() * 2, hipMemcpyDeviceToHost, st));
+        sync();
+        for (size_t j = 0; j < n; j++) std::memcpy(out + j * hd, all.data() + (j * cfg.n_kv_heads + head) * hd, hd * 2);
+        return;
+    }
+    const uint16_t *base = kv + (((int64_t)layer * 2 + which) * cfg.n_kv_heads + head) * cap * hd;
+    // copy the whole 32-position blocks covering the rows, then gather the
+    // rows out of the blocked layout (sd_common.hpp: kv_k_off / kv_v_off)
+    const int64_t b0 = (int64_t)pos0 / 32, b1 = ((int64_t)(pos0 + n) + 31) / 32;
+    std::vector<uint16_t> blk((size_t)(b1 - b0) * 32 * hd);
+    SD_HIP_CHECK(hipMemcpy(blk.data(), base + b0 * 32 * hd, blk.size() * 2, hipMemcpyDeviceToHost));
+    const int64_t off0 = b0 * 32 * hd;
+    for (size_t j = 0; j < n; j++)
+        for (int d = 0; d < hd; d++) out[j * hd + d] = blk[kv_off(which, (int64_t)(pos0 + j), d, hd) - off0];
+}
+
+void Model::sample_rows(const float *rows, int n, const SampleParams &filters, const float *uniforms, int32_t *tokens) {
+    if (!sampler) {
+        if (!smp_u) smp_u = dalloc<float>(cfg.max_batch);
+        if (!smp_tok) smp_tok = dalloc<int>(cfg.max_batch);
+        sampler = std::make_unique<Sampler>(cfg.vocab, cfg.max_batch, cfg.device);
+    }
+    // through the pinned staging block of the acceptance walks
+    float *in = (float *)acc_stage;
+    int *out = acc_stage + (size_t)kAccTreeInts * cfg.max_batch;
+    std::memcpy(in, uniforms, (size_t)n * sizeof(float));
+    SD_HIP_CHECK(hipMemcpyAsync(smp_u, in, (size_t)n * sizeof(float), hipMemcpyHostToDevice, st));
+    SampleParams p = filters;
+    p.logits = rows;
+    p.ld = cfg.vocab;
+    p.rows = n;
+    p.u = smp_u;
+    p.tokens = smp_tok;
+    p.probs = nullptr;
+    sampler->run(p, st);
+    SD_HIP_CHECK(hipMemcpyAsync(out, smp_tok, (size_t)n * sizeof(int), hipMemcpyDeviceToHost, st));
+    sync();
+    for (int i = 0; i < n; i++)
+        if (out[i] < 0) throw SamplingError("row " + std::to_string(i) + " has no distribution (NaN, +inf or -inf only)");
+    std::memcpy(tokens, out, (size_t)n * sizeof(int));
+}
+
 void Model::fill_kv_synthetic(int P, uint64_t seed) {
     fwd_count++;
     if (P < 0 || P > cfg.ctx_len) throw ArgError("prefix longer than the KV capacity");
     const float mult = (float)(std::sqrt(3.0) / 65536.0);
+    if (kvq) {
+        // the same fp16 values, appended unrotated (position 0) and quantised
+        const int chunk = std::min(P, 4096);
+        if (!chunk) return;
+        const size_t row = (size_t)cfg.n_kv_heads * cfg.head_dim;
+        std::unique_ptr<uint16_t, void (*)(uint16_t *)> buf(dalloc<uint16_t>(2 * chunk * row + 2 * chunk),
+                                                            [](uint16_t *p) { (void)hipFree(p); });
+        uint16_t *k = buf.get(), *v = k + chunk * row;
+        KvqAppend a{};
+        a.pos = (const int *)(v + chunk * row);  // zeros
+        a.cos_t = cos_t;
+        a.sin_t = sin_t;
+        a.max_pos = 1;
+        a.interleaved = 1;
+        a.n_heads = cfg.n_heads;
+        a.k = k;
+        a.v = v;
+        a.k_ld = a.v_ld = (int64_t)row;
+        for (int l = 0; l < cfg.n_layers; l++)
+            for (int p0 = 0; p0 < P; p0 += chunk) {
+                const int n = std::min(chunk, P - p0);
+                launch_synth_kv_rows(k, v, l, cfg.n_kv_heads, cfg.head_dim, P, p0, n, seed, mult, st);
+                a.L = kvq->layer(l);
+                a.rows = KvqRows{n, nullptr, nullptr, p0, kvq_table, 1, kvq->cfg.n_pages};
+                launch_kvq_append(a, st);
+            }
+        SD_HIP_CHECK(hipStreamSynchronize(st));
+        return;
+    }
     launch_fill_kv(kv, cfg.n_layers, cfg.n_kv_heads, cap, cfg.head_dim, P, seed, mult, st);
     SD_HIP_CHECK(hipStreamSynchronize(st));
 }
@@ -673,11 +793,13 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
     const bool spread = !fused && M > 16 && M <= 64;
     const int sp_parts = resid_u_parts(H);
     // K and V rows read once per layer by the attention: [0, P + M) of every KV head
-    const double kv_bytes = 2.0 * c.n_kv_heads * (double)(P + M) * c.head_dim * 2.0;
+    const double kv_bytes = 2.0 * c.n_kv_heads * (double)(P + M) * (kvq ? kvq_block_bytes(c.head_dim) / 64.0 : c.head_dim * 2.0);
+    KvqPlan kvq_plan{};
+    if (kvq) kvq_plan = kvq->plan(M, 1, M, P + M);
     // up to 16 rows, with the epilogues fused, the attention's workgroups join
     // the Q/K/V launch where its shape allows (qkv_attention_fits)
     auto qa_fits = [&](const GemmParams &g, const AttnParams &at) {
-        return fused && fused_qkv_attn && qkv_attention_fits(g, at, n_cus);
+        return fused && fused_qkv_attn && !kvq && qkv_attention_fits(g, at, n_cus);
     };
     for (int l = 0; l < c.n_layers; l++) {
         auto &L = lw[l];
@@ -689,8 +811,8 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
         bool qa_launched = false;
         AttnParams a{};
         a.q16 = q16;
-        a.kc = kc(l);
-        a.vc = vc(l);
+        a.kc = kvq ? nullptr : kc(l);
+        a.vc = kvq ? nullptr : vc(l);
         a.cap = cap;
         a.mask = d_mask;
         a.mask_words = mask_words;
@@ -726,7 +848,7 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
             p.K = H;
             p.M = M;
             p.mode = GM_STORE;
-            p.allow_split = split_ok;
+            p.allow_split = kvq ? 0 : split_ok;  // the 4-bit append reads whole sums
             if (spread) {
                 p.norm_ssq = ssq;
                 p.norm_parts = sp_parts;
@@ -736,6 +858,8 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
                 p.norm_ssq = ssq;
                 p.norm_parts = np;
                 p.norm_eps = c.rms_eps;
+            }
+            if (fused && !kvq) {
                 RopeOut &R = p.rope;
                 R.pos = pos_dev;
                 R.cos_t = cos_t;
@@ -770,7 +894,48 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
                 nks_qkv = qgemm_slices(p);
             }
         }
-        {
+        if (kvq) {
+            KvqAppend ka{};
+            ka.L = kvq->layer(l);
+            ka.rows = KvqRows{M, nullptr, nullptr, P, kvq_table, 1, kvq->cfg.n_pages};
+            ka.pos = pos_dev;
+            ka.cos_t = cos_t;
+            ka.sin_t = sin_t;
+            ka.max_pos = (int)cap;
+            ka.interleaved = c.arch == 0;
+            ka.n_heads = c.n_heads;
+            ka.f32 = 1;
+            ka.q = qkv;
+            ka.k = qkv + QD;
+            ka.v = qkv + QD + KVD;
+            ka.q_ld = ka.k_ld = ka.v_ld = QKVD;
+            ka.q_out = q16;
+            ka.q_out_row = QD;
+            ka.q_out_head = c.head_dim;
+            KvqAttn kt{};
+            kt.L = ka.L;
+            kt.q = q16;
+            kt.q_row = QD;
+            kt.q_head = c.head_dim;
+            kt.out = ap;
+            kt.out_ld = ap_ld;
+            kt.out_act = tiled ? 2 : 1;
+            kt.rows = M;
+            kt.n_seqs = 1;
+            kt.len0 = P + M;
+            kt.table = kvq_table;
+            kt.table_ld = kvq->cfg.n_pages;
+            kt.mask = prompt ? nullptr : d_mask;
+            kt.mask_words = mask_words;
+            kt.max_rows = M;
+            kt.n_heads = c.n_heads;
+            kt.n_rep = c.n_heads / c.n_kv_heads;
+            kt.scale = a.scale;
+            const int ev = prof_on ? prof_begin() : 0;
+            launch_kvq_append(ka, st);
+            launch_kvq_attention(kt, kvq_plan, kvq_ws, st);
+            if (prof_on) prof_end(ev, PC_ATTN, kv_bytes);
+        } else {
             RopeKvParams r{};
             r.qkv = qkv;
             r.ld_qkv = QKVD;
@@ -926,6 +1091,7 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
         run_gemm(p, PC_LM_HEAD, wbytes(W));
         launch_argmax_reduce(amax_v, amax_i, p.amax_ld, rows, argmax, st);
         logits_rows_last = rows;
+        rows_last = logits;
     }
     if (!collect.empty() && collect_out) {
         SD_HIP_CHECK(hipMemcpyAsync(collect_out, collect_buf, collect.size() * H * 4, hipMemcpyDeviceToHost, st));
@@ -999,6 +1165,10 @@ void Model::compact_tail(int P, const std::vector<int> &src) {
     std::memcpy(h_stage, src.data(), n * sizeof(int));
     SD_HIP_CHECK(hipMemcpyAsync(d_src, h_stage, n * sizeof(int), hipMemcpyHostToDevice, st));
     stage_done();
+    if (kvq) {
+        launch_kvq_keep_tail(kvq->layer(0), kvq->layer_bytes, cfg.n_layers, kvq_table, P, d_src, n, st);
+        return;
+    }
     launch_keep_kv_tail(kv, cfg.n_layers * 2 * cfg.n_kv_heads, cap * cfg.head_dim, cfg.n_kv_heads, cfg.head_dim, P, d_src,
                         n, st);
 }
@@ -1386,6 +1556,18 @@ void Decoder::argmax_rows(int32_t *out, size_t n) {
     std::memcpy(out, pin, n * 4);
 }
 
+void Decoder::sample_next(const SampleParams &filters, float u, int32_t *token) {
+    Sampler::check(filters.temperature, filters.top_k, filters.top_p, filters.min_p);
+    next_logits(nullptr);
+    model->sample_rows(model->last_row, 1, filters, &u, token);
+}
+
+void Decoder::sample_rows(const SampleParams &filters, const float *uniforms, size_t n, int32_t *tokens) {
+    Sampler::check(filters.temperature, filters.top_k, filters.top_p, filters.min_p);
+    if (n > (size_t)model->logits_rows_last) throw ArgError("fewer rows in the last verify pass");
+    if (n) model->sample_rows(model->rows_last, (int)n, filters, uniforms, tokens);
+}
+
 // batched_logits + greedy acceptance with the logits kept in HBM:
 // accept drafts while draft[i] == argmax(row i); the first mismatch (or the
 // bonus row k) contributes argmax of that row (vanilla.rs:178-210 at T=0,
@@ -1397,6 +1579,7 @@ void Decoder::verify_greedy_linear(const uint32_t *drafts, size_t k, uint32_t *c
     if (k == 0) {
         launch_argmax_rows(model->last_row, model->cfg.vocab, model->cfg.vocab, 1, model->argmax, model->st);
         model->logits_rows_last = 1;
+        model->rows_last = model->last_row;
     }
     argmax_rows(am.data(), k + 1);
     size_t a = 0;
@@ -1667,6 +1850,7 @@ void Decoder::verify_rejection_linear(const uint32_t *drafts, size_t k, const fl
         // next_logits left the row in last_row; the walk reads logits row 0
         SD_HIP_CHECK(hipMemcpyAsync(m.logits, m.last_row, (size_t)m.cfg.vocab * 4, hipMemcpyDeviceToDevice, m.st));
         m.logits_rows_last = 1;
+        m.rows_last = m.logits;
     }
     const int n = (int)k + 1;
     std::vector<int> parents(n), tokens(n), qrow(n);

@@ -14,6 +14,7 @@
 #include "sd_kernels_attn.hpp"
 #include "sd_kernels_accept.hpp"
 #include "sd_kernels_elem.hpp"
+#include "sd_kvpool.hpp"
 
 namespace sd {
 
@@ -141,6 +142,24 @@ class Model {
     static constexpr int kPromptRows = 2048;
     int prompt_rows = 0;
 
+    // The cache's format: fp16 in `kv`, or 4 bits in the pages of `kvq` (whose
+    // table names them in order, so that a position's place is its own).  Either
+    // one is allocated.  Changing it drops what is cached.
+    enum { KV_F16 = 1, KV_Q4 = 2 };
+    static constexpr int kKvqPage = 256;
+    void set_kv_format(int fmt);
+    // cache rows [pos0, pos0 + n) of one (layer, K or V, KV head) as fp16 [n][hd]
+    void read_kv_rows(int layer, int which, int head, size_t pos0, size_t n, uint16_t *out);
+    std::unique_ptr<KvPool> kvq;
+    int *kvq_table = nullptr;
+    void *kvq_ws = nullptr;
+
+    // sampling: made on first use, max_batch rows
+    std::unique_ptr<Sampler> sampler;
+    float *smp_u = nullptr;
+    int *smp_tok = nullptr;
+    void sample_rows(const float *rows, int n, const SampleParams &filters, const float *uniforms, int32_t *tokens);
+
     // device buffers
     uint16_t *kv = nullptr;  // [L][2][n_kv][cap][hd]
     int64_t cap = 0;
@@ -198,6 +217,7 @@ class Model {
     int nsplit_max = 0;
     int64_t part_rows = 0;     // (split, row) pairs of part_o, part_ml
     int logits_rows_last = 0;  // rows of `logits` / `argmax` produced by the last forward
+    const float *rows_last = nullptr;  // those rows: `logits`, or the cached next-token row alone
     // apply_lm_head / embed_tokens work buffers (kAuxRows rows per chunk),
     // apart from the verify pass's
     static constexpr int kAuxRows = 16;
@@ -277,6 +297,9 @@ class Decoder {
                                size_t n_uniforms, float temperature, int use_t2d, int siblings, size_t max_commit,
                                uint32_t *path, size_t *path_len, int32_t *token, size_t *n_used,
                                bool q_on_device = false);
+    // tokens drawn from the cached next-token row / from rows [0, n) of the last pass
+    void sample_next(const SampleParams &filters, float u, int32_t *token);
+    void sample_rows(const SampleParams &filters, const float *uniforms, size_t n, int32_t *tokens);
     // EAGLE-3 vocabulary map (eagle3.rs:377-397, 476-513)
     void set_d2t(const int64_t *d2t, size_t n);
     std::vector<int64_t> d2t_host;

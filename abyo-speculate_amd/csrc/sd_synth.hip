@@ -194,6 +194,16 @@ __global__ void k_fill_kv(uint16_t *kv, int L, int n_kv, int64_t cap, int hd, in
     kv[stream * cap * hd + kv_off(which, r / hd, (int)(r % hd), hd)] = f2h(synth_value(seed, idx, mult));
 }
 
+__global__ void k_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int P, int p0, int64_t total,
+                                uint64_t seed, float mult) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= 2 * total) return;
+    const int which = i >= total;
+    const int64_t j = i - which * total, d = j % hd, h = j / hd % n_kv, pos = p0 + j / hd / n_kv;
+    const uint64_t stream = (uint64_t)(layer * 2 + which) * n_kv + h;
+    (which ? v : k)[j] = f2h(synth_value(seed, (stream << 32) | (uint64_t)(pos * hd + d), mult));
+}
+
 // ---- exact f32 dequantisation: one thread per 32 outputs ----------------
 __device__ inline float ldh(const uint8_t *p) { return h2f((uint16_t)(p[0] | (p[1] << 8))); }
 
@@ -272,6 +282,13 @@ void launch_fill_kv(uint16_t *kv, int L, int n_kv, int64_t cap, int hd, int P, u
     if (total == 0) return;
     hipLaunchKernelGGL(k_fill_kv, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, kv, L, n_kv, cap, hd, P,
                        seed, mult);
+}
+
+void launch_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int P, int p0, int n, uint64_t seed,
+                          float mult, hipStream_t st) {
+    const int64_t total = (int64_t)n * n_kv * hd;
+    hipLaunchKernelGGL(k_synth_kv_rows, dim3((unsigned)((2 * total + 255) / 256)), dim3(256), 0, st, k, v, layer, n_kv,
+                       hd, P, p0, total, seed, mult);
 }
 
 void launch_dequant(int fmt, const uint8_t *w, int64_t n_elems, float *y, hipStream_t st) {

@@ -35,6 +35,7 @@ SD_OK, SD_ERR_SAMPLING, SD_ERR_ROLLBACK, SD_ERR_BACKEND, SD_ERR_ARG, SD_ERR_UNSU
 # formats (GGML type ids)
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
 F16 = 1  # rows of the operators on device memory
+KV_F16, KV_Q4 = 1, 2  # formats of a decoder's cache
 # tensor kinds
 (TOK_EMBD, OUTPUT, OUTPUT_NORM, ATTN_Q, ATTN_K, ATTN_V, ATTN_OUTPUT, FFN_GATE, FFN_UP, FFN_DOWN,
  ATTN_NORM, FFN_NORM, ATTN_Q_BIAS, ATTN_K_BIAS, ATTN_V_BIAS) = range(15)
@@ -96,6 +97,7 @@ class Config:
     max_batch: int = 128
     tied_output: int = 0
     device: int = 0
+    kv_format: int = KV_F16  # KV_Q4: the cache in 4 bits (sd_model_set_kv_format)
 
     def to_c(self) -> SdConfig:
         return SdConfig(**{k: getattr(self, k) for k, _ in SdConfig._fields_})
@@ -235,6 +237,9 @@ def load_library(path: str = LIB_PATH):
         "sd_draft2_reset": ([P], I32),
         "sd_draft2_forward": ([P, P, SZ, ctypes.c_uint32, SZ, P], I32),
         "sd_draft2_round": ([P, P, P, SZ, P, P, P], I32),
+        "sd_model_set_kv_format": ([P, I32], I32),
+        "sd_sample_next": ([P, ctypes.POINTER(Sampling), ctypes.c_float, ctypes.POINTER(ctypes.c_int32)], I32),
+        "sd_sample_rows": ([P, ctypes.POINTER(Sampling), P, SZ, P], I32),
         "sd_kvpool_create": ([ctypes.POINTER(KvPoolConfig), ctypes.POINTER(P)], I32),
         "sd_kvpool_destroy": ([P], None),
         "sd_kvpool_page_bytes": ([P], SZ),
@@ -615,14 +620,16 @@ class HipQuantDecoder:
 
     @classmethod
     def from_gguf(cls, gguf_path: str, arch: int = -1, ctx_len: Optional[int] = None, max_batch: int = 128,
-                  device: int = 0, eos_token_ids: Sequence[int] = ()) -> "HipQuantDecoder":
+                  device: int = 0, eos_token_ids: Sequence[int] = (), kv_format: int = KV_F16) -> "HipQuantDecoder":
         """LlamaQuantDecoder::from_gguf / Qwen2QuantDecoder::from_gguf
         (quantized_llama.rs:57-98, quantized_qwen2.rs:55-100) without the
         tokenizer: the config from the file's metadata, then every tensor.
         arch picks the decoder type (ARCH_LLAMA reads llama.* keys); -1 follows
         general.architecture."""
         with GgufFile(gguf_path) as g:
-            dec = cls(g.config(arch, ctx_len=ctx_len, max_batch=max_batch, device=device))
+            cfg = g.config(arch, ctx_len=ctx_len, max_batch=max_batch, device=device)
+            cfg.kv_format = kv_format
+            dec = cls(cfg)
             try:
                 _check(_lib.sd_model_load_gguf(dec._h, g._h))
             except Exception:
@@ -642,6 +649,12 @@ class HipQuantDecoder:
         self.vocab = cfg.vocab
         self.hidden = cfg.hidden
         _pinned.acquire()
+        if cfg.kv_format != KV_F16:
+            try:
+                self.set_kv_format(cfg.kv_format)
+            except Exception:
+                self.close()
+                raise
 
     def close(self):
         if getattr(self, "_h", None):
@@ -654,6 +667,10 @@ class HipQuantDecoder:
             self.close()
         except Exception:
             pass
+
+    def set_kv_format(self, fmt: int):
+        """KV_F16 or KV_Q4, while the cache is empty."""
+        _check(_lib.sd_model_set_kv_format(self._h, fmt))
 
     # ---- weights ----
     def set_tensor(self, layer: int, kind: int, fmt: int, data: np.ndarray):
@@ -917,6 +934,23 @@ class HipQuantDecoder:
         out = np.empty(n, np.int32)
         _check(_lib.sd_last_argmax(self._h, _ptr(out), n))
         return out
+
+    # ---- sampling ----
+    def sample_next(self, uniform: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                    min_p: float = 0.0) -> int:
+        """A token drawn from the next-token row with the given random number
+        in [0, 1) and filters (sd_sampling); the row stays on the device."""
+        s, tok = Sampling(temperature, top_k, top_p, min_p), ctypes.c_int32()
+        _check(_lib.sd_sample_next(self._h, ctypes.byref(s), float(uniform), ctypes.byref(tok)))
+        return int(tok.value)
+
+    def sample_rows(self, uniforms: Sequence[float], temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                    min_p: float = 0.0) -> List[int]:
+        """A token from each of the first len(uniforms) rows of the last verify pass."""
+        u = np.ascontiguousarray(uniforms, np.float32)
+        s, out = Sampling(temperature, top_k, top_p, min_p), np.empty(u.size, np.int32)
+        _check(_lib.sd_sample_rows(self._h, ctypes.byref(s), _ptr(u), u.size, _ptr(out)))
+        return [int(v) for v in out]
 
     # ---- synthetic state / measurement ----
     def prime_synthetic(self, ids: Sequence[int], kv_seed: int):

@@ -106,6 +106,15 @@ typedef struct sd_model sd_model;
 sd_status sd_model_create(const sd_config *cfg, sd_model **out);
 void sd_model_destroy(sd_model *m);
 
+/* The KV cache's format, while it is empty (after creation or sd_reset;
+ * SD_ERR_ARG otherwise): fp16 as created, or the 4-bit blocks of sd_kvpool_*
+ * below, 4.5 bits a value, which every entry point of the handle then appends
+ * to and attends over.  Rows are rotated with the handle's own RoPE tables.
+ * A handle of the 4-bit format does not keep row i of an M-row call equal
+ * to the one-row call bit for bit.  On failure the format stays. */
+enum { SD_KV_F16 = 1, SD_KV_Q4 = 2 };
+sd_status sd_model_set_kv_format(sd_model *m, int32_t format);
+
 /* Uploads one tensor given in its GGUF byte layout (`layer` = -1 for the
  * global tensors).  Replaces the `ct.tensor(reader, name, device)` loads at
  * quantized_llama_local.rs:242-281. */
@@ -317,7 +326,8 @@ enum { SD_BENCH_QKV = 100, SD_BENCH_GATE_UP = 101, SD_BENCH_ALL_LAYERS = -2 };
 sd_status sd_bench_qmatmul(sd_model *m, int32_t layer, int32_t kind, size_t rows, int32_t iters, double *us,
                            double *bytes);
 /* Copies n fp16 cache rows [pos0, pos0+n) of one (layer, K=0/V=1, kv head):
- * out [n][head_dim] (checks of the in-place KV layout). */
+ * out [n][head_dim] (checks of the in-place KV layout; in the 4-bit format the
+ * values that the codes stand for). */
 sd_status sd_read_kv_rows(sd_model *m, int32_t layer, int32_t which, int32_t head, size_t pos0, size_t n,
                           uint16_t *out);
 /* Number of positions currently held in the KV cache. */
@@ -494,6 +504,14 @@ typedef struct sd_sampling {
     int32_t top_k;
     float top_p, min_p;
 } sd_sampling;
+/* A token drawn from the next-token row (as sd_next_logits would return it,
+ * with the same effects), and one from each of rows [0, n) of the last verify
+ * pass (sd_batched_logits, sd_tree_logits_keep_kv; n at most its rows), on the
+ * device: the logits do not cross to the host.  params, uniforms and tokens are
+ * host memory.  SD_ERR_SAMPLING for filters out of range or a row without a
+ * distribution. */
+sd_status sd_sample_next(sd_model *m, const sd_sampling *params, float uniform, int32_t *token);
+sd_status sd_sample_rows(sd_model *m, const sd_sampling *params, const float *uniforms, size_t n, int32_t *tokens);
 typedef struct sd_sampler sd_sampler;
 /* A workspace for up to max_rows rows of vocab (<= 262144) logits.  Calls on
  * one handle, replays of graphs that captured them among these, must be

@@ -3,26 +3,13 @@
 its fp16 weights, at the lengths, masks, strides and pages where it can go wrong."""
 import numpy as np
 import pytest
-import torch
 
 import _kvq
+from _devmem import Graph, Stream, dev, full, ptr, synchronize, zeros
 
 pytestmark = pytest.mark.gpu
 
 MAX_POS = 5000
-
-
-def dev(a):
-    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
-
-
-def host(t):
-    torch.cuda.synchronize()
-    return t.cpu().numpy()
-
-
-def ptr(t):
-    return 0 if t is None else t.data_ptr()
 
 
 class Pool:
@@ -50,19 +37,19 @@ class Pool:
         dk, dv, ds, dl = dev(k), dev(v), dev(np.asarray(seq, np.int32)), dev(np.asarray(slot, np.int32))
         dp = None if pos is None else dev(np.asarray(pos, np.int32))
         dq = None if q is None else dev(q)
-        qo = None if q is None else torch.full((len(k), self.H, self.hd), 77.0, dtype=torch.float16, device="cuda")
-        torch.cuda.synchronize()
+        qo = None if q is None else full((len(k), self.H, self.hd), 77.0, np.float16)
+        synchronize()
         self.pool.append(layer, len(k), ptr(dk), ptr(dv), ptr(dl), ptr(self.dtable), *self.table.shape, dtype=dt,
                          seqs=ptr(ds), pos=ptr(dp), q=ptr(dq), q_out=ptr(qo), stream=stream)
-        torch.cuda.synchronize()
-        return None if q is None else host(qo)
+        synchronize()
+        return None if q is None else qo.get()
 
     def read(self, seq, slot, layer=0, fill=5.0):
         n = len(slot)
         ds, dl = dev(np.asarray(seq, np.int32)), dev(np.asarray(slot, np.int32))
-        ko, vo = (torch.full((n, self.KV, self.hd), fill, dtype=torch.float16, device="cuda") for _ in range(2))
+        ko, vo = (full((n, self.KV, self.hd), fill, np.float16) for _ in range(2))
         self.pool.read(layer, n, ptr(dl), ptr(self.dtable), *self.table.shape, ptr(ko), ptr(vo), seqs=ptr(ds))
-        return host(ko), host(vo)
+        return ko.get(), vo.get()
 
     def fill(self, layer=0, edit=None):
         """all positions of all sequences; returns the values they stand for, a (k, v) pair per sequence"""
@@ -83,20 +70,20 @@ class Pool:
         lens = self.lens if lens is None else lens
         rows = int(sum(counts))
         start = dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
-        dl, dq, dm = dev(np.asarray(lens, np.int32)), dev(q), None if mask is None else dev(mask.view(np.int64))
+        dl, dq, dm = dev(np.asarray(lens, np.int32)), dev(q), None if mask is None else dev(mask)
         if out is None:
-            out = torch.full((rows, self.H, self.hd), 9.0, dtype=torch.float16, device="cuda")
+            out = full((rows, self.H, self.hd), 9.0, np.float16)
         table = self.dtable if table is None else table
         max_rows = max(counts) if max_rows is None else max_rows
         max_len = max(lens) if max_len is None else max_len
         if ws is None:
-            ws = torch.zeros(self.pool.attend_workspace(rows, len(counts), max_rows, max_len), dtype=torch.uint8, device="cuda")
-        torch.cuda.synchronize()
+            ws = zeros(self.pool.attend_workspace(rows, len(counts), max_rows, max_len), np.uint8)
+        synchronize()
         self.pool.attend(layer, ptr(dq), ptr(out), ptr(start), ptr(dl), ptr(table), *table.shape, rows=rows,
-                         max_rows=max_rows, max_len=max_len, ws=ptr(ws) if ws.numel() else 0, ws_bytes=ws.numel(),
+                         max_rows=max_rows, max_len=max_len, ws=ptr(ws) if ws.nbytes else 0, ws_bytes=ws.nbytes,
                          mask=ptr(dm), mask_words=0 if mask is None else mask.shape[1], scale=scale, q_ld=q_ld,
                          out_ld=out_ld, stream=stream)
-        return host(out)
+        return out.get()
 
 
 def causal(n, T):
@@ -201,8 +188,8 @@ def test_strided_rows(hip):
     n, w = 50, 8 * 64
     x = p.rng.standard_normal((n, w)).astype(np.float32)
     dx, ds = dev(x), dev(np.arange(n, dtype=np.int32))
-    qo = torch.zeros((n, 4, 64), dtype=torch.float16, device="cuda")
-    torch.cuda.synchronize()
+    qo = zeros((n, 4, 64), np.float16)
+    synchronize()
     p.pool.append(0, n, ptr(dx) + 4 * 256, ptr(dx) + 4 * 384, ptr(ds), ptr(p.dtable), 1, 1, dtype=hip.F32, q=ptr(dx),
                   q_out=ptr(qo), q_ld=w, k_ld=w, v_ld=w)
     gk, gv = p.read([0] * n, range(n))
@@ -210,7 +197,7 @@ def test_strided_rows(hip):
     assert np.array_equal(gk, _kvq.store(_kvq.rotate(k, np.arange(n), p.cos, p.sin, False)))
     assert np.array_equal(gv, _kvq.store(x[:, 384:].reshape(n, 2, 64)))
     want = _kvq.rotate(x[:, :256].reshape(n, 4, 64).astype(np.float64), np.arange(n), p.cos, p.sin, False)
-    assert np.all(np.abs(host(qo) - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * np.abs(x).max())
+    assert np.all(np.abs(qo.get() - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * np.abs(x).max())
 
 
 # ---- attention -------------------------------------------------------------------
@@ -328,14 +315,14 @@ def test_attention_strides_scale_and_untouched_rows(hip):
     wide = np.zeros((9, 4 * 64 + 24), np.float16)
     q = p.rows(9, 4)
     wide[:, :256] = q.reshape(9, 256)
-    out = torch.full((9, 4 * 64 + 12), 3.0, dtype=torch.float16, device="cuda")
+    out = full((9, 4 * 64 + 12), 3.0, np.float16)
     # rows 0-2 of the first sequence, 3-5 of the second; max_rows 2 leaves each one's third; 6-8 belong to nobody
     start, lens, dq = dev(np.array([0, 3, 6], np.int32)), dev(np.array([200, 90], np.int32)), dev(wide)
-    ws = torch.zeros(max(16, p.pool.attend_workspace(9, 2, 2, 200)), dtype=torch.uint8, device="cuda")
-    torch.cuda.synchronize()
+    ws = zeros(max(16, p.pool.attend_workspace(9, 2, 2, 200)), np.uint8)
+    synchronize()
     p.pool.attend(0, ptr(dq), ptr(out), ptr(start), ptr(lens), ptr(p.dtable), *p.table.shape, rows=9, max_rows=2, max_len=200,
-                  ws=ptr(ws), ws_bytes=ws.numel(), scale=0.3, q_ld=280, out_ld=268)
-    got = host(out)
+                  ws=ptr(ws), ws_bytes=ws.nbytes, scale=0.3, q_ld=280, out_ld=268)
+    got = out.get()
     assert (got[:, 256:] == 3.0).all() and (got[[2, 5, 6, 7, 8]] == 3.0).all()
     for s, T in ((0, 200), (1, 90)):
         vis = causal(3, T)[:2]
@@ -378,37 +365,31 @@ def test_captured_and_replayed(hip, rows):
     (kv,) = p.fill()
     ks, vs = kv[0].copy(), kv[1].copy()
     slots = dev(np.arange(T - rows, T, dtype=np.int32))
-    q, k, v = (torch.zeros((rows, h, 128), dtype=torch.float16, device="cuda") for h in (8, 2, 2))
-    qo = torch.zeros_like(q)
-    out = torch.zeros((rows, 8, 128), dtype=torch.float16, device="cuda")
+    q, k, v = (zeros((rows, h, 128), np.float16) for h in (8, 2, 2))
+    qo, out = zeros((rows, 8, 128), np.float16), zeros((rows, 8, 128), np.float16)
     start, lens = dev(np.array([0, rows], np.int32)), dev(np.array([T], np.int32))
-    ws = torch.zeros(max(16, p.pool.attend_workspace(rows, 1, rows, T)), dtype=torch.uint8, device="cuda")
+    ws = zeros(max(16, p.pool.attend_workspace(rows, 1, rows, T)), np.uint8)
 
-    def step():
-        st = torch.cuda.current_stream().cuda_stream
+    def step(st):
         p.pool.append(0, rows, ptr(k), ptr(v), ptr(slots), ptr(p.dtable), *p.table.shape, q=ptr(q), q_out=ptr(qo), stream=st)
         p.pool.attend(0, ptr(qo), ptr(out), ptr(start), ptr(lens), ptr(p.dtable), *p.table.shape, rows=rows, max_rows=rows,
-                      max_len=T, ws=ptr(ws), ws_bytes=ws.numel(), stream=st)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        step()
-    for i in range(3):
+                      max_len=T, ws=ptr(ws), ws_bytes=ws.nbytes, stream=st)
+    graph, side = Graph(step), Stream()
+    for i in range(4):
         nq, nk, nv = p.rows(rows, 8), p.rows(rows, 2), p.rows(rows, 2)
         for t, a in ((q, nq), (k, nk), (v, nv)):
-            t.copy_(torch.from_numpy(a))
-        out.zero_()
-        graph.replay()
-        got, turned = host(out), host(qo)
+            t.put(a)
+        out.put(np.zeros(out.shape))
+        graph.launch()
+        got, turned = out.get(), qo.get()
         pos = np.arange(T - rows, T)
         ks[T - rows:] = _kvq.store(_kvq.rotate(nk.astype(np.float64), pos, p.cos, p.sin, True))
         vs[T - rows:] = _kvq.store(nv.astype(np.float64))
         check_rows(got, turned, (ks, vs), causal(rows, T), 128 ** -0.5)
-        side = torch.cuda.Stream()
-        with torch.cuda.stream(side):
-            out.zero_()
-            step()
-        assert np.array_equal(host(out), got), i
+        out.put(np.zeros(out.shape))
+        step(side.handle)
+        side.wait()
+        assert np.array_equal(out.get(), got), i
 
 
 def test_repeated_calls_agree_bit_for_bit(hip):
@@ -423,7 +404,7 @@ def test_repeated_calls_agree_bit_for_bit(hip):
 # ---- refusals ---------------------------------------------------------------------
 def test_refusals(hip):
     p = Pool(hip, 61, 4, 2, 64, [10], page=32, layers=2)
-    buf = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    buf = zeros(1 << 16, np.uint8)
     b, P = ptr(buf), p.pool
     ok = dict(n=1, k=b, v=b, slots=b, table=b, n_seqs=1, table_ld=1)
     for bad in (dict(k=0), dict(v=0), dict(slots=0), dict(table=0), dict(n_seqs=0), dict(table_ld=0), dict(k=b + 2),

@@ -1,9 +1,9 @@
 """Filtered sampling (sd_sampler_*) against a 64-bit restatement: tokens equal, distributions to an fp32 rounding."""
 import numpy as np
 import pytest
-import torch
 
 import _kvq
+from _devmem import Graph, Stream, dev, full, ptr, zeros
 
 pytestmark = pytest.mark.gpu
 
@@ -12,14 +12,11 @@ def draw(hip, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probs=True, 
     x = np.ascontiguousarray(x, np.float32)
     rows, V = x.shape[0], V or x.shape[1]
     s = sampler or hip.HipSampler(V, rows)
-    dx, du = torch.from_numpy(x).cuda(), torch.from_numpy(np.ascontiguousarray(u, np.float32)).cuda()
-    tok = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
-    pr = torch.full((rows, V), 5.0, device="cuda") if probs else None
-    torch.cuda.synchronize()
-    s.sample(dx.data_ptr(), rows, du.data_ptr(), tok.data_ptr(), temperature, top_k, top_p, min_p,
-             probs=pr.data_ptr() if probs else 0, ld=ld)
-    torch.cuda.synchronize()
-    return tok.cpu().numpy(), pr.cpu().numpy() if probs else None
+    dx, du = dev(x), dev(np.asarray(u, np.float32))
+    tok = full(rows, -7, np.int32)
+    pr = full((rows, V), 5.0) if probs else None
+    s.sample(ptr(dx), rows, ptr(du), ptr(tok), temperature, top_k, top_p, min_p, probs=ptr(pr), ld=ld)
+    return tok.get(), pr.get() if probs else None
 
 
 def check(hip, x, u, **kw):
@@ -129,37 +126,30 @@ def test_captured_and_replayed(hip, kw):
     rng = np.random.default_rng(5)
     V, rows = 33333, 3
     s = hip.HipSampler(V, rows)
-    x, u = torch.zeros((rows, V), device="cuda"), torch.zeros(rows, device="cuda")
-    tok, pr = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros((rows, V), device="cuda")
+    x, u, tok, pr = zeros((rows, V)), zeros(rows), zeros(rows, np.int32), zeros((rows, V))
 
-    def step():
-        s.sample(x.data_ptr(), rows, u.data_ptr(), tok.data_ptr(), probs=pr.data_ptr(),
-                 stream=torch.cuda.current_stream().cuda_stream, **kw)
-    torch.cuda.synchronize()
-    g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
-        step()
-    for i in range(3):
+    def step(st):
+        s.sample(ptr(x), rows, ptr(u), ptr(tok), probs=ptr(pr), stream=st, **kw)
+    graph, side = Graph(step), Stream()
+    for i in range(4):
         a, b = (rng.standard_normal((rows, V)) * 2).astype(np.float32), rng.random(rows).astype(np.float32)
-        x.copy_(torch.from_numpy(a))
-        u.copy_(torch.from_numpy(b))
-        g.replay()
-        torch.cuda.synchronize()
-        got, dist = tok.cpu().numpy(), pr.cpu().numpy()
+        x.put(a)
+        u.put(b)
+        graph.launch()
+        got, dist = tok.get(), pr.get()
         for r in range(rows):
             want, p = _kvq.sample(a[r], b[r], 1.0, **kw)
             assert got[r] == want and np.all(np.abs(dist[r] - p) <= 2.0 ** -24 * p * 1.01 + 2.0 ** -150)
-        side = torch.cuda.Stream()
-        with torch.cuda.stream(side):
-            tok.fill_(-9)
-            step()
-        torch.cuda.synchronize()
-        assert np.array_equal(tok.cpu().numpy(), got)
+        tok.put(np.full(rows, -9))
+        step(side.handle)
+        side.wait()
+        assert np.array_equal(tok.get(), got)
 
 
 def test_refusals(hip):
     s = hip.HipSampler(100, 4)
-    b = torch.zeros(4096, device="cuda").data_ptr()
+    buf = zeros(4096)
+    b = ptr(buf)
     for kw in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_k=-1),
                dict(top_p=-0.1), dict(top_p=1.1), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=2.0)):
         with pytest.raises(hip.SamplingError):
