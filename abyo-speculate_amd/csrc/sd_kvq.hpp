@@ -122,13 +122,13 @@ struct KvqAttn {
     int max_rows;          // most rows of one sequence
     int n_heads, n_rep;
     float scale;
-    // filled in by kvq_attn_plan
-    int nsplit, qt, tiles;
+    // from the plan
+    int nsplit, tile_q, tiles;
     float *part_o, *part_ml;
 };
 // The work split of a call: query tiles, key splits and the workspace they need.
 struct KvqPlan {
-    int qt, tiles, nsplit;
+    int tile_q, tiles, nsplit;  // queries of a tile, tiles, key ranges
     size_t ws_bytes;
 };
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus);

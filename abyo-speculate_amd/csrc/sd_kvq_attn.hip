@@ -1,18 +1,29 @@
 // Attention over the 4-bit paged KV cache (sd_kvq.hpp).
 //
-// Split flash-decoding: a workgroup takes one query tile (QT x 16 queries of
-// one KV head: rows times the heads that share it) and one range of 32-position
-// blocks; its four waves take the range's blocks in turn.  A block's codes
-// become fp16 values in registers (exactly the values the codes stand for),
-// scores are computed transposed, S^T = K Q^T, so that a lane's eight
-// probabilities are the operand of O^T = V^T P^T, and each wave keeps a running
-// maximum and sum in f32.  The waves meet in LDS, the splits in a second launch.
+// Split flash-decoding in two kernels.  A block's codes become fp16 values
+// (exactly the values the codes stand for), scores are computed transposed,
+// S^T = K Q^T, so that a lane's probabilities are its operand of O^T = V^T P^T,
+// and a running maximum and sum in f32 follow the blocks.
+//
+// Up to 32 queries of a KV head (rows times the heads that share it):
+// k_kvq_attn, whose four waves take the blocks of a key range in turn, codes
+// straight from memory into registers.  A value costs two VALU operations
+// (mask and exponent, then the exact subtraction and the step, two values
+// each), so a block is about 300 VALU instructions for 4.6 KB: half of what a
+// CU can spend on its share of the memory's rate.
+// More: k_kvq_wide, whose waves have 32 queries each and share the values of
+// 64 positions through LDS, expanded once for up to 256 queries.
+// Key ranges (splits) meet in k_kvq_combine.
+#include <atomic>
+
 #include "sd_attn_dev.hpp"
 #include "sd_kvq_dev.hpp"
 
 #pragma clang fp contract(fast)
 
 namespace sd {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kKvqT = 256, kKvqWaves = kKvqT / 64;
 
@@ -36,12 +47,6 @@ __device__ __forceinline__ void kvq_load(KvqStep<HD> &b, const uint8_t *blk, int
     b.vs = *(const uintx4 *)(blk + 34 * HD + ((HD == 128 ? r16 >> 2 : r16 >> 3) * 4 + g) * 16);
 }
 
-template <int HD, int QT> struct KvqState {
-    uintx4 q[QT][HD / 32];
-    floatx4 o[QT][HD / 16];
-    float m[QT], l[QT];
-};
-
 // the rows of sequence s: n of them from r0; false where there are none inside the call's
 __device__ __forceinline__ bool kvq_seq_rows(const KvqAttn &p, int s, int &r0, int &n) {
     r0 = p.row_start ? p.row_start[s] : 0;
@@ -61,168 +66,239 @@ __device__ __forceinline__ uint32_t kvq_nan_steps(const uintx4 &vs) {
     return bad;
 }
 
+// C channels from tc of a query's result: normalised, or a split's part (o, and once per query its maximum and sum)
+template <int C>
+__device__ __forceinline__ void kvq_emit(const KvqAttn &p, int split, int row, int head, int tc, float (&o)[C], float M, float l,
+                                         bool first) {
+    if (p.nsplit == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int hd = p.L.hd;
+        if (p.out_act) {
+#pragma unroll
+            for (int c = 0; c < C; c += 4)
+                *(uintx2 *)(p.out + act_index(row, (int64_t)head * hd + tc + c, (int)p.out_ld, p.out_act == 2)) =
+                    uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 2] * inv) << 16),
+                           (uint32_t)f2h(o[c + 1] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
+        } else {
+            uint16_t *dst = p.out + (int64_t)row * p.out_ld + (int64_t)head * hd + tc;
+#pragma unroll
+            for (int c = 0; c < C; c += 4)
+                *(uintx2 *)(dst + c) = uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 1] * inv) << 16),
+                                              (uint32_t)f2h(o[c + 2] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
+        }
+        return;
+    }
+    const int64_t at = ((int64_t)split * p.rows + row) * p.n_heads + head;
+    float *po = p.part_o + at * p.L.hd + tc;
+#pragma unroll
+    for (int c = 0; c < C; c += 4) *(float4 *)(po + c) = float4{o[c], o[c + 1], o[c + 2], o[c + 3]};
+    if (first) *(float2 *)(p.part_ml + 2 * at) = float2{M, l};
+}
+
+// What a workgroup works on: rows and positions of its sequence, its queries,
+// its range of blocks.  False: nothing.
+struct KvqWork {
+    int r0, n, T, P;  // row i of n is row r0 + i of the call and position P + i
+    int nq, q0;       // queries of the KV head, the tile's first
+    int t_end, t_all; // positions that some of the tile's rows see end before t_end, all of them see those before t_all
+    int b0, b1;       // blocks
+};
+__device__ __forceinline__ bool kvq_work(const KvqAttn &p, int s, int split, int tile, int tile_q, KvqWork &w) {
+    if (!kvq_seq_rows(p, s, w.r0, w.n)) return false;
+    w.T = p.row_start ? p.kv_len[s] : p.len0;
+    w.nq = min(w.n, p.max_rows) * p.n_rep;
+    w.q0 = tile * tile_q;
+    if (w.q0 >= w.nq) return false;
+    w.P = w.T - w.n;
+    const int m_first = w.q0 / p.n_rep, m_last = (min(w.q0 + tile_q, w.nq) - 1) / p.n_rep;
+    w.t_end = p.mask ? w.T : min(w.T, w.P + m_last + 1);
+    w.t_all = p.mask ? w.P : w.P + m_first + 1;
+    const int nblk =
+        w.t_end > 0 ? (int)min((int64_t)((w.t_end - 1) / 32 + 1), (int64_t)p.table_ld << (p.L.page_shift - 5)) : 0;
+    w.b0 = (int)((int64_t)nblk * split / p.nsplit);
+    w.b1 = (int)((int64_t)nblk * (split + 1) / p.nsplit);
+    return true;
+}
+
+// bit j: row m sees position key0 + j, j < 8
+__device__ __forceinline__ uint32_t kvq_visible(const KvqAttn &p, const KvqWork &w, int m, int key0) {
+    if (!p.mask) return (1u << min(max(w.P + m + 1 - key0, 0), 8)) - 1u;
+    const uint64_t *mk = p.mask + (int64_t)(w.r0 + m) * p.mask_words;
+    uint32_t vis = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int x = key0 + j - w.P;
+        bool see = x < 0;
+        if (x >= 0 && x < w.n && (x >> 6) < p.mask_words) see = (mk[x >> 6] >> (x & 63)) & 1;
+        vis |= (uint32_t)see << j;
+    }
+    return vis;
+}
+
+// one query's 8 channels from c, negated where the scale is (scores are compared before they are scaled)
+__device__ __forceinline__ uintx4 kvq_query(const KvqAttn &p, const KvqWork &w, int h, int q, int c) {
+    q = min(q, w.nq - 1);
+    const uint16_t *qr = p.q + (int64_t)(w.r0 + q / p.n_rep) * p.q_row + (int64_t)(h * p.n_rep + q % p.n_rep) * p.q_head;
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    return *(const uintx4 *)(qr + c) ^ uintx4{flip, flip, flip, flip};
+}
+
+// fp16 weights of eight scores (scaled by sl2 against the maximum), and their sum
+__device__ __forceinline__ uintx4 kvq_weights(const float (&s)[8], float sl2, float mu, float &sum) {
+    uintx4 pk;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float a = __builtin_amdgcn_exp2f(s[2 * j] * sl2 - mu), b = __builtin_amdgcn_exp2f(s[2 * j + 1] * sl2 - mu);
+        sum += a + b;
+        pk[j] = h2bits(half2v{(_Float16)a, (_Float16)b});
+    }
+    return pk;
+}
+
+// ---- up to 32 queries ------------------------------------------------------------
 template <int HD, int QT>
-__global__ __launch_bounds__(kKvqT) void k_kvq_attn(const KvqAttn p) {
+__global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void k_kvq_attn(const KvqAttn p) {
     constexpr int NDC = HD / 32, NDT = HD / 16;
     __shared__ float sh_o[kKvqWaves][16][HD];
     __shared__ float sh_ml[kKvqWaves][16][2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x, s = blockIdx.z;
-    const int h = blockIdx.y % p.L.n_kv, tile = blockIdx.y / p.L.n_kv;
-    int r0, n;
-    if (!kvq_seq_rows(p, s, r0, n)) return;
-    const int T = p.row_start ? p.kv_len[s] : p.len0;
-    const int nq = min(n, p.max_rows) * p.n_rep, q0 = tile * QT * 16;
-    if (q0 >= nq) return;
-    const int P = T - n;  // row i is position P + i
-    const int m_last = (min(q0 + QT * 16, nq) - 1) / p.n_rep, m_first = q0 / p.n_rep;
-    // positions any of the tile's rows may see, and those that all of them see
-    const int t_end = p.mask ? T : min(T, P + m_last + 1);
-    const int t_all = p.mask ? P : P + m_first + 1;
-    const int nblk = t_end > 0 ? (int)min((int64_t)((t_end - 1) / 32 + 1), (int64_t)p.table_ld << (p.L.page_shift - 5)) : 0;
-    const int b0 = (int)((int64_t)nblk * split / p.nsplit), b1 = (int)((int64_t)nblk * (split + 1) / p.nsplit);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+    const int split = blockIdx.x, h = blockIdx.y % p.L.n_kv;
+    KvqWork W;
+    if (!kvq_work(p, blockIdx.z, split, blockIdx.y / p.L.n_kv, QT * 16, W)) return;
 
-    KvqState<HD, QT> S;
+    uintx4 qf[QT][NDC];
+    floatx4 o[QT][NDT];
+    float m[QT], l[QT];  // the maximum in raw scores
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        const int q = min(q0 + t * 16 + r16, nq - 1);
-        const uint16_t *qr = p.q + (int64_t)(r0 + q / p.n_rep) * p.q_row + (int64_t)(h * p.n_rep + q % p.n_rep) * p.q_head;
 #pragma unroll
-        for (int dc = 0; dc < NDC; dc++) S.q[t][dc] = *(const uintx4 *)(qr + 8 * (g * NDC + dc));
+        for (int dc = 0; dc < NDC; dc++) qf[t][dc] = kvq_query(p, W, h, W.q0 + t * 16 + r16, 8 * (g * NDC + dc));
 #pragma unroll
-        for (int dt = 0; dt < NDT; dt++) S.o[t][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
-        S.m[t] = -INFINITY;
-        S.l[t] = 0.f;
+        for (int dt = 0; dt < NDT; dt++) o[t][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+        m[t] = -INFINITY;
+        l[t] = 0.f;
     }
-    const float sl2 = p.scale * 1.4426950408889634f;
-    const int *table = p.table + (int64_t)s * p.table_ld;
-    for (int b = b0 + wave; b < b1; b += kKvqWaves) {
-        const int page = __builtin_amdgcn_readfirstlane(table[b >> (p.L.page_shift - 5)]);
-        if (page < 0 || page >= p.L.n_pages) continue;  // holds no positions
-        KvqStep<HD> k;
-        kvq_load<HD>(k, p.L.block(page, h, b * 32), lane);
-        const int key0 = b * 32 + 8 * g;
-        const bool full = b * 32 + 32 <= t_all && b * 32 + 32 <= T;
-        // K operands
-        uintx4 ka[2][NDC];
+    const float sl2 = fabsf(p.scale) * 1.4426950408889634f;
+    const float rise = 8.f / fmaxf(sl2, 1e-30f);
+    const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
+    const int steps = (W.b1 - W.b0 - wave + kKvqWaves - 1) / kKvqWaves;  // blocks b0 + wave + 4 i
+    // lane i holds the page of step i of 64; -1: holds no positions
+    auto pages = [&](int i0) {
+        const int b = W.b0 + wave + (i0 + lane) * kKvqWaves;
+        const int pg = i0 + lane < steps ? table[b >> (p.L.page_shift - 5)] : -1;
+        return pg >= 0 && pg < p.L.n_pages ? pg : -1;
+    };
+    auto fetch = [&](KvqStep<HD> &k, int i, int page) {
+        if (page >= 0) kvq_load<HD>(k, p.L.block(page, h, (W.b0 + wave + i * kKvqWaves) * 32), lane);
+    };
+    int pg = pages(0);
+    KvqStep<HD> next{};
+    int page = __builtin_amdgcn_readlane(pg, 0);
+    if (steps > 0) fetch(next, 0, page);
+    for (int i = 0; i < steps; i++) {
+        KvqStep<HD> k = next;
+        const bool have = page >= 0;
+        if (i + 1 < steps) {
+            if (((i + 1) & 63) == 0) pg = pages(i + 1);
+            page = __builtin_amdgcn_readlane(pg, (i + 1) & 63);
+            fetch(next, i + 1, page);
+        }
+        if (!have) continue;
+        const int b = W.b0 + wave + i * kKvqWaves, key0 = b * 32 + 8 * g;
+        const bool full = b * 32 + 32 <= W.t_all && b * 32 + 32 <= W.T;
+        float st[QT][8];
         {
             const uint32_t k0 = k.ks & 0xffffu, k1 = k.ks >> 16;
             const half2v d0 = __builtin_bit_cast(half2v, k0 | (k0 << 16)), d1 = __builtin_bit_cast(half2v, k1 | (k1 << 16));
+            floatx4 acc[QT][2];
+#pragma unroll
+            for (int t = 0; t < QT; t++) acc[t][0] = acc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int dc = 0; dc < NDC; dc++) {
-                ka[0][dc] = kvq_expand_k(HD == 128 ? k.kc[0][dc] : k.kc[0][dc], d0);
-                ka[1][dc] = kvq_expand_k(HD == 128 ? k.kc[HD / 64 - 1][dc] : k.kc[0][2 + dc], d1);
+                const half8 a0 = __builtin_bit_cast(half8, kvq_expand_k(k.kc[0][dc], d0));
+                const half8 a1 = __builtin_bit_cast(half8, kvq_expand_k(HD == 128 ? k.kc[HD / 64 - 1][dc] : k.kc[0][2 + dc], d1));
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    acc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, __builtin_bit_cast(half8, qf[t][dc]), acc[t][0], 0, 0, 0);
+                    acc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, __builtin_bit_cast(half8, qf[t][dc]), acc[t][1], 0, 0, 0);
+                }
             }
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) st[t][j] = acc[t][j >> 2][j & 3];
         }
-        // V operands: a position pair's nibbles n are channels n (hd 128) or 4 (r16 & 1) + n (64) of the lane's word
-        uintx4 va[NDT];
-        uint32_t bad = 0;
+        uint32_t bad = 0, vis[QT];
         if (!full) {
             bad = kvq_nan_steps(k.vs);
-            if (bad) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (bad >> (2 * i) & 1) k.vs[i] &= 0xffff0000u;
-                    if (bad >> (2 * i + 1) & 1) k.vs[i] &= 0x0000ffffu;
-                }
+            for (int j = 0; j < 4; j++) {
+                if (bad >> (2 * j) & 1) k.vs[j] &= 0xffff0000u;
+                if (bad >> (2 * j + 1) & 1) k.vs[j] &= 0x0000ffffu;
+            }
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                vis[t] = kvq_visible(p, W, min(W.q0 + t * 16 + r16, W.nq - 1) / p.n_rep, key0);
+#pragma unroll
+                for (int j = 0; j < 8; j++) st[t][j] = (vis[t] >> j) & 1 ? st[t][j] : -INFINITY;
             }
         }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t wa = k.vc[j >> 1][(2 * j) & 3], wb = k.vc[j >> 1][(2 * j + 1) & 3];
-            const half2v d = __builtin_bit_cast(half2v, (uint32_t)k.vs[j]);
-#pragma unroll
-            for (int u = 0; u < NDT / 4; u++) {
-                const uint32_t sel = HD == 128 ? (u ? 0x07060302u : 0x05040100u) : (r16 & 1 ? 0x07060302u : 0x05040100u);
-                const uint32_t x = __builtin_amdgcn_perm(wb, wa, sel);
-                va[4 * u][j] = h2bits(kvq_low(x) * d);
-                va[4 * u + 1][j] = h2bits(kvq_high(x) * d);
-                va[4 * u + 2][j] = h2bits(kvq_low(x >> 8) * d);
-                va[4 * u + 3][j] = h2bits(kvq_high(x >> 8) * d);
-            }
-        }
+        uintx4 pk[QT];
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-            if (q0 + t * 16 >= nq) break;
-            floatx4 st[2];
+            float top = st[t][0];
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                st[kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 1; j < 8; j++) top = fmaxf(top, st[t][j]);
+            // the maximum moves only for a score that would weigh more than 2^8
+            if (__builtin_amdgcn_ballot_w64(top > m[t] + rise) != 0) {
+                const float cm = xmax4(top);
+                if (cm > m[t] + rise) {
+                    const float alpha = __builtin_amdgcn_exp2f((m[t] - cm) * sl2);
+                    m[t] = cm;
+                    l[t] *= alpha;
 #pragma unroll
-                for (int dc = 0; dc < NDC; dc++)
-                    st[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[kt][dc]),
-                                                                    __builtin_bit_cast(half8, S.q[t][dc]), st[kt], 0, 0, 0);
-            }
-            // bit j: the query sees position key0 + j
-            uint32_t vis = 0xffu;
-            if (!full) {
-                const int m = min(q0 + t * 16 + r16, nq - 1) / p.n_rep;
-                vis = 0;
-                if (p.mask) {
-                    const uint64_t *mk = p.mask + (int64_t)(r0 + m) * p.mask_words;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int x = key0 + j - P;
-                        bool see = x < 0;
-                        if (x >= 0 && x < n && (x >> 6) < p.mask_words) see = (mk[x >> 6] >> (x & 63)) & 1;
-                        vis |= (uint32_t)see << j;
-                    }
-                } else {
-                    const int seen = min(max(P + m + 1 - key0, 0), 8);  // of the lane's 8
-                    vis = (1u << seen) - 1u;
+                    for (int dt = 0; dt < NDT; dt++) o[t][dt] *= alpha;
                 }
             }
-            float lmax = -INFINITY;
+            pk[t] = kvq_weights(st[t], sl2, m[t] == -INFINITY ? 0.f : m[t] * sl2, l[t]);
+        }
+        // V operands: a position pair's nibbles n are channels n (hd 128) or 4 (r16 & 1) + n (64) of the lane's word
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float v = st[j >> 2][j & 3] * sl2;
-                if (!full) v = (vis >> j) & 1 ? v : -INFINITY;
-                st[j >> 2][j & 3] = v;
-                lmax = fmaxf(lmax, v);
+        for (int u = 0; u < NDT / 4; u++) {
+            uintx4 va[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t wa = k.vc[j >> 1][(2 * j) & 3], wb = k.vc[j >> 1][(2 * j + 1) & 3];
+                const half2v d = __builtin_bit_cast(half2v, (uint32_t)k.vs[j]);
+                const uint32_t sel = HD == 128 ? (u ? 0x07060302u : 0x05040100u) : (r16 & 1 ? 0x07060302u : 0x05040100u);
+                const uint32_t x = __builtin_amdgcn_perm(wb, wa, sel);
+                va[0][j] = h2bits(kvq_low(x) * d);
+                va[1][j] = h2bits(kvq_high(x) * d);
+                va[2][j] = h2bits(kvq_low(x >> 8) * d);
+                va[3][j] = h2bits(kvq_high(x >> 8) * d);
             }
-            // the maximum moves only for a score above it by more than 8: weights stay below 2^8
-            if (__builtin_amdgcn_ballot_w64(lmax > S.m[t] + 8.f) != 0) {
-                const float cm = xmax4(lmax);
-                if (cm > S.m[t] + 8.f) {
-                    const float alpha = __builtin_amdgcn_exp2f(S.m[t] - cm);
-                    S.m[t] = cm;
-                    S.l[t] *= alpha;
 #pragma unroll
-                    for (int dt = 0; dt < NDT; dt++) S.o[t][dt] *= alpha;
-                }
-            }
-            const float mu = S.m[t] == -INFINITY ? 0.f : S.m[t];
-            float ps = 0.f, e[8];
+            for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                e[j] = __builtin_amdgcn_exp2f(st[j >> 2][j & 3] - mu);
-                ps += e[j];
-            }
-            S.l[t] += ps;
-            uintx4 pk;
+                for (int t = 0; t < QT; t++)
+                    o[t][4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(half8, va[e]), __builtin_bit_cast(half8, pk[t]), o[t][4 * u + e], 0, 0, 0);
+        }
+        if (!full && __builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+            // NaN groups among the block's values reach the queries that see them and no others.  Lane (q, g) knows what
+            // q sees of the positions 8 g ..; their flags for group e are in the lanes of the same g with its words.
 #pragma unroll
-            for (int j = 0; j < 4; j++) pk[j] = (uint32_t)f2h(e[2 * j]) | ((uint32_t)f2h(e[2 * j + 1]) << 16);
-#pragma unroll
-            for (int dt = 0; dt < NDT; dt++)
-                S.o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, va[dt]),
-                                                                    __builtin_bit_cast(half8, pk), S.o[t][dt], 0, 0, 0);
-            if (!full && __builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-                // NaN groups among the block's values: they reach the queries that see them and no others.
-                // Lane (q, g) knows the visibility of its 8 positions; the groups' flags are in lanes with the
-                // same g: one flag byte per group e, from lane e * (64 / HD * 8 ...) of this g.
+            for (int t = 0; t < QT; t++) {
                 uint32_t hit = 0;
 #pragma unroll
-                for (int e2 = 0; e2 < HD / 32; e2++) {
-                    const int from = g * 16 + e2 * (16 / (HD / 32));
-                    const uint32_t fl = (uint32_t)__shfl((int)bad, from);
-                    hit |= (uint32_t)((fl & vis) != 0) << e2;
-                }
+                for (int e = 0; e < HD / 32; e++)
+                    hit |= (uint32_t)(((uint32_t)__shfl((int)bad, g * 16 + e * (512 / HD)) & vis[t]) != 0) << e;
                 hit |= (uint32_t)__shfl_xor((int)hit, 16);
                 hit |= (uint32_t)__shfl_xor((int)hit, 32);
                 // the lane's accumulators are channels (HD / 4) g ..: group (HD / 4) g / 32
                 if ((hit >> (HD == 128 ? g : g >> 1)) & 1) {
 #pragma unroll
-                    for (int dt = 0; dt < NDT; dt++) S.o[t][dt] = floatx4{NAN, NAN, NAN, NAN};
+                    for (int dt = 0; dt < NDT; dt++) o[t][dt] = floatx4{NAN, NAN, NAN, NAN};
                 }
             }
         }
@@ -230,133 +306,388 @@ __global__ __launch_bounds__(kKvqT) void k_kvq_attn(const KvqAttn p) {
     // the four waves' states, one query tile at a time
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        if (q0 + t * 16 >= nq) break;
-        const float l = xsum4(S.l[t]);
+        if (W.q0 + t * 16 >= W.nq) break;
+        const float lq = xsum4(l[t]);
         if (g == 0) {
-            sh_ml[wave][r16][0] = S.m[t];
-            sh_ml[wave][r16][1] = l;
+            sh_ml[wave][r16][0] = m[t] * sl2;
+            sh_ml[wave][r16][1] = lq;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int dt = 0; dt < NDT; dt++) sh_o[wave][r16][(HD / 4) * g + NDT * i + dt] = S.o[t][dt][i];
+            for (int dt = 0; dt < NDT; dt += 4)
+                *(floatx4 *)&sh_o[wave][r16][(HD / 4) * g + NDT * i + dt] =
+                    floatx4{o[t][dt][i], o[t][dt + 1][i], o[t][dt + 2][i], o[t][dt + 3][i]};
         __syncthreads();
         // thread: query tq, HD / 16 channels from tc
-        const int tq = threadIdx.x >> 4, tc = (threadIdx.x & 15) * (HD / 16);
-        const int q = q0 + t * 16 + tq;
+        const int tq = threadIdx.x >> 4, tc = (threadIdx.x & 15) * (HD / 16), q = W.q0 + t * 16 + tq;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kKvqWaves; w++) M = fmaxf(M, sh_ml[w][tq][0]);
         const float Mu = M == -INFINITY ? 0.f : M;
-        float lw = 0.f, o[HD / 16];
+        float lw = 0.f, oc[HD / 16];
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) o[c] = 0.f;
+        for (int c = 0; c < HD / 16; c++) oc[c] = 0.f;
 #pragma unroll
         for (int w = 0; w < kKvqWaves; w++) {
             const float f = __builtin_amdgcn_exp2f(sh_ml[w][tq][0] - Mu);
             lw += sh_ml[w][tq][1] * f;
 #pragma unroll
-            for (int c = 0; c < HD / 16; c++) o[c] += sh_o[w][tq][tc + c] * f;
+            for (int c = 0; c < HD / 16; c++) oc[c] += sh_o[w][tq][tc + c] * f;
         }
-        if (q < nq) {
-            const int row = r0 + q / p.n_rep, head = h * p.n_rep + q % p.n_rep;
-            if (p.nsplit == 1) {
-                const float inv = lw == 0.f ? 0.f : 1.f / lw;
-                if (p.out_act) {
-#pragma unroll
-                    for (int c = 0; c < HD / 16; c += 4)
-                        *(uintx2 *)(p.out + act_index(row, (int64_t)head * HD + tc + c, (int)p.out_ld, p.out_act == 2)) =
-                            uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 2] * inv) << 16),
-                                   (uint32_t)f2h(o[c + 1] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
-                } else {
-                    uint16_t *dst = p.out + (int64_t)row * p.out_ld + (int64_t)head * HD + tc;
-#pragma unroll
-                    for (int c = 0; c < HD / 16; c += 4)
-                        *(uintx2 *)(dst + c) = uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 1] * inv) << 16),
-                                                      (uint32_t)f2h(o[c + 2] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
-                }
-            } else {
-                const int64_t at = ((int64_t)split * p.rows + row) * p.n_heads + head;
-                float *po = p.part_o + at * HD + tc;
-#pragma unroll
-                for (int c = 0; c < HD / 16; c += 4) *(float4 *)(po + c) = float4{o[c], o[c + 1], o[c + 2], o[c + 3]};
-                if (tc == 0) {
-                    p.part_ml[2 * at] = M;
-                    p.part_ml[2 * at + 1] = lw;
-                }
-            }
-        }
+        if (q < W.nq) kvq_emit<HD / 16>(p, split, W.r0 + q / p.n_rep, h * p.n_rep + q % p.n_rep, tc, oc, M, lw, tc == 0);
         __syncthreads();
     }
 }
 
-// One wave per (row, head): the splits in order.
-template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const KvqAttn p) {
-    const int s = blockIdx.y, lane = threadIdx.x & 63;
-    int r0, n;
-    if (!kvq_seq_rows(p, s, r0, n)) return;
-    const int at = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int m = at / p.n_heads, head = at % p.n_heads;
-    if (m >= min(n, p.max_rows)) return;
-    const int row = r0 + m;
-    float M = -INFINITY;
-    for (int k = 0; k < p.nsplit; k++) M = fmaxf(M, p.part_ml[2 * (((int64_t)k * p.rows + row) * p.n_heads + head)]);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    constexpr int C = HD / 64;
-    float l = 0.f, o[C] = {};
-    for (int k = 0; k < p.nsplit; k++) {
-        const int64_t i = ((int64_t)k * p.rows + row) * p.n_heads + head;
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * i] - Mu);
-        l += p.part_ml[2 * i + 1] * f;
+// ---- more ------------------------------------------------------------------------
+// NW waves of 32 queries (32x32x16 MFMA: column = query).  Stages of two blocks
+// go through LDS as operands, 1 KiB each: lane r + 32 h of an operand holds 8
+// values.  K, chunk c of 16 channels: row r (position k with bits 2 and 3
+// exchanged), channels 16 c + 8 h ..; so a lane's scores 8 c .. 8 c + 7 are the
+// positions 16 c + 8 h ..  V, tile tt and chunk c of 16 positions: positions
+// 16 c + 8 h .. of channel (hd 128) 8 (r >> 1) + 2 tt + (r & 1) or (64)
+// 8 (r >> 2) + 4 tt + (r & 3): the channels of a word are rows next to each other.
+// A stage is expanded by all waves while the one before it is multiplied (two
+// buffers, one barrier a stage).
+template <int HD> struct KvqStage {
+    uintx4 k[2][HD / 16][64];  // [block][chunk][lane]
+    uintx4 v[2][HD / 16][64];  // [block][2 tile + chunk][lane]
+    uint32_t bad[2][HD / 32];  // [block][group]: positions whose values are NaN (held as 0)
+};
+
+// A unit of a stage: 0, 1 the K halves of block 0 (kt), 2, 3 its V halves, 4 .. 7 block 1's.
+template <int HD> struct KvqUnit {
+    uintx4 a, b, s;
+};
+
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_kvq_wide(const KvqAttn p) {
+    constexpr int NC = HD / 16, NT = HD / 32, NU = 8 / NW;
+    extern __shared__ __align__(16) uint8_t smem[];
+    KvqStage<HD> *stage = (KvqStage<HD> *)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
+    const int split = blockIdx.x, h = blockIdx.y % p.L.n_kv;
+    KvqWork W;
+    if (!kvq_work(p, blockIdx.z, split, blockIdx.y / p.L.n_kv, NW * 32, W)) return;
+    const int q0 = W.q0 + wave * 32;            // this wave's queries
+    const bool idle = q0 >= W.nq;
+    const int m_first = min(q0, W.nq - 1) / p.n_rep, m_last = (min(q0 + 32, W.nq) - 1) / p.n_rep;
+    const int t_end = p.mask ? W.T : min(W.T, W.P + m_last + 1), t_all = p.mask ? W.P : min(W.T, W.P + m_first + 1);
+    const int my_m = min(q0 + r32, W.nq - 1) / p.n_rep;
+
+    uintx4 qf[NC];
 #pragma unroll
-        for (int c = 0; c < C; c++) o[c] += p.part_o[i * HD + lane * C + c] * f;
+    for (int c = 0; c < NC; c++) qf[c] = kvq_query(p, W, h, q0 + r32, 16 * c + 8 * hh);
+    floatx16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[t][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float sl2 = fabsf(p.scale) * 1.4426950408889634f;
+    const float rise = 8.f / fmaxf(sl2, 1e-30f);
+    const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
+    const int stages = (W.b1 - W.b0 + 1) / 2;
+
+    // pages of stage i's two blocks, -1 where there is none
+    auto page_of = [&](int b) {
+        const int pg = b < W.b1 ? table[b >> (p.L.page_shift - 5)] : -1;
+        return __builtin_amdgcn_readfirstlane(pg >= 0 && pg < p.L.n_pages ? pg : -1);
+    };
+    KvqUnit<HD> un[NU];
+    int page[2];
+    auto fetch = [&](int i) {
+        page[0] = page_of(W.b0 + 2 * i);
+        page[1] = page_of(W.b0 + 2 * i + 1);
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const int id = wave * NU + u, blk = id >> 2, part = id & 3;
+            const int pg = blk ? page[1] : page[0];
+            if (pg < 0) continue;
+            const uint8_t *base = p.L.block(pg, h, (W.b0 + 2 * i + blk) * 32);
+            if (part < 2) {
+                // K half: position rows of key tile `part`; the lane's (rho, lane group) as stored
+                const int rho = lane & 15, g = lane >> 4;
+                if constexpr (HD == 128) {
+                    un[u].a = *(const uintx4 *)(base + part * 1024 + lane * 16);
+                    un[u].s.x = *(const uint16_t *)(base + 16 * HD + (rho + 16 * g) * 4 + 2 * part);
+                } else {
+                    const uintx2 w = *(const uintx2 *)(base + lane * 16 + 8 * part);
+                    un[u].a = uintx4{w.x, w.y, 0, 0};
+                    un[u].s.x = *(const uint16_t *)(base + 16 * HD + (rho + 16 * (g >> 1)) * 4 + 2 * part);
+                }
+            } else {
+                // V half: hd 128: word lane & 15, positions 8 (lane >> 4) ..; 64: word lane & 7, positions 8 ((lane >> 3) & 3) ..
+                const int w = HD == 128 ? lane & 15 : lane & 7, g = HD == 128 ? lane >> 4 : (lane >> 3) & 3;
+                const uint8_t *v = base + 18 * HD + (w + (HD / 8) * g) * 32;
+                un[u].a = *(const uintx4 *)v;
+                un[u].b = *(const uintx4 *)(v + 16);
+                un[u].s = *(const uintx4 *)(base + 34 * HD + ((w >> 2) * 4 + g) * 16);
+            }
+        }
+    };
+    auto expand = [&](KvqStage<HD> &S) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const int id = wave * NU + u, blk = id >> 2, part = id & 3;
+            if ((blk ? page[1] : page[0]) < 0) {
+                if (part == 2 && lane < HD / 32) S.bad[blk][lane] = 0;
+                continue;
+            }
+            if (part < 2) {
+                const int rho = lane & 15, g = lane >> 4;
+                // position 8 (rho >> 2) + 4 part + (rho & 3) is row 16 (rho >> 3) + 8 part + 4 ((rho >> 2) & 1) + (rho & 3)
+                const int row = 16 * (rho >> 3) + 8 * part + 4 * ((rho >> 2) & 1) + (rho & 3);
+                const uint32_t s = un[u].s.x & 0xffffu;
+                const half2v d = __builtin_bit_cast(half2v, s | (s << 16));
+#pragma unroll
+                for (int e = 0; e < HD / 32; e++) {
+                    const int w = g * (HD / 32) + e;  // channels 8 w ..: chunk w >> 1, half w & 1
+                    S.k[blk][w >> 1][row + 32 * (w & 1)] = kvq_expand_k(un[u].a[e], d);
+                }
+            } else {
+                const int w = HD == 128 ? lane & 15 : lane & 7, g = HD == 128 ? lane >> 4 : (lane >> 3) & 3;
+                const uint32_t bad = kvq_nan_steps(un[u].s);
+                if (bad) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (bad >> (2 * j) & 1) un[u].s[j] &= 0xffff0000u;
+                        if (bad >> (2 * j + 1) & 1) un[u].s[j] &= 0x0000ffffu;
+                    }
+                }
+                if (part == 2 && (w & 3) == 0 && (HD == 128 || lane < 32)) ((uint8_t *)&S.bad[blk][w >> 2])[g] = (uint8_t)bad;
+                // nibbles 4 (part - 2) .. of the words; hd 64 gives each half of the wave two of them
+                const uint32_t sel = part == 3 ? 0x07060302u : 0x05040100u;
+                uintx4 va[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uintx4 &x4 = j < 2 ? un[u].a : un[u].b;
+                    const uint32_t x = __builtin_amdgcn_perm(x4[(2 * j + 1) & 3], x4[(2 * j) & 3], sel);
+                    const half2v d = __builtin_bit_cast(half2v, (uint32_t)un[u].s[j]);
+                    va[0][j] = h2bits(kvq_low(x) * d);
+                    va[1][j] = h2bits(kvq_high(x) * d);
+                    va[2][j] = h2bits(kvq_low(x >> 8) * d);
+                    va[3][j] = h2bits(kvq_high(x >> 8) * d);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int n = 4 * (part - 2) + e;  // nibble: hd 128: tile n >> 1, row 2 w + (n & 1); 64: tile n >> 2, row 4 w + (n & 3)
+                    const int tt = HD == 128 ? n >> 1 : n >> 2, row = HD == 128 ? 2 * w + (n & 1) : 4 * w + (n & 3);
+                    if (HD == 128 || lane < 32) S.v[blk][2 * tt + (g >> 1)][row + 32 * (g & 1)] = va[e];
+                }
+            }
+        }
+    };
+    if (stages > 0) {
+        fetch(0);
+        expand(stage[0]);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __syncthreads();
+    for (int i = 0; i < stages; i++) {
+        const KvqStage<HD> &S = stage[i & 1];
+        const int have0 = page[0], have1 = page[1];
+        if (i + 1 < stages) fetch(i + 1);
+#pragma unroll 1
+        for (int blk = 0; blk < 2; blk++) {
+            const int base = (W.b0 + 2 * i + blk) * 32;
+            if (idle || (blk ? have1 : have0) < 0 || base >= t_end) continue;
+            const bool full = base + 32 <= t_all;
+            floatx16 st;
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-        const int64_t k = (int64_t)head * HD + lane * C + c;
-        p.out[p.out_act ? act_index(row, k, (int)p.out_ld, p.out_act == 2) : (int64_t)row * p.out_ld + k] = f2h(o[c] * inv);
+            for (int j = 0; j < 16; j++) st[j] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.k[blk][c][lane]),
+                                                            __builtin_bit_cast(half8, qf[c]), st, 0, 0, 0);
+            uint32_t vis[2] = {0xffu, 0xffu};
+            if (!full) {
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    vis[c] = kvq_visible(p, W, my_m, base + 16 * c + 8 * hh);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) st[8 * c + j] = (vis[c] >> j) & 1 ? st[8 * c + j] : -INFINITY;
+                }
+            }
+            float top = st[0];
+#pragma unroll
+            for (int j = 1; j < 16; j++) top = fmaxf(top, st[j]);
+            if (__builtin_amdgcn_ballot_w64(top > m + rise) != 0) {
+                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                if (cm > m + rise) {
+                    const float alpha = __builtin_amdgcn_exp2f((m - cm) * sl2);
+                    m = cm;
+                    l *= alpha;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[t][j] *= alpha;
+                }
+            }
+            const float mu = m == -INFINITY ? 0.f : m * sl2;
+            uintx4 pk[2];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float s8[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) s8[j] = st[8 * c + j];
+                pk[c] = kvq_weights(s8, sl2, mu, l);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.v[blk][2 * t + c][lane]),
+                                                                  __builtin_bit_cast(half8, pk[c]), o[t], 0, 0, 0);
+            // NaN groups among the values reach the queries that see them
+            uint32_t any = 0;
+#pragma unroll
+            for (int e = 0; e < HD / 32; e++) any |= S.bad[blk][e];
+            if (any) {
+                uint32_t seen = vis[0] << (8 * hh) | vis[1] << (16 + 8 * hh);
+                seen |= (uint32_t)__shfl_xor((int)seen, 32);
+#pragma unroll
+                for (int e = 0; e < HD / 32; e++)
+                    if (S.bad[blk][e] & seen) {
+                        // accumulator j of any tile is a channel of word (hd 128) 4 (j >> 2) + 2 hh + ((j >> 1) & 1),
+                        // (64) 2 (j >> 2) + hh
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const int w = HD == 128 ? 4 * (j >> 2) + 2 * hh + ((j >> 1) & 1) : 2 * (j >> 2) + hh;
+                            if (w >> 2 == e)
+#pragma unroll
+                                for (int t = 0; t < NT; t++) o[t][j] = NAN;
+                        }
+                    }
+            }
+        }
+        if (i + 1 < stages) expand(stage[(i + 1) & 1]);
+        __syncthreads();
+    }
+    if (idle) return;
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    const int q = q0 + r32;
+    if (q >= W.nq) return;
+    const int row = W.r0 + q / p.n_rep, head = h * p.n_rep + q % p.n_rep;
+    // a word's 8 channels: hd 128: tiles 0 .. 3 of accumulators j, j + 1 (j even); 64: tiles 0, 1 of four accumulators
+#pragma unroll
+    for (int j = 0; j < 16; j += HD == 128 ? 2 : 4) {
+        float oc[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) oc[n] = HD == 128 ? o[n >> 1][j + (n & 1)] : o[(n >> 2) % NT][(j + (n & 3)) & 15];
+        const int w = HD == 128 ? 4 * (j >> 2) + 2 * hh + ((j >> 1) & 1) : 2 * (j >> 2) + hh;
+        kvq_emit<8>(p, split, row, head, 8 * w, oc, m * sl2, l, w == 0);
     }
 }
 
-// Splits so that the workgroups fill the card about twice, each with at least
-// one block for each of its waves.
+// ---- the splits ------------------------------------------------------------------
+// One workgroup per (row, head): every wave knows all weights (lane k: split
+// k's), and takes each fourth split's part, four in flight.
+template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const KvqAttn p) {
+    constexpr int C = HD / 64;
+    __shared__ float sh[4][HD];
+    const int s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int r0, n;
+    if (!kvq_seq_rows(p, s, r0, n)) return;
+    const int mr = blockIdx.x / p.n_heads, head = blockIdx.x % p.n_heads;
+    if (mr >= min(n, p.max_rows)) return;
+    const int row = r0 + mr;
+    const int64_t at = (int64_t)row * p.n_heads + head, step = (int64_t)p.rows * p.n_heads;
+    const float2 ml = lane < p.nsplit ? *(const float2 *)(p.part_ml + 2 * (at + lane * step)) : float2{-INFINITY, 0.f};
+    float M = ml.x;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float f = lane < p.nsplit ? __builtin_amdgcn_exp2f(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
+    float l = ml.y * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    float acc[C] = {};
+    for (int k0 = wave; k0 < p.nsplit; k0 += 16) {
+        float v[4][C];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int k = min(k0 + 4 * u, p.nsplit - 1);
+#pragma unroll
+            for (int c = 0; c < C; c++) v[u][c] = p.part_o[(at + k * step) * HD + lane * C + c];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int k = k0 + 4 * u;
+            const float w = k < p.nsplit ? __shfl(f, k & 63) : 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[c] += k < p.nsplit ? v[u][c] * w : 0.f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) sh[wave][lane * C + c] = acc[c];
+    __syncthreads();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int d = threadIdx.x;
+    if (d < HD) {
+        const float v = (sh[0][d] + sh[1][d]) + (sh[2][d] + sh[3][d]);
+        const int64_t k = (int64_t)head * HD + d;
+        p.out[p.out_act ? act_index(row, k, (int)p.out_ld, p.out_act == 2) : (int64_t)row * p.out_ld + k] = f2h(v * inv);
+    }
+}
+
+// Up to 32 queries: one or two tiles of 16; more: tiles of 64, 128 or 256, the
+// smallest that holds them all.  Splits so that the workgroups fill the card
+// (four waves of the small kernel: twice), each wave with at least one block.
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus) {
     KvqPlan r{};
-    const int nq = max_rows * (n_heads / n_kv);
-    r.qt = nq <= 16 ? 1 : nq <= 32 ? 2 : 4;
-    r.tiles = (nq + 16 * r.qt - 1) / (16 * r.qt);
+    const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
+    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq <= 128 ? 128 : 256;
+    r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
-    const int64_t want = (2 * cus + groups - 1) / groups, most = std::max<int64_t>(1, blocks / kKvqWaves);
+    const int64_t fill = r.tile_q <= 32 ? 2 * cus : cus, least = r.tile_q <= 32 ? kKvqWaves : 4;
+    const int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
     return r;
+}
+
+template <int HD, int NW> static void launch_wide(const KvqAttn &p, hipStream_t st) {
+    constexpr int lds = 2 * (int)sizeof(KvqStage<HD>);
+    static_assert(lds <= 160 * 1024, "two stages in LDS");
+    if constexpr (lds > 64 * 1024) {
+        static std::atomic<uint64_t> done{0};  // bit per device
+        int dev = 0;
+        SD_HIP_CHECK(hipGetDevice(&dev));
+        const uint64_t bit = 1ull << (dev & 63);
+        if (!(done.load(std::memory_order_acquire) & bit) || dev > 63) {
+            SD_HIP_CHECK(hipFuncSetAttribute((const void *)k_kvq_wide<HD, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            done.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    k_kvq_wide<HD, NW><<<dim3((unsigned)p.nsplit, (unsigned)(p.tiles * p.L.n_kv), (unsigned)p.n_seqs), dim3(64 * NW), lds, st>>>(p);
+}
+
+template <int HD> static void launch_attn(const KvqAttn &p, hipStream_t st) {
+    const dim3 g((unsigned)p.nsplit, (unsigned)(p.tiles * p.L.n_kv), (unsigned)p.n_seqs), b(kKvqT);
+    switch (p.tile_q) {
+    case 16: k_kvq_attn<HD, 1><<<g, b, 0, st>>>(p); break;
+    case 32: k_kvq_attn<HD, 2><<<g, b, 0, st>>>(p); break;
+    case 64: launch_wide<HD, 2>(p, st); break;
+    case 128: launch_wide<HD, 4>(p, st); break;
+    default: launch_wide<HD, 8>(p, st); break;
+    }
+    SD_HIP_CHECK(hipGetLastError());
+    if (p.nsplit > 1) {
+        k_kvq_combine<HD><<<dim3((unsigned)(p.max_rows * p.n_heads), (unsigned)p.n_seqs), dim3(256), 0, st>>>(p);
+        SD_HIP_CHECK(hipGetLastError());
+    }
 }
 
 void launch_kvq_attention(const KvqAttn &in, const KvqPlan &plan, void *ws, hipStream_t st) {
     KvqAttn p = in;
     p.nsplit = plan.nsplit;
-    p.qt = plan.qt;
+    p.tile_q = plan.tile_q;
     p.tiles = plan.tiles;
     p.part_o = (float *)ws;
     p.part_ml = p.part_o + (int64_t)p.nsplit * p.rows * p.n_heads * p.L.hd;
-    const dim3 g((unsigned)p.nsplit, (unsigned)(p.tiles * p.L.n_kv), (unsigned)p.n_seqs), b(kKvqT);
-#define KVQ_ATTN(HD)                                            \
-    if (p.qt == 1) k_kvq_attn<HD, 1><<<g, b, 0, st>>>(p);       \
-    else if (p.qt == 2) k_kvq_attn<HD, 2><<<g, b, 0, st>>>(p);  \
-    else k_kvq_attn<HD, 4><<<g, b, 0, st>>>(p)
-    if (p.L.hd == 128) {
-        KVQ_ATTN(128);
-    } else {
-        KVQ_ATTN(64);
-    }
-#undef KVQ_ATTN
-    SD_HIP_CHECK(hipGetLastError());
-    if (p.nsplit > 1) {
-        const dim3 cg((unsigned)((p.max_rows * p.n_heads + 3) / 4), (unsigned)p.n_seqs);
-        if (p.L.hd == 128) k_kvq_combine<128><<<cg, dim3(256), 0, st>>>(p);
-        else k_kvq_combine<64><<<cg, dim3(256), 0, st>>>(p);
-        SD_HIP_CHECK(hipGetLastError());
-    }
+    if (p.L.hd == 128) launch_attn<128>(p, st);
+    else launch_attn<64>(p, st);
 }
 
 }  // namespace sd
