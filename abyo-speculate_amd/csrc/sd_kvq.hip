@@ -27,28 +27,6 @@ template <int X> __device__ __forceinline__ double quad_xor(double v) {
     return __builtin_bit_cast(double, (uint64_t)quad_xor<X>((uint32_t)b) | ((uint64_t)quad_xor<X>((uint32_t)(b >> 32)) << 32));
 }
 
-// The step of the 32 channels that four lanes hold, 8 each.
-__device__ __forceinline__ _Float16 group_step(const double (&x)[8]) {
-    double hi = x[0], lo = x[0];
-    uint32_t bad = x[0] != x[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) {
-        hi = fmax(hi, x[i]);
-        lo = fmin(lo, x[i]);
-        bad |= x[i] != x[i];
-    }
-    hi = fmax(hi, quad_xor<1>(hi));
-    lo = fmin(lo, quad_xor<1>(lo));
-    bad |= quad_xor<1>(bad);
-    hi = fmax(hi, quad_xor<2>(hi));
-    lo = fmin(lo, quad_xor<2>(lo));
-    bad |= quad_xor<2>(bad);
-    const double a = fmax(hi, -lo);
-    if (bad || !(a <= 65504.0)) return (_Float16)__builtin_nanf("");
-    const _Float16 d = (_Float16)(float)(a * 0.125);
-    return hi > -lo ? -d : d;
-}
-
 // c + 8 of clamp(rint(x / d), -8, 7).  The product with 1 / d is within 2^-49
 // of the quotient, so only a value that close to a half needs the division.
 __device__ __forceinline__ uint32_t group_code(double x, double d, double rd) {
@@ -113,79 +91,119 @@ void launch_kvq_tables(float *cos_t, float *sin_t, int max_pos, int hd, double b
 
 constexpr int kAppendT = 256;
 
-// One thread per 8 channels of one head of one row: a row's units are its K
-// heads, V heads and q heads.
+// c + 8 for a value that fp32 holds: the fp32 quotient is within 2^-22 of its
+// own size of the exact one, so only a value that close to a half needs more.
+__device__ __forceinline__ uint32_t group_code(float x, float d, float rd) {
+    const float y = x * rd;
+    float r = rintf(y);
+    if (fabsf(y - r) > 0.5f - 1e-5f) r = (float)rint((double)x / (double)d);
+    return (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8);
+}
+
+// the step of 32 channels from the extremes of four lanes' 8 each
+template <typename T> __device__ __forceinline__ T quad_max(T v) {
+    v = fmax(v, quad_xor<1>(v));
+    return fmax(v, quad_xor<2>(v));
+}
+template <> __device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __uint_as_float(quad_xor<1>(__float_as_uint(v))));
+    return fmaxf(v, __uint_as_float(quad_xor<2>(__float_as_uint(v))));
+}
+template <typename T> __device__ __forceinline__ _Float16 group_step(const T (&x)[8]) {
+    T hi = x[0], lo = -x[0];
+    uint32_t bad = x[0] != x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        hi = fmax(hi, x[i]);
+        lo = fmax(lo, -x[i]);
+        bad |= x[i] != x[i];
+    }
+    hi = quad_max(hi);
+    lo = quad_max(lo);
+    bad |= quad_xor<1>(bad);
+    bad |= quad_xor<2>(bad);
+    const T a = fmax(hi, lo);
+    if (bad || !(a <= (T)65504)) return (_Float16)__builtin_nanf("");
+    const _Float16 d = (_Float16)(float)(a * (T)0.125);
+    return hi > lo ? -d : d;
+}
+
+// the codes of a word's 8 channels; 8s where the step is 0 or NaN
+template <typename T> __device__ __forceinline__ uint32_t group_word(const T (&x)[8], _Float16 d, bool is_v) {
+    if (!(d != (_Float16)0.f && d == d)) return 0x88888888u;
+    const T dd = (T)(float)d, rd = (T)1 / dd;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int n = is_v ? i : (i >> 1) + 4 * (i & 1);
+        word |= group_code(x[i], dd, rd) << (4 * n);
+    }
+    return word;
+}
+
+// One thread per 8 channels of one head of one row.  grid (rows, chunks of
+// units): first the row's K and V heads, then its q heads.  K values are
+// rotated and divided in f64: a code that lies at a border in fp32 (about one
+// value in a million) would depend on the order of two roundings.
 template <int HD, bool F32>
-__global__ __launch_bounds__(kAppendT) void k_kvq_append(const KvqAppend p) {
-    constexpr int W = HD / 8;
-    const int units = 2 * p.L.n_kv + (p.q ? p.n_heads : 0);
-    const int64_t id = ((int64_t)blockIdx.x * kAppendT + threadIdx.x) / W;
-    const int w = threadIdx.x % W;
-    const int r = (int)(id / units), u = (int)(id % units);
-    if (r >= p.rows.n) return;
+__global__ __launch_bounds__(kAppendT) void k_kvq_append(const KvqAppend p, int kv_chunks) {
+    constexpr int W = HD / 8, U = kAppendT / W;  // units of a workgroup
+    const int r = blockIdx.x, w = threadIdx.x % W, unit = threadIdx.x / W, n_kv = p.L.n_kv;
+    const bool is_q = (int)blockIdx.y >= kv_chunks;
+    const int u = (is_q ? (int)blockIdx.y - kv_chunks : (int)blockIdx.y) * U + unit;
+    if (u >= (is_q ? p.n_heads : 2 * n_kv)) return;
+    const bool is_v = !is_q && u >= n_kv;
+    const int h = is_v ? u - n_kv : u, other = (w + W / 2) % W;
+    const bool pairs = p.interleaved != 0;
+    // the row's values do not wait for its place
+    float a[8], b[8] = {};
+    {
+        const void *src = is_q ? p.q : is_v ? p.v : p.k;
+        const int64_t at = (int64_t)r * (is_q ? p.q_ld : is_v ? p.v_ld : p.k_ld) + h * HD;
+        load8<F32>(src, at + 8 * w, a);
+        if (!pairs && !is_v) load8<F32>(src, at + 8 * other, b);
+    }
     int slot;
     const int page = kvq_row_page(p.rows, p.L, r, slot);
     const int pos = p.pos ? p.pos[r] : slot;
     if (page < 0 || pos < 0 || pos >= p.max_pos) return;
     const float *cos_r = p.cos_t + (int64_t)pos * (HD / 2), *sin_r = p.sin_t + (int64_t)pos * (HD / 2);
-    const bool pairs = p.interleaved != 0;
-    const int n_kv = p.L.n_kv, other = (w + W / 2) % W;
-    if (u >= 2 * n_kv) {
-        const int h = u - 2 * n_kv;
-        float x[8], y[8] = {}, o[8];
-        load8<F32>(p.q, (int64_t)r * p.q_ld + h * HD + 8 * w, x);
-        if (!pairs) load8<F32>(p.q, (int64_t)r * p.q_ld + h * HD + 8 * other, y);
-        rotate8<float, HD>(x, y, cos_r, sin_r, w, pairs, o);
-        uintx4 b;
-        b.x = (uint32_t)f2h(o[0]) | ((uint32_t)f2h(o[1]) << 16);
-        b.y = (uint32_t)f2h(o[2]) | ((uint32_t)f2h(o[3]) << 16);
-        b.z = (uint32_t)f2h(o[4]) | ((uint32_t)f2h(o[5]) << 16);
-        b.w = (uint32_t)f2h(o[6]) | ((uint32_t)f2h(o[7]) << 16);
-        *(uintx4 *)(p.q_out + (int64_t)r * p.q_out_row + (int64_t)h * p.q_out_head + 8 * w) = b;
+    if (is_q) {
+        float o[8];
+        rotate8<float, HD>(a, b, cos_r, sin_r, w, pairs, o);
+        uintx4 v;
+        v.x = (uint32_t)f2h(o[0]) | ((uint32_t)f2h(o[1]) << 16);
+        v.y = (uint32_t)f2h(o[2]) | ((uint32_t)f2h(o[3]) << 16);
+        v.z = (uint32_t)f2h(o[4]) | ((uint32_t)f2h(o[5]) << 16);
+        v.w = (uint32_t)f2h(o[6]) | ((uint32_t)f2h(o[7]) << 16);
+        *(uintx4 *)(p.q_out + (int64_t)r * p.q_out_row + (int64_t)h * p.q_out_head + 8 * w) = v;
         return;
     }
-    const bool is_v = u >= n_kv;
-    const int h = is_v ? u - n_kv : u, k = slot & 31;
-    double x[8];
-    {
-        float a[8], b[8] = {};
-        load8<F32>(is_v ? p.v : p.k, (int64_t)r * (is_v ? p.v_ld : p.k_ld) + h * HD + 8 * w, a);
-        if (is_v) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = a[i];
-        } else {
-            if (!pairs) load8<F32>(p.k, (int64_t)r * p.k_ld + h * HD + 8 * other, b);
-            rotate8<double, HD>(a, b, cos_r, sin_r, w, pairs, x);
-        }
-    }
-    const _Float16 d = group_step(x);
-    uint32_t word = 0x88888888u;  // a step of 0, and a NaN group
-    if (d != (_Float16)0.f && d == d) {
-        const double dd = (double)(float)d, rd = 1.0 / dd;
-        word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int n = is_v ? i : (i >> 1) + 4 * (i & 1);
-            word |= group_code(x[i], dd, rd) << (4 * n);
-        }
-    }
+    const int k = slot & 31;
     uint8_t *blk = p.L.block(page, h, slot);
-    *(uint32_t *)(blk + (is_v ? kvq_v_code(k, w, HD) : kvq_k_code(k, w, HD))) = word;
-    if ((w & 3) == 0)
-        *(_Float16 *)(blk + (is_v ? kvq_v_step(k, w >> 2, HD) : kvq_k_step(k, w >> 2, HD))) = d;
+    if (is_v) {
+        const _Float16 d = group_step(a);
+        *(uint32_t *)(blk + kvq_v_code(k, w, HD)) = group_word(a, d, true);
+        if ((w & 3) == 0) *(_Float16 *)(blk + kvq_v_step(k, w >> 2, HD)) = d;
+    } else {
+        double x[8];
+        rotate8<double, HD>(a, b, cos_r, sin_r, w, pairs, x);
+        const _Float16 d = group_step(x);
+        *(uint32_t *)(blk + kvq_k_code(k, w, HD)) = group_word(x, d, false);
+        if ((w & 3) == 0) *(_Float16 *)(blk + kvq_k_step(k, w >> 2, HD)) = d;
+    }
 }
 
 void launch_kvq_append(const KvqAppend &p, hipStream_t st) {
     if (p.rows.n < 1) return;
-    const int64_t units = 2 * p.L.n_kv + (p.q ? p.n_heads : 0);
-    const int64_t groups = (p.rows.n * units * (p.L.hd / 8) + kAppendT - 1) / kAppendT;
-    const dim3 g((unsigned)groups), b(kAppendT);
+    const int U = kAppendT / (p.L.hd / 8), kv = (2 * p.L.n_kv + U - 1) / U, q = p.q ? (p.n_heads + U - 1) / U : 0;
+    const dim3 g((unsigned)p.rows.n, (unsigned)(kv + q)), b(kAppendT);
     if (p.L.hd == 128) {
-        if (p.f32) k_kvq_append<128, true><<<g, b, 0, st>>>(p);
-        else k_kvq_append<128, false><<<g, b, 0, st>>>(p);
+        if (p.f32) k_kvq_append<128, true><<<g, b, 0, st>>>(p, kv);
+        else k_kvq_append<128, false><<<g, b, 0, st>>>(p, kv);
     } else {
-        if (p.f32) k_kvq_append<64, true><<<g, b, 0, st>>>(p);
-        else k_kvq_append<64, false><<<g, b, 0, st>>>(p);
+        if (p.f32) k_kvq_append<64, true><<<g, b, 0, st>>>(p, kv);
+        else k_kvq_append<64, false><<<g, b, 0, st>>>(p, kv);
     }
     SD_HIP_CHECK(hipGetLastError());
 }
@@ -195,10 +213,8 @@ template <int HD>
 __global__ __launch_bounds__(kAppendT) void k_kvq_read(const KvqLayer L, const KvqRows rows, uint16_t *k_out,
                                                        uint16_t *v_out) {
     constexpr int W = HD / 8;
-    const int64_t id = ((int64_t)blockIdx.x * kAppendT + threadIdx.x) / W;
-    const int w = threadIdx.x % W;
-    const int r = (int)(id / (2 * L.n_kv)), u = (int)(id % (2 * L.n_kv));
-    if (r >= rows.n) return;
+    const int r = blockIdx.x, w = threadIdx.x % W, u = blockIdx.y * (kAppendT / W) + threadIdx.x / W;
+    if (u >= 2 * L.n_kv) return;
     const bool is_v = u >= L.n_kv;
     uint16_t *out = is_v ? v_out : k_out;
     int slot;
@@ -220,9 +236,10 @@ __global__ __launch_bounds__(kAppendT) void k_kvq_read(const KvqLayer L, const K
 
 void launch_kvq_read(const KvqLayer &L, const KvqRows &rows, uint16_t *k_out, uint16_t *v_out, hipStream_t st) {
     if (rows.n < 1) return;
-    const int64_t groups = ((int64_t)rows.n * 2 * L.n_kv * (L.hd / 8) + kAppendT - 1) / kAppendT;
-    if (L.hd == 128) k_kvq_read<128><<<dim3((unsigned)groups), dim3(kAppendT), 0, st>>>(L, rows, k_out, v_out);
-    else k_kvq_read<64><<<dim3((unsigned)groups), dim3(kAppendT), 0, st>>>(L, rows, k_out, v_out);
+    const int U = kAppendT / (L.hd / 8);
+    const dim3 g((unsigned)rows.n, (unsigned)((2 * L.n_kv + U - 1) / U)), b(kAppendT);
+    if (L.hd == 128) k_kvq_read<128><<<g, b, 0, st>>>(L, rows, k_out, v_out);
+    else k_kvq_read<64><<<g, b, 0, st>>>(L, rows, k_out, v_out);
     SD_HIP_CHECK(hipGetLastError());
 }
 

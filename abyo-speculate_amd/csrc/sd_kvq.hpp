@@ -123,12 +123,12 @@ struct KvqAttn {
     int n_heads, n_rep;
     float scale;
     // from the plan
-    int nsplit, tile_q, tiles;
+    int nsplit, tile_q, tiles, chunk;
     float *part_o, *part_ml;
 };
 // The work split of a call: query tiles, key splits and the workspace they need.
 struct KvqPlan {
-    int tile_q, tiles, nsplit;  // queries of a tile, tiles, key ranges
+    int tile_q, tiles, nsplit, chunk;  // queries of a tile, tiles, key ranges, blocks of a range
     size_t ws_bytes;
 };
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus);

@@ -95,6 +95,15 @@ __device__ __forceinline__ void kvq_emit(const KvqAttn &p, int split, int row, i
     if (first) *(float2 *)(p.part_ml + 2 * at) = float2{M, l};
 }
 
+// blocks of t positions that the table has pages for
+__device__ __forceinline__ int kvq_blocks(const KvqAttn &p, int t) {
+    return t > 0 ? (int)min((int64_t)((t - 1) / 32 + 1), (int64_t)p.table_ld << (p.L.page_shift - 5)) : 0;
+}
+// splits of a sequence of T positions: at least one
+__device__ __forceinline__ int kvq_splits(const KvqAttn &p, int T) {
+    return min(p.nsplit, max(1, (kvq_blocks(p, T) + p.chunk - 1) / p.chunk));
+}
+
 // What a workgroup works on: rows and positions of its sequence, its queries,
 // its range of blocks.  False: nothing.
 struct KvqWork {
@@ -113,42 +122,40 @@ __device__ __forceinline__ bool kvq_work(const KvqAttn &p, int s, int split, int
     const int m_first = w.q0 / p.n_rep, m_last = (min(w.q0 + tile_q, w.nq) - 1) / p.n_rep;
     w.t_end = p.mask ? w.T : min(w.T, w.P + m_last + 1);
     w.t_all = p.mask ? w.P : w.P + m_first + 1;
-    const int nblk =
-        w.t_end > 0 ? (int)min((int64_t)((w.t_end - 1) / 32 + 1), (int64_t)p.table_ld << (p.L.page_shift - 5)) : 0;
-    w.b0 = (int)((int64_t)nblk * split / p.nsplit);
-    w.b1 = (int)((int64_t)nblk * (split + 1) / p.nsplit);
+    // split k: blocks [k chunk, (k + 1) chunk), the last one to the end
+    if (split >= kvq_splits(p, w.T)) return false;
+    const int nblk = kvq_blocks(p, w.t_end);
+    w.b0 = min(split * p.chunk, nblk);
+    w.b1 = split == p.nsplit - 1 ? nblk : min(w.b0 + p.chunk, nblk);
     return true;
 }
 
 // bit j: row m sees position key0 + j, j < 8
 __device__ __forceinline__ uint32_t kvq_visible(const KvqAttn &p, const KvqWork &w, int m, int key0) {
     if (!p.mask) return (1u << min(max(w.P + m + 1 - key0, 0), 8)) - 1u;
+    // eight bits from x0 of the row's words: both words they can lie in are loaded at once, whatever x0 is
     const uint64_t *mk = p.mask + (int64_t)(w.r0 + m) * p.mask_words;
-    uint32_t vis = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const int x = key0 + j - w.P;
-        bool see = x < 0;
-        if (x >= 0 && x < w.n && (x >> 6) < p.mask_words) see = (mk[x >> 6] >> (x & 63)) & 1;
-        vis |= (uint32_t)see << j;
-    }
+    const int x0 = key0 - w.P, a = x0 >> 6, s = x0 & 63, left = w.n - x0;
+    const uint64_t w0 = mk[min(max(a, 0), p.mask_words - 1)], w1 = mk[min(max(a + 1, 0), p.mask_words - 1)];
+    const uint64_t lo = a >= 0 && a < p.mask_words ? w0 : 0, hi = a + 1 >= 0 && a + 1 < p.mask_words ? w1 : 0;
+    uint32_t vis = (uint32_t)(lo >> s | (hi << 1) << (63 - s)) & 0xffu;
+    if (left < 8) vis &= (1u << max(left, 0)) - 1u;
+    if (x0 < 0) vis |= (1u << min(-x0, 8)) - 1u;  // the prefix
     return vis;
 }
 
-// one query's 8 channels from c, negated where the scale is (scores are compared before they are scaled)
-__device__ __forceinline__ uintx4 kvq_query(const KvqAttn &p, const KvqWork &w, int h, int q, int c) {
+// a query's channels
+__device__ __forceinline__ const uint16_t *kvq_query(const KvqAttn &p, const KvqWork &w, int h, int q) {
     q = min(q, w.nq - 1);
-    const uint16_t *qr = p.q + (int64_t)(w.r0 + q / p.n_rep) * p.q_row + (int64_t)(h * p.n_rep + q % p.n_rep) * p.q_head;
-    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    return *(const uintx4 *)(qr + c) ^ uintx4{flip, flip, flip, flip};
+    return p.q + (int64_t)(w.r0 + q / p.n_rep) * p.q_row + (int64_t)(h * p.n_rep + q % p.n_rep) * p.q_head;
 }
 
-// fp16 weights of eight scores (scaled by sl2 against the maximum), and their sum
-__device__ __forceinline__ uintx4 kvq_weights(const float (&s)[8], float sl2, float mu, float &sum) {
+// fp16 weights of eight scores (in base-2 units) against the maximum, and their sum
+__device__ __forceinline__ uintx4 kvq_weights(const float (&s)[8], float mu, float &sum) {
     uintx4 pk;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const float a = __builtin_amdgcn_exp2f(s[2 * j] * sl2 - mu), b = __builtin_amdgcn_exp2f(s[2 * j + 1] * sl2 - mu);
+        const float a = __builtin_amdgcn_exp2f(s[2 * j] - mu), b = __builtin_amdgcn_exp2f(s[2 * j + 1] - mu);
         sum += a + b;
         pk[j] = h2bits(half2v{(_Float16)a, (_Float16)b});
     }
@@ -168,18 +175,18 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 
     uintx4 qf[QT][NDC];
     floatx4 o[QT][NDT];
-    float m[QT], l[QT];  // the maximum in raw scores
+    float m[QT], l[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
+        const uint16_t *qr = kvq_query(p, W, h, W.q0 + t * 16 + r16);
 #pragma unroll
-        for (int dc = 0; dc < NDC; dc++) qf[t][dc] = kvq_query(p, W, h, W.q0 + t * 16 + r16, 8 * (g * NDC + dc));
+        for (int dc = 0; dc < NDC; dc++) qf[t][dc] = *(const uintx4 *)(qr + 8 * (g * NDC + dc));
 #pragma unroll
         for (int dt = 0; dt < NDT; dt++) o[t][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
         m[t] = -INFINITY;
         l[t] = 0.f;
     }
-    const float sl2 = fabsf(p.scale) * 1.4426950408889634f;
-    const float rise = 8.f / fmaxf(sl2, 1e-30f);
+    const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
     const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
     const int steps = (W.b1 - W.b0 - wave + kKvqWaves - 1) / kKvqWaves;  // blocks b0 + wave + 4 i
     // lane i holds the page of step i of 64; -1: holds no positions
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
             for (int t = 0; t < QT; t++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) st[t][j] = acc[t][j >> 2][j & 3];
+                for (int j = 0; j < 8; j++) st[t][j] = acc[t][j >> 2][j & 3] * sl2;
         }
         uint32_t bad = 0, vis[QT];
         if (!full) {
@@ -250,17 +257,17 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
             for (int j = 1; j < 8; j++) top = fmaxf(top, st[t][j]);
             // the maximum moves only for a score that would weigh more than 2^8
-            if (__builtin_amdgcn_ballot_w64(top > m[t] + rise) != 0) {
+            if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.f) != 0) {
                 const float cm = xmax4(top);
-                if (cm > m[t] + rise) {
-                    const float alpha = __builtin_amdgcn_exp2f((m[t] - cm) * sl2);
+                if (cm > m[t] + 8.f) {
+                    const float alpha = __builtin_amdgcn_exp2f(m[t] - cm);
                     m[t] = cm;
                     l[t] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < NDT; dt++) o[t][dt] *= alpha;
                 }
             }
-            pk[t] = kvq_weights(st[t], sl2, m[t] == -INFINITY ? 0.f : m[t] * sl2, l[t]);
+            pk[t] = kvq_weights(st[t], m[t] == -INFINITY ? 0.f : m[t], l[t]);
         }
         // V operands: a position pair's nibbles n are channels n (hd 128) or 4 (r16 & 1) + n (64) of the lane's word
 #pragma unroll
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
         if (W.q0 + t * 16 >= W.nq) break;
         const float lq = xsum4(l[t]);
         if (g == 0) {
-            sh_ml[wave][r16][0] = m[t] * sl2;
+            sh_ml[wave][r16][0] = m[t];
             sh_ml[wave][r16][1] = lq;
         }
 #pragma unroll
@@ -350,10 +357,11 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 // 8 (r >> 2) + 4 tt + (r & 3): the channels of a word are rows next to each other.
 // A stage is expanded by all waves while the one before it is multiplied (two
 // buffers, one barrier a stage).
+constexpr int kMfma = 0x008, kDsRead = 0x100;  // instruction classes of a scheduling group
 template <int HD> struct KvqStage {
     uintx4 k[2][HD / 16][64];  // [block][chunk][lane]
     uintx4 v[2][HD / 16][64];  // [block][2 tile + chunk][lane]
-    uint32_t bad[2][HD / 32];  // [block][group]: positions whose values are NaN (held as 0)
+    __align__(16) uint32_t bad[2][HD / 32];  // [block][group]: positions whose values are NaN (held as 0)
 };
 
 // A unit of a stage: 0, 1 the K halves of block 0 (kt), 2, 3 its V halves, 4 .. 7 block 1's.
@@ -377,29 +385,31 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int my_m = min(q0 + r32, W.nq - 1) / p.n_rep;
 
     uintx4 qf[NC];
+    const uint16_t *qr = kvq_query(p, W, h, q0 + r32);
 #pragma unroll
-    for (int c = 0; c < NC; c++) qf[c] = kvq_query(p, W, h, q0 + r32, 16 * c + 8 * hh);
+    for (int c = 0; c < NC; c++) qf[c] = *(const uintx4 *)(qr + 16 * c + 8 * hh);
     floatx16 o[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const float sl2 = fabsf(p.scale) * 1.4426950408889634f;
-    const float rise = 8.f / fmaxf(sl2, 1e-30f);
+    const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
     const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
     const int stages = (W.b1 - W.b0 + 1) / 2;
 
-    // pages of stage i's two blocks, -1 where there is none
-    auto page_of = [&](int b) {
-        const int pg = b < W.b1 ? table[b >> (p.L.page_shift - 5)] : -1;
-        return __builtin_amdgcn_readfirstlane(pg >= 0 && pg < p.L.n_pages ? pg : -1);
-    };
+    // lane k holds the page of block b0 + 64 j + k; -1: holds no positions
+    int pages = -1;
     KvqUnit<HD> un[NU];
-    int page[2];
+    int page[2] = {-1, -1};  // of the stage in un
     auto fetch = [&](int i) {
-        page[0] = page_of(W.b0 + 2 * i);
-        page[1] = page_of(W.b0 + 2 * i + 1);
+        if ((i & 31) == 0) {
+            const int b = W.b0 + 2 * i + lane;
+            pages = b < W.b1 ? table[b >> (p.L.page_shift - 5)] : -1;
+            pages = pages >= 0 && pages < p.L.n_pages ? pages : -1;
+        }
+        page[0] = __builtin_amdgcn_readlane(pages, 2 * i & 63);
+        page[1] = __builtin_amdgcn_readlane(pages, (2 * i + 1) & 63);
 #pragma unroll
         for (int u = 0; u < NU; u++) {
             const int id = wave * NU + u, blk = id >> 2, part = id & 3;
@@ -432,7 +442,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int u = 0; u < NU; u++) {
             const int id = wave * NU + u, blk = id >> 2, part = id & 3;
             if ((blk ? page[1] : page[0]) < 0) {
+                // nobody sees the positions: their weights are 0, and so must the values be
                 if (part == 2 && lane < HD / 32) S.bad[blk][lane] = 0;
+                if (part >= 2)
+                    for (int e = 0; e < HD / 32; e++) S.v[blk][(part - 2) * (HD / 32) + e][lane] = uintx4{0, 0, 0, 0};
                 continue;
             }
             if (part < 2) {
@@ -479,77 +492,112 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
         }
     };
-    if (stages > 0) {
-        fetch(0);
-        expand(stage[0]);
-    }
-    __syncthreads();
-    for (int i = 0; i < stages; i++) {
-        const KvqStage<HD> &S = stage[i & 1];
-        const int have0 = page[0], have1 = page[1];
-        if (i + 1 < stages) fetch(i + 1);
-#pragma unroll 1
-        for (int blk = 0; blk < 2; blk++) {
-            const int base = (W.b0 + 2 * i + blk) * 32;
-            if (idle || (blk ? have1 : have0) < 0 || base >= t_end) continue;
-            const bool full = base + 32 <= t_all;
-            floatx16 st;
+    auto multiply = [&](const KvqStage<HD> &S, int base, bool first, bool second) {
+        const bool full = first && second && base + 64 <= t_all;
+        floatx16 st[2];
 #pragma unroll
-            for (int j = 0; j < 16; j++) st[j] = 0.f;
+        for (int j = 0; j < 16; j++) st[0][j] = st[1][j] = 0.f;
+        // Two chains, and a group order that keeps six operands requested ahead of them (the compiler would read each
+        // operand just before its product and wait for it: 2.7 us a stage instead of KVQ_STAGE_US)
+        uintx4 vf[4];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.k[blk][c][lane]),
-                                                            __builtin_bit_cast(half8, qf[c]), st, 0, 0, 0);
-            uint32_t vis[2] = {0xffu, 0xffu};
-            if (!full) {
+        for (int c = 0; c < NC; c++) {
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++)
+                st[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.k[blk][c][lane]),
+                                                                 __builtin_bit_cast(half8, qf[c]), st[blk], 0, 0, 0);
+        }
+        // the first tile's values are requested under the softmax
+#pragma unroll
+        for (int c = 0; c < 4; c++) vf[c] = S.v[c >> 1][c & 1][lane];
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
+#pragma unroll
+        for (int c = 0; c < 2 * NC - 2; c++) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) st[blk][j] *= sl2;
+        uint32_t seen[2] = {~0u, ~0u};  // of the lane's query: byte 2 c + hh of a block, the lane's own positions
+        if (!full) {
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                seen[blk] = 0;
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    vis[c] = kvq_visible(p, W, my_m, base + 16 * c + 8 * hh);
+                    const int b = 2 * c + hh;
+                    const uint32_t vis = !(blk ? second : first) ? 0 : kvq_visible(p, W, my_m, base + 32 * blk + 8 * b);
+                    seen[blk] |= vis << (8 * b);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) st[8 * c + j] = (vis[c] >> j) & 1 ? st[8 * c + j] : -INFINITY;
+                    for (int j = 0; j < 8; j++) st[blk][8 * c + j] = (vis >> j) & 1 ? st[blk][8 * c + j] : -INFINITY;
                 }
             }
-            float top = st[0];
+        }
+        float top = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
-            for (int j = 1; j < 16; j++) top = fmaxf(top, st[j]);
-            if (__builtin_amdgcn_ballot_w64(top > m + rise) != 0) {
-                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-                if (cm > m + rise) {
-                    const float alpha = __builtin_amdgcn_exp2f((m - cm) * sl2);
-                    m = cm;
-                    l *= alpha;
+        for (int j = 1; j < 16; j++) top = fmaxf(top, fmaxf(st[0][j], st[1][j]));
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            if (cm > m + 8.f) {
+                const float alpha = __builtin_amdgcn_exp2f(m - cm);
+                m = cm;
+                l *= alpha;
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int j = 0; j < 16; j++) o[t][j] *= alpha;
-                }
+                    for (int j = 0; j < 16; j++) o[t][j] *= alpha;
             }
-            const float mu = m == -INFINITY ? 0.f : m * sl2;
-            uintx4 pk[2];
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        uintx4 pk[4];
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                float s8[8];
+        for (int c = 0; c < 4; c++) {
+            float s8[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) s8[j] = st[8 * c + j];
-                pk[c] = kvq_weights(s8, sl2, mu, l);
+            for (int j = 0; j < 8; j++) s8[j] = st[c >> 1][8 * (c & 1) + j];
+            pk[c] = kvq_weights(s8, mu, l);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const uintx4 v = t ? S.v[c >> 1][2 * t + (c & 1)][lane] : vf[c];
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), __builtin_bit_cast(half8, pk[c]), o[t], 0, 0, 0);
             }
+        }
+        uintx4 bad[2];
+        if constexpr (HD == 128) {
+            bad[0] = *(const uintx4 *)S.bad[0], bad[1] = *(const uintx4 *)S.bad[1];
+        } else {
+            const uintx4 b = *(const uintx4 *)S.bad[0];
+            bad[0] = uintx4{b.x, b.y, 0, 0}, bad[1] = uintx4{b.z, b.w, 0, 0};
+        }
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+        for (int c = 0; c < 4 * (NT - 1) - 2; c++) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4 + 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // NaN groups among the values reach the queries that see them
+        uint32_t any = 0;
 #pragma unroll
-                for (int c = 0; c < 2; c++)
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.v[blk][2 * t + c][lane]),
-                                                                  __builtin_bit_cast(half8, pk[c]), o[t], 0, 0, 0);
-            // NaN groups among the values reach the queries that see them
-            uint32_t any = 0;
+        for (int e = 0; e < HD / 32; e++) any |= bad[0][e] | bad[1][e];
+        if (__builtin_amdgcn_readfirstlane(any) != 0) {
 #pragma unroll
-            for (int e = 0; e < HD / 32; e++) any |= S.bad[blk][e];
-            if (any) {
-                uint32_t seen = vis[0] << (8 * hh) | vis[1] << (16 + 8 * hh);
-                seen |= (uint32_t)__shfl_xor((int)seen, 32);
+            for (int blk = 0; blk < 2; blk++) {
+                seen[blk] |= (uint32_t)__shfl_xor((int)seen[blk], 32);
 #pragma unroll
                 for (int e = 0; e < HD / 32; e++)
-                    if (S.bad[blk][e] & seen) {
+                    if (bad[blk][e] & seen[blk]) {
                         // accumulator j of any tile is a channel of word (hd 128) 4 (j >> 2) + 2 hh + ((j >> 1) & 1),
                         // (64) 2 (j >> 2) + hh
 #pragma unroll
@@ -562,7 +610,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                     }
             }
         }
-        if (i + 1 < stages) expand(stage[(i + 1) & 1]);
+    };
+    // In an interval stage i is multiplied, stage i + 1 expanded and stage i + 2 requested.  Half of the waves, one of the
+    // two of a SIMD, expand first: the matrix instructions of one wave then run beside the other's VALU work.
+    const bool early = NW == 8 && wave >= NW / 2;
+    int now = 0, next = 0;  // bit b: block b of the stage holds positions
+    if (stages > 0) fetch(0);
+    auto prepare = [&](int i) {
+        if (i + 1 >= stages) return;
+        next = (page[0] >= 0) | (page[1] >= 0) << 1;
+        expand(stage[(i + 1) & 1]);
+        if (i + 2 < stages) fetch(i + 2);
+    };
+    for (int i = -1; i < stages; i++) {
+        if (early) prepare(i);
+        const int base = (W.b0 + 2 * i) * 32;
+        if (i >= 0 && !idle && now && base < t_end) multiply(stage[i & 1], base, now & 1, now >> 1);
+        if (!early) prepare(i);
+        now = next;
         __syncthreads();
     }
     if (idle) return;
@@ -578,7 +643,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
         for (int n = 0; n < 8; n++) oc[n] = HD == 128 ? o[n >> 1][j + (n & 1)] : o[(n >> 2) % NT][(j + (n & 3)) & 15];
         const int w = HD == 128 ? 4 * (j >> 2) + 2 * hh + ((j >> 1) & 1) : 2 * (j >> 2) + hh;
-        kvq_emit<8>(p, split, row, head, 8 * w, oc, m * sl2, l, w == 0);
+        kvq_emit<8>(p, split, row, head, 8 * w, oc, m, l, w == 0);
     }
 }
 
@@ -595,29 +660,30 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
     if (mr >= min(n, p.max_rows)) return;
     const int row = r0 + mr;
     const int64_t at = (int64_t)row * p.n_heads + head, step = (int64_t)p.rows * p.n_heads;
-    const float2 ml = lane < p.nsplit ? *(const float2 *)(p.part_ml + 2 * (at + lane * step)) : float2{-INFINITY, 0.f};
+    const int ns = kvq_splits(p, p.row_start ? p.kv_len[s] : p.len0);
+    const float2 ml = lane < ns ? *(const float2 *)(p.part_ml + 2 * (at + lane * step)) : float2{-INFINITY, 0.f};
     float M = ml.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float f = lane < p.nsplit ? __builtin_amdgcn_exp2f(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
+    const float f = lane < ns ? __builtin_amdgcn_exp2f(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
     float l = ml.y * f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
     float acc[C] = {};
-    for (int k0 = wave; k0 < p.nsplit; k0 += 16) {
+    for (int k0 = wave; k0 < ns; k0 += 16) {
         float v[4][C];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int k = min(k0 + 4 * u, p.nsplit - 1);
+            const int k = min(k0 + 4 * u, ns - 1);
 #pragma unroll
             for (int c = 0; c < C; c++) v[u][c] = p.part_o[(at + k * step) * HD + lane * C + c];
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int k = k0 + 4 * u;
-            const float w = k < p.nsplit ? __shfl(f, k & 63) : 0.f;
+            const float w = k < ns ? __shfl(f, k & 63) : 0.f;
 #pragma unroll
-            for (int c = 0; c < C; c++) acc[c] += k < p.nsplit ? v[u][c] * w : 0.f;
+            for (int c = 0; c < C; c++) acc[c] += k < ns ? v[u][c] * w : 0.f;
         }
     }
 #pragma unroll
@@ -642,8 +708,10 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
     const int64_t fill = r.tile_q <= 32 ? 2 * cus : cus, least = r.tile_q <= 32 ? kKvqWaves : 4;
-    const int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
+    int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
+    if (const char *e = getenv("KVQ_CHUNK")) want = std::max<int64_t>(1, blocks / atoi(e));
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
+    r.chunk = (int)std::max<int64_t>(1, (blocks + r.nsplit - 1) / r.nsplit);
     return r;
 }
 
@@ -684,6 +752,7 @@ void launch_kvq_attention(const KvqAttn &in, const KvqPlan &plan, void *ws, hipS
     p.nsplit = plan.nsplit;
     p.tile_q = plan.tile_q;
     p.tiles = plan.tiles;
+    p.chunk = plan.chunk;
     p.part_o = (float *)ws;
     p.part_ml = p.part_o + (int64_t)p.nsplit * p.rows * p.n_heads * p.L.hd;
     if (p.L.hd == 128) launch_attn<128>(p, st);
