@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 // 8 (r >> 2) + 4 tt + (r & 3): the channels of a word are rows next to each other.
 // A stage is expanded by all waves while the one before it is multiplied (two
 // buffers, one barrier a stage).
-constexpr int kMfma = 0x008, kDsRead = 0x100;  // instruction classes of a scheduling group
+constexpr int kMfma = 0x008, kDsRead = 0x100, kValu = 0x402;  // instruction classes of a scheduling group
 template <int HD> struct KvqStage {
     uintx4 k[2][HD / 16][64];  // [block][chunk][lane]
     uintx4 v[2][HD / 16][64];  // [block][2 tile + chunk][lane]
@@ -492,86 +492,125 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
         }
     };
+    const float hidden = sl2 < 0.f ? INFINITY : -INFINITY;  // a masked score before it is scaled
+    // the maximum of a block's scores joins the query's
+    auto raise = [&](const floatx16 &st) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; j++) top = fmaxf(top, st[j] * sl2);
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        if (cm > m) {
+            const float alpha = __builtin_amdgcn_exp2f(m - cm);
+            m = cm;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[t][j] *= alpha;
+        }
+    };
+    // fp16 weights of a block's scores and their sum
+    auto weigh = [&](const floatx16 &st, uintx4 (&pk)[2]) {
+        const float mu = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = __builtin_amdgcn_exp2f(st[8 * c + 2 * j] * sl2 - mu);
+                const float y = __builtin_amdgcn_exp2f(st[8 * c + 2 * j + 1] * sl2 - mu);
+                sum += x + y;
+                pk[c][j] = h2bits(half2v{(_Float16)x, (_Float16)y});
+            }
+        return sum;
+    };
+    // A stage: the products of one block run beside the softmax of the other.  The maximum is not looked for: a query
+    // keeps the one of its first block until its weights add up to more than 2^14 in some block (they stay below
+    // fp16's range, and their relative precision is the same at any size); then it is raised and they are taken again.
+    constexpr float kMost = 16384.f;
     auto multiply = [&](const KvqStage<HD> &S, int base, bool first, bool second) {
         const bool full = first && second && base + 64 <= t_all;
         floatx16 st[2];
+        uintx4 pk[2][2];
+        uint32_t seen[2] = {~0u, ~0u};  // of the lane's query: byte 2 c + hh of a block, the lane's own positions
 #pragma unroll
         for (int j = 0; j < 16; j++) st[0][j] = st[1][j] = 0.f;
-        // Two chains, and a group order that keeps six operands requested ahead of them (the compiler would read each
-        // operand just before its product and wait for it: 2.7 us a stage instead of KVQ_STAGE_US)
-        uintx4 vf[4];
-        __builtin_amdgcn_sched_barrier(0);
+        auto mask = [&](int blk) {
+            if (full) return;
+            seen[blk] = 0;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
+            for (int c = 0; c < 2; c++) {
+                const int b = 2 * c + hh;
+                const uint32_t vis = !(blk ? second : first) ? 0 : kvq_visible(p, W, my_m, base + 32 * blk + 8 * b);
+                seen[blk] |= vis << (8 * b);
 #pragma unroll
-            for (int blk = 0; blk < 2; blk++)
+                for (int j = 0; j < 8; j++) st[blk][8 * c + j] = (vis >> j) & 1 ? st[blk][8 * c + j] : hidden;
+            }
+        };
+        auto scores = [&](int blk) {
+#pragma unroll
+            for (int c = 0; c < NC; c++)
                 st[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.k[blk][c][lane]),
                                                                  __builtin_bit_cast(half8, qf[c]), st[blk], 0, 0, 0);
-        }
-        // the first tile's values are requested under the softmax
+        };
+        auto values = [&](int blk) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) vf[c] = S.v[c >> 1][c & 1][lane];
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
+            for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int c = 0; c < 2 * NC - 2; c++) {
+                for (int t = 0; t < NT; t++)
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, S.v[blk][2 * t + c][lane]),
+                                                                  __builtin_bit_cast(half8, pk[blk][c]), o[t], 0, 0, 0);
+        };
+        // scores of block 0, its operands requested four ahead
+        __builtin_amdgcn_sched_barrier(0);
+        scores(0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+        for (int c = 0; c < NC - 4; c++) {
             __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
         __builtin_amdgcn_sched_barrier(0);
+        mask(0);
+        // scores of block 1 beside the weights of block 0
+        __builtin_amdgcn_sched_barrier(0);
+        scores(1);
+        float sum = weigh(st[0], pk[0]);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
 #pragma unroll
-        for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) st[blk][j] *= sl2;
-        uint32_t seen[2] = {~0u, ~0u};  // of the lane's query: byte 2 c + hh of a block, the lane's own positions
-        if (!full) {
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++) {
-                seen[blk] = 0;
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int b = 2 * c + hh;
-                    const uint32_t vis = !(blk ? second : first) ? 0 : kvq_visible(p, W, my_m, base + 32 * blk + 8 * b);
-                    seen[blk] |= vis << (8 * b);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) st[blk][8 * c + j] = (vis >> j) & 1 ? st[blk][8 * c + j] : -INFINITY;
-                }
-            }
-        }
-        float top = fmaxf(st[0][0], st[1][0]);
-#pragma unroll
-        for (int j = 1; j < 16; j++) top = fmaxf(top, fmaxf(st[0][j], st[1][j]));
-        if (__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0) {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-            if (cm > m + 8.f) {
-                const float alpha = __builtin_amdgcn_exp2f(m - cm);
-                m = cm;
-                l *= alpha;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) o[t][j] *= alpha;
-            }
-        }
-        const float mu = m == -INFINITY ? 0.f : m;
-        uintx4 pk[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            float s8[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) s8[j] = st[c >> 1][8 * (c & 1) + j];
-            pk[c] = kvq_weights(s8, mu, l);
+        for (int c = 0; c < NC; c++) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kValu, 56 / NC, 0);
+            if (c + 4 < NC) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const uintx4 v = t ? S.v[c >> 1][2 * t + (c & 1)][lane] : vf[c];
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), __builtin_bit_cast(half8, pk[c]), o[t], 0, 0, 0);
-            }
+        if (__builtin_amdgcn_ballot_w64(sum > kMost || m == -INFINITY) != 0) {
+            raise(st[0]);
+            sum = weigh(st[0], pk[0]);
         }
+        l += sum;
+        mask(1);
+        // values of block 0 beside the weights of block 1
+        __builtin_amdgcn_sched_barrier(0);
+        values(0);
+        sum = weigh(st[1], pk[1]);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+        for (int c = 0; c < 2 * NT; c++) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kValu, 56 / (2 * NT), 0);
+            if (c + 4 < 2 * NT) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (__builtin_amdgcn_ballot_w64(sum > kMost || m == -INFINITY) != 0) {
+            raise(st[1]);
+            sum = weigh(st[1], pk[1]);
+        }
+        l += sum;
+        __builtin_amdgcn_sched_barrier(0);
+        values(1);
         uintx4 bad[2];
         if constexpr (HD == 128) {
             bad[0] = *(const uintx4 *)S.bad[0], bad[1] = *(const uintx4 *)S.bad[1];
@@ -581,11 +620,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
         __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
 #pragma unroll
-        for (int c = 0; c < 4 * (NT - 1) - 2; c++) {
+        for (int c = 0; c < 2 * NT - 3; c++) {
             __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 4 + 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, 3, 0);
         __builtin_amdgcn_sched_barrier(0);
         // NaN groups among the values reach the queries that see them
         uint32_t any = 0;
@@ -707,7 +746,7 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq <= 128 ? 128 : 256;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
-    const int64_t fill = r.tile_q <= 32 ? 2 * cus : cus, least = r.tile_q <= 32 ? kKvqWaves : 4;
+    const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus, least = r.tile_q <= 32 && n_seqs > 1 ? 8 : 4;
     int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
     if (const char *e = getenv("KVQ_CHUNK")) want = std::max<int64_t>(1, blocks / atoi(e));
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
