@@ -78,7 +78,8 @@ KvqPlan KvPool::plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max
     if (max_rows < 1 || max_rows > rows) throw ArgError("kvpool: max_rows must be in [1, rows]");
     if (max_len < 0 || max_len > 0x7fffffc0) throw ArgError("kvpool: max_len out of range");
     KvqPlan p = kvq_attn_plan(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, (int)n_seqs, (int)max_rows, max_len, cus);
-    if ((int64_t)p.tiles * cfg.n_kv_heads > 65535) throw UnsupportedError("kvpool: too many rows of one sequence in one call");
+    // a grid holds fewer than 2^32 threads, at up to 512 a workgroup
+    if ((int64_t)p.tiles * cfg.n_kv_heads * n_seqs > (1 << 22)) throw UnsupportedError("kvpool: too many rows in one call");
     p.ws_bytes = p.nsplit > 1 ? (size_t)p.nsplit * (size_t)rows * cfg.n_heads * (cfg.head_dim + 2) * sizeof(float) : 0;
     return p;
 }

@@ -123,7 +123,7 @@ struct KvqAttn {
     int n_heads, n_rep;
     float scale;
     // from the plan
-    int nsplit, tile_q, tiles, chunk;
+    int nsplit, tile_q, tiles, chunk, groups;
     float *part_o, *part_ml;
 };
 // The work split of a call: query tiles, key splits and the workspace they need.

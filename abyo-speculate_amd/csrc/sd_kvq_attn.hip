@@ -27,6 +27,13 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kKvqT = 256, kKvqWaves = kKvqT / 64;
 
+// Weights are 2^(score - m) in fp16 with m, a query's reference, this much below
+// a maximum of its scores: the largest of the scores so far weighs 2^7 or more,
+// so that a million positions of 2^-24 of its weight each still count (fp16 ends
+// at 2^-24; a weight is rounded by 2^-11 of itself, or by 2^-32 of the largest).
+// 2048 rows over 8191 positions take 295 us with it and 287 without.
+constexpr float kKvqHead = 7.f;
+
 // What a wave loads of one block: the words of its lane.
 template <int HD> struct KvqStep {
     uintx4 kc[HD / 64];  // [kt] at hd 128, both kt at 64
@@ -112,6 +119,27 @@ struct KvqWork {
     int t_end, t_all; // positions that some of the tile's rows see end before t_end, all of them see those before t_all
     int b0, b1;       // blocks
 };
+// Workgroup id -> (sequence, KV head, tile, split): the splits one after the
+// other, a split's groups turned by its number.  XCDs take workgroups in turn
+// (8 of them), and the first splits are the ones every sequence has: with the
+// splits next to each other all short sequences of a batch met on one XCD
+// (16 sequences of up to 9001 positions in 32 splits: 19.5 us, in 35 14.8).
+// With heads next to each other a head's tiles read its blocks through one L2.
+struct KvqPlace {
+    int s, h, tile, split;
+};
+__device__ __forceinline__ KvqPlace kvq_place(const KvqAttn &p) {
+    KvqPlace r;
+    const uint32_t id = blockIdx.x, n = (uint32_t)p.groups;
+    r.split = (int)(id / n);
+    uint32_t i = id % n + (uint32_t)r.split;
+    i = i >= n ? i % n : i;
+    r.h = (int)(i % (uint32_t)p.L.n_kv);
+    i /= (uint32_t)p.L.n_kv;
+    r.tile = (int)(i % (uint32_t)p.tiles);
+    r.s = (int)(i / (uint32_t)p.tiles);
+    return r;
+}
 __device__ __forceinline__ bool kvq_work(const KvqAttn &p, int s, int split, int tile, int tile_q, KvqWork &w) {
     if (!kvq_seq_rows(p, s, w.r0, w.n)) return false;
     w.T = p.row_start ? p.kv_len[s] : p.len0;
@@ -150,7 +178,7 @@ __device__ __forceinline__ const uint16_t *kvq_query(const KvqAttn &p, const Kvq
     return p.q + (int64_t)(w.r0 + q / p.n_rep) * p.q_row + (int64_t)(h * p.n_rep + q % p.n_rep) * p.q_head;
 }
 
-// fp16 weights of eight scores (in base-2 units) against the maximum, and their sum
+// fp16 weights of eight scores (in base-2 units) against the reference, and their sum
 __device__ __forceinline__ uintx4 kvq_weights(const float (&s)[8], float mu, float &sum) {
     uintx4 pk;
 #pragma unroll
@@ -169,9 +197,10 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
     __shared__ float sh_o[kKvqWaves][16][HD];
     __shared__ float sh_ml[kKvqWaves][16][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x, h = blockIdx.y % p.L.n_kv;
+    const KvqPlace at = kvq_place(p);
+    const int split = at.split, h = at.h;
     KvqWork W;
-    if (!kvq_work(p, blockIdx.z, split, blockIdx.y / p.L.n_kv, QT * 16, W)) return;
+    if (!kvq_work(p, at.s, split, at.tile, QT * 16, W)) return;
 
     uintx4 qf[QT][NDC];
     floatx4 o[QT][NDT];
@@ -187,7 +216,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
         l[t] = 0.f;
     }
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
-    const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
+    const int *table = p.table + (int64_t)at.s * p.table_ld;
     const int steps = (W.b1 - W.b0 - wave + kKvqWaves - 1) / kKvqWaves;  // blocks b0 + wave + 4 i
     // lane i holds the page of step i of 64; -1: holds no positions
     auto pages = [&](int i0) {
@@ -256,10 +285,10 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
             float top = st[t][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) top = fmaxf(top, st[t][j]);
-            // the maximum moves only for a score that would weigh more than 2^8
-            if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.f) != 0) {
-                const float cm = xmax4(top);
-                if (cm > m[t] + 8.f) {
+            // the reference moves only for a score that would weigh more than 2^15
+            if (__builtin_amdgcn_ballot_w64(top > m[t] + 15.f) != 0) {
+                const float cm = xmax4(top) - kKvqHead;
+                if (cm > m[t] + 15.f - kKvqHead) {
                     const float alpha = __builtin_amdgcn_exp2f(m[t] - cm);
                     m[t] = cm;
                     l[t] *= alpha;
@@ -375,9 +404,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     extern __shared__ __align__(16) uint8_t smem[];
     KvqStage<HD> *stage = (KvqStage<HD> *)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
-    const int split = blockIdx.x, h = blockIdx.y % p.L.n_kv;
+    const KvqPlace at = kvq_place(p);
+    const int split = at.split, h = at.h;
     KvqWork W;
-    if (!kvq_work(p, blockIdx.z, split, blockIdx.y / p.L.n_kv, NW * 32, W)) return;
+    if (!kvq_work(p, at.s, split, at.tile, NW * 32, W)) return;
     const int q0 = W.q0 + wave * 32;            // this wave's queries
     const bool idle = q0 >= W.nq;
     const int m_first = min(q0, W.nq - 1) / p.n_rep, m_last = (min(q0 + 32, W.nq) - 1) / p.n_rep;
@@ -395,7 +425,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
-    const int *table = p.table + (int64_t)blockIdx.z * p.table_ld;
+    const int *table = p.table + (int64_t)at.s * p.table_ld;
     const int stages = (W.b1 - W.b0 + 1) / 2;
 
     // lane k holds the page of block b0 + 64 j + k; -1: holds no positions
@@ -493,13 +523,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
     };
     const float hidden = sl2 < 0.f ? INFINITY : -INFINITY;  // a masked score before it is scaled
-    // the maximum of a block's scores joins the query's
+    // a block's scores move their query's reference
     auto raise = [&](const floatx16 &st) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; j++) top = fmaxf(top, st[j] * sl2);
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        const float cm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) - kKvqHead;
         if (cm > m) {
             const float alpha = __builtin_amdgcn_exp2f(m - cm);
             m = cm;
@@ -525,10 +555,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
         return sum;
     };
-    // A stage: the products of one block run beside the softmax of the other.  The maximum is not looked for: a query
-    // keeps the one of its first block until its weights add up to more than 2^14 in some block (they stay below
-    // fp16's range, and their relative precision is the same at any size); then it is raised and they are taken again.
-    constexpr float kMost = 16384.f;
+    // A stage: the products of one block run beside the softmax of the other.  No maximum is looked for: a query
+    // keeps the reference of its first block until its weights add up to more than 2^15 in half a block (they stay
+    // below fp16's range); then the reference is raised and they are taken again.
+    constexpr float kMost = 32768.f;
     auto multiply = [&](const KvqStage<HD> &S, int base, bool first, bool second) {
         const bool full = first && second && base + 64 <= t_all;
         floatx16 st[2];
@@ -651,7 +681,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
     };
     // In an interval stage i is multiplied, stage i + 1 expanded and stage i + 2 requested.  Half of the waves, one of the
-    // two of a SIMD, expand first: the matrix instructions of one wave then run beside the other's VALU work.
+    // two of a SIMD, expand first: the matrix instructions of one wave then run beside the other's VALU work (2048 rows
+    // over 8191 positions 295 us, all expanding first some 10 us more).
     const bool early = NW == 8 && wave >= NW / 2;
     int now = 0, next = 0;  // bit b: block b of the stage holds positions
     if (stages > 0) fetch(0);
@@ -738,8 +769,13 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
 }
 
 // Up to 32 queries: one or two tiles of 16; more: tiles of 64, 128 or 256, the
-// smallest that holds them all.  Splits so that the workgroups fill the card
-// (four waves of the small kernel: twice), each wave with at least one block.
+// smallest that holds them all (60 rows of 4 heads over 8191 positions, one tile
+// of 256 for a KV head: 34 us with the combine; tiles of 128 39, of 64 52).
+// Splits: the wide kernel's workgroup has a CU to itself, the small one's four
+// waves share it with another (5 rows over 120000 positions 21 us in 64 splits of
+// 8 heads, 25 in 32).  In a batch the lengths differ, so more and shorter ranges
+// even the load, but not below two blocks a wave, whose merge then costs as much
+// (16 sequences of up to 9001 positions: ranges of 4 blocks 22 us, 8 18.5).
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
@@ -748,7 +784,6 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
     const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus, least = r.tile_q <= 32 && n_seqs > 1 ? 8 : 4;
     int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
-    if (const char *e = getenv("KVQ_CHUNK")) want = std::max<int64_t>(1, blocks / atoi(e));
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
     r.chunk = (int)std::max<int64_t>(1, (blocks + r.nsplit - 1) / r.nsplit);
     return r;
@@ -767,11 +802,11 @@ template <int HD, int NW> static void launch_wide(const KvqAttn &p, hipStream_t 
             done.fetch_or(bit, std::memory_order_release);
         }
     }
-    k_kvq_wide<HD, NW><<<dim3((unsigned)p.nsplit, (unsigned)(p.tiles * p.L.n_kv), (unsigned)p.n_seqs), dim3(64 * NW), lds, st>>>(p);
+    k_kvq_wide<HD, NW><<<dim3((unsigned)(p.nsplit * p.groups)), dim3(64 * NW), lds, st>>>(p);
 }
 
 template <int HD> static void launch_attn(const KvqAttn &p, hipStream_t st) {
-    const dim3 g((unsigned)p.nsplit, (unsigned)(p.tiles * p.L.n_kv), (unsigned)p.n_seqs), b(kKvqT);
+    const dim3 g((unsigned)(p.nsplit * p.groups)), b(kKvqT);
     switch (p.tile_q) {
     case 16: k_kvq_attn<HD, 1><<<g, b, 0, st>>>(p); break;
     case 32: k_kvq_attn<HD, 2><<<g, b, 0, st>>>(p); break;
@@ -792,6 +827,7 @@ void launch_kvq_attention(const KvqAttn &in, const KvqPlan &plan, void *ws, hipS
     p.tile_q = plan.tile_q;
     p.tiles = plan.tiles;
     p.chunk = plan.chunk;
+    p.groups = p.tiles * p.L.n_kv * p.n_seqs;
     p.part_o = (float *)ws;
     p.part_ml = p.part_o + (int64_t)p.nsplit * p.rows * p.n_heads * p.L.hd;
     if (p.L.hd == 128) launch_attn<128>(p, st);
