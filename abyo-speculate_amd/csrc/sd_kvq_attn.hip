@@ -73,26 +73,26 @@ __device__ __forceinline__ uint32_t kvq_nan_steps(const uintx4 &vs) {
     return bad;
 }
 
+__device__ __forceinline__ uint32_t kvq_pair(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
+// C channels from k of a row of the result, in the activation layout or in rows
+template <int C>
+__device__ __forceinline__ void kvq_put(const KvqAttn &p, int row, int64_t k, const float (&o)[C], float inv) {
+#pragma unroll
+    for (int c = 0; c < C; c += 4) {
+        if (p.out_act)
+            *(uintx2 *)(p.out + act_index(row, k + c, (int)p.out_ld, p.out_act == 2)) =
+                uintx2{kvq_pair(o[c] * inv, o[c + 2] * inv), kvq_pair(o[c + 1] * inv, o[c + 3] * inv)};
+        else
+            *(uintx2 *)(p.out + (int64_t)row * p.out_ld + k + c) =
+                uintx2{kvq_pair(o[c] * inv, o[c + 1] * inv), kvq_pair(o[c + 2] * inv, o[c + 3] * inv)};
+    }
+}
 // C channels from tc of a query's result: normalised, or a split's part (o, and once per query its maximum and sum)
 template <int C>
 __device__ __forceinline__ void kvq_emit(const KvqAttn &p, int split, int row, int head, int tc, float (&o)[C], float M, float l,
                                          bool first) {
     if (p.nsplit == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int hd = p.L.hd;
-        if (p.out_act) {
-#pragma unroll
-            for (int c = 0; c < C; c += 4)
-                *(uintx2 *)(p.out + act_index(row, (int64_t)head * hd + tc + c, (int)p.out_ld, p.out_act == 2)) =
-                    uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 2] * inv) << 16),
-                           (uint32_t)f2h(o[c + 1] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
-        } else {
-            uint16_t *dst = p.out + (int64_t)row * p.out_ld + (int64_t)head * hd + tc;
-#pragma unroll
-            for (int c = 0; c < C; c += 4)
-                *(uintx2 *)(dst + c) = uintx2{(uint32_t)f2h(o[c] * inv) | ((uint32_t)f2h(o[c + 1] * inv) << 16),
-                                              (uint32_t)f2h(o[c + 2] * inv) | ((uint32_t)f2h(o[c + 3] * inv) << 16)};
-        }
+        kvq_put<C>(p, row, (int64_t)head * p.L.hd + tc, o, l == 0.f ? 0.f : 1.f / l);
         return;
     }
     const int64_t at = ((int64_t)split * p.rows + row) * p.n_heads + head;
@@ -169,6 +169,22 @@ __device__ __forceinline__ uint32_t kvq_visible(const KvqAttn &p, const KvqWork 
     uint32_t vis = (uint32_t)(lo >> s | (hi << 1) << (63 - s)) & 0xffu;
     if (left < 8) vis &= (1u << max(left, 0)) - 1u;
     if (x0 < 0) vis |= (1u << min(-x0, 8)) - 1u;  // the prefix
+    return vis;
+}
+
+// bit j: row m sees position key0 + j, j < 64
+__device__ __forceinline__ uint64_t kvq_visible64(const KvqAttn &p, const KvqWork &w, int m, int key0) {
+    if (!p.mask) {
+        const int n = w.P + m + 1 - key0;
+        return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1u;
+    }
+    const uint64_t *mk = p.mask + (int64_t)(w.r0 + m) * p.mask_words;
+    const int x0 = key0 - w.P, a = x0 >> 6, s = x0 & 63, left = w.n - x0;
+    const uint64_t w0 = mk[min(max(a, 0), p.mask_words - 1)], w1 = mk[min(max(a + 1, 0), p.mask_words - 1)];
+    const uint64_t lo = a >= 0 && a < p.mask_words ? w0 : 0, hi = a + 1 >= 0 && a + 1 < p.mask_words ? w1 : 0;
+    uint64_t vis = lo >> s | (hi << 1) << (63 - s);
+    if (left < 64) vis &= (1ull << max(left, 0)) - 1u;
+    if (x0 < 0) vis |= x0 <= -64 ? ~0ull : (1ull << -x0) - 1u;  // the prefix
     return vis;
 }
 
@@ -563,20 +579,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const bool full = first && second && base + 64 <= t_all;
         floatx16 st[2];
         uintx4 pk[2][2];
-        uint32_t seen[2] = {~0u, ~0u};  // of the lane's query: byte 2 c + hh of a block, the lane's own positions
+        uint64_t seen = ~0ull;  // bit j: the lane's query sees position base + j
+        if (!full) seen = kvq_visible64(p, W, my_m, base) & ((first ? 0xffffffffull : 0) | (second ? 0xffffffffull << 32 : 0));
 #pragma unroll
         for (int j = 0; j < 16; j++) st[0][j] = st[1][j] = 0.f;
         auto mask = [&](int blk) {
             if (full) return;
-            seen[blk] = 0;
+            const uint32_t vis = (uint32_t)(seen >> (32 * blk + 8 * hh));
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int b = 2 * c + hh;
-                const uint32_t vis = !(blk ? second : first) ? 0 : kvq_visible(p, W, my_m, base + 32 * blk + 8 * b);
-                seen[blk] |= vis << (8 * b);
-#pragma unroll
-                for (int j = 0; j < 8; j++) st[blk][8 * c + j] = (vis >> j) & 1 ? st[blk][8 * c + j] : hidden;
-            }
+            for (int j = 0; j < 16; j++) st[blk][j] = (vis >> (j + (j & 8))) & 1 ? st[blk][j] : hidden;
         };
         auto scores = [&](int blk) {
 #pragma unroll
@@ -663,10 +674,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         if (__builtin_amdgcn_readfirstlane(any) != 0) {
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
-                seen[blk] |= (uint32_t)__shfl_xor((int)seen[blk], 32);
 #pragma unroll
                 for (int e = 0; e < HD / 32; e++)
-                    if (bad[blk][e] & seen[blk]) {
+                    if (bad[blk][e] & (uint32_t)(seen >> (32 * blk))) {
                         // accumulator j of any tile is a channel of word (hd 128) 4 (j >> 2) + 2 hh + ((j >> 1) & 1),
                         // (64) 2 (j >> 2) + hh
 #pragma unroll
@@ -706,15 +716,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int q = q0 + r32;
     if (q >= W.nq) return;
     const int row = W.r0 + q / p.n_rep, head = h * p.n_rep + q % p.n_rep;
-    // a word's 8 channels: hd 128: tiles 0 .. 3 of accumulators j, j + 1 (j even); 64: tiles 0, 1 of four accumulators
+    // word w's 8 channels: hd 128: tiles 0 .. 3 of accumulators j, j + 1 (j even); 64: tiles 0, 1 of four accumulators
+    auto words = [&](auto &&put) {
 #pragma unroll
-    for (int j = 0; j < 16; j += HD == 128 ? 2 : 4) {
-        float oc[8];
+        for (int j = 0; j < 16; j += HD == 128 ? 2 : 4) {
+            float oc[8];
 #pragma unroll
-        for (int n = 0; n < 8; n++) oc[n] = HD == 128 ? o[n >> 1][j + (n & 1)] : o[(n >> 2) % NT][(j + (n & 3)) & 15];
-        const int w = HD == 128 ? 4 * (j >> 2) + 2 * hh + ((j >> 1) & 1) : 2 * (j >> 2) + hh;
-        kvq_emit<8>(p, split, row, head, 8 * w, oc, m, l, w == 0);
+            for (int n = 0; n < 8; n++) oc[n] = HD == 128 ? o[n >> 1][j + (n & 1)] : o[(n >> 2) % NT][(j + (n & 3)) & 15];
+            put((HD == 128 ? 4 * (j >> 2) + ((j >> 1) & 1) : 2 * (j >> 2)) * 8, oc);
+        }
+    };
+    const int c0 = (HD == 128 ? 2 : 1) * 8 * hh;  // the lane's first channel
+    if (p.nsplit > 1) {
+        const int64_t i = ((int64_t)split * p.rows + row) * p.n_heads + head;
+        float *po = p.part_o + i * HD + c0;
+        words([&](int c, const float (&oc)[8]) {
+            *(float4 *)(po + c) = float4{oc[0], oc[1], oc[2], oc[3]};
+            *(float4 *)(po + c + 4) = float4{oc[4], oc[5], oc[6], oc[7]};
+        });
+        if (hh == 0) *(float2 *)(p.part_ml + 2 * i) = float2{m, l};
+        return;
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    words([&](int c, const float (&oc)[8]) { kvq_put<8>(p, row, (int64_t)head * HD + c0 + c, oc, inv); });
 }
 
 // ---- the splits ------------------------------------------------------------------
