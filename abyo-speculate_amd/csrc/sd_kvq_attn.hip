@@ -141,8 +141,8 @@ __device__ __forceinline__ KvqPlace kvq_place(const KvqAttn &p) {
     return r;
 }
 __device__ __forceinline__ bool kvq_work(const KvqAttn &p, int s, int split, int tile, int tile_q, KvqWork &w) {
-    if (!kvq_seq_rows(p, s, w.r0, w.n)) return false;
     w.T = p.row_start ? p.kv_len[s] : p.len0;
+    if (!kvq_seq_rows(p, s, w.r0, w.n)) return false;
     w.nq = min(w.n, p.max_rows) * p.n_rep;
     w.q0 = tile * tile_q;
     if (w.q0 >= w.nq) return false;
@@ -156,6 +156,12 @@ __device__ __forceinline__ bool kvq_work(const KvqAttn &p, int s, int split, int
     w.b0 = min(split * p.chunk, nblk);
     w.b1 = split == p.nsplit - 1 ? nblk : min(w.b0 + p.chunk, nblk);
     return true;
+}
+
+// The page of block b, asked for before it is known whether the sequence has
+// the block: one round trip to memory less before the first one is requested.
+__device__ __forceinline__ int kvq_page(const KvqAttn &p, int s, int b) {
+    return p.table[(int64_t)s * p.table_ld + min(b >> (p.L.page_shift - 5), p.table_ld - 1)];
 }
 
 // bit j: row m sees position key0 + j, j < 8
@@ -215,6 +221,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
     const KvqPlace at = kvq_place(p);
     const int split = at.split, h = at.h;
+    const int pg0 = kvq_page(p, at.s, split * p.chunk + wave + lane * kKvqWaves);
     KvqWork W;
     if (!kvq_work(p, at.s, split, at.tile, QT * 16, W)) return;
 
@@ -232,18 +239,13 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
         l[t] = 0.f;
     }
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
-    const int *table = p.table + (int64_t)at.s * p.table_ld;
     const int steps = (W.b1 - W.b0 - wave + kKvqWaves - 1) / kKvqWaves;  // blocks b0 + wave + 4 i
     // lane i holds the page of step i of 64; -1: holds no positions
-    auto pages = [&](int i0) {
-        const int b = W.b0 + wave + (i0 + lane) * kKvqWaves;
-        const int pg = i0 + lane < steps ? table[b >> (p.L.page_shift - 5)] : -1;
-        return pg >= 0 && pg < p.L.n_pages ? pg : -1;
-    };
+    auto pages = [&](int i0, int pg) { return i0 + lane < steps && pg >= 0 && pg < p.L.n_pages ? pg : -1; };
     auto fetch = [&](KvqStep<HD> &k, int i, int page) {
         if (page >= 0) kvq_load<HD>(k, p.L.block(page, h, (W.b0 + wave + i * kKvqWaves) * 32), lane);
     };
-    int pg = pages(0);
+    int pg = pages(0, pg0);
     KvqStep<HD> next{};
     int page = __builtin_amdgcn_readlane(pg, 0);
     if (steps > 0) fetch(next, 0, page);
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
         KvqStep<HD> k = next;
         const bool have = page >= 0;
         if (i + 1 < steps) {
-            if (((i + 1) & 63) == 0) pg = pages(i + 1);
+            if (((i + 1) & 63) == 0) pg = pages(i + 1, kvq_page(p, at.s, W.b0 + wave + (i + 1 + lane) * kKvqWaves));
             page = __builtin_amdgcn_readlane(pg, (i + 1) & 63);
             fetch(next, i + 1, page);
         }
@@ -422,6 +424,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
     const KvqPlace at = kvq_place(p);
     const int split = at.split, h = at.h;
+    int pages = kvq_page(p, at.s, split * p.chunk + lane);
     KvqWork W;
     if (!kvq_work(p, at.s, split, at.tile, NW * 32, W)) return;
     const int q0 = W.q0 + wave * 32;            // this wave's queries
@@ -441,18 +444,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
-    const int *table = p.table + (int64_t)at.s * p.table_ld;
     const int stages = (W.b1 - W.b0 + 1) / 2;
 
-    // lane k holds the page of block b0 + 64 j + k; -1: holds no positions
-    int pages = -1;
+    // in `pages` lane k holds the page of block b0 + 64 j + k; -1: holds no positions
     KvqUnit<HD> un[NU];
     int page[2] = {-1, -1};  // of the stage in un
     auto fetch = [&](int i) {
         if ((i & 31) == 0) {
             const int b = W.b0 + 2 * i + lane;
-            pages = b < W.b1 ? table[b >> (p.L.page_shift - 5)] : -1;
-            pages = pages >= 0 && pages < p.L.n_pages ? pages : -1;
+            if (i > 0) pages = kvq_page(p, at.s, b);
+            pages = b < W.b1 && pages >= 0 && pages < p.L.n_pages ? pages : -1;
         }
         page[0] = __builtin_amdgcn_readlane(pages, 2 * i & 63);
         page[1] = __builtin_amdgcn_readlane(pages, (2 * i + 1) & 63);
@@ -743,19 +744,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 
 // ---- the splits ------------------------------------------------------------------
 // One workgroup per (row, head): every wave knows all weights (lane k: split
-// k's), and takes each fourth split's part, four in flight.
+// k's) and takes a part of the splits, HD / 4 lanes to a split, four loads in
+// flight; the first of them go out with those of the maxima and sums.
 template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const KvqAttn p) {
-    constexpr int C = HD / 64;
-    __shared__ float sh[4][HD];
-    const int s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int LS = HD / 4, N = 256 / LS, U = 4;  // lanes of a split, splits of a round, rounds in flight
+    __shared__ __align__(16) float sh[N][HD];
+    const int s = blockIdx.y, lane = threadIdx.x & 63, mine = threadIdx.x / LS, c = threadIdx.x % LS * 4;
+    const int T = p.row_start ? p.kv_len[s] : p.len0;
     int r0, n;
     if (!kvq_seq_rows(p, s, r0, n)) return;
     const int mr = blockIdx.x / p.n_heads, head = blockIdx.x % p.n_heads;
     if (mr >= min(n, p.max_rows)) return;
-    const int row = r0 + mr;
+    const int row = r0 + mr, ns = kvq_splits(p, T);
     const int64_t at = (int64_t)row * p.n_heads + head, step = (int64_t)p.rows * p.n_heads;
-    const int ns = kvq_splits(p, p.row_start ? p.kv_len[s] : p.len0);
     const float2 ml = lane < ns ? *(const float2 *)(p.part_ml + 2 * (at + lane * step)) : float2{-INFINITY, 0.f};
+    float4 v[U];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = *(const float4 *)(p.part_o + (at + min(k0 + u * N + mine, ns - 1) * step) * HD + c);
+    };
+    load(0);
     float M = ml.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -763,32 +771,26 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
     float l = ml.y * f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    float acc[C] = {};
-    for (int k0 = wave; k0 < ns; k0 += 16) {
-        float v[4][C];
+    float4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < ns; k0 += U * N) {
+        if (k0 > 0) load(k0);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int k = min(k0 + 4 * u, ns - 1);
-#pragma unroll
-            for (int c = 0; c < C; c++) v[u][c] = p.part_o[(at + k * step) * HD + lane * C + c];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int k = k0 + 4 * u;
-            const float w = k < ns ? __shfl(f, k & 63) : 0.f;
-#pragma unroll
-            for (int c = 0; c < C; c++) acc[c] += k < ns ? v[u][c] * w : 0.f;
+        for (int u = 0; u < U; u++) {
+            const int k = k0 + u * N + mine;
+            const float w = __shfl(f, k & 63);
+            if (k < ns) acc.x += v[u].x * w, acc.y += v[u].y * w, acc.z += v[u].z * w, acc.w += v[u].w * w;
         }
     }
-#pragma unroll
-    for (int c = 0; c < C; c++) sh[wave][lane * C + c] = acc[c];
+    *(float4 *)&sh[mine][c] = acc;
     __syncthreads();
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int d = threadIdx.x;
     if (d < HD) {
-        const float v = (sh[0][d] + sh[1][d]) + (sh[2][d] + sh[3][d]);
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) x += sh[i][d];
         const int64_t k = (int64_t)head * HD + d;
-        p.out[p.out_act ? act_index(row, k, (int)p.out_ld, p.out_act == 2) : (int64_t)row * p.out_ld + k] = f2h(v * inv);
+        p.out[p.out_act ? act_index(row, k, (int)p.out_ld, p.out_act == 2) : (int64_t)row * p.out_ld + k] = f2h(x * inv);
     }
 }
 
