@@ -416,12 +416,13 @@ template <int HD> struct KvqUnit {
     uintx4 a, b, s;
 };
 
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void k_kvq_wide(const KvqAttn p) {
+template <int HD, int NW, int KG>
+__global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2))) void k_kvq_wide(const KvqAttn p) {
     constexpr int NC = HD / 16, NT = HD / 32, NU = 8 / NW;
     extern __shared__ __align__(16) uint8_t smem[];
-    KvqStage<HD> *stage = (KvqStage<HD> *)smem;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
+    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
+    const int wave = id % NW, kg = id / NW;
+    KvqStage<HD> *stage = (KvqStage<HD> *)smem + 2 * kg;
     const KvqPlace at = kvq_place(p);
     const int split = at.split, h = at.h;
     int pages = kvq_page(p, at.s, split * p.chunk + lane);
@@ -444,15 +445,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int i = 0; i < 16; i++) o[t][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
-    const int stages = (W.b1 - W.b0 + 1) / 2;
+    const int all = (W.b1 - W.b0 + 1) / 2, stages = (all - kg + KG - 1) / KG;  // the range's and this key group's
 
     // in `pages` lane k holds the page of block b0 + 64 j + k; -1: holds no positions
     KvqUnit<HD> un[NU];
     int page[2] = {-1, -1};  // of the stage in un
-    auto fetch = [&](int i) {
-        if ((i & 31) == 0) {
-            const int b = W.b0 + 2 * i + lane;
-            if (i > 0) pages = kvq_page(p, at.s, b);
+    auto fetch = [&](int n) {
+        const int i = n * KG + kg;
+        if ((i & 31) < KG) {
+            const int b = W.b0 + 2 * (i & ~31) + lane;
+            if (n > 0) pages = kvq_page(p, at.s, b);
             pages = b < W.b1 && pages >= 0 && pages < p.L.n_pages ? pages : -1;
         }
         page[0] = __builtin_amdgcn_readlane(pages, 2 * i & 63);
@@ -694,7 +696,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     // In an interval stage i is multiplied, stage i + 1 expanded and stage i + 2 requested.  Half of the waves, one of the
     // two of a SIMD, expand first: the matrix instructions of one wave then run beside the other's VALU work (2048 rows
     // over 8191 positions 295 us, all expanding first some 10 us more).
-    const bool early = NW == 8 && wave >= NW / 2;
+    const bool early = NW * KG == 8 && id >= 4;
     int now = 0, next = 0;  // bit b: block b of the stage holds positions
     if (stages > 0) fetch(0);
     auto prepare = [&](int i) {
@@ -703,13 +705,42 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         expand(stage[(i + 1) & 1]);
         if (i + 2 < stages) fetch(i + 2);
     };
-    for (int i = -1; i < stages; i++) {
+    for (int i = -1; i < (all + KG - 1) / KG; i++) {
         if (early) prepare(i);
-        const int base = (W.b0 + 2 * i) * 32;
-        if (i >= 0 && !idle && now && base < t_end) multiply(stage[i & 1], base, now & 1, now >> 1);
+        const int base = (W.b0 + 2 * (i * KG + kg)) * 32;
+        if (i >= 0 && i < stages && !idle && now && base < t_end) multiply(stage[i & 1], base, now & 1, now >> 1);
         if (!early) prepare(i);
         now = next;
         __syncthreads();
+    }
+    if constexpr (KG == 2) {
+        // group 1's state goes to the wave of group 0 with the same queries, lane to lane
+        float4 *box = (float4 *)smem + wave * 64 * (4 * NT + 1) + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    box[64 * (4 * t + i)] = float4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+            box[64 * 4 * NT] = float4{m, l, 0.f, 0.f};
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float4 ml = box[64 * 4 * NT];
+        const float M = fmaxf(m, ml.x), Mu = M == -INFINITY ? 0.f : M;
+        const float f0 = __builtin_amdgcn_exp2f(m - Mu), f1 = __builtin_amdgcn_exp2f(ml.x - Mu);
+        m = M;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 b = box[64 * (4 * t + i)];
+                o[t][4 * i] = o[t][4 * i] * f0 + b.x * f1;
+                o[t][4 * i + 1] = o[t][4 * i + 1] * f0 + b.y * f1;
+                o[t][4 * i + 2] = o[t][4 * i + 2] * f0 + b.z * f1;
+                o[t][4 * i + 3] = o[t][4 * i + 3] * f0 + b.w * f1;
+            }
     }
     if (idle) return;
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -805,7 +836,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
-    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq <= 128 ? 128 : 256;
+    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : (nq + 255) / 256 * n_kv * n_seqs < cus ? 128 : 256;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
     const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus, least = r.tile_q <= 32 && n_seqs > 1 ? 8 : 4;
@@ -815,20 +846,21 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     return r;
 }
 
-template <int HD, int NW> static void launch_wide(const KvqAttn &p, hipStream_t st) {
-    constexpr int lds = 2 * (int)sizeof(KvqStage<HD>);
-    static_assert(lds <= 160 * 1024, "two stages in LDS");
+template <int HD, int NW, int KG> static void launch_wide(const KvqAttn &p, hipStream_t st) {
+    constexpr int lds = 2 * KG * (int)sizeof(KvqStage<HD>);
+    static_assert(lds <= 160 * 1024, "two stages of each key group in LDS");
+    static_assert(KG == 1 || NW * 64 * (HD / 8 + 1) * 16 <= lds, "a key group's state in LDS");
     if constexpr (lds > 64 * 1024) {
         static std::atomic<uint64_t> done{0};  // bit per device
         int dev = 0;
         SD_HIP_CHECK(hipGetDevice(&dev));
         const uint64_t bit = 1ull << (dev & 63);
         if (!(done.load(std::memory_order_acquire) & bit) || dev > 63) {
-            SD_HIP_CHECK(hipFuncSetAttribute((const void *)k_kvq_wide<HD, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            SD_HIP_CHECK(hipFuncSetAttribute((const void *)k_kvq_wide<HD, NW, KG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
             done.fetch_or(bit, std::memory_order_release);
         }
     }
-    k_kvq_wide<HD, NW><<<dim3((unsigned)(p.nsplit * p.groups)), dim3(64 * NW), lds, st>>>(p);
+    k_kvq_wide<HD, NW, KG><<<dim3((unsigned)(p.nsplit * p.groups)), dim3(64 * NW * KG), lds, st>>>(p);
 }
 
 template <int HD> static void launch_attn(const KvqAttn &p, hipStream_t st) {
@@ -836,9 +868,9 @@ template <int HD> static void launch_attn(const KvqAttn &p, hipStream_t st) {
     switch (p.tile_q) {
     case 16: k_kvq_attn<HD, 1><<<g, b, 0, st>>>(p); break;
     case 32: k_kvq_attn<HD, 2><<<g, b, 0, st>>>(p); break;
-    case 64: launch_wide<HD, 2>(p, st); break;
-    case 128: launch_wide<HD, 4>(p, st); break;
-    default: launch_wide<HD, 8>(p, st); break;
+    case 64: launch_wide<HD, 2, 2>(p, st); break;
+    case 128: launch_wide<HD, 4, 2>(p, st); break;
+    default: launch_wide<HD, 8, 1>(p, st); break;
     }
     SD_HIP_CHECK(hipGetLastError());
     if (p.nsplit > 1) {
