@@ -392,6 +392,94 @@ def test_captured_and_replayed(hip, rows):
         assert np.array_equal(out.get(), got), i
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("KV,H,seqs,most", [(8, 32, 32, 20), (16, 16, 8, 300)])
+def test_attention_many_rows_in_many_sequences(hip, hd, KV, H, seqs, most):
+    """Enough rows for tiles of 256 queries, the sequences with from none to `most` of them."""
+    rng = np.random.default_rng(seqs)
+    counts = [most, 0, 1] + [int(v) for v in rng.integers(1, most, seqs - 3)]
+    lens = [n + int(v) for n, v in zip(counts, rng.integers(0, 90, seqs))]
+    p = Pool(hip, hd + seqs, H, KV, hd, lens, page=32)
+    kvs = p.fill()
+    q = p.rows(sum(counts), H)
+    got = p.attend(q, counts)
+    at = 0
+    for s, n in enumerate(counts):
+        if n:
+            check_rows(got[at:at + n], q[at:at + n], kvs[s], causal(n, lens[s]), hd ** -0.5)
+        at += n
+
+
+@pytest.mark.parametrize("rows,H", [(1, 1), (1, 20), (40, 1), (60, 4)])
+def test_attention_long_tail_of_small_weights(hip, rows, H):
+    """One position 16 nats above thousands of others whose values alone are not zero: a weight is rounded by 2^-11 of itself
+    or 2^-32 of the largest, so the result by 2^-11 of itself, the positions times 2^-32 of the largest value, its own fp16
+    rounding, and what the fp32 scores (64 products) do to the exponentials."""
+    T, hd = 4000, 64
+    p = Pool(hip, 71, H, 1, hd, [T], page=256)
+    k, v = np.zeros((T, 1, hd), np.float16), np.ones((T, 1, hd), np.float16)
+    k[0], v[0] = 2.0, 0.0
+    p.append(k, v, [0] * T, range(T), pos=[0] * T)
+    q = np.ones((rows, H, hd), np.float16)  # scores 2 hd / sqrt(hd) = 16 and 0
+    got = p.attend(q, [rows], mask=None).astype(np.float64)
+    n = T - rows + np.arange(rows, dtype=np.float64)  # positions after the first that row i sees
+    want = (n * np.exp(-16.0) / (1 + n * np.exp(-16.0)))[:, None, None]
+    tol = 2.0 ** -11 * want * 2.01 + T * 2.0 ** -32 + 2.0 ** -25 + 2 * hd * 2.0 ** -24 * 16 * want
+    assert np.all(np.abs(got - want) <= tol), float(np.max(np.abs(got - want) - tol))
+
+
+def test_pages_past_32_bits(hip):
+    """Pages that begin more than 2^32 bytes into a layer, of the second layer: appended, read and attended as the first ones."""
+    hd, KV, page, n_pages, T = 128, 8, 4096, 1000, 300
+    pool = hip.HipKvPool(n_layers=2, n_heads=8, n_kv_heads=KV, head_dim=hd, n_pages=n_pages, page_tokens=page, max_pos=MAX_POS)
+    assert pool.page_bytes() * (n_pages - 2) > 1 << 32
+    rng = np.random.default_rng(5)
+    dk, dv, dq = (dev(rng.standard_normal((n, 8, hd)).astype(np.float16)) for n in (T, T, 2))
+    slots, start, lens = dev(np.arange(T, dtype=np.int32)), dev(np.array([0, 2], np.int32)), dev(np.array([T], np.int32))
+    ws = zeros(max(16, pool.attend_workspace(2, 1, 2, T)), np.uint8)
+    seen = []
+    for layer, pg in ((0, 0), (0, n_pages - 1), (1, n_pages - 2)):
+        table = dev(np.array([[pg]], np.int32))
+        ko, vo, out = (full((n, 8, hd), 3.0, np.float16) for n in (T, T, 2))
+        synchronize()
+        pool.append(layer, T, ptr(dk), ptr(dv), ptr(slots), ptr(table), 1, 1)
+        pool.read(layer, T, ptr(slots), ptr(table), 1, 1, ptr(ko), ptr(vo))
+        pool.attend(layer, ptr(dq), ptr(out), ptr(start), ptr(lens), ptr(table), 1, 1, rows=2, max_rows=2, max_len=T,
+                    ws=ptr(ws), ws_bytes=ws.nbytes)
+        seen.append((ko.get(), vo.get(), out.get()))
+    assert seen[0][0].any() and seen[0][2].any()
+    for other in seen[1:]:
+        for a, b in zip(seen[0], other):
+            assert np.array_equal(a, b)
+    pool.close()
+
+
+def test_two_streams_over_the_same_pages(hip):
+    """Calls on two streams, each with its workspace, read the same pages and give what they give one after the other."""
+    T = 3000
+    p = Pool(hip, 81, 8, 2, 128, [T], page=64)
+    p.fill()
+    start, lens = dev(np.array([0, 5], np.int32)), dev(np.array([T], np.int32))
+    qs, outs = [dev(p.rows(5, 8)) for _ in range(2)], [full((5, 8, 128), 9.0, np.float16) for _ in range(2)]
+    wss = [zeros(max(16, p.pool.attend_workspace(5, 1, 5, T)), np.uint8) for _ in range(2)]
+
+    def call(i, st):
+        p.pool.attend(0, ptr(qs[i]), ptr(outs[i]), ptr(start), ptr(lens), ptr(p.dtable), *p.table.shape, rows=5, max_rows=5,
+                      max_len=T, ws=ptr(wss[i]), ws_bytes=wss[i].nbytes, stream=st)
+    synchronize()
+    want = []
+    for i in range(2):
+        call(i, 0)
+        want.append(outs[i].get())
+    streams = [Stream(), Stream()]
+    for _ in range(8):
+        for i in range(2):
+            call(i, streams[i].handle)
+    for s in streams:
+        s.wait()
+    assert all(np.array_equal(outs[i].get(), want[i]) for i in range(2)) and not np.array_equal(*want)
+
+
 def test_repeated_calls_agree_bit_for_bit(hip):
     p = Pool(hip, 51, 8, 2, 128, [3000, 40, 1500], page=64)
     p.fill()
