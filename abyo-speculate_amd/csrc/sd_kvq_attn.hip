@@ -825,9 +825,13 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
     }
 }
 
-// Up to 32 queries: one or two tiles of 16; more: tiles of 64, 128 or 256, the
-// smallest that holds them all (60 rows of 4 heads over 8191 positions, one tile
-// of 256 for a KV head: 34 us with the combine; tiles of 128 39, of 64 52).
+// Queries of a KV head: up to 32 in one or two tiles of 16, up to 64 in a tile
+// of 64.  More: tiles of 256 expand every value once but leave, with the splits
+// that a short context needs to fill the card, twice the partial results of
+// tiles of 128 in two key groups.  They are taken where they fill the card alone
+// or a split is more than 12 blocks long (a decoder's pass of 60 rows, 32 heads
+// over 8, 8 layers: 8192 positions 1113 us with 128 and 1126 with 256, 32768
+// 1451 and 1394; tiles of 64 lose more to expansion than they save in partials).
 // Splits: the wide kernel's workgroup has a CU to itself, the small one's four
 // waves share it with another (5 rows over 120000 positions 21 us in 64 splits of
 // 8 heads, 25 in 32).  In a batch the lengths differ, so more and shorter ranges
@@ -836,9 +840,10 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
-    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : (nq + 255) / 256 * n_kv * n_seqs < cus ? 128 : 256;
+    const int64_t blocks = (max_len + 31) / 32, big = (nq + 255) / 256 * n_kv * n_seqs;
+    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq > 128 && (big >= cus || big * blocks > 12 * cus) ? 256 : 128;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
-    const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, blocks = (max_len + 31) / 32;
+    const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs;
     const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus, least = r.tile_q <= 32 && n_seqs > 1 ? 8 : 4;
     int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
