@@ -833,10 +833,11 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
 // over 8, 8 layers: 8192 positions 1113 us with 128 and 1126 with 256, 32768
 // 1451 and 1394; tiles of 64 lose more to expansion than they save in partials).
 // Splits: the wide kernel's workgroup has a CU to itself, the small one's four
-// waves share it with another (5 rows over 120000 positions 21 us in 64 splits of
-// 8 heads, 25 in 32).  In a batch the lengths differ, so more and shorter ranges
-// even the load, but not below two blocks a wave, whose merge then costs as much
-// (16 sequences of up to 9001 positions: ranges of 4 blocks 22 us, 8 18.5).
+// waves share it with another (8 layers of 32 heads over 8, 120000 positions, one
+// row: a pass of 720 us, 763 with one to a CU; 32768 positions, 5 rows: no
+// difference).  In a batch the lengths differ, so four times as many ranges even
+// the load (16 sequences of up to 9001 positions: 17.6 us, 19.2 without).  No
+// range is shorter than a block for each wave.
 KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
@@ -844,8 +845,8 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq > 128 && (big >= cus || big * blocks > 12 * cus) ? 256 : 128;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs;
-    const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus, least = r.tile_q <= 32 && n_seqs > 1 ? 8 : 4;
-    int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / least);
+    const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus;
+    int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / 4);
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
     r.chunk = (int)std::max<int64_t>(1, (blocks + r.nsplit - 1) / r.nsplit);
     return r;
