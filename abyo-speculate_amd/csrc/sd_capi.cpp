@@ -86,7 +86,8 @@ static void need_aligned(const void *p, int64_t row_bytes, int align, const char
 }
 static sd::KvqRows kv_rows(const sd_kv_rows *r) {
     if (!r || !r->slot || !r->table) throw sd::ArgError("null argument");
-    if (r->n > ((size_t)1 << 24)) throw sd::ArgError("at most 2^24 rows");
+    // a grid holds fewer than 2^32 threads, 256 of them to a row
+    if (r->n > ((size_t)1 << 23)) throw sd::ArgError("at most 2^23 rows");
     if (r->n_seqs < 1 || r->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
     return sd::KvqRows{(int)r->n, r->seq, r->slot, 0, r->table, r->n_seqs, r->table_ld};
 }
@@ -949,6 +950,7 @@ sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, 
         a.rows = kv_rows(rows);
         if (fmt != SD_F16 && fmt != SD_F32) throw sd::UnsupportedError("append: rows must be F16 or F32");
         if (!k || !v || (q && !q_out)) throw sd::ArgError("null argument");
+        if (q && (const void *)q_out == q) throw sd::ArgError("q_out must not be q");
         const int size = fmt == SD_F32 ? 4 : 2, hd = P.cfg.head_dim;
         a.L = P.layer(layer);
         a.pos = pos;
@@ -1010,6 +1012,7 @@ sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *qy, v
         if (qy->rows == 0) return;
         if (!qy->q || !qy->out || !qy->row_start || !qy->kv_len || !qy->table) throw sd::ArgError("null argument");
         if (qy->n_seqs < 1 || qy->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
+        if (qy->out == qy->q) throw sd::ArgError("out must not be q");
         if (qy->mask && qy->mask_words < 1) throw sd::ArgError("mask_words must be positive");
         const size_t most = (size_t)1 << 40;
         const sd::KvqPlan plan = P.plan((int64_t)std::min(qy->rows, most), qy->n_seqs, (int64_t)std::min(qy->max_rows, most),

@@ -114,6 +114,7 @@ void Sampler::run(SampleParams p, hipStream_t st) {
     if (!p.logits || !p.u || !p.tokens) throw ArgError("sampler: null argument");
     if (p.ld == 0) p.ld = vocab;
     if (p.ld < vocab) throw ArgError("sampler: rows overlap (ld < vocab)");
+    if (p.probs == p.logits) throw ArgError("sampler: probs must not be the logits");
     DeviceScope dev(device);
     p.V = vocab;
     p.ws = ws;

@@ -141,10 +141,17 @@ template <typename T> __device__ __forceinline__ uint32_t group_word(const T (&x
     return word;
 }
 
-// One thread per 8 channels of one head of one row.  grid (rows, chunks of
-// units): first the row's K and V heads, then its q heads.  K values are
-// rotated and divided in f64: a code that lies at a border in fp32 (about one
-// value in a million) would depend on the order of two roundings.
+// One thread per 8 channels of one head of one row, so a group of 32 is four
+// neighbouring lanes and its extremes two quad exchanges.  grid (rows, chunks of
+// units): first the row's K and V heads, then its q heads, which keeps the two
+// kinds of work in different workgroups and gives a single row three of them.
+// K values are rotated and divided in f64: a code that lies at a border in fp32
+// (about one value in a million) would depend on the order of two roundings.
+// Values need no rotation, and fp32 with a check near the borders decides their
+// codes; with the grid by rows that took append and read of 16384 rows from 136
+// to 114 us.  Memory bounds it: 16384 fp16 rows of 32 query heads and 8 KV heads
+// of 128 channels take 88 us, 74 at the rate of a large copy; 2501 fp32 rows 20
+// (18).
 template <int HD, bool F32>
 __global__ __launch_bounds__(kAppendT) void k_kvq_append(const KvqAppend p, int kv_chunks) {
     constexpr int W = HD / 8, U = kAppendT / W;  // units of a workgroup
@@ -209,6 +216,8 @@ void launch_kvq_append(const KvqAppend &p, hipStream_t st) {
 }
 
 // ---- read ----------------------------------------------------------------------
+// The same threads the other way: 16384 rows of 8 heads 27 us, 18 at the rate of
+// a large copy, most of it the 4-byte words that lie 32 bytes apart.
 template <int HD>
 __global__ __launch_bounds__(kAppendT) void k_kvq_read(const KvqLayer L, const KvqRows rows, uint16_t *k_out,
                                                        uint16_t *v_out) {

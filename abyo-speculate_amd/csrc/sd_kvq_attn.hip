@@ -11,9 +11,17 @@
 // (mask and exponent, then the exact subtraction and the step, two values
 // each), so a block is about 300 VALU instructions for 4.6 KB: half of what a
 // CU can spend on its share of the memory's rate.
+// 5 rows of 32 heads over 8 and 32768 positions, 37.7 MB of blocks: 15 us, 7.8 at
+// the rate of a large copy; some 8 us are a chain that runs once.
 // More: k_kvq_wide, whose waves have 32 queries each and share the values of
-// 64 positions through LDS, expanded once for up to 256 queries.
-// Key ranges (splits) meet in k_kvq_combine.
+// 64 positions through LDS, expanded once for up to 256 queries (two key groups
+// of fewer queries halve the partial results where the context is short).
+// 2048 rows of 32 heads over 8191 positions: 290 us, 830 TFLOP/s; a large
+// product of fp16 matrices reaches 1190.  A stage of 64 positions is 2048 cycles
+// of matrix instructions and as many of VALU work (246 instructions a wave, 32
+// of them exponentials) on a SIMD, whose two waves overlap them in part.
+// Key ranges (splits) meet in k_kvq_combine (60 rows of 32 heads in 16 ranges,
+// 16 MB of fp32: 5.8 us; 5 rows in 64 ranges 4.3, most of it latency).
 #include <atomic>
 
 #include "sd_attn_dev.hpp"
@@ -31,7 +39,7 @@ constexpr int kKvqT = 256, kKvqWaves = kKvqT / 64;
 // a maximum of its scores: the largest of the scores so far weighs 2^7 or more,
 // so that a million positions of 2^-24 of its weight each still count (fp16 ends
 // at 2^-24; a weight is rounded by 2^-11 of itself, or by 2^-32 of the largest).
-// 2048 rows over 8191 positions take 295 us with it and 287 without.
+// The headroom costs the many-row kernel 3 % (2048 rows over 8191 positions).
 constexpr float kKvqHead = 7.f;
 
 // What a wave loads of one block: the words of its lane.
@@ -695,7 +703,7 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
     };
     // In an interval stage i is multiplied, stage i + 1 expanded and stage i + 2 requested.  Half of the waves, one of the
     // two of a SIMD, expand first: the matrix instructions of one wave then run beside the other's VALU work (2048 rows
-    // over 8191 positions 295 us, all expanding first some 10 us more).
+    // over 8191 positions: 3 % less time than with all expanding first).
     const bool early = NW * KG == 8 && id >= 4;
     int now = 0, next = 0;  // bit b: block b of the stage holds positions
     if (stages > 0) fetch(0);

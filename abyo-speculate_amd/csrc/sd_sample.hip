@@ -21,7 +21,8 @@
 // the bin in which the bound lies, takes that bin's entries (or, when they are
 // few, all entries down to that bin) into LDS, finds the bound among them and
 // draws: a slice by the slices' sums, then an entry of it.  k_smp_probs writes
-// the kept distribution when asked.
+// the kept distribution when asked.  (One row of 128256 with top-k 40: 6.5 us of
+// slices and 10 of draw; 60 rows of 152064 with top-p: 29 and 23.)
 //
 // A row's draw is a chain of short steps that each run once, so its time is
 // memory round trips and instruction fetches (about 0.15 us for a cache line of
@@ -169,16 +170,23 @@ enum SmpMode : int { kSmpSum = 0, kSmpTopK = 1, kSmpHist = 2 };
 // A workgroup's time is the length of its chain (one row of 128256 is 16
 // workgroups on 256 CUs) and of the code that it runs once: 1024 threads with
 // two loads of four entries each, rolled loops over the entries (32 entries a
-// thread, unrolled: 10 us for one row, 4 of them fetching the last loop's code).
+// thread, unrolled: 10 us for one row, 4 of them fetching the last loop's code;
+// now 6.5).  Many rows are bound by VALU work, some 90 instructions an entry and
+// a quarter of them f64: 60 rows of 152064 take 29 us, 8 at the rate of a large
+// copy.  The histogram's loop therefore takes two entries a turn (one: 31 us;
+// four: the same as two; entries in LDS instead of turned registers: 31).
 constexpr int kSlT = 1024, kSlPer = kSmpSlice / kSlT;
 typedef float floatx4r __attribute__((ext_vector_type(4), aligned(4)));
 
-// the next of a thread's entries into l[0]
-__device__ __forceinline__ void next_entry(float (&l)[kSlPer]) {
-    const float first = l[0];
+// the next N of a thread's entries into l[0] ..
+template <int N, typename T> __device__ __forceinline__ void turn(T (&l)[kSlPer]) {
+    T first[N];
 #pragma unroll
-    for (int k = 0; k + 1 < kSlPer; k++) l[k] = l[k + 1];
-    l[kSlPer - 1] = first;
+    for (int k = 0; k < N; k++) first[k] = l[k];
+#pragma unroll
+    for (int k = 0; k + N < kSlPer; k++) l[k] = l[k + N];
+#pragma unroll
+    for (int k = 0; k < N; k++) l[kSlPer - N + k] = first[k];
 }
 
 template <int MODE> __global__ __launch_bounds__(kSlT) void k_smp_slices(const SmpCfg p) {
@@ -234,27 +242,29 @@ template <int MODE> __global__ __launch_bounds__(kSlT) void k_smp_slices(const S
     const int top = bin_of(m, p.bins_per);
     uint64_t sum = 0;
     uint32_t at[kSlPer];  // kSmpHist: the entry's bin and its rank in it (bin << 16 | rank)
+    constexpr int kStep = MODE == kSmpHist ? 2 : 1;
 #pragma unroll 1
-    for (int i = 0; i < kSlPer; i++) {
-        uint32_t place_of = ~0u;
-        if constexpr (MODE == kSmpSum) {
-            sum += to_int(weight(l[0], m, p.c) * kOne);  // -inf weighs 0
-        } else if (l[0] > -INFINITY) {
-            const int b = min(top - bin_of(l[0], p.bins_per), kSmpBins - 1);
-            if constexpr (MODE == kSmpTopK)
-                atomicAdd(&cnt[b], 1u);
-            else
-                place_of = (uint32_t)b << 16 |
-                           ((uint32_t)atomicAdd((unsigned long long *)&hist[b],
-                                                (unsigned long long)((to_int(weight(l[0], m, p.c) * kBinOne) << kCountBits) + 1)) &
-                            ((1u << kCountBits) - 1));
-        }
-        if constexpr (MODE == kSmpHist) {
+    for (int i = 0; i < kSlPer; i += kStep) {
 #pragma unroll
-            for (int k = 0; k + 1 < kSlPer; k++) at[k] = at[k + 1];
-            at[kSlPer - 1] = place_of;
+        for (int k = 0; k < kStep; k++) {
+            if constexpr (MODE == kSmpSum) {
+                sum += to_int(weight(l[k], m, p.c) * kOne);  // -inf weighs 0
+                continue;
+            }
+            at[k] = ~0u;
+            if (l[k] > -INFINITY) {
+                const int b = min(top - bin_of(l[k], p.bins_per), kSmpBins - 1);
+                if constexpr (MODE == kSmpTopK)
+                    atomicAdd(&cnt[b], 1u);
+                else
+                    at[k] = (uint32_t)b << 16 |
+                            ((uint32_t)atomicAdd((unsigned long long *)&hist[b],
+                                                 (unsigned long long)((to_int(weight(l[k], m, p.c) * kBinOne) << kCountBits) + 1)) &
+                             ((1u << kCountBits) - 1));
+            }
         }
-        next_entry(l);
+        if constexpr (MODE == kSmpHist) turn<kStep>(at);
+        turn<kStep>(l);
     }
     if constexpr (MODE == kSmpSum) {
         sum = wave_sum(sum);
@@ -279,13 +289,10 @@ template <int MODE> __global__ __launch_bounds__(kSlT) void k_smp_slices(const S
         p.ws.hist[((int64_t)r * p.nsl + sl) * kSmpBins + t] = h;
         p.ws.first[((int64_t)r * p.nsl + sl) * kSmpBins + t] = (uint16_t)(run - c);
         __syncthreads();
-#pragma unroll 1
-        for (int i = 0; i < kSlPer; i++) {
-            if (at[0] != ~0u)
-                place[(uint32_t)hist[at[0] >> 16] + (at[0] & 0xffffu)] = (uint16_t)((i >> 2) * 4 * kSlT + 4 * t + (i & 3));
 #pragma unroll
-            for (int k = 0; k + 1 < kSlPer; k++) at[k] = at[k + 1];
-        }
+        for (int i = 0; i < kSlPer; i++)
+            if (at[i] != ~0u)
+                place[(uint32_t)hist[at[i] >> 16] + (at[i] & 0xffffu)] = (uint16_t)((i >> 2) * 4 * kSlT + 4 * t + (i & 3));
         __syncthreads();
         // (places past the finite entries are not read)
         *(uintx4 *)(p.ws.place + ((int64_t)r * p.nsl + sl) * kSmpSlice + 8 * t) = *(const uintx4 *)(place + 8 * t);
@@ -300,7 +307,7 @@ template <int MODE> __global__ __launch_bounds__(kSlT) void k_smp_slices(const S
         for (int i = 0; i < kSlPer; i++) {
             if (l[0] > -INFINITY && min(top - bin_of(l[0], p.bins_per), kSmpBins - 1) < bins)
                 cand[atomicAdd(&s_n, 1u)] = order_of(key_of(l[0]), sl * kSmpSlice + (i >> 2) * 4 * kSlT + 4 * t + (i & 3));
-            next_entry(l);
+            turn<1>(l);
         }
         __syncthreads();
         if (t == 0) *out = SmpSlice{key, 0, 0, (int)s_n, bins};

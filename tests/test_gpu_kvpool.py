@@ -496,7 +496,8 @@ def test_refusals(hip):
     b, P = ptr(buf), p.pool
     ok = dict(n=1, k=b, v=b, slots=b, table=b, n_seqs=1, table_ld=1)
     for bad in (dict(k=0), dict(v=0), dict(slots=0), dict(table=0), dict(n_seqs=0), dict(table_ld=0), dict(k=b + 2),
-                dict(q=b), dict(q=b, q_out=b + 8), dict(k_ld=64), dict(v_ld=100), dict(k_ld=132), dict(n=1 << 25)):
+                dict(q=b), dict(q=b, q_out=b + 8), dict(q=b, q_out=b), dict(k_ld=64), dict(v_ld=100), dict(k_ld=132), dict(n=1 << 25),
+                dict(n=1 << 24)):
         with pytest.raises(hip.ArgError):
             P.append(0, **dict(ok, **bad))
     with pytest.raises(hip.UnsupportedMethod):
@@ -510,11 +511,11 @@ def test_refusals(hip):
         P.read(0, 1, b, b, 1, 1, b + 2, b)
     need = P.attend_workspace(2, 1, 1, 100000)
     assert need > 0 and P.attend_workspace(2, 1, 3, 10) == 0 and P.attend_workspace(0, 1, 1, 10) == 0
-    at = dict(q=b, out=b, row_start=b, kv_len=b, table=b, n_seqs=1, table_ld=1, rows=2, max_rows=1, max_len=100000, ws=b,
+    at = dict(q=b, out=b + 32768, row_start=b, kv_len=b, table=b, n_seqs=1, table_ld=1, rows=2, max_rows=1, max_len=100000, ws=b,
               ws_bytes=need)
     for bad in (dict(q=0), dict(out=0), dict(row_start=0), dict(kv_len=0), dict(table=0), dict(n_seqs=0), dict(table_ld=0),
-                dict(max_rows=0), dict(max_rows=3), dict(ws=0), dict(ws_bytes=need - 1), dict(ws=b + 8), dict(q=b + 8),
-                dict(out=b + 4), dict(mask=b), dict(scale=float("nan")), dict(q_ld=128), dict(out_ld=255), dict(out_ld=258),
+                dict(out=b), dict(max_rows=0), dict(max_rows=3), dict(ws=0), dict(ws_bytes=need - 1), dict(ws=b + 8), dict(q=b + 8),
+                dict(out=b + 32772), dict(mask=b), dict(scale=float("nan")), dict(q_ld=128), dict(out_ld=255), dict(out_ld=258),
                 dict(n_seqs=70000), dict(max_len=1 << 40)):
         with pytest.raises(hip.ArgError):
             P.attend(0, **dict(at, **bad))

@@ -155,7 +155,7 @@ def test_refusals(hip):
         with pytest.raises(hip.SamplingError):
             s.sample(b, 1, b, b, **kw)
     for args, kw in (((0, 1, b, b), {}), ((b, 1, 0, b), {}), ((b, 1, b, 0), {}), ((b, 5, b, b), {}), ((b, 1, b, b), dict(ld=99)),
-                     ((b, 1 << 20, b, b), {})):
+                     ((b, 1 << 20, b, b), {}), ((b, 1, b, b), dict(probs=b))):
         with pytest.raises(hip.ArgError):
             s.sample(*args, **kw)
     s.sample(b, 0, b, b)
