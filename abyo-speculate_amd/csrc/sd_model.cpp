@@ -411,9 +411,12 @@ void Model::set_kv_format(int fmt) {
             SD_HIP_CHECK(hipMemcpy(kvq_table, ids.data(), ids.size() * sizeof(int), hipMemcpyHostToDevice));
         }
         if (!kvq_ws) {
+            // (a shorter context never needs more)
             size_t most = 16;
-            for (int M = 1; M <= prompt_rows; M++) most = std::max(most, pool->plan(M, 1, M, cfg.ctx_len).ws_bytes);
+            for (int M = 1; M <= std::max(prompt_rows, cfg.max_batch); M++)
+                most = std::max(most, pool->plan(M, 1, M, cfg.ctx_len).ws_bytes);
             kvq_ws = dalloc<uint8_t>(most);
+            kvq_ws_bytes = most;
         }
         SD_HIP_CHECK(hipFree(kv));
         kv = nullptr;
@@ -796,6 +799,7 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
     const double kv_bytes = 2.0 * c.n_kv_heads * (double)(P + M) * (kvq ? kvq_block_bytes(c.head_dim) / 64.0 : c.head_dim * 2.0);
     KvqPlan kvq_plan{};
     if (kvq) kvq_plan = kvq->plan(M, 1, M, P + M);
+    if (kvq_plan.ws_bytes > kvq_ws_bytes) throw BackendError("the 4-bit attention's workspace is too small");
     // up to 16 rows, with the epilogues fused, the attention's workgroups join
     // the Q/K/V launch where its shape allows (qkv_attention_fits)
     auto qa_fits = [&](const GemmParams &g, const AttnParams &at) {

@@ -153,6 +153,7 @@ class Model {
     std::unique_ptr<KvPool> kvq;
     int *kvq_table = nullptr;
     void *kvq_ws = nullptr;
+    size_t kvq_ws_bytes = 0;
 
     // sampling: made on first use, max_batch rows
     std::unique_ptr<Sampler> sampler;
