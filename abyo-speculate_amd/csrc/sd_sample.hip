@@ -764,7 +764,6 @@ __global__ __launch_bounds__(kSmpT) void k_smp_draw(const SmpCfg p) {
     const BinSource src{S, p, row, max, r, 0};
     if (p.mode == kSmpSum) {
         const Kept k{p, row, max, 0};
-        if (p.min_p > 0.0) row_sums(S, k);  // the slices' sums are of all entries
         token = draw_slices(S, k, u, total);
     } else if (p.mode == kSmpTopK) {
         // the candidates of all slices, in registers, and their counts by bin
@@ -988,8 +987,9 @@ void launch_sample(const SampleParams &in, hipStream_t st) {
     p.top_k = greedy ? 1 : in.top_k;
     p.top_p = in.top_p;
     p.min_p = in.min_p;
-    // a slice's candidates hold a top-k of up to 256 (of the whole row, so of any slice)
-    p.mode = p.top_k > 0 && p.top_k <= kSmpCand ? kSmpTopK : p.top_k > 0 || p.top_p < 1.0 ? kSmpHist : kSmpSum;
+    // A slice's candidates hold a top-k of up to 256 (of the whole row, so of any slice); histograms for the other
+    // bounds, min-p alone among them (2 rows of 128256: 21 us; the draw's one workgroup adding up its row again 60).
+    p.mode = p.top_k > 0 && p.top_k <= kSmpCand ? kSmpTopK : p.top_k > 0 || p.top_p < 1.0 || p.min_p > 0.0 ? kSmpHist : kSmpSum;
     p.u = in.u;
     p.tokens = in.tokens;
     p.probs = in.probs;

@@ -1187,7 +1187,7 @@ class HipKvPool:
         _check(_lib.sd_kvpool_read(self._h, layer, ctypes.byref(r), k_out, v_out, stream))
 
     def attend_workspace(self, rows: int, n_seqs: int, max_rows: int, max_len: int) -> int:
-        """Bytes of zeroed device memory attend() needs for these sizes."""
+        """Bytes of device memory attend() needs for these sizes; one workspace per call in flight."""
         return int(_lib.sd_kvpool_attend_workspace(self._h, rows, n_seqs, max_rows, max_len))
 
     def attend(self, layer: int, q: int, out: int, row_start: int, kv_len: int, table: int, n_seqs: int, table_ld: int,

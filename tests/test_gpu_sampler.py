@@ -67,6 +67,16 @@ def test_ties(hip, f):
     check(hip, x, [0.5, 0.25, 0.75, 0.0], **FILTERS[f])
 
 
+@pytest.mark.parametrize("V", [1, 9000, 152064])
+@pytest.mark.parametrize("min_p", [1.0, 0.5, 1e-3, 1e-9, 1e-30])
+def test_min_p_alone(hip, V, min_p):
+    """From the ties of the maximum to every entry kept: flat, ordinary and steep rows, and one of equal values."""
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal((4, V)) * np.array([[0.01], [1.0], [4.0], [0.0]])).astype(np.float32)
+    for T in (0.3, 5.0):
+        check(hip, x, rng.random(4), min_p=min_p, temperature=T)
+
+
 def test_two_near_values(hip):
     """A bin full of values that differ in their last bits only."""
     rng = np.random.default_rng(1)
