@@ -5,7 +5,7 @@
 // S^T = K Q^T, so that a lane's probabilities are its operand of O^T = V^T P^T,
 // and a running maximum and sum in f32 follow the blocks.
 //
-// Up to 32 queries of a KV head (rows times the heads that share it):
+// Up to 64 queries of a KV head (rows times the heads that share it):
 // k_kvq_attn, whose four waves take the blocks of a key range in turn, codes
 // straight from memory into registers.  A value costs two VALU operations
 // (mask and exponent, then the exact subtraction and the step, two values
@@ -15,7 +15,7 @@
 // the rate of a large copy; some 8 us are a chain that runs once.
 // More: k_kvq_wide, whose waves have 32 queries each and share the values of
 // 64 positions through LDS, expanded once for up to 256 queries (two key groups
-// of fewer queries halve the partial results where the context is short).
+// of 128 queries halve the partial results where the context is short).
 // 2048 rows of 32 heads over 8191 positions: 290 us, 830 TFLOP/s; a large
 // product of fp16 matrices reaches 1190.  A stage of 64 positions is 2048 cycles
 // of matrix instructions and as many of VALU work (246 instructions a wave, 32
@@ -220,7 +220,7 @@ __device__ __forceinline__ uintx4 kvq_weights(const float (&s)[8], float mu, flo
     return pk;
 }
 
-// ---- up to 32 queries ------------------------------------------------------------
+// ---- up to 64 queries, 16 or 32 to a workgroup ------------------------------------
 template <int HD, int QT>
 __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void k_kvq_attn(const KvqAttn p) {
     constexpr int NDC = HD / 32, NDT = HD / 16;
@@ -833,13 +833,16 @@ template <int HD> __global__ __launch_bounds__(256) void k_kvq_combine(const Kvq
     }
 }
 
-// Queries of a KV head: up to 32 in one or two tiles of 16, up to 64 in a tile
-// of 64.  More: tiles of 256 expand every value once but leave, with the splits
+// Queries of a KV head: up to 64 in tiles of 16 or 32 of the small kernel, which
+// for two tiles expands every value twice but waits for no LDS (a decoder's pass
+// of 16 rows, 32 heads over 8, 8 layers: 32768 positions 858 us, 120000 1199; in
+// a tile of 64 of the wide kernel 959 and 1438, of 128 946 and 1459).
+// More: tiles of 256 expand every value once but leave, with the splits
 // that a short context needs to fill the card, twice the partial results of
 // tiles of 128 in two key groups.  They are taken where they fill the card alone
 // or a split is more than 12 blocks long (a decoder's pass of 60 rows, 32 heads
 // over 8, 8 layers: 8192 positions 1113 us with 128 and 1126 with 256, 32768
-// 1451 and 1394; tiles of 64 lose more to expansion than they save in partials).
+// 1451 and 1394).
 // Splits: the wide kernel's workgroup has a CU to itself, the small one's four
 // waves share it with another (8 layers of 32 heads over 8, 120000 positions, one
 // row: a pass of 720 us, 763 with one to a CU; 32768 positions, 5 rows: no
@@ -850,7 +853,7 @@ KvqPlan kvq_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
     const int64_t blocks = (max_len + 31) / 32, big = (nq + 255) / 256 * n_kv * n_seqs;
-    r.tile_q = nq <= 16 ? 16 : nq <= 32 ? 32 : nq <= 64 ? 64 : nq > 128 && (big >= cus || big * blocks > 12 * cus) ? 256 : 128;
+    r.tile_q = nq <= 16 ? 16 : nq <= 64 ? 32 : nq > 128 && (big >= cus || big * blocks > 12 * cus) ? 256 : 128;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs;
     const int64_t fill = r.tile_q > 32 ? cus : n_seqs > 1 ? 8 * cus : 2 * cus;
@@ -882,7 +885,6 @@ template <int HD> static void launch_attn(const KvqAttn &p, hipStream_t st) {
     switch (p.tile_q) {
     case 16: k_kvq_attn<HD, 1><<<g, b, 0, st>>>(p); break;
     case 32: k_kvq_attn<HD, 2><<<g, b, 0, st>>>(p); break;
-    case 64: launch_wide<HD, 2, 2>(p, st); break;
     case 128: launch_wide<HD, 4, 2>(p, st); break;
     default: launch_wide<HD, 8, 1>(p, st); break;
     }
