@@ -9,8 +9,9 @@
 //          sum of the kept
 // Weights are computed in f64 and summed as integers, so no sum depends on an
 // order: of 2^-44 in the sums that a token is drawn from, of 2^-36 in the
-// histograms (a decision can differ from exact arithmetic only within about
-// 1e-11 of a border, for top-p V * 2^-37 of the sum at worst).
+// histograms.  A rounded sum of V weights loses at most half a unit for each, so
+// a decision can differ from exact arithmetic only within V * 2^-45 of the sum
+// (with histograms V * 2^-37) of a border, usually within the 1e-11 of a weight.
 //
 // Both top-k and top-p keep a prefix of the order (value descending, index
 // ascending), so together they are one bound on the pair (value, index).  Two
@@ -41,7 +42,7 @@ constexpr double kOne = 17592186044416.0;  // 2^44
 // A histogram word: the bin's weight in units of 2^-36 above 14 bits of its
 // count (8192 weights of at most 1 make 49 bits).
 constexpr double kBinOne = 68719476736.0;  // 2^36
-constexpr int kCountBits = 14;
+constexpr int kCountBits = 14, kFactorBits = 8;  // kOne / kBinOne: 2^8
 
 // Per slice: the largest entry's order key, whether an entry is NaN or +inf,
 // the sum of the weights relative to the slice's maximum (kSmpSum), the entries
@@ -504,16 +505,16 @@ __device__ __forceinline__ uint64_t select_list(SmpShared &S, int n, uint64_t le
     return select(S, ListSource{S, n, least}, by_mass, target, shift, some >> (shift + 8));
 }
 
-// The weight of an entry if it is kept.
+// The weight of an entry if it is kept, `one` units for a weight of 1.
 struct Kept {
     const SmpCfg &p;
     const float *row;
     float max;
     uint64_t cut;
-    __device__ __forceinline__ uint64_t mass(int i, float l) const {
+    __device__ __forceinline__ uint64_t mass(int i, float l, double one = kOne) const {
         if (l == -INFINITY || order_of(key_of(l), i) < cut) return 0;
         const double w = weight(l, max, p.c);
-        return w >= p.min_p ? to_int(w * kOne) : 0;
+        return w >= p.min_p ? to_int(w * one) : 0;
     }
 };
 // the slices' kept weights from the row itself, a slice to a wave, into S.smass
@@ -551,6 +552,11 @@ __device__ __forceinline__ uint64_t draw_target(float u, uint64_t sum) {
 // The draw: a slice by the slices' sums, then the first of its entries whose
 // running kept weight reaches what is left of the target (the last kept one
 // where rounded sums leave more than the slice has).
+// A slice may be far below the row's maximum (its sum some units of 2^-44, each
+// of its entries less than half a unit), so inside it weights and target are
+// in units of 2^-44 of its maximum's power of two: the maximum, which is
+// kept where anything of the slice is, weighs 2^44 or more, and a slice that
+// is picked always has an entry to give.
 __device__ __forceinline__ int draw_slices(SmpShared &S, const Kept &k, float u, uint64_t &total) {
     const int t = threadIdx.x, lane = t & 63;
     const uint64_t sm = lane < k.p.nsl ? S.smass[lane & (kMaxSlices - 1)] : 0, sr = wave_run(sm);
@@ -560,6 +566,12 @@ __device__ __forceinline__ int draw_slices(SmpShared &S, const Kept &k, float u,
     if (!hit) hit = 1;  // no weight at all
     const int pick = __ffsll((unsigned long long)hit) - 1;
     target -= min(__shfl(sr - sm, pick), target - 1);
+    // its maximum's exponent, from the factor of its sums; a sum of a unit or more has a maximum of 2^-58 or more (8192
+    // entries, half a unit lost to rounding)
+    const int e = (int)(__builtin_bit_cast(uint64_t, S.f[pick]) >> 52) - (k.p.mode == kSmpHist ? kFactorBits : 0);
+    const int down = min(1023 - e, 58);
+    const double one = __builtin_bit_cast(double, (uint64_t)(1023 + 44 + down) << 52);
+    target = ((target - 1) << down) + 1;
     // eight entries to a thread, in order
     const int x0 = pick * kSmpSlice + 8 * t, len = k.p.V - x0;
     float l[8];
@@ -575,7 +587,7 @@ __device__ __forceinline__ int draw_slices(SmpShared &S, const Kept &k, float u,
     uint64_t mine = 0, m[8];
 #pragma unroll 1
     for (int e = 0; e < 8; e++) {
-        const uint64_t w = k.mass(x0 + e, l[0]);
+        const uint64_t w = k.mass(x0 + e, l[0], one);
         mine += w;
 #pragma unroll
         for (int i = 0; i < 7; i++) l[i] = l[i + 1], m[i] = m[i + 1];

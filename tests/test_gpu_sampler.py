@@ -172,3 +172,33 @@ def test_refusals(hip):
     s.close()
     with pytest.raises(hip.ArgError):
         s.sample(b, 1, b, b)
+
+
+def far_rows(V, first, rest=-200.0):
+    """A row whose slices but the last lie `first` below its maximum (8192 entries each), the last one's single 0 apart."""
+    x = np.full((1, V), rest, np.float32)
+    for s, at in enumerate(first):
+        x[0, 8192 * s:8192 * (s + 1)] = at
+    x[0, V - 5] = 0.0
+    return x
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(min_p=1e-30), dict(top_k=9000), dict(top_p=1 - 2.0 ** -24), dict(temperature=0.05),
+                                dict(temperature=0.05, min_p=1e-30), dict(top_k=40)])
+@pytest.mark.parametrize("first", [[-32.0], [-31.5], [-31.0, -31.9], [-36.0, -31.9], [-40.0], [-40.0, -31.2, -38.5], [-300.0, -31.4]])
+def test_draws_from_slices_far_below_the_maximum(hip, first, kw):
+    """Small uniforms lead to slices none of whose entries weighs 2^-45 of the row's maximum: still an entry that is kept, and the
+    rule's own but for what sums lose.  Each of V weights is rounded to 2^-44 of the row's maximum, half a unit: V 2^-45 of the
+    sum, which is at least 1; where histograms add them up, to 2^-36 of the slice's maximum: V 2^-37.  The weights themselves
+    are within 1e-11."""
+    T = kw.get("temperature", 1.0)
+    x = far_rows(8192 * (len(first) + 1), [a * T for a in first], -200.0 * T)
+    u = np.array([0.0, 1e-14, 1e-12, 1e-11, 5e-11, 0.25], np.float32)
+    tol = x.shape[1] * 2.0 ** (-45 if set(kw) <= {"temperature"} or kw.get("top_k") == 40 else -37) + 1e-11
+    tok, pr = draw(hip, np.repeat(x, len(u), 0), u, **kw)
+    for r in range(len(u)):
+        p = _kvq.sample(x[0], u[r], **dict(dict(temperature=1.0), **kw))[1]
+        c = np.cumsum(p)
+        assert 0 <= tok[r] < x.shape[1], (r, tok[r])
+        assert p[tok[r]] > 0 and pr[r, tok[r]] > 0
+        assert c[tok[r]] - p[tok[r]] <= u[r] + tol and c[tok[r]] >= u[r] - tol, (r, tok[r])
