@@ -802,7 +802,11 @@ __global__ __launch_bounds__(kSmpT) void k_smp_draw(const SmpCfg p) {
         }
         const int hi = S.n, few = (int)S.count[hi];
         const int s = lane & (kMaxSlices - 1);
-        const bool whole = few <= kSmpList && __ballot(s < p.nsl && S.shift[s] >= 0 && hi - S.shift[s] >= S.bins[s]) == 0;
+        // A slice's entries down to hi are all listed (the row's last bin takes what lies below it, however far down), or
+        // top_k of its largest are, and what it does not list is none of the row's top_k.
+        const int need = hi == kSmpBins - 1 ? kSmpBins : hi - S.shift[s] + 1;
+        const bool short_of = s < p.nsl && S.shift[s] >= 0 && need > S.bins[s] && S.n_in[s] < p.top_k;
+        const bool whole = few <= kSmpList && __ballot(short_of) == 0;
         const bool p_on = p.top_p < 1.0;
         __syncthreads();
         if (t == 0) S.n = 0;

@@ -202,3 +202,30 @@ def test_draws_from_slices_far_below_the_maximum(hip, first, kw):
         assert 0 <= tok[r] < x.shape[1], (r, tok[r])
         assert p[tok[r]] > 0 and pr[r, tok[r]] > 0
         assert c[tok[r]] - p[tok[r]] <= u[r] + tol and c[tok[r]] >= u[r] - tol, (r, tok[r])
+
+
+@pytest.mark.parametrize("top_k", [11, 40, 256])
+@pytest.mark.parametrize("spread", [0.0, 0.001, 3.0])
+@pytest.mark.parametrize("slices", [2, 5])
+def test_top_k_reaches_slices_far_below(hip, top_k, spread, slices):
+    """Fewer finite entries near the maximum than top-k: the rest come, in order, from slices more than 32 nats below."""
+    rng = np.random.default_rng(top_k + slices)
+    x = np.full((2, 8192 * slices), -np.inf, np.float32)
+    x[:, 100:110] = rng.standard_normal((2, 10))
+    for s in range(1, slices):
+        x[:, 8192 * s + 7:8192 * s + 307] = -40.0 - s + spread * rng.random((2, 300))
+    check(hip, x, [0.3, 0.9], top_k=top_k)
+    check(hip, x, [0.3, 0.9], top_k=top_k, temperature=0.5)
+    check(hip, x, [0.3, 0.9], top_k=top_k, top_p=0.9)
+
+
+@pytest.mark.parametrize("top_k", [1, 40, 256])
+@pytest.mark.parametrize("V", [20000, 128256])
+def test_top_k_of_sharp_rows(hip, top_k, V):
+    """At low temperatures nearly all of a row, and all but a few of its top-k, lie more than 32 nats below its maximum."""
+    rng = np.random.default_rng(top_k + V)
+    x = (rng.standard_normal((3, V)) * 2).astype(np.float32)
+    x[0, 17] = x[1, V - 1] = 30.0
+    x[2, 9000:9300] = 7.0  # more than a slice lists in one bin
+    for T in (0.05, 0.2):
+        check(hip, x, rng.random(3), top_k=top_k, temperature=T)
