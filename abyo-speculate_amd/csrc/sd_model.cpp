@@ -1347,6 +1347,10 @@ void Decoder::next_logits(float *out) {
 void Decoder::batched_logits(const uint32_t *drafts, size_t k, float *out) {
     if (k == 0) {
         next_logits(out);
+        // the pass's one row, whatever pass (of more rows, perhaps) left it
+        launch_argmax_rows(model->last_row, model->cfg.vocab, model->cfg.vocab, 1, model->argmax, model->st);
+        model->logits_rows_last = 1;
+        model->rows_last = model->last_row;
         return;
     }
     if (history.empty()) throw SamplingError("batched_logits with empty history");
@@ -1580,11 +1584,6 @@ void Decoder::verify_greedy_linear(const uint32_t *drafts, size_t k, uint32_t *c
                                    size_t *n_accepted) {
     batched_logits(drafts, k, nullptr);
     std::vector<int32_t> am(k + 1);
-    if (k == 0) {
-        launch_argmax_rows(model->last_row, model->cfg.vocab, model->cfg.vocab, 1, model->argmax, model->st);
-        model->logits_rows_last = 1;
-        model->rows_last = model->last_row;
-    }
     argmax_rows(am.data(), k + 1);
     size_t a = 0;
     while (a < k && (uint32_t)am[a] == drafts[a]) a++;
@@ -1853,8 +1852,6 @@ void Decoder::verify_rejection_linear(const uint32_t *drafts, size_t k, const fl
     if (k == 0) {
         // next_logits left the row in last_row; the walk reads logits row 0
         SD_HIP_CHECK(hipMemcpyAsync(m.logits, m.last_row, (size_t)m.cfg.vocab * 4, hipMemcpyDeviceToDevice, m.st));
-        m.logits_rows_last = 1;
-        m.rows_last = m.logits;
     }
     const int n = (int)k + 1;
     std::vector<int> parents(n), tokens(n), qrow(n);

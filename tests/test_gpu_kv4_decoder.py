@@ -259,3 +259,22 @@ def test_sampled_decoding_over_a_4_bit_cache(hip):
     d.rollback_to(n0)
     b = d.verify_rejection_linear(drafts, q, uni, 1.0)
     assert a == b
+
+
+@pytest.mark.parametrize("q4", [False, True])
+def test_a_verify_pass_without_drafts_is_the_last_pass(hip, q4):
+    """batched_logits of no drafts gives one row, the next token's: that row is what sample_rows and last_argmax then see,
+    not the first of the pass before."""
+    ocfg = oracle_cfg(**SHAPES["llama"])
+    d, V = decoder(hip, ocfg, q4), ocfg.vocab
+    d.observe(ids(14, 50, V))
+    rows = d.batched_logits(ids(15, 4, V))
+    us = [0.05, 0.35, 0.65, 0.95]
+    want, stale = ([_kvq.sample(rows[i], u, 1.0)[0] for u in us] for i in (4, 0))
+    assert want != stale and np.argmax(rows[0]) != np.argmax(rows[4])
+    assert np.array_equal(d.batched_logits([])[0], rows[4])
+    assert [d.sample_rows([u])[0] for u in us] == want
+    assert int(d.last_argmax(1)[0]) == int(np.argmax(rows[4]))
+    for call in (lambda: d.sample_rows([0.5, 0.5]), lambda: d.last_argmax(2)):
+        with pytest.raises(hip.ArgError):
+            call()
