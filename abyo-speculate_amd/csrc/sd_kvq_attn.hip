@@ -23,6 +23,7 @@
 // Key ranges (splits) meet in k_kvq_combine (60 rows of 32 heads in 16 ranges,
 // 16 MB of fp32: 5.8 us; 5 rows in 64 ranges 4.3, most of it latency).
 #include <atomic>
+#include <type_traits>
 
 #include "sd_attn_dev.hpp"
 #include "sd_kvq_dev.hpp"
@@ -288,7 +289,12 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
             for (int t = 0; t < QT; t++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) st[t][j] = acc[t][j >> 2][j & 3] * sl2;
+                for (int j = 0; j < 8; j++) {
+                    // rounded here, not inside the weight: beyond 2^28 the rounding is more than fp16 has room for, so what is
+                    // weighed must be what the maximum is taken of
+#pragma clang fp contract(off)
+                    st[t][j] = acc[t][j >> 2][j & 3] * sl2;
+                }
         }
         uint32_t bad = 0, vis[QT];
         if (!full) {
@@ -311,11 +317,12 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
             float top = st[t][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) top = fmaxf(top, st[t][j]);
-            // the reference moves only for a score that would weigh more than 2^15
-            if (__builtin_amdgcn_ballot_w64(top > m[t] + 15.f) != 0) {
-                const float cm = xmax4(top) - kKvqHead;
-                if (cm > m[t] + 15.f - kKvqHead) {
-                    const float alpha = __builtin_amdgcn_exp2f(m[t] - cm);
+            // The reference moves only for a score that would weigh more than 2^15.  By the difference, which is exact for
+            // neighbouring scores: beyond 2^27 the reference and 15 add up to the score that is 16 above it.
+            if (__builtin_amdgcn_ballot_w64(top - m[t] > 15.f) != 0) {
+                const float tm = xmax4(top);
+                if (tm - m[t] > 15.f) {
+                    const float cm = tm - kKvqHead, alpha = __builtin_amdgcn_exp2f(m[t] - cm);
                     m[t] = cm;
                     l[t] *= alpha;
 #pragma unroll
@@ -567,16 +574,20 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
                 for (int j = 0; j < 16; j++) o[t][j] *= alpha;
         }
     };
-    // fp16 weights of a block's scores and their sum
-    auto weigh = [&](const floatx16 &st, uintx4 (&pk)[2]) {
+    // fp16 weights of a block's scores and their sum; with `rounded` of the scaled scores as raise() compares them, else in
+    // one fused operation each
+    auto weigh = [&](const floatx16 &st, uintx4 (&pk)[2], auto rounded) {
         const float mu = m == -INFINITY ? 0.f : m;
         float sum = 0.f;
+        auto weight = [&](float s) {
+#pragma clang fp contract(off)
+            return __builtin_amdgcn_exp2f(decltype(rounded)::value ? s * sl2 - mu : __builtin_fmaf(s, sl2, -mu));
+        };
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float x = __builtin_amdgcn_exp2f(st[8 * c + 2 * j] * sl2 - mu);
-                const float y = __builtin_amdgcn_exp2f(st[8 * c + 2 * j + 1] * sl2 - mu);
+                const float x = weight(st[8 * c + 2 * j]), y = weight(st[8 * c + 2 * j + 1]);
                 sum += x + y;
                 pk[c][j] = h2bits(half2v{(_Float16)x, (_Float16)y});
             }
@@ -584,8 +595,10 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
     };
     // A stage: the products of one block run beside the softmax of the other.  No maximum is looked for: a query
     // keeps the reference of its first block until its weights add up to more than 2^15 in half a block (they stay
-    // below fp16's range); then the reference is raised and they are taken again.
-    constexpr float kMost = 32768.f;
+    // below fp16's range); then the reference is raised and they are taken again.  A fused weight is of the unrounded
+    // score, which beyond 2^28 may lie more than 16 from the rounded one that the reference came from, past fp16's end
+    // on either side: where the reference is beyond 2^24, weights are always taken again, of the rounded scores.
+    constexpr float kMost = 32768.f, kFused = 16777216.f;
     auto multiply = [&](const KvqStage<HD> &S, int base, bool first, bool second) {
         const bool full = first && second && base + 64 <= t_all;
         floatx16 st[2];
@@ -629,7 +642,7 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
         // scores of block 1 beside the weights of block 0
         __builtin_amdgcn_sched_barrier(0);
         scores(1);
-        float sum = weigh(st[0], pk[0]);
+        float sum = weigh(st[0], pk[0], std::false_type{});
         __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
@@ -638,16 +651,16 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
             if (c + 4 < NC) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (__builtin_amdgcn_ballot_w64(sum > kMost || m == -INFINITY) != 0) {
+        if (__builtin_amdgcn_ballot_w64(sum > kMost || !(fabsf(m) < kFused)) != 0) {
             raise(st[0]);
-            sum = weigh(st[0], pk[0]);
+            sum = weigh(st[0], pk[0], std::true_type{});
         }
         l += sum;
         mask(1);
         // values of block 0 beside the weights of block 1
         __builtin_amdgcn_sched_barrier(0);
         values(0);
-        sum = weigh(st[1], pk[1]);
+        sum = weigh(st[1], pk[1], std::false_type{});
         __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
 #pragma unroll
         for (int c = 0; c < 2 * NT; c++) {
@@ -656,9 +669,9 @@ __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(2)
             if (c + 4 < 2 * NT) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (__builtin_amdgcn_ballot_w64(sum > kMost || m == -INFINITY) != 0) {
+        if (__builtin_amdgcn_ballot_w64(sum > kMost || !(fabsf(m) < kFused)) != 0) {
             raise(st[1]);
-            sum = weigh(st[1], pk[1]);
+            sum = weigh(st[1], pk[1], std::true_type{});
         }
         l += sum;
         __builtin_amdgcn_sched_barrier(0);

@@ -526,3 +526,70 @@ def test_refusals(hip):
     P.close()
     with pytest.raises(hip.ArgError):
         P.append(0, **ok)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,H", [(1, 1), (1, 20), (5, 8), (20, 4), (60, 4), (300, 1)])
+@pytest.mark.parametrize("T", [40, 1000])
+def test_attention_scores_near_the_formats_end(hip, hd, rows, H, T):
+    """Queries and keys of 65504 and a little less in one channel: scores of some 5e8, whose fp32 neighbours are 32 or 64 apart.
+    A position that is alone at the top is the answer, positions that share it are averaged; nothing overflows."""
+    T = max(T, rows)
+    p = Pool(hip, hd + rows, H, 1, hd, [T], page=32)
+    rng = np.random.default_rng(hd + rows + T)
+    k = np.zeros((T, 1, hd), np.float16)
+    k[:, 0, 3] = rng.integers(0, 3, T) * 32 + 65408  # 65408, 65440, 65472
+    k[:, 0, 40] = rng.standard_normal(T)
+    v = rng.integers(-7, 8, (T, 1, hd)).astype(np.float16)
+    v[:, 0, 5] = 0
+    v[:, 0, ::32] = 8  # steps of 1: the values are stored as they are
+    top, low = T - rows, max(0, T - rows - 17)  # seen by every row
+    k[top, 0, 3] = 65504
+    p.append(k, v, [0] * T, range(T), pos=[0] * T)
+    q = np.zeros((rows, H, hd), np.float16)
+    half = 2.0 ** -11  # an fp16 rounding: of a weight, of the result
+    for big in (4096.0, 60000.0, 65504.0):
+        q[:, :, 3] = big
+        got = p.attend(q, [rows]).astype(np.float64)
+        want = v[top, 0].astype(np.float64)
+        assert np.all(np.abs(got - want) <= 2.01 * half * np.abs(want)), big
+    # two at the top, in blocks of their own where there is room
+    k[low, 0, 3] = 65504
+    k[:, 0, 40] = 0
+    p.append(k, v, [0] * T, range(T), pos=[0] * T)
+    got = p.attend(q, [rows]).astype(np.float64)
+    both = v[[top, low], 0].astype(np.float64)
+    assert np.all(np.abs(got - both.mean(0)) <= 1.01 * half * (np.abs(both.mean(0)) + np.abs(both).mean(0)))
+    # all positions alike, far below zero: their mean
+    k[:] = 0
+    k[:, 0, 3] = 65504
+    p.append(k, v, [0] * T, range(T), pos=[0] * T)
+    q[:, :, 3] = -65504.0
+    got = p.attend(q, [rows]).astype(np.float64)
+    for r in range(rows):
+        n = T - rows + r + 1
+        seen = v[:n, 0].astype(np.float64)
+        # besides, fp32 sums of up to n terms of up to 8, and the result below fp16's normal range
+        tol = 1.01 * half * (np.abs(seen.mean(0)) + np.abs(seen).mean(0)) + n * 2.0 ** -24 * 8 + 2.0 ** -25
+        assert np.all(np.abs(got[r] - seen.mean(0)) <= tol), r
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,H", [(1, 1), (5, 8), (20, 4), (60, 4), (300, 1)])
+def test_attention_a_later_score_one_fp32_step_higher(hip, hd, rows, H):
+    """Products of 2^30 and 2^30 + 128: scores of some 1.9e8 and 1.4e8, whose fp32 neighbours are 16 apart, one step from each
+    other.  In any rounding the second weighs 2^8 times the first or more (they are 23 and 16 apart, less half a step)."""
+    T = max(200, rows + 200)
+    p = Pool(hip, hd * rows, H, 1, hd, [T], page=32)
+    k, v = np.zeros((T, 1, hd), np.float16), np.zeros((T, 1, hd), np.float16)
+    k[[0, 130], 0, 1] = 2.0 ** 15
+    k[130, 0, 33] = 8.0
+    v[0, 0, 7], v[130, 0, 9] = 7.0, 5.0
+    p.append(k, v, [0] * T, range(T), pos=[0] * T)
+    q = np.zeros((rows, H, hd), np.float16)
+    q[:, :, 1], q[:, :, 33] = 2.0 ** 15, 16.0
+    got = p.attend(q, [rows]).astype(np.float64)
+    assert np.all(np.abs(got[..., 9] - 5.0) <= 5.0 * (2.0 ** -8 + 2.01 * 2.0 ** -11)), float(got[..., 9].min())
+    assert np.all((got[..., 7] >= 0) & (got[..., 7] <= 7.0 * 2.0 ** -8))
+    got[..., [7, 9]] = 0
+    assert not got.any()
