@@ -136,10 +136,13 @@ __device__ inline float norm_inv_rms(const float *ssq_row, int np, int K, float 
 
 }  // namespace sd
 
+// A failed call is the exception's to report: the runtime's copy of the error is
+// taken too, or the check behind the next launch would find it there.
 #define SD_HIP_CHECK(expr)                                                        \
     do {                                                                          \
         hipError_t _e = (expr);                                                   \
         if (_e != hipSuccess) {                                                   \
+            (void)hipGetLastError();                                              \
             throw sd::BackendError(std::string(#expr) + ": " + hipGetErrorString(_e)); \
         }                                                                         \
     } while (0)

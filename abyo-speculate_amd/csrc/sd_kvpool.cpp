@@ -43,7 +43,6 @@ KvPool::KvPool(const KvPoolCfg &c) : cfg(c) {
     } catch (...) {
         for (void *p : {(void *)mem, (void *)cos_t, (void *)sin_t})
             if (p) (void)hipFree(p);
-        (void)hipGetLastError();
         throw;
     }
 }

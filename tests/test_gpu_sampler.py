@@ -1,9 +1,11 @@
 """Filtered sampling (sd_sampler_*) against a 64-bit restatement: tokens equal, distributions to an fp32 rounding."""
+import ctypes
+
 import numpy as np
 import pytest
 
 import _kvq
-from _devmem import Graph, Stream, dev, full, ptr, zeros
+from _devmem import Dev, Graph, Stream, dev, full, ptr, runtime, zeros
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +231,28 @@ def test_top_k_of_sharp_rows(hip, top_k, V):
     x[2, 9000:9300] = 7.0  # more than a slice lists in one bin
     for T in (0.05, 0.2):
         check(hip, x, rng.random(3), top_k=top_k, temperature=T)
+
+
+def test_a_refused_handle_leaves_no_error_behind(hip):
+    """A handle that cannot be made says so once: the runtime's last error is clear and the next launch is taken."""
+    rt = runtime()
+    x = np.random.default_rng(6).standard_normal((1, 500)).astype(np.float32)
+    s = hip.HipSampler(500, 1)
+
+    def refused(make):
+        with pytest.raises(hip.BackendError):
+            make()
+        tok, _ = draw(hip, x, [0.5], sampler=s)
+        assert tok[0] == _kvq.sample(x[0], 0.5, 1.0)[0]
+        assert rt.hipGetLastError() == 0
+
+    refused(lambda: hip.HipSampler(500, 1, device=9999))
+    refused(lambda: hip.HipKvPool(n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, n_pages=1, device=9999))
+    # memory that is not there: 60 GB where 30 are left
+    free, total = ctypes.c_size_t(), ctypes.c_size_t()
+    assert rt.hipMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+    if free.value < 80 << 30:
+        pytest.skip("less than 80 GiB of GPU memory free")
+    held = Dev(free.value - (30 << 30), np.uint8)
+    refused(lambda: hip.HipSampler(262144, 65535))
+    del held
