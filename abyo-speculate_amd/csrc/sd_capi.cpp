@@ -950,7 +950,6 @@ sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, 
         a.rows = kv_rows(rows);
         if (fmt != SD_F16 && fmt != SD_F32) throw sd::UnsupportedError("append: rows must be F16 or F32");
         if (!k || !v || (q && !q_out)) throw sd::ArgError("null argument");
-        if (q && (const void *)q_out == q) throw sd::ArgError("q_out must not be q");
         const int size = fmt == SD_F32 ? 4 : 2, hd = P.cfg.head_dim;
         a.L = P.layer(layer);
         a.pos = pos;
@@ -972,7 +971,14 @@ sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, 
         if (q) need_aligned(q, a.q_ld * size, 16, "q");
         need_aligned(k, a.k_ld * size, 16, "k");
         need_aligned(v, a.v_ld * size, 16, "v");
-        if (q) need_aligned(q_out, 16, 16, "q_out");
+        if (q) {
+            need_aligned(q_out, 16, 16, "q_out");
+            const int64_t n = a.rows.n, qb = (int64_t)P.cfg.n_heads * hd, kb = (int64_t)P.cfg.n_kv_heads * hd * size;
+            const sd::RowBytes out{q_out, qb * 2, qb * 2, n};
+            if (rows_meet(out, {q, a.q_ld * size, qb * size, n}) || rows_meet(out, {k, a.k_ld * size, kb, n}) ||
+                rows_meet(out, {v, a.v_ld * size, kb, n}))
+                throw sd::ArgError("q_out must not overlap q, k or v");
+        }
         sd::DeviceScope dev(P.cfg.device);
         sd::launch_kvq_append(a, (hipStream_t)stream);
     });
@@ -1012,7 +1018,6 @@ sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *qy, v
         if (qy->rows == 0) return;
         if (!qy->q || !qy->out || !qy->row_start || !qy->kv_len || !qy->table) throw sd::ArgError("null argument");
         if (qy->n_seqs < 1 || qy->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
-        if (qy->out == qy->q) throw sd::ArgError("out must not be q");
         if (qy->mask && qy->mask_words < 1) throw sd::ArgError("mask_words must be positive");
         const size_t most = (size_t)1 << 40;
         const sd::KvqPlan plan = P.plan((int64_t)std::min(qy->rows, most), qy->n_seqs, (int64_t)std::min(qy->max_rows, most),
@@ -1031,6 +1036,11 @@ sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *qy, v
         a.out_ld = row_stride(qy->out_ld, (int64_t)P.cfg.n_heads * hd, "out");
         need_aligned(a.q, a.q_row * 2, 16, "q");
         need_aligned(a.out, a.out_ld * 2, 8, "out");
+        const int64_t row = (int64_t)P.cfg.n_heads * hd * 2;
+        const sd::RowBytes q{a.q, a.q_row * 2, row, (int64_t)qy->rows}, out{a.out, a.out_ld * 2, row, (int64_t)qy->rows};
+        const sd::RowBytes work{ws, 0, (int64_t)plan.ws_bytes, 1};
+        if (rows_meet(q, out) || rows_meet(q, work) || rows_meet(out, work))
+            throw sd::ArgError("attend: q, out and the workspace must not overlap");
         a.rows = (int)qy->rows;
         a.n_seqs = qy->n_seqs;
         a.row_start = qy->row_start;

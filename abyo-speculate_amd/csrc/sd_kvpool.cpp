@@ -16,6 +16,20 @@ DeviceScope::~DeviceScope() {
     if (prev >= 0) (void)hipSetDevice(prev);
 }
 
+bool rows_meet(const RowBytes &a, const RowBytes &b) {
+    if (!a.at || !b.at || a.n < 1 || b.n < 1 || a.row < 1 || b.row < 1) return false;
+    // (a stride of 2^42 bytes times 2^24 rows passes 64 bits)
+    typedef unsigned __int128 wide;
+    auto start = [](const RowBytes &x, int64_t i) { return (wide)(uintptr_t)x.at + (wide)i * (wide)x.ld; };
+    if (start(a, a.n - 1) + a.row <= start(b, 0) || start(b, b.n - 1) + b.row <= start(a, 0)) return false;
+    for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
+        const wide ea = start(a, i) + a.row, eb = start(b, j) + b.row;
+        if (start(a, i) < eb && start(b, j) < ea) return true;
+        (ea < eb ? i : j)++;
+    }
+    return false;
+}
+
 KvPool::KvPool(const KvPoolCfg &c) : cfg(c) {
     if (c.n_layers < 1 || c.n_heads < 1 || c.n_kv_heads < 1 || c.n_pages < 1) throw ArgError("kvpool: all sizes must be positive");
     if (c.n_heads % c.n_kv_heads) throw ArgError("kvpool: n_heads must be a multiple of n_kv_heads");
@@ -113,7 +127,9 @@ void Sampler::run(SampleParams p, hipStream_t st) {
     if (!p.logits || !p.u || !p.tokens) throw ArgError("sampler: null argument");
     if (p.ld == 0) p.ld = vocab;
     if (p.ld < vocab) throw ArgError("sampler: rows overlap (ld < vocab)");
-    if (p.probs == p.logits) throw ArgError("sampler: probs must not be the logits");
+    const int64_t row = (int64_t)vocab * sizeof(float);
+    if (rows_meet({p.probs, row, row, p.rows}, {p.logits, p.ld * (int64_t)sizeof(float), row, p.rows}))
+        throw ArgError("sampler: probs must not overlap the logits");
     DeviceScope dev(device);
     p.V = vocab;
     p.ws = ws;

@@ -25,6 +25,14 @@ class DeviceScope {
     int prev = -1;
 };
 
+// Whether two sets of rows (n rows of `row` bytes, `ld` bytes apart) have a byte
+// in common.  Rows of one buffer may lie between the other's.
+struct RowBytes {
+    const void *at;
+    int64_t ld, row, n;
+};
+bool rows_meet(const RowBytes &a, const RowBytes &b);
+
 // The pages of every layer in one allocation.
 class KvPool {
   public:

@@ -439,9 +439,10 @@ typedef struct sd_kv_rows {
 /* Appends k and v [n][n_kv_heads][head_dim] (fmt SD_F16 or SD_F32, row strides
  * k_ld and v_ld elements, 0: dense) to a layer: k rotated to pos[r] (slot[r]
  * with pos NULL), both quantised.  With q [n][n_heads][head_dim], the rotated
- * queries go to q_out [n][n_heads][head_dim] fp16, which overlaps no input; q
- * NULL: keys and values only.  Rows at a rotation position outside [0, max_pos) are padding.  Rows
- * must start at multiples of 16 bytes. */
+ * queries go to q_out [n][n_heads][head_dim] fp16, which overlaps none of the
+ * rows of q, k and v (SD_ERR_ARG); q NULL: keys and values only.  Rows at a
+ * rotation position outside [0, max_pos) are padding.  Rows must start at
+ * multiples of 16 bytes. */
 sd_status sd_kvpool_append(sd_kvpool *c, int32_t layer, const sd_kv_rows *rows, int32_t fmt, const void *q, size_t q_ld,
                            const void *k, size_t k_ld, const void *v, size_t v_ld, const int32_t *pos, uint16_t *q_out,
                            void *stream);
@@ -481,7 +482,8 @@ typedef struct sd_kv_query {
 size_t sd_kvpool_attend_workspace(const sd_kvpool *c, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len);
 /* ws: device memory of at least that many bytes, 16-byte aligned, whatever it
  * holds; each call in flight needs its own, and two graphs that may run at once
- * must not share one.  out overlaps neither q nor ws. */
+ * must not share one.  q's rows, out's rows (between which q's may lie) and the
+ * bytes of ws that the call needs do not overlap (SD_ERR_ARG). */
 sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *query, void *ws, size_t ws_bytes,
                            void *stream);
 
@@ -524,10 +526,10 @@ sd_status sd_sampler_create(int32_t vocab, int32_t max_rows, int32_t device, sd_
 void sd_sampler_destroy(sd_sampler *s);
 /* logits f32 [rows] of stride ld (0: vocab), uniforms f32 [rows] in [0, 1),
  * tokens int32 [rows], probs f32 [rows][vocab] (the filtered distributions,
- * e.g. the draft rows of sd_verify_rejection_*_device_q; not the logits' own
- * memory) or NULL: device memory of the handle's GPU.  Enqueues on `stream` (NULL: the default
- * stream); allocates nothing and can be captured.  SD_ERR_SAMPLING for
- * filters out of range. */
+ * e.g. the draft rows of sd_verify_rejection_*_device_q; overlapping no row of
+ * the logits, SD_ERR_ARG) or NULL: device memory of the handle's GPU.  Enqueues
+ * on `stream` (NULL: the default stream); allocates nothing and can be captured.
+ * SD_ERR_SAMPLING for filters out of range. */
 sd_status sd_sampler_run(sd_sampler *s, const float *logits, size_t ld, size_t rows, const sd_sampling *params,
                          const float *uniforms, int32_t *tokens, float *probs, void *stream);
 

@@ -593,3 +593,49 @@ def test_attention_a_later_score_one_fp32_step_higher(hip, hd, rows, H):
     assert np.all((got[..., 7] >= 0) & (got[..., 7] <= 7.0 * 2.0 ** -8))
     got[..., [7, 9]] = 0
     assert not got.any()
+
+
+def test_overlapping_rows_are_refused(hip):
+    """Outputs that share a byte with an input or the workspace, at either end or between strided rows; rows that lie between
+    another's are taken."""
+    H, KV, hd, n, T = 4, 2, 64, 5, 2000  # (shorter ones need no workspace)
+    p = Pool(hip, 91, H, KV, hd, [T], page=64)
+    (kv,) = p.fill()
+    P, w, kw = p.pool, 2 * H * hd, 2 * KV * hd  # bytes of a query's and of a key's row
+    slots = dev(np.arange(n, dtype=np.int32))
+    buf = zeros(1 << 20, np.uint8)
+    at = ptr(buf) + (1 << 19)  # q; k, v and the outputs around it
+    far = dict(k=at + 65536, v=at + 131072)
+
+    def append(**k):
+        P.append(0, n, **dict(dict(far, slots=ptr(slots), table=ptr(p.dtable), n_seqs=1, table_ld=p.table.shape[1], q=at), **k))
+    for out in (at, at + 16, at + n * w - 16, at - n * w + 16, far["k"] + kw, far["v"] + n * kw - 16, far["k"] - n * w + 16):
+        with pytest.raises(hip.ArgError):
+            append(q_out=out)
+    with pytest.raises(hip.ArgError):  # in the gaps of strided q, but longer than they are
+        append(q_out=at + w, q_ld=H * hd + 64)
+    start, lens = dev(np.array([0, n], np.int32)), dev(np.array([T], np.int32))
+    need = P.attend_workspace(n, 1, n, T)
+    assert need > 0
+
+    def attend(**k):
+        P.attend(0, **dict(dict(q=at, out=at + 65536, row_start=ptr(start), kv_len=ptr(lens), table=ptr(p.dtable), n_seqs=1,
+                                table_ld=p.table.shape[1], rows=n, max_rows=n, max_len=T, ws=at + 131072, ws_bytes=need), **k))
+    for bad in (dict(out=at), dict(out=at + 8), dict(out=at - n * w + 8), dict(out=at + n * w - 8), dict(ws=at + n * w - 16),
+                dict(ws=at - need // 16 * 16 + 16), dict(ws=at + 65536 + 16), dict(out=at + w - 8, q_ld=2 * H * hd, out_ld=2 * H * hd),
+                dict(out=at + w, q_ld=2 * H * hd, out_ld=3 * H * hd)):
+        with pytest.raises(hip.ArgError):
+            attend(**bad)
+    # q and out as the halves of one buffer's rows, and one right behind the other
+    q = p.rows(n, H)
+    both = np.full((n, 2, H, hd), 9.0, np.float16)
+    both[:, 0] = q
+    d = dev(both)
+    ws = zeros(need, np.uint8)
+    attend(q=ptr(d), out=ptr(d) + w, q_ld=2 * H * hd, out_ld=2 * H * hd, ws=ptr(ws))
+    got = d.get()
+    assert np.array_equal(got[:, 0], q)
+    check_rows(got[:, 1], q, kv, causal(n, T), hd ** -0.5)
+    d = dev(np.concatenate([q, q]))
+    attend(q=ptr(d), out=ptr(d) + n * w, ws=ptr(ws))
+    assert np.array_equal(d.get(), np.concatenate([q, got[:, 1]]))

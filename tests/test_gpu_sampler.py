@@ -256,3 +256,22 @@ def test_a_refused_handle_leaves_no_error_behind(hip):
     held = Dev(free.value - (30 << 30), np.uint8)
     refused(lambda: hip.HipSampler(262144, 65535))
     del held
+
+
+def test_overlapping_probabilities_are_refused(hip):
+    V, ld, rows = 100, 220, 3
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((rows, ld)).astype(np.float32)
+    s = hip.HipSampler(V, rows)
+    d, u, tok = dev(x), dev(np.full(rows, 0.5, np.float32)), zeros(rows, np.int32)
+    end = 4 * ((rows - 1) * ld + V)
+    for at in (4, 4 * (V - 1), -4 * (rows * V - 1), end - 4, 4 * V):
+        with pytest.raises(hip.ArgError):
+            s.sample(ptr(d), rows, ptr(u), ptr(tok), probs=ptr(d) + at, ld=ld)
+    # one row's fits behind it, before the next one's logits
+    s.sample(ptr(d), 1, ptr(u), ptr(tok), probs=ptr(d) + 4 * V, ld=ld)
+    got = d.get()
+    want, p = _kvq.sample(x[0, :V], 0.5, 1.0)
+    assert tok.get()[0] == want and np.all(np.abs(got[0, V:2 * V] - p) <= 2.0 ** -24 * p * 1.01)
+    got[0, V:2 * V] = x[0, V:2 * V]
+    assert np.array_equal(got, x)
