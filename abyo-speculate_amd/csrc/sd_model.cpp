@@ -426,7 +426,7 @@ void Model::set_kv_format(int fmt) {
 }
 
 void Model::read_kv_rows(int layer, int which, int head, size_t pos0, size_t n, uint16_t *out) {
-    if (pos0 + n > (size_t)cap) throw ArgError("kv rows out of range");
+    if (n > (size_t)cap || pos0 > (size_t)cap - n) throw ArgError("kv rows out of range");
     if (n == 0) return;
     SD_HIP_CHECK(hipSetDevice(cfg.device));
     const int hd = cfg.head_dim;

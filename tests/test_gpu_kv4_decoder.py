@@ -278,3 +278,18 @@ def test_a_verify_pass_without_drafts_is_the_last_pass(hip, q4):
     for call in (lambda: d.sample_rows([0.5, 0.5]), lambda: d.last_argmax(2)):
         with pytest.raises(hip.ArgError):
             call()
+
+
+@pytest.mark.parametrize("q4", [False, True])
+def test_cache_rows_out_of_range_are_refused(hip, q4):
+    """Positions whose end wraps around 64 bits among them."""
+    ocfg = oracle_cfg(**SHAPES["llama"])
+    d = decoder(hip, ocfg, q4)
+    d.observe(ids(16, 40, ocfg.vocab))
+    out = np.zeros((64, ocfg.head_dim), np.uint16)
+    cap = (ocfg.ctx_len + 128 + 31) // 32 * 32  # positions that the cache holds
+    for pos0, n in ((cap, 1), (cap - 3, 4), (2 ** 64 - 1, 2), (2 ** 64 - 64, 64), (2 ** 63, 1), (0, cap + 1), (1, 2 ** 64 - 1)):
+        with pytest.raises(hip.ArgError):
+            hip._check(hip._lib.sd_read_kv_rows(d._h, 0, 0, 0, pos0, n, out.ctypes.data))
+    assert not out.any()
+    assert d.read_kv_rows(0, 0, 0, cap - 4, 4).shape == (4, ocfg.head_dim) and d.read_kv_rows(0, 1, 0, cap, 0).size == 0
