@@ -293,3 +293,20 @@ def test_cache_rows_out_of_range_are_refused(hip, q4):
             hip._check(hip._lib.sd_read_kv_rows(d._h, 0, 0, 0, pos0, n, out.ctypes.data))
     assert not out.any()
     assert d.read_kv_rows(0, 0, 0, cap - 4, 4).shape == (4, ocfg.head_dim) and d.read_kv_rows(0, 1, 0, cap, 0).size == 0
+
+
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+@pytest.mark.parametrize("rows", [17, 33, 64, 128])
+def test_many_rows_against_the_oracle_with_a_4_bit_cache(hip, shape, rows):
+    """As test_logits_against_the_oracle_with_a_4_bit_cache, by the kernels that more than 16 rows take: weights in fp16 besides,
+    2^-11 of each, which move a value no more than the activations do."""
+    ocfg = oracle_cfg(**SHAPES[shape])
+    om = O.OracleModel(ocfg)
+    f16, q4 = O.OracleDecoder(om), O.OracleDecoder(FourBitOracle(ocfg, om.raw))
+    d, prefix, drafts = decoder(hip, ocfg), ids(1, 90, ocfg.vocab), ids(rows, rows - 1, ocfg.vocab)
+    for x in (f16, q4, d):
+        x.observe(prefix)
+    want, plain, got = (np.asarray(x.batched_logits(drafts)).astype(np.float64) for x in (q4, f16, d))
+    change = np.linalg.norm(want - plain)
+    assert np.linalg.norm(got - want) <= 0.5 * change
+    assert np.linalg.norm(got - plain) >= 0.5 * change

@@ -639,3 +639,99 @@ def test_overlapping_rows_are_refused(hip):
     d = dev(np.concatenate([q, q]))
     attend(q=ptr(d), out=ptr(d) + n * w, ws=ptr(ws))
     assert np.array_equal(d.get(), np.concatenate([q, got[:, 1]]))
+
+
+# ---- every kernel's masks, NaN groups and absent pages, in batches ---------------------
+def check_but_holes(got, q, kv, visible, scale):
+    """check_rows for what is a number; NaN exactly where a row sees a key of one (everywhere) or a value of one (that group)."""
+    rows, H, hd = q.shape
+    KV, T = kv[0].shape[1], len(kv[0])
+    bad_k, bad_v = np.isnan(kv[0]).any(-1), np.isnan(kv[1])  # [T][KV], [T][KV][hd]
+    hole = np.zeros((rows, H, hd), bool)
+    for t in np.nonzero(bad_k.any(-1) | bad_v.any((1, 2)))[0]:
+        for h in range(H):
+            g = h // (H // KV)
+            hole[visible[:, t], h] |= bad_k[t, g] | bad_v[t, g]
+    assert np.array_equal(np.isnan(got), hole)
+    k, v, q = (np.where(np.isnan(x), 0, x).astype(np.float64) for x in (*kv, q))
+    want, mag, smax = np.zeros((rows, H, hd)), np.zeros((rows, H, hd)), 0.0
+    for h in range(H):
+        kh, vh = k[:, h // (H // KV)], v[:, h // (H // KV)]
+        s = np.where(visible, q[:, h] @ kh.T * scale, -np.inf)
+        smax = max(smax, float(np.max(np.abs(q[:, h]) @ np.abs(kh).T)) * scale)
+        m = s.max(-1, keepdims=True)
+        w = np.exp(s - np.where(m == -np.inf, 0, m))
+        w /= np.where(m == -np.inf, 1, w.sum(-1, keepdims=True))
+        want[:, h], mag[:, h] = w @ vh, w @ np.abs(vh)
+    score = 2 * hd * 2.0 ** -24 * smax + 2.0 ** -20  # as in check_rows
+    vmax = float(np.max(np.abs(v.astype(np.float64)))) if T else 0.0
+    tol = 2.0 ** -11 * (np.abs(want) + mag) * 1.01 + 2 * score * mag + T * 2.0 ** -25 * vmax + 2.0 ** -25
+    bad = (np.abs(got.astype(np.float64) - want) > tol) & ~hole
+    assert not bad.any(), np.argwhere(bad)[:4].tolist()
+
+
+def fill_long(p, edit):
+    """Pool.fill with rotation positions that start again at MAX_POS."""
+    out = []
+    for s, n in enumerate(p.lens):
+        k, v, pos = p.rows(n, p.KV), p.rows(n, p.KV), np.arange(n) % MAX_POS
+        edit(s, k, v)
+        p.append(k, v, [s] * n, range(n), pos=pos)
+        with np.errstate(invalid="ignore"):
+            out.append((_kvq.store(_kvq.rotate(k.astype(np.float64), pos, p.cos, p.sin, p.inter)), _kvq.store(v.astype(np.float64))))
+    return out
+
+
+# counts of rows, prefixes before them, heads, KV heads; the kernel and tile that these sizes take
+BATCHES = {
+    "16 queries": ([1, 0, 3, 2], [70, 9, 300, 0], 8, 4),
+    "32 queries, two tiles": ([25, 7, 30], [40, 500, 3], 4, 2),
+    "128 queries in two key groups, ranges": ([60, 33, 0, 41], [440, 900, 50, 7], 4, 2),
+    "256 queries in one range": ([300, 1, 70, 129, 200, 5, 64, 300], [0, 90, 33, 64, 5, 200, 1, 31], 16, 16),
+    "256 queries, ranges": ([150], [12350], 8, 8),
+}
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("name", sorted(BATCHES))
+def test_batches_with_masks_holes_and_absent_pages(hip, name, masked, hd):
+    counts, before, H, KV = BATCHES[name]
+    held = [n + b for n, b in zip(counts, before)]
+    rng = np.random.default_rng(len(name) + hd + masked)
+
+    def edit(s, k, v):
+        """Numbers that are none: in the sequence's own rows, where masks hide them from some rows, and behind its end."""
+        n, T = counts[s], held[s]
+        for at in {T - n // 2, T - 1} if n > 1 else ():
+            v[at, rng.integers(KV), rng.integers(hd)] = rng.choice([np.nan, np.inf, -np.inf])
+        if n > 2:
+            k[T - n // 3, 0, 5] = np.nan
+        v[T:], k[T:] = np.nan, np.inf
+    p = Pool(hip, hd + masked, H, KV, hd, [n + 3 for n in held], page=32)
+    kvs = fill_long(p, edit)
+    q, total, words = p.rows(sum(counts), H), sum(counts), -(-max(counts) // 64)
+    mask, seen, table, at = np.zeros((total, words), np.uint64), [], p.table.copy(), 0
+    for s, (n, T) in enumerate(zip(counts, held)):
+        vis = causal(n, T)
+        if masked:
+            bits = rng.random((n, n)) < 0.3
+            bits[::7] = False
+            vis = np.concatenate([np.ones((n, T - n), bool), bits], 1)
+            for i, j in np.argwhere(bits):
+                mask[at + i, j // 64] |= np.uint64(1) << np.uint64(j % 64)
+            if n % 64 and n:
+                mask[at:at + n, n // 64] |= np.uint64(1) << np.uint64(63)  # past the sequence's rows: nothing
+        if s % 2 == 0:  # every other sequence has pages that are not there
+            for pg, bad in ((T // 64, -1), (max(0, T // 32 - 1), p.n_pages + 3)):
+                table[s, pg] = bad
+                vis[:, 32 * pg:32 * pg + 32] = False
+        seen.append(vis)
+        at += n
+    got = p.attend(q, counts, lens=held, mask=mask if masked else None, table=dev(table))
+    at = 0
+    for s, n in enumerate(counts):
+        if n:
+            kv = [x[:held[s]] for x in kvs[s]]
+            check_but_holes(got[at:at + n], q[at:at + n], kv, seen[s], hd ** -0.5)
+        at += n
