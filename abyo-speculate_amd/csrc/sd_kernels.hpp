@@ -30,8 +30,8 @@ void launch_synth_f32(float *out, int64_t n, uint64_t seed, float mult, hipStrea
 void launch_fill_f32(float *out, int64_t n, float v, hipStream_t st);
 void launch_fill_kv(uint16_t *kv, int L, int n_kv, int64_t cap, int hd, int P, uint64_t seed, float mult,
                     hipStream_t st);
-// the same values as fp16 rows [n][n_kv][hd] of positions [p0, p0 + n) of one layer (P: positions of the fill)
-void launch_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int P, int p0, int n, uint64_t seed,
+// the same values as fp16 rows [n][n_kv][hd] of positions [p0, p0 + n) of one layer
+void launch_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int p0, int n, uint64_t seed,
                           float mult, hipStream_t st);
 // GGUF block bytes -> f32, exact (input must be in GGUF layout)
 void launch_dequant(int fmt, const uint8_t *w, int64_t n_elems, float *y, hipStream_t st);

@@ -150,8 +150,8 @@ template <typename T> __device__ __forceinline__ uint32_t group_word(const T (&x
 // Values need no rotation, and fp32 with a check near the borders decides their
 // codes; with the grid by rows that took append and read of 16384 rows from 136
 // to 114 us.  Memory bounds it: 16384 fp16 rows of 32 query heads and 8 KV heads
-// of 128 channels take 88 us, 74 at the rate of a large copy; 2501 fp32 rows 20
-// (18).
+// of 128 channels take 87 us, 74 at the rate of a large copy (4-byte words of codes
+// 32 bytes apart: 235 MB are written where 172 would do); 2501 fp32 rows 20 (18).
 template <int HD, bool F32>
 __global__ __launch_bounds__(kAppendT) void k_kvq_append(const KvqAppend p, int kv_chunks) {
     constexpr int W = HD / 8, U = kAppendT / W;  // units of a workgroup
@@ -216,8 +216,9 @@ void launch_kvq_append(const KvqAppend &p, hipStream_t st) {
 }
 
 // ---- read ----------------------------------------------------------------------
-// The same threads the other way: 16384 rows of 8 heads 27 us, 18 at the rate of
-// a large copy, most of it the 4-byte words that lie 32 bytes apart.
+// The same threads the other way: 16384 rows of 8 heads 29 us, 18 at the rate of
+// a large copy.  A workgroup has one row, whose 4-byte words lie 32 bytes apart,
+// so that the seven rows beside it fetch the same sectors again.
 template <int HD>
 __global__ __launch_bounds__(kAppendT) void k_kvq_read(const KvqLayer L, const KvqRows rows, uint16_t *k_out,
                                                        uint16_t *v_out) {

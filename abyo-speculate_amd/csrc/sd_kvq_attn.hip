@@ -9,19 +9,28 @@
 // k_kvq_attn, whose four waves take the blocks of a key range in turn, codes
 // straight from memory into registers.  A value costs two VALU operations
 // (mask and exponent, then the exact subtraction and the step, two values
-// each), so a block is about 300 VALU instructions for 4.6 KB: half of what a
-// CU can spend on its share of the memory's rate.
-// 5 rows of 32 heads over 8 and 32768 positions, 37.7 MB of blocks: 15 us, 7.8 at
-// the rate of a large copy; some 8 us are a chain that runs once.
+// each); with softmax, products, prologue and merge a block of 4.6 KB is some 540
+// VALU instructions of a wave for up to 32 queries, 540 cycles of a CU, whose
+// share of the memory's rate brings it in 410.
+// 5 rows of 32 heads over 8 and 32768 positions, 37.7 MB of blocks: 17 us, 6.2 at
+// the rate of a large read.  VALU instructions are issued in 59 % of the CUs' busy
+// cycles, matrix instructions take 13 %, and waves wait for 27 % of theirs: each
+// has four blocks here, of which it requests one ahead.
 // More: k_kvq_wide, whose waves have 32 queries each and share the values of
 // 64 positions through LDS, expanded once for up to 256 queries (two key groups
 // of 128 queries halve the partial results where the context is short).
-// 2048 rows of 32 heads over 8191 positions: 290 us, 830 TFLOP/s; a large
-// product of fp16 matrices reaches 1190.  A stage of 64 positions is 2048 cycles
-// of matrix instructions and as many of VALU work (246 instructions a wave, 32
-// of them exponentials) on a SIMD, whose two waves overlap them in part.
+// 2048 rows of 32 heads over 8191 positions: 291 us once the clocks have settled
+// (307 in the first ten calls), 825 TFLOP/s; a large product of fp16 matrices
+// reaches 1190.  A stage of 64 positions is 2048 cycles of matrix instructions
+// and some 2300 of VALU work (253 instructions a wave, 32 of them exponentials)
+// on a SIMD, whose two waves overlap them in part: of the CUs' busy cycles the
+// matrix pipes take 40 % and VALU instructions 50 %.  A CU has one tile, and causal
+// tiles differ in length: the longest is 1.14 times the mean here, 1.94 times in
+// the first 2048 positions of a prompt (83 us, 416 TFLOP/s).
+// 60 rows over 8192 positions: 29 us, in which the CUs' matrix pipes take 17 %,
+// VALU instructions 36 %, and waves wait for 39 % (four stages to a key group).
 // Key ranges (splits) meet in k_kvq_combine (60 rows of 32 heads in 16 ranges,
-// 16 MB of fp32: 5.8 us; 5 rows in 64 ranges 4.3, most of it latency).
+// 16 MB of fp32: 6.1 us; 5 rows in 64 ranges 4.3, most of it latency).
 #include <atomic>
 #include <type_traits>
 
@@ -71,7 +80,7 @@ __device__ __forceinline__ bool kvq_seq_rows(const KvqAttn &p, int s, int &r0, i
     return r0 >= 0 && end > r0 && end <= p.rows;
 }
 
-// bit j: position j of the lane's 8 is a number's (its V step is not NaN)
+// bit j: the V step of position j of the lane's 8 is NaN
 __device__ __forceinline__ uint32_t kvq_nan_steps(const uintx4 &vs) {
     uint32_t bad = 0;
 #pragma unroll

@@ -503,7 +503,7 @@ void Model::fill_kv_synthetic(int P, uint64_t seed) {
         for (int l = 0; l < cfg.n_layers; l++)
             for (int p0 = 0; p0 < P; p0 += chunk) {
                 const int n = std::min(chunk, P - p0);
-                launch_synth_kv_rows(k, v, l, cfg.n_kv_heads, cfg.head_dim, P, p0, n, seed, mult, st);
+                launch_synth_kv_rows(k, v, l, cfg.n_kv_heads, cfg.head_dim, p0, n, seed, mult, st);
                 a.L = kvq->layer(l);
                 a.rows = KvqRows{n, nullptr, nullptr, p0, kvq_table, 1, kvq->cfg.n_pages};
                 launch_kvq_append(a, st);

@@ -172,10 +172,11 @@ enum SmpMode : int { kSmpSum = 0, kSmpTopK = 1, kSmpHist = 2 };
 // workgroups on 256 CUs) and of the code that it runs once: 1024 threads with
 // two loads of four entries each, rolled loops over the entries (32 entries a
 // thread, unrolled: 10 us for one row, 4 of them fetching the last loop's code;
-// now 6.5).  Many rows are bound by VALU work, some 90 instructions an entry and
-// a quarter of them f64: 60 rows of 152064 take 29 us, 8 at the rate of a large
-// copy.  The histogram's loop therefore takes two entries a turn (one: 31 us;
-// four: the same as two; entries in LDS instead of turned registers: 31).
+// now 6.5).  Many rows are bound by VALU work, 82 instructions an entry and a
+// quarter of them f64, issued in 91 % of the CUs' busy cycles: 60 rows of 152064
+// take 29 us, 6 at the rate of a large read (and 30 MB of places and histograms
+// are written).  The histogram's loop therefore takes two entries a turn (one: 31
+// us; four: the same as two; entries in LDS instead of turned registers: 31).
 constexpr int kSlT = 1024, kSlPer = kSmpSlice / kSlT;
 typedef float floatx4r __attribute__((ext_vector_type(4), aligned(4)));
 

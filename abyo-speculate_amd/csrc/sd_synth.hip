@@ -194,7 +194,7 @@ __global__ void k_fill_kv(uint16_t *kv, int L, int n_kv, int64_t cap, int hd, in
     kv[stream * cap * hd + kv_off(which, r / hd, (int)(r % hd), hd)] = f2h(synth_value(seed, idx, mult));
 }
 
-__global__ void k_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int P, int p0, int64_t total,
+__global__ void k_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int p0, int64_t total,
                                 uint64_t seed, float mult) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= 2 * total) return;
@@ -284,11 +284,11 @@ void launch_fill_kv(uint16_t *kv, int L, int n_kv, int64_t cap, int hd, int P, u
                        seed, mult);
 }
 
-void launch_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int P, int p0, int n, uint64_t seed,
+void launch_synth_kv_rows(uint16_t *k, uint16_t *v, int layer, int n_kv, int hd, int p0, int n, uint64_t seed,
                           float mult, hipStream_t st) {
     const int64_t total = (int64_t)n * n_kv * hd;
     hipLaunchKernelGGL(k_synth_kv_rows, dim3((unsigned)((2 * total + 255) / 256)), dim3(256), 0, st, k, v, layer, n_kv,
-                       hd, P, p0, total, seed, mult);
+                       hd, p0, total, seed, mult);
 }
 
 void launch_dequant(int fmt, const uint8_t *w, int64_t n_elems, float *y, hipStream_t st) {

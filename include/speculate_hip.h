@@ -111,7 +111,9 @@ void sd_model_destroy(sd_model *m);
  * below, 4.5 bits a value, which every entry point of the handle then appends
  * to and attends over.  Rows are rotated with the handle's own RoPE tables.
  * A handle of the 4-bit format does not keep row i of an M-row call equal
- * to the one-row call bit for bit.  On failure the format stays. */
+ * to the one-row call bit for bit.  On failure the format stays.  A handle is
+ * created with the fp16 cache, and both exist while the format changes: the
+ * context has to fit both. */
 enum { SD_KV_F16 = 1, SD_KV_Q4 = 2 };
 sd_status sd_model_set_kv_format(sd_model *m, int32_t format);
 
@@ -426,7 +428,8 @@ size_t sd_kvpool_page_bytes(const sd_kvpool *c);
  * with seq NULL); that position lives in page
  * table[seq * table_ld + slot / page_tokens].  A row whose sequence is outside
  * [0, n_seqs), whose slot is negative or past the table, or whose page id is
- * outside the pool is padding: nothing is read or written for it.  No two rows
+ * outside the pool is padding: no page and no output is read or written for it
+ * (its rows of the inputs exist and may hold anything).  No two rows
  * of an append may be the same position of the same page (its content is then
  * a mixture of the two). */
 typedef struct sd_kv_rows {
@@ -475,7 +478,9 @@ typedef struct sd_kv_query {
     const uint64_t *mask;       /* [rows][mask_words] or NULL: causal */
     int32_t mask_words;
     size_t max_rows;            /* most rows of one sequence (host bound of row_start) */
-    size_t max_len;             /* most positions of one sequence: plans the work, larger kv_len stay correct */
+    size_t max_len;             /* most positions of one sequence: plans the work.  Larger kv_len stay correct; with
+                                   far smaller ones most of the key ranges are empty and few CUs work (60 rows over
+                                   4096 positions: 30 us, with max_len 131072 147; one row 12 and 23) */
     float scale;                /* 0: 1 / sqrt(head_dim) */
 } sd_kv_query;
 /* Bytes of workspace sd_kvpool_attend needs for these sizes (0 for a bad handle or bad sizes, or where none is needed). */
