@@ -20,7 +20,7 @@
 // 64 positions through LDS, expanded once for up to 256 queries (two key groups
 // of 128 queries halve the partial results where the context is short).
 // 2048 rows of 32 heads over 8191 positions: 291 us once the clocks have settled
-// (307 in the first ten calls), 825 TFLOP/s; a large product of fp16 matrices
+// (307 to 332 in the first ten calls), 825 TFLOP/s; a large product of fp16 matrices
 // reaches 1190.  A stage of 64 positions is 2048 cycles of matrix instructions
 // and some 2300 of VALU work (253 instructions a wave, 32 of them exponentials)
 // on a SIMD, whose two waves overlap them in part: of the CUs' busy cycles the
