@@ -9,9 +9,10 @@
 //          sum of the kept
 // Weights are computed in f64 and summed as integers, so no sum depends on an
 // order: of 2^-44 in the sums that a token is drawn from, of 2^-36 in the
-// histograms.  A rounded sum of V weights loses at most half a unit for each, so
-// a decision can differ from exact arithmetic only within V * 2^-45 of the sum
-// (with histograms V * 2^-37) of a border, usually within the 1e-11 of a weight.
+// histograms.  A weight is within 1e-11 of itself, and a rounded sum of V of them
+// loses at most half a unit for each, so a decision can differ from exact
+// arithmetic only within 1e-11 and V * 2^-45 of the sum (with histograms V * 2^-37)
+// of a border.
 //
 // Both top-k and top-p keep a prefix of the order (value descending, index
 // ascending), so together they are one bound on the pair (value, index).  Two

@@ -504,9 +504,10 @@ sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *query
  *   min-p  of those the ones with w_i >= min_p (0: off)
  *   token  the first kept i whose running sum, by index, exceeds u times the
  *          kept sum
- * Sums are rounded: a bound or a draw can differ from exact arithmetic within
- * vocab * 2^-37 of the sum (vocab * 2^-45 with neither top-p, min-p nor a top-k
- * above 256).  A token that is drawn is one that is kept.
+ * Weights are within 1e-11 of themselves and sums are rounded: a bound or a draw
+ * can differ from exact arithmetic within 1e-11 and vocab * 2^-37 of the sum
+ * (vocab * 2^-45 with neither top-p, min-p nor a top-k above 256).  A token that
+ * is drawn is one that is kept.
  * A row with a NaN or +inf, or of -inf only, has no distribution: token -1,
  * its probabilities zeros. */
 typedef struct sd_sampling {
