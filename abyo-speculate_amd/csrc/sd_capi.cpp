@@ -33,6 +33,9 @@ struct sd_draft3 {
 struct sd_kvpool {
     std::unique_ptr<sd::KvPool> p;
 };
+struct sd_kv8 {
+    std::unique_ptr<sd::KvPool> p;
+};
 struct sd_sampler {
     std::unique_ptr<sd::Sampler> s;
 };
@@ -74,6 +77,9 @@ static void need_weights(const sd_model *m) {
 static void need(const sd_kvpool *c) {
     if (!c || !c->p) throw sd::ArgError("null pool handle");
 }
+static void need(const sd_kv8 *c) {
+    if (!c || !c->p) throw sd::ArgError("null pool handle");
+}
 // elements of a row: the caller's stride, or a dense row's
 static int64_t row_stride(size_t ld, int64_t dense, const char *what) {
     if (ld == 0) return dense;
@@ -91,6 +97,65 @@ static sd::KvqRows kv_rows(const sd_kv_rows *r) {
     if (r->n_seqs < 1 || r->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
     return sd::KvqRows{(int)r->n, r->seq, r->slot, 0, r->table, r->n_seqs, r->table_ld};
 }
+static std::unique_ptr<sd::KvPool> make_pool(const sd_kvpool_config &cfg, int bits) {
+    sd::KvPoolCfg c;
+    c.n_layers = cfg.n_layers;
+    c.n_heads = cfg.n_heads;
+    c.n_kv_heads = cfg.n_kv_heads;
+    c.head_dim = cfg.head_dim;
+    c.n_pages = cfg.n_pages;
+    c.page_tokens = cfg.page_tokens;
+    c.max_pos = cfg.max_pos;
+    c.interleaved = cfg.interleaved != 0;
+    c.rope_theta = cfg.rope_theta;
+    c.device = cfg.device;
+    c.bits = bits;
+    if (c.max_pos < 1) throw sd::ArgError("kvpool: max_pos must be positive");
+    return std::make_unique<sd::KvPool>(c);
+}
+// What an attention call and a call for its weights have in common: the rows, the
+// sequences, the mask and the window of a query over an 8-bit pool.
+static sd::Kv8Attn kv8_query(const sd::KvPool &P, int32_t layer, const sd_kv_query *qy, const sd_kv_window *win) {
+    P.check_layer(layer);
+    if (!qy->q || !qy->row_start || !qy->kv_len || !qy->table) throw sd::ArgError("null argument");
+    if (qy->n_seqs < 1 || qy->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
+    if (qy->mask && qy->mask_words < 1) throw sd::ArgError("mask_words must be positive");
+    if (!std::isfinite(qy->scale)) throw sd::ArgError("scale must be finite");
+    const int hd = P.cfg.head_dim;
+    const size_t most = (size_t)1 << 30;
+    sd::Kv8Attn a{};
+    a.L = P.layer(layer);
+    a.q = qy->q;
+    a.q_row = row_stride(qy->q_ld, (int64_t)P.cfg.n_heads * hd, "q");
+    a.q_head = hd;
+    need_aligned(a.q, a.q_row * 2, 16, "q");
+    a.rows = (int)std::min(qy->rows, most);
+    a.n_seqs = qy->n_seqs;
+    a.row_start = qy->row_start;
+    a.kv_len = qy->kv_len;
+    a.table = qy->table;
+    a.table_ld = qy->table_ld;
+    a.mask = qy->mask;
+    a.mask_words = qy->mask_words;
+    a.max_rows = (int)std::min(qy->max_rows, most);
+    a.n_heads = P.cfg.n_heads;
+    a.n_rep = P.cfg.n_heads / P.cfg.n_kv_heads;
+    a.scale = qy->scale == 0.f ? (float)(1.0 / std::sqrt((double)hd)) : qy->scale;
+    if (win) {
+        a.window = (int)std::min(win->window, most);
+        a.sinks = (int)std::min(win->sinks, most);
+    }
+    return a;
+}
+static sd::KvqPlan kv8_plan(const sd::KvPool &P, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len,
+                            const sd_kv_window *win) {
+    const size_t most = (size_t)1 << 40, wide = (size_t)1 << 30;
+    return P.plan((int64_t)std::min(rows, most), (int64_t)std::min(n_seqs, most), (int64_t)std::min(max_rows, most),
+                  (int64_t)std::min(max_len, most), win ? (int)std::min(win->window, wide) : 0,
+                  win ? (int)std::min(win->sinks, wide) : 0);
+}
+// one range of memory
+static sd::RowBytes bytes_at(const void *p, int64_t bytes) { return {p, 0, bytes, 1}; }
 static void setdev(sd_model *m) { SD_HIP_CHECK(hipSetDevice(m->model->cfg.device)); }
 
 extern "C" {
@@ -919,20 +984,8 @@ sd_status sd_kvpool_create(const sd_kvpool_config *cfg, sd_kvpool **out) {
     return guard([&] {
         if (!cfg || !out) throw sd::ArgError("null argument");
         *out = nullptr;
-        sd::KvPoolCfg c;
-        c.n_layers = cfg->n_layers;
-        c.n_heads = cfg->n_heads;
-        c.n_kv_heads = cfg->n_kv_heads;
-        c.head_dim = cfg->head_dim;
-        c.n_pages = cfg->n_pages;
-        c.page_tokens = cfg->page_tokens;
-        c.max_pos = cfg->max_pos;
-        c.interleaved = cfg->interleaved != 0;
-        c.rope_theta = cfg->rope_theta;
-        c.device = cfg->device;
-        if (c.max_pos < 1) throw sd::ArgError("kvpool: max_pos must be positive");
         auto h = std::make_unique<sd_kvpool>();
-        h->p = std::make_unique<sd::KvPool>(c);
+        h->p = make_pool(*cfg, 4);
         *out = h.release();
     });
 }
@@ -1055,6 +1108,234 @@ sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *qy, v
         a.scale = qy->scale == 0.f ? (float)(1.0 / std::sqrt((double)hd)) : qy->scale;
         sd::DeviceScope dev(P.cfg.device);
         sd::launch_kvq_attention(a, plan, ws, (hipStream_t)stream);
+    });
+}
+
+sd_status sd_kv8_create(const sd_kvpool_config *cfg, sd_kv8 **out) {
+    return guard([&] {
+        if (!cfg || !out) throw sd::ArgError("null argument");
+        *out = nullptr;
+        auto h = std::make_unique<sd_kv8>();
+        h->p = make_pool(*cfg, 8);
+        *out = h.release();
+    });
+}
+void sd_kv8_destroy(sd_kv8 *c) { delete c; }
+size_t sd_kv8_page_bytes(const sd_kv8 *c) { return c && c->p ? (size_t)c->p->page_bytes() : 0; }
+
+sd_status sd_kv8_append(sd_kv8 *c, int32_t layer, const sd_kv_seqs *seqs, int32_t fmt, const void *q, size_t q_ld,
+                        const void *k, size_t k_ld, const void *v, size_t v_ld, const int32_t *pos, uint16_t *q_out,
+                        void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        if (!seqs) throw sd::ArgError("null argument");
+        if (fmt != SD_F16 && fmt != SD_F32) throw sd::UnsupportedError("append: rows must be F16 or F32");
+        if (seqs->rows == 0) return;
+        if (!seqs->row_start || !seqs->kv_len || !seqs->table || !k || !v || (q && !q_out)) throw sd::ArgError("null argument");
+        if (seqs->rows > ((size_t)1 << 24)) throw sd::ArgError("append: at most 2^24 rows");
+        if (seqs->max_rows < 1 || seqs->max_rows > seqs->rows) throw sd::ArgError("append: max_rows must be in [1, rows]");
+        if (seqs->n_seqs < 1 || seqs->n_seqs > 65535) throw sd::ArgError("append: n_seqs must be in [1, 65535]");
+        if (seqs->table_ld < 1) throw sd::ArgError("append: table_ld must be positive");
+        // a grid holds fewer than 2^32 threads
+        if ((int64_t)seqs->n_seqs * (2 * P.cfg.n_kv_heads + P.cfg.n_heads) > (1 << 23))
+            throw sd::UnsupportedError("append: too many sequences and heads in one call");
+        const int size = fmt == SD_F32 ? 4 : 2, hd = P.cfg.head_dim;
+        sd::Kv8Append a{};
+        a.L = sd::Kv8Layer(P.layer(layer));
+        a.seqs = {(int)seqs->rows, seqs->n_seqs, (int)seqs->max_rows, seqs->row_start, seqs->kv_len, 0, seqs->table, seqs->table_ld};
+        a.pos = pos;
+        a.cos_t = P.cos_t;
+        a.sin_t = P.sin_t;
+        a.max_pos = P.cfg.max_pos;
+        a.interleaved = P.cfg.interleaved;
+        a.n_heads = P.cfg.n_heads;
+        a.f32 = fmt == SD_F32;
+        a.q = q;
+        a.k = k;
+        a.v = v;
+        a.q_ld = row_stride(q_ld, (int64_t)P.cfg.n_heads * hd, "q");
+        a.k_ld = row_stride(k_ld, (int64_t)P.cfg.n_kv_heads * hd, "k");
+        a.v_ld = row_stride(v_ld, (int64_t)P.cfg.n_kv_heads * hd, "v");
+        a.q_out = q_out;
+        need_aligned(k, a.k_ld * size, 16, "k");
+        need_aligned(v, a.v_ld * size, 16, "v");
+        if (q) {
+            need_aligned(q, a.q_ld * size, 16, "q");
+            need_aligned(q_out, 16, 16, "q_out");
+            const int64_t n = a.seqs.rows, qb = (int64_t)P.cfg.n_heads * hd, kb = (int64_t)P.cfg.n_kv_heads * hd * size;
+            const sd::RowBytes out{q_out, qb * 2, qb * 2, n};
+            if (rows_meet(out, {q, a.q_ld * size, qb * size, n}) || rows_meet(out, {k, a.k_ld * size, kb, n}) ||
+                rows_meet(out, {v, a.v_ld * size, kb, n}))
+                throw sd::ArgError("q_out must not overlap q, k or v");
+        }
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kv8_append(a, (hipStream_t)stream);
+    });
+}
+
+sd_status sd_kv8_read(sd_kv8 *c, int32_t layer, const sd_kv_rows *rows, uint16_t *k_out, uint16_t *v_out, void *stream) {
+    return guard([&] {
+        need(c);
+        c->p->check_layer(layer);
+        const sd::KvqRows r = kv_rows(rows);
+        need_aligned(k_out, 16, 16, "k_out");
+        need_aligned(v_out, 16, 16, "v_out");
+        const int64_t bytes = (int64_t)r.n * c->p->cfg.n_kv_heads * c->p->cfg.head_dim * 2;
+        if (rows_meet(bytes_at(k_out, bytes), bytes_at(v_out, bytes))) throw sd::ArgError("read: k_out and v_out must not overlap");
+        if (!k_out && !v_out) return;
+        sd::DeviceScope dev(c->p->cfg.device);
+        sd::launch_kv8_read(sd::Kv8Layer(c->p->layer(layer)), r, k_out, v_out, (hipStream_t)stream);
+    });
+}
+
+size_t sd_kv8_attend_workspace(const sd_kv8 *c, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len,
+                               const sd_kv_window *window) {
+    size_t bytes = 0;
+    guard([&] {
+        need(c);
+        bytes = kv8_plan(*c->p, rows, n_seqs, max_rows, max_len, window).ws_bytes;
+    });
+    return bytes;
+}
+
+sd_status sd_kv8_attend(sd_kv8 *c, int32_t layer, const sd_kv_query *qy, const sd_kv_window *window, float *lse, void *ws,
+                        size_t ws_bytes, void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        if (!qy) throw sd::ArgError("null argument");
+        if (qy->rows == 0) return;
+        if (!qy->out) throw sd::ArgError("null argument");
+        sd::Kv8Attn a = kv8_query(P, layer, qy, window);
+        const sd::KvqPlan plan = kv8_plan(P, qy->rows, (size_t)qy->n_seqs, qy->max_rows, qy->max_len, window);
+        if (plan.ws_bytes && (!ws || ws_bytes < plan.ws_bytes))
+            throw sd::ArgError("attend: the workspace needs " + std::to_string(plan.ws_bytes) + " bytes");
+        need_aligned(ws, 16, 16, "workspace");
+        need_aligned(lse, 4, 4, "lse");
+        a.out = qy->out;
+        a.out_ld = row_stride(qy->out_ld, (int64_t)P.cfg.n_heads * P.cfg.head_dim, "out");
+        need_aligned(a.out, a.out_ld * 2, 8, "out");
+        a.lse = lse;
+        const int64_t row = (int64_t)P.cfg.n_heads * P.cfg.head_dim * 2, n = a.rows;
+        const sd::RowBytes q{a.q, a.q_row * 2, row, n}, out{a.out, a.out_ld * 2, row, n};
+        const sd::RowBytes work = bytes_at(ws, (int64_t)plan.ws_bytes), stat = bytes_at(lse, n * P.cfg.n_heads * 4);
+        if (rows_meet(q, out) || rows_meet(q, work) || rows_meet(out, work) || rows_meet(stat, q) || rows_meet(stat, out) ||
+            rows_meet(stat, work))
+            throw sd::ArgError("attend: q, out, lse and the workspace must not overlap");
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kv8_attention(a, plan, ws, (hipStream_t)stream);
+    });
+}
+
+sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *qy, const sd_kv_window *window, const float *lse,
+                         const sd_kv_scores *scores, void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        if (!qy || !scores) throw sd::ArgError("null argument");
+        if (qy->rows == 0) return;
+        if (!lse || !scores->out) throw sd::ArgError("null argument");
+        kv8_plan(P, qy->rows, (size_t)std::max(qy->n_seqs, 0), qy->max_rows, qy->max_len, window);  // the sizes
+        sd::Kv8Weights w{};
+        w.a = kv8_query(P, layer, qy, window);
+        w.a.lse = (float *)lse;
+        w.in = scores->in;
+        w.out = scores->out;
+        if (scores->ld < 1 || scores->ld > ((size_t)1 << 30)) throw sd::ArgError("weights: ld must be in [1, 2^30]");
+        if (!std::isfinite(scores->decay)) throw sd::ArgError("weights: decay must be finite");
+        w.ld = (int64_t)scores->ld;
+        w.decay = scores->decay;
+        w.max_len = (int64_t)qy->max_len;
+        need_aligned(lse, 4, 4, "lse");
+        need_aligned(w.in, 4, 4, "scores");
+        need_aligned(w.out, 4, 4, "scores");
+        const int64_t n = (int64_t)w.a.n_seqs * P.cfg.n_kv_heads * w.ld * 4, row = (int64_t)P.cfg.n_heads * P.cfg.head_dim * 2;
+        const sd::RowBytes out = bytes_at(w.out, n);
+        if (w.in != w.out && rows_meet(out, bytes_at(w.in, n))) throw sd::ArgError("weights: the scores overlap in part");
+        if (rows_meet(out, {w.a.q, w.a.q_row * 2, row, w.a.rows}) || rows_meet(out, bytes_at(lse, (int64_t)w.a.rows * P.cfg.n_heads * 4)))
+            throw sd::ArgError("weights: the scores must not overlap q or lse");
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kv8_weights(w, (hipStream_t)stream);
+    });
+}
+
+// whether n_seqs x budget is a size that a call can have
+static void check_evict(const sd::KvPool &P, int64_t n_seqs, size_t budget) {
+    if (n_seqs < 1 || n_seqs > 65535) throw sd::ArgError("evict: n_seqs must be in [1, 65535]");
+    if (budget > ((size_t)1 << 30)) throw sd::ArgError("evict: budget must be at most 2^30");
+    // a grid holds fewer than 2^32 threads
+    const int64_t blocks = std::max<int64_t>(4, ((int64_t)budget + 31) / 32);
+    if (blocks > ((int64_t)1 << 23) / (2 * P.cfg.n_kv_heads * n_seqs))
+        throw sd::UnsupportedError("evict: too many sequences and blocks in one call");
+}
+
+size_t sd_kv8_evict_workspace(const sd_kv8 *c, size_t n_seqs, size_t budget) {
+    size_t bytes = 0;
+    guard([&] {
+        need(c);
+        check_evict(*c->p, (int64_t)std::min(n_seqs, (size_t)1 << 40), budget);
+        bytes = sd::kv8_evict_ws_bytes((int)n_seqs, c->p->cfg.n_kv_heads, c->p->cfg.head_dim, (int)budget);
+    });
+    return bytes;
+}
+
+sd_status sd_kv8_evict(sd_kv8 *c, int32_t layer, const sd_kv_evict *e, void *ws, size_t ws_bytes, void *stream) {
+    return guard([&] {
+        need(c);
+        const sd::KvPool &P = *c->p;
+        P.check_layer(layer);
+        if (!e || !e->kv_len || !e->table || !e->scores || !e->new_len || (e->budget && !e->kept)) throw sd::ArgError("null argument");
+        if (e->table_ld < 1 || (e->new_table && e->new_table_ld < 1)) throw sd::ArgError("table_ld must be positive");
+        check_evict(P, e->n_seqs, e->budget);
+        if (e->sinks > e->budget || e->recent > e->budget - e->sinks) throw sd::ArgError("evict: sinks and recent exceed the budget");
+        if (e->scores_ld < 1 || e->scores_ld > ((size_t)1 << 30)) throw sd::ArgError("evict: scores_ld must be in [1, 2^30]");
+        const size_t out_ld = e->scores_out_ld ? e->scores_out_ld : e->budget;
+        if (e->scores_out && (out_ld < e->budget || out_ld > ((size_t)1 << 30))) throw sd::ArgError("evict: scores_out: rows overlap");
+        const int kv = P.cfg.n_kv_heads;
+        const int64_t need_ws = e->new_table ? 0 : (int64_t)sd::kv8_evict_ws_bytes(e->n_seqs, kv, P.cfg.head_dim, (int)e->budget);
+        if (need_ws && (!ws || ws_bytes < (size_t)need_ws))
+            throw sd::ArgError("evict: the workspace needs " + std::to_string(need_ws) + " bytes");
+        need_aligned(ws, 16, 16, "workspace");
+        for (const void *p : {(const void *)e->scores, (const void *)e->scores_out, (const void *)e->kept, (const void *)e->new_len})
+            need_aligned(p, 4, 4, "evict");
+        const int64_t heads = (int64_t)e->n_seqs * kv;
+        const bool same = e->scores_out == e->scores && out_ld == e->scores_ld;
+        // (tables of several layers' calls, kv_len and scores are inputs; nothing written may meet them or each other)
+        const sd::RowBytes outs[] = {bytes_at(e->kept, heads * (int64_t)e->budget * 4), bytes_at(e->new_len, (int64_t)e->n_seqs * 4),
+                                     bytes_at(ws, need_ws), bytes_at(e->scores_out, heads * (int64_t)out_ld * 4)};
+        const sd::RowBytes ins[] = {bytes_at(e->kv_len, (int64_t)e->n_seqs * 4), bytes_at(e->table, (int64_t)e->n_seqs * e->table_ld * 4),
+                                    bytes_at(e->new_table, (int64_t)e->n_seqs * e->new_table_ld * 4),
+                                    bytes_at(e->scores, heads * (int64_t)e->scores_ld * 4)};
+        for (int i = 0; i < 4; i++) {
+            for (int j = 0; j < i; j++)
+                if (rows_meet(outs[i], outs[j])) throw sd::ArgError("evict: outputs and the workspace must not overlap");
+            for (int j = 0; j < 4; j++)
+                if (!(i == 3 && j == 3 && same) && rows_meet(outs[i], ins[j]))
+                    throw sd::ArgError("evict: outputs and the workspace must not overlap the inputs");
+        }
+        sd::Kv8Evict a{};
+        a.L = sd::Kv8Layer(P.layer(layer));
+        a.n_seqs = e->n_seqs;
+        a.kv_len = e->kv_len;
+        a.table = e->table;
+        a.table_ld = e->table_ld;
+        a.new_table = e->new_table;
+        a.new_ld = e->new_table_ld;
+        a.scores = e->scores;
+        a.scores_ld = (int64_t)e->scores_ld;
+        a.scores_out = e->scores_out;
+        a.scores_out_ld = (int64_t)out_ld;
+        a.budget = (int)e->budget;
+        a.sinks = (int)e->sinks;
+        a.recent = (int)e->recent;
+        a.kept = e->kept;
+        a.new_len = e->new_len;
+        sd::DeviceScope dev(P.cfg.device);
+        sd::launch_kv8_evict(a, ws, (hipStream_t)stream);
     });
 }
 

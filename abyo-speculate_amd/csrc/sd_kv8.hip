@@ -1,0 +1,257 @@
+// The 8-bit paged KV cache: appending rows (RoPE and quantisation on the way),
+// reading them back, moving accepted tree rows.  The format and the block layout
+// are in sd_kv8.hpp.
+#include "sd_kv8_dev.hpp"
+
+namespace sd {
+
+// C channels from c0 of a head's row, rotated in T by the pairs' or halves' angles
+template <typename T, int HD, bool F32>
+__device__ __forceinline__ void kv8_rotated(const void *src, int64_t at, int c0, const float *cos_r, const float *sin_r,
+                                            bool pairs, T (&x)[HD / 8]) {
+    constexpr int W = HD / 8;
+#pragma unroll
+    for (int i = 0; i < HD / 64; i++) {
+        const int w = c0 / 8 + i;
+        float a[8], b[8] = {};
+        load8<F32>(src, at + 8 * w, a);
+        if (!pairs) load8<F32>(src, at + 8 * ((w + W / 2) % W), b);
+        T o[8];
+        rotate8<T, HD>(a, b, cos_r, sin_r, w, pairs, o);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[8 * i + j] = o[j];
+    }
+}
+
+// One workgroup per block and unit: the keys of a KV head, the values of one, or
+// 32 pairs of a row and a query head; 8 threads to a position or pair.  Blocks of a
+// sequence are dealt round gridDim.x workgroups.  What a block holds in front of the
+// call's rows is read, and the whole block written: its scale may have changed.  Keys
+// are rotated and rounded in f64, so that no code depends on the order of roundings.
+template <int HD, bool F32>
+__global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
+    constexpr int C = HD / 8;
+    __shared__ Kv8Sh sh;
+    const int s = blockIdx.z, n_kv = p.L.n_kv, tid = threadIdx.x;
+    const int r0 = p.seqs.row_start ? p.seqs.row_start[s] : 0;
+    const int end = p.seqs.row_start ? p.seqs.row_start[s + 1] : p.seqs.rows;
+    const int T = p.seqs.row_start ? p.seqs.kv_len[s] : p.seqs.len0;
+    if (r0 < 0 || end <= r0 || end > p.seqs.rows || T < 1 || T > kKv8MaxLen) return;
+    // row i is position P + i; of the positions [first, last)
+    const int n = end - r0, P = T - n, first = max(P, 0), last = P + min(n, p.seqs.max_rows);
+    const bool pairs = p.interleaved != 0;
+    const int unit = blockIdx.y;
+    for (int b = (first >> 5) + (int)blockIdx.x; (int64_t)b * 32 < last; b += gridDim.x) {
+        const int lo = max(first, b * 32), hi = min(last, b * 32 + 32);
+        if (unit >= 2 * n_kv) {
+            const int u = (unit - 2 * n_kv) * 32 + (tid >> 3), pos = lo + u / p.n_heads, h = u % p.n_heads, c0 = (tid & 7) * C;
+            if (pos >= hi) continue;
+            const int row = r0 + pos - P, at = p.pos ? p.pos[row] : pos;
+            float x[C];
+            if (at >= 0 && at < p.max_pos) {
+                kv8_rotated<float, HD, F32>(p.q, (int64_t)row * p.q_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
+                                            p.sin_t + (int64_t)at * (HD / 2), pairs, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < C; i++) x[i] = NAN;
+            }
+            uint16_t *out = p.q_out + ((int64_t)row * p.n_heads + h) * HD + c0;
+#pragma unroll
+            for (int i = 0; i < C; i += 8) {
+                uintx4 v;
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] = (uint32_t)f2h(x[i + 2 * j]) | (uint32_t)f2h(x[i + 2 * j + 1]) << 16;
+                *(uintx4 *)(out + i) = v;
+            }
+            continue;
+        }
+        const bool is_v = unit >= n_kv;
+        const int h = is_v ? unit - n_kv : unit, slot = b >> (p.L.page_shift - 5);
+        const int page = slot < p.seqs.table_ld ? p.seqs.table[(int64_t)s * p.seqs.table_ld + slot] : -1;
+        if (page < 0 || page >= p.L.n_pages) continue;
+        uint8_t *codes = p.L.codes(page, h, b * 32) + (is_v ? 32 * HD : 0);
+        Kv8Head *head = p.L.head(page, h, b * 32);
+        const int k = tid >> 3, c0 = (tid & 7) * C, pos = b * 32 + k;
+        const bool live = pos < hi, held = pos < lo;
+        float scale = 1.f;
+        uint32_t nans = 0;
+        if (lo > b * 32) {
+            scale = head->scale[is_v];
+            nans = head->nan[is_v];
+            kv8_codes_in<HD>(sh, codes);
+            __syncthreads();
+        }
+        const int row = r0 + pos - P;
+        if (is_v) {
+            float x[C] = {};
+            if (held) {
+                kv8_row<HD, true>(sh.codes, k, c0, scale, x);
+            } else if (live) {
+                const int64_t at = (int64_t)row * p.v_ld + (int64_t)h * HD + c0;
+#pragma unroll
+                for (int i = 0; i < C; i += 8) {
+                    float a[8];
+                    load8<F32>(p.v, at + i, a);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[i + j] = a[j];
+                }
+            }
+            // a row whose rotation position does not exist is NaN in its values too
+            const bool lost = live && !held && p.pos && (p.pos[row] < 0 || p.pos[row] >= p.max_pos);
+            const bool past = live && !held && !p.pos && pos >= p.max_pos;
+            kv8_build<HD, true>(sh, x, live, lost || past || (held && (nans >> k & 1)), scale, nans);
+        } else {
+            double x[C] = {};
+            bool lost = held && (nans >> k & 1);
+            if (held) {
+                kv8_row<HD, false>(sh.codes, k, c0, scale, x);
+            } else if (live) {
+                const int at = p.pos ? p.pos[row] : pos;
+                lost = at < 0 || at >= p.max_pos;
+                if (!lost)
+                    kv8_rotated<double, HD, F32>(p.k, (int64_t)row * p.k_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
+                                                 p.sin_t + (int64_t)at * (HD / 2), pairs, x);
+            }
+            kv8_build<HD, false>(sh, x, live, lost, scale, nans);
+        }
+        kv8_codes_out<HD>(sh, codes);
+        if (tid == 0) {
+            head->scale[is_v] = scale;
+            head->nan[is_v] = nans;
+        }
+        __syncthreads();  // the codes in LDS are free again
+    }
+}
+
+void launch_kv8_append(const Kv8Append &p, hipStream_t st) {
+    if (p.seqs.rows < 1) return;
+    // blocks that max_rows rows can touch; a sequence's are dealt round as many workgroups as even ragged lengths need
+    const int64_t blocks = (p.seqs.max_rows + 30) / 32 + 1;
+    const int64_t mean = (p.seqs.rows / 32 + 2 * (int64_t)p.seqs.n_seqs + p.seqs.n_seqs - 1) / p.seqs.n_seqs;
+    const int q = p.q ? (int)(((int64_t)std::min(32, p.seqs.max_rows) * p.n_heads + 31) / 32) : 0;
+    // (a grid holds fewer than 2^32 threads)
+    const int64_t units = 2 * p.L.n_kv + q, most = ((int64_t)1 << 23) / (units * p.seqs.n_seqs);
+    if (most < 1) throw BackendError("append: too many sequences and heads in one call");
+    const dim3 g((unsigned)std::min({blocks, 4 * mean, most}), (unsigned)units, (unsigned)p.seqs.n_seqs), b(kKv8T);
+    if (p.L.hd == 128) {
+        if (p.f32) k_kv8_append<128, true><<<g, b, 0, st>>>(p);
+        else k_kv8_append<128, false><<<g, b, 0, st>>>(p);
+    } else {
+        if (p.f32) k_kv8_append<64, true><<<g, b, 0, st>>>(p);
+        else k_kv8_append<64, false><<<g, b, 0, st>>>(p);
+    }
+    SD_HIP_CHECK(hipGetLastError());
+}
+
+// ---- read ----------------------------------------------------------------------
+// 16 rows of one KV head's keys or values to a workgroup, 16 or 8 threads to a row:
+// rows next to each other share the lines that their values' bytes lie in.
+constexpr int kReadRows = 16;
+template <int HD>
+__global__ __launch_bounds__(2 * HD) void k_kv8_read(const Kv8Layer L, const KvqRows rows, uint16_t *k_out, uint16_t *v_out) {
+    constexpr int W = HD / 8;
+    const int r = blockIdx.x * kReadRows + threadIdx.x / W, c0 = threadIdx.x % W * 8;
+    const bool is_v = (int)blockIdx.y >= L.n_kv;
+    const int h = is_v ? (int)blockIdx.y - L.n_kv : (int)blockIdx.y;
+    uint16_t *out = is_v ? v_out : k_out;
+    if (!out || r >= rows.n) return;
+    int slot;
+    const int page = kvq_row_page(rows, L, r, slot);
+    if (page < 0) return;
+    const int k = slot & 31;
+    const uint8_t *codes = L.codes(page, h, slot) + (is_v ? 32 * HD : 0);
+    const Kv8Head *head = L.head(page, h, slot);
+    const float scale = head->scale[is_v];
+    uintx2 w = {0, 0};
+    if (is_v) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)codes[kv8_v_at(k, c0 + i, HD)] << (8 * (i & 3));
+    } else {
+        w = *(const uintx2 *)(codes + kv8_k_at(k, c0, HD));
+    }
+    uintx4 v = kv8_expand(w.x, w.y, scale);
+    if (head->nan[is_v] >> k & 1) v = uintx4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+    *(uintx4 *)(out + ((int64_t)r * L.n_kv + h) * HD + c0) = v;
+}
+
+void launch_kv8_read(const Kv8Layer &L, const KvqRows &rows, uint16_t *k_out, uint16_t *v_out, hipStream_t st) {
+    if (rows.n < 1) return;
+    const dim3 g((unsigned)((rows.n + kReadRows - 1) / kReadRows), (unsigned)(2 * L.n_kv));
+    if (L.hd == 128) k_kv8_read<128><<<g, dim3(256), 0, st>>>(L, rows, k_out, v_out);
+    else k_kv8_read<64><<<g, dim3(128), 0, st>>>(L, rows, k_out, v_out);
+    SD_HIP_CHECK(hipGetLastError());
+}
+
+// ---- keep accepted tree rows ------------------------------------------------------
+// One workgroup per (layer, KV head, keys or values): the accepted rows' codes go to
+// LDS, with their scales, then the blocks from P's on are built again from what stays
+// in front of P and the rows.
+constexpr int kKeepMax = 128;
+template <int HD, bool V>
+__device__ void kv8_keep(Kv8Sh &sh, uint8_t (&code)[kKeepMax][HD], float (&scales)[kKeepMax], uint32_t (&bad)[kKeepMax],
+                         const Kv8Layer &L, int h, const int *table, int P, const int *src, int n) {
+    constexpr int C = HD / 8;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < n * 8; i += kKv8T) {
+        const int j = i >> 3, c0 = (i & 7) * C, pos = P + src[j], page = table[pos >> L.page_shift];
+        const uint8_t *b = L.codes(page, h, pos) + (V ? 32 * HD : 0);
+#pragma unroll
+        for (int c = 0; c < C; c++) code[j][c0 + c] = b[V ? kv8_v_at(pos & 31, c0 + c, HD) : kv8_k_at(pos & 31, c0 + c, HD)];
+        if ((i & 7) == 0) {
+            const Kv8Head *head = L.head(page, h, pos);
+            scales[j] = head->scale[V];
+            bad[j] = head->nan[V] >> (pos & 31) & 1;
+        }
+    }
+    __syncthreads();
+    const int k = tid >> 3, c0 = (tid & 7) * C;
+    for (int b = P >> 5; b * 32 < P + n; b++) {
+        const int page = table[b * 32 >> L.page_shift], pos = b * 32 + k, j = pos - P;
+        uint8_t *codes = L.codes(page, h, b * 32) + (V ? 32 * HD : 0);
+        Kv8Head *head = L.head(page, h, b * 32);
+        float scale = head->scale[V];
+        uint32_t nans = head->nan[V];
+        float x[C] = {};
+        bool lost = false;
+        if (j < 0) {
+            kv8_row<HD, V>(codes, k, c0, scale, x);
+            lost = nans >> k & 1;
+        } else if (j < n) {
+#pragma unroll
+            for (int c = 0; c < C; c++) x[c] = kv8_value(code[j][c0 + c], scales[j]);
+            lost = bad[j] != 0;
+        }
+        kv8_build<HD, V>(sh, x, j < n, lost, scale, nans);  // (its first barrier: the block has been read)
+        kv8_codes_out<HD>(sh, codes);
+        if (tid == 0) {
+            head->scale[V] = scale;
+            head->nan[V] = nans;
+        }
+        __syncthreads();
+    }
+}
+template <int HD>
+__global__ __launch_bounds__(kKv8T) void k_kv8_keep_tail(const Kv8Layer L0, int64_t layer_bytes, const int *table, int P,
+                                                         const int *src, int n) {
+    __shared__ Kv8Sh sh;
+    __shared__ uint8_t code[kKeepMax][HD];
+    __shared__ float scales[kKeepMax];
+    __shared__ uint32_t bad[kKeepMax];
+    Kv8Layer L = L0;
+    const int u = blockIdx.x % (2 * L.n_kv);
+    L.base += (int64_t)(blockIdx.x / (2 * L.n_kv)) * layer_bytes;
+    if (u < L.n_kv) kv8_keep<HD, false>(sh, code, scales, bad, L, u, table, P, src, n);
+    else kv8_keep<HD, true>(sh, code, scales, bad, L, u - L.n_kv, table, P, src, n);
+}
+
+void launch_kv8_keep_tail(const Kv8Layer &L0, int64_t layer_bytes, int n_layers, const int *table, int P, const int *src,
+                          int n, hipStream_t st) {
+    if (n < 1) return;
+    if (n > kKeepMax) throw BackendError("keep_tail: at most 128 rows");
+    const dim3 g((unsigned)(n_layers * 2 * L0.n_kv)), b(kKv8T);
+    if (L0.hd == 128) k_kv8_keep_tail<128><<<g, b, 0, st>>>(L0, layer_bytes, table, P, src, n);
+    else k_kv8_keep_tail<64><<<g, b, 0, st>>>(L0, layer_bytes, table, P, src, n);
+    SD_HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace sd

@@ -1,0 +1,72 @@
+// What the attention over the 8-bit cache and the sums of its weights share:
+// which blocks a tile of queries sees, and which of their positions.
+#pragma once
+#include "sd_kv8_dev.hpp"
+#include "sd_kvq_attn_dev.hpp"
+
+namespace sd {
+
+// Rows and positions of a workgroup's sequence, its queries and their blocks.
+struct Kv8Work {
+    int r0, n, T, P;   // row i of n is row r0 + i of the call and position P + i
+    int nq, q0;        // queries of the KV head, the tile's first
+    int t_end, t_all;  // positions that some of the tile's rows see end before t_end, without a window all see those before t_all
+    int w_any, w_all;  // with a window: besides the first `sinks`, some rows see positions from w_any on, all of them from w_all
+    int nsink, b_win;  // blocks: [0, nsink) for the first positions, then from b_win to the end
+    int total;         // blocks in all
+};
+
+// the k-th block that a tile sees
+__device__ __forceinline__ int kv8_nth(const Kv8Work &w, int k) { return k < w.nsink ? k : k - w.nsink + w.b_win; }
+
+__device__ __forceinline__ bool kv8_work(const Kv8Attn &p, int s, int tile, int tile_q, Kv8Work &w) {
+    w.T = p.row_start ? p.kv_len[s] : p.len0;
+    if (!kvq_seq_rows(p, s, w.r0, w.n)) return false;
+    w.nq = min(w.n, p.max_rows) * p.n_rep;
+    w.q0 = tile * tile_q;
+    if (w.q0 >= w.nq) return false;
+    w.T = min(w.T, kKv8MaxLen);
+    w.P = w.T - w.n;
+    const int m_first = w.q0 / p.n_rep, m_last = (min(w.q0 + tile_q, w.nq) - 1) / p.n_rep;
+    w.t_end = p.mask ? w.T : min(w.T, w.P + m_last + 1);
+    w.t_all = p.mask ? w.P : w.P + m_first + 1;
+    // blocks that hold positions the table has pages for
+    const int nblk = w.t_end > 0 ? (int)min((int64_t)((w.t_end - 1) / 32 + 1), (int64_t)p.table_ld << (p.L.page_shift - 5)) : 0;
+    w.w_any = w.w_all = w.nsink = w.b_win = 0;
+    if (p.window > 0) {
+        w.w_any = max(0, w.P + m_first - p.window + 1);
+        w.w_all = max(0, w.P + m_last - p.window + 1);
+        w.b_win = min(w.w_any >> 5, nblk);
+        w.nsink = min((int)(((int64_t)p.sinks + 31) >> 5), w.b_win);
+    }
+    w.total = w.nsink + nblk - w.b_win;
+    return true;
+}
+// whether every row of the tile sees all of positions [a, a + n)
+__device__ __forceinline__ bool kv8_full(const Kv8Attn &p, const Kv8Work &w, int a, int n) {
+    return a + n <= w.t_all && a + n <= w.T && (p.window <= 0 || a >= w.w_all || a + n <= p.sinks);
+}
+
+// the lowest n of N bits
+template <int N> __device__ __forceinline__ uint32_t kv8_low(int n) {
+    return n >= N ? (N == 32 ? ~0u : (1u << (N & 31)) - 1u) : (1u << max(n, 0)) - 1u;
+}
+// bit j: row m sees position key0 + j, j < N (8 or 32); key0 a multiple of N
+template <int N> __device__ __forceinline__ uint32_t kv8_visible(const Kv8Attn &p, const Kv8Work &w, int m, int key0) {
+    uint32_t vis;
+    if (!p.mask) {
+        vis = kv8_low<N>(w.P + m + 1 - key0);
+    } else {
+        // N bits from x0 of the row's words: both words they can lie in are loaded at once, whatever x0 is
+        const uint64_t *mk = p.mask + (int64_t)(w.r0 + m) * p.mask_words;
+        const int x0 = key0 - w.P, a = x0 >> 6, s = x0 & 63;
+        const uint64_t w0 = mk[min(max(a, 0), p.mask_words - 1)], w1 = mk[min(max(a + 1, 0), p.mask_words - 1)];
+        const uint64_t lo = a >= 0 && a < p.mask_words ? w0 : 0, hi = a + 1 >= 0 && a + 1 < p.mask_words ? w1 : 0;
+        vis = (uint32_t)(lo >> s | (hi << 1) << (63 - s)) & kv8_low<N>(w.n - x0);
+        if (x0 < 0) vis |= kv8_low<N>(-x0);  // the prefix
+    }
+    if (p.window > 0) vis &= kv8_low<N>(p.sinks - key0) | ~kv8_low<N>(w.P + m - p.window + 1 - key0);
+    return vis;
+}
+
+}  // namespace sd

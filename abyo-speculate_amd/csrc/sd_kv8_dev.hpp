@@ -1,0 +1,129 @@
+// Device code shared by the kernels of the 8-bit KV cache.
+#pragma once
+#include "sd_kv8.hpp"
+#include "sd_kvq_dev.hpp"
+
+namespace sd {
+
+typedef float float2v __attribute__((ext_vector_type(2)));
+
+constexpr int kKv8T = 256;  // threads that build a block: 8 to a position
+
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float kv8_two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The smallest e with a <= 448 * 2^e = 1.75 * 2^(8 + e), for a finite a >= 0.
+__device__ __forceinline__ int kv8_exp(double a) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, a);
+    return (int)(b >> 52) - 1023 - 8 + ((b & 0xfffffffffffffull) > 0xc000000000000ull);
+}
+__device__ __forceinline__ int kv8_exp(float a) {
+    const uint32_t b = __float_as_uint(a);
+    return (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u);
+}
+// (a subnormal's result is wrong, but below the least scale in any case)
+
+// x in 32 bits such that a later rounding to fewer bits gives what rounding x
+// itself would: what does not fit goes into the last bit
+__device__ __forceinline__ float kv8_odd(double x) {
+    const float f = (float)x;
+    const double d = (double)f;
+    if (d == x) return f;
+    const uint32_t b = __float_as_uint(f);
+    return __uint_as_float((fabs(d) > fabs(x) ? b - 1 : b) | 1u);
+}
+__device__ __forceinline__ float kv8_odd(float x) { return x; }
+
+// four codes of x * r
+__device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return (uint32_t)w;
+}
+__device__ __forceinline__ float kv8_value(uint32_t code, float scale) {
+    return __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * scale;
+}
+// eight codes as fp16 values, exactly
+__device__ __forceinline__ uintx4 kv8_expand(uint32_t a, uint32_t b, float scale) {
+    return uintx4{h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false))),
+                  h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true))),
+                  h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false))),
+                  h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true)))};
+}
+
+// A block's keys or values from the values of its positions: thread t has the
+// channels (HD / 8) (t & 7) .. of position t >> 3 in x (live: the position holds
+// something), in LDS `codes` come the block's 32 HD bytes of codes.  Returns the
+// scale and the NaN bits.  All 256 threads call it; what they read of `codes`
+// before, they have read when the first barrier is passed.
+struct Kv8Sh {
+    __align__(16) uint8_t codes[32 * 128];
+    int exp[4];
+    uint32_t nan[4];
+};
+template <int HD, bool V, typename T>
+__device__ __forceinline__ void kv8_build(Kv8Sh &sh, const T (&x)[HD / 8], bool live, bool nan, float &scale, uint32_t &nans) {
+    constexpr int C = HD / 8;
+    const int tid = threadIdx.x, k = tid >> 3, c0 = (tid & 7) * C, lane = tid & 63;
+    T top = fabs(x[0]);
+    bool bad = !(top <= (T)65504);
+#pragma unroll
+    for (int i = 1; i < C; i++) {
+        const T a = fabs(x[i]);
+        bad |= !(a <= (T)65504);
+        top = fmax(top, a);
+    }
+    const uint64_t wave_bad = __builtin_amdgcn_ballot_w64(live && (bad || nan));
+    const bool row_bad = (wave_bad >> (lane & 56) & 0xff) != 0;
+    int e = live && !row_bad && top > (T)0 ? min(max(kv8_exp(top), kKv8MinExp), kKv8MaxExp) : kKv8MinExp;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o));
+    if (lane == 0) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m |= (uint32_t)((wave_bad >> (8 * i) & 0xff) != 0) << i;
+        sh.exp[tid >> 6] = e;
+        sh.nan[tid >> 6] = m;
+    }
+    __syncthreads();
+    e = max(max(sh.exp[0], sh.exp[1]), max(sh.exp[2], sh.exp[3]));
+    nans = sh.nan[0] | sh.nan[1] << 8 | sh.nan[2] << 16 | sh.nan[3] << 24;
+    scale = kv8_two_to(e);
+    const float r = live && !row_bad ? kv8_two_to(-e) : 0.f;
+    uint32_t w[C / 4];
+#pragma unroll
+    for (int i = 0; i < C; i += 4) {
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            y[j] = r == 0.f ? 0.f : kv8_odd(x[i + j]) * r;  // (not NaN or infinity times 0)
+            if (e == kKv8MaxExp) y[j] = fminf(fmaxf(y[j], -240.f), 240.f);  // 256 of it are more than fp16 holds
+        }
+        w[i / 4] = kv8_pack(y[0], y[1], y[2], y[3]);
+    }
+    if constexpr (!V) {
+#pragma unroll
+        for (int i = 0; i < C / 4; i += 2) *(uintx2 *)(sh.codes + kv8_k_at(k, c0 + 4 * i, HD)) = uintx2{w[i], w[i + 1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i++) sh.codes[kv8_v_at(k, c0 + i, HD)] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+    }
+    __syncthreads();
+}
+// the codes in LDS to or from a block's keys or values in memory
+template <int HD> __device__ __forceinline__ void kv8_codes_out(const Kv8Sh &sh, uint8_t *at) {
+    if constexpr (HD == 128) *(uintx4 *)(at + threadIdx.x * 16) = *(const uintx4 *)(sh.codes + threadIdx.x * 16);
+    else *(uintx2 *)(at + threadIdx.x * 8) = *(const uintx2 *)(sh.codes + threadIdx.x * 8);
+}
+template <int HD> __device__ __forceinline__ void kv8_codes_in(Kv8Sh &sh, const uint8_t *at) {
+    if constexpr (HD == 128) *(uintx4 *)(sh.codes + threadIdx.x * 16) = *(const uintx4 *)(at + threadIdx.x * 16);
+    else *(uintx2 *)(sh.codes + threadIdx.x * 8) = *(const uintx2 *)(at + threadIdx.x * 8);
+}
+// the C channels from c0 of position k of a block's codes
+template <int HD, bool V, typename T>
+__device__ __forceinline__ void kv8_row(const uint8_t *codes, int k, int c0, float scale, T (&x)[HD / 8]) {
+#pragma unroll
+    for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[V ? kv8_v_at(k, c0 + i, HD) : kv8_k_at(k, c0 + i, HD)], scale);
+}
+
+}  // namespace sd

@@ -1,4 +1,4 @@
-// Host side of the 4-bit paged KV cache and the sampler.  See sd_kvpool.hpp.
+// Host side of the paged KV caches and the sampler.  See sd_kvpool.hpp.
 #include "sd_kvpool.hpp"
 
 #include <cmath>
@@ -39,11 +39,11 @@ KvPool::KvPool(const KvPoolCfg &c) : cfg(c) {
         throw UnsupportedError("kvpool: page_tokens must be a power of two from 32 to 4096");
     if (c.max_pos < 0 || c.max_pos > (1 << 24)) throw ArgError("kvpool: max_pos must be in [0, 2^24]");
     if (c.max_pos && !(c.rope_theta > 0.f && std::isfinite(c.rope_theta))) throw ArgError("kvpool: rope_theta must be positive");
-    const double bytes = (double)c.n_layers * c.n_pages * c.n_kv_heads * (c.page_tokens / kKvqBlock) * kvq_block_bytes(c.head_dim);
+    const double bytes = (double)c.n_layers * c.n_pages * (double)page_bytes();
     if (bytes > 1e12) throw ArgError("kvpool: more than 1 TB of pages");
     DeviceScope dev(c.device);
     SD_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, c.device));
-    layer_bytes = (int64_t)c.n_pages * c.n_kv_heads * (c.page_tokens / kKvqBlock) * kvq_block_bytes(c.head_dim);
+    layer_bytes = c.n_pages * page_bytes();
     try {
         SD_HIP_CHECK(hipMalloc(&mem, (size_t)layer_bytes * c.n_layers + 256));
         SD_HIP_CHECK(hipMemset(mem, 0, (size_t)layer_bytes * c.n_layers + 256));
@@ -70,10 +70,15 @@ KvPool::~KvPool() {
     if (prev >= 0) (void)hipSetDevice(prev);
 }
 
+int64_t KvPool::page_bytes() const {
+    return cfg.bits == 8 ? kv8_page_bytes(cfg.n_kv_heads, cfg.head_dim, cfg.page_tokens)
+                         : (int64_t)cfg.n_kv_heads * (cfg.page_tokens / kKvqBlock) * kvq_block_bytes(cfg.head_dim);
+}
+
 KvqLayer KvPool::layer(int l) const {
     KvqLayer L;
     L.base = mem + (int64_t)l * layer_bytes;
-    L.page_bytes = (int64_t)cfg.n_kv_heads * (cfg.page_tokens / kKvqBlock) * kvq_block_bytes(cfg.head_dim);
+    L.page_bytes = page_bytes();
     L.n_pages = cfg.n_pages;
     L.page_shift = __builtin_ctz((unsigned)cfg.page_tokens);
     L.n_kv = cfg.n_kv_heads;
@@ -85,12 +90,14 @@ void KvPool::check_layer(int l) const {
     if (l < 0 || l >= cfg.n_layers) throw ArgError("kvpool: layer out of range");
 }
 
-KvqPlan KvPool::plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max_len) const {
+KvqPlan KvPool::plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max_len, int window, int sinks) const {
     if (rows < 1 || rows > (1 << 24)) throw ArgError("kvpool: rows must be in [1, 2^24]");
     if (n_seqs < 1 || n_seqs > 65535) throw ArgError("kvpool: n_seqs must be in [1, 65535]");
     if (max_rows < 1 || max_rows > rows) throw ArgError("kvpool: max_rows must be in [1, rows]");
     if (max_len < 0 || max_len > 0x7fffffc0) throw ArgError("kvpool: max_len out of range");
-    KvqPlan p = kvq_attn_plan(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, (int)n_seqs, (int)max_rows, max_len, cus);
+    KvqPlan p = cfg.bits == 8 ? kv8_attn_plan(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, (int)n_seqs, (int)max_rows, max_len,
+                                              window, sinks, cus)
+                              : kvq_attn_plan(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, (int)n_seqs, (int)max_rows, max_len, cus);
     // a grid holds fewer than 2^32 threads, at up to 512 a workgroup
     if ((int64_t)p.tiles * cfg.n_kv_heads * n_seqs > (1 << 22)) throw UnsupportedError("kvpool: too many rows in one call");
     p.ws_bytes = p.nsplit > 1 ? (size_t)p.nsplit * (size_t)rows * cfg.n_heads * (cfg.head_dim + 2) * sizeof(float) : 0;

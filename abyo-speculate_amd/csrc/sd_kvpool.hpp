@@ -1,7 +1,7 @@
-// Host handles of the operators on device memory: the 4-bit paged KV cache
-// and the sampler.
+// Host handles of the operators on device memory: the paged KV caches in 4 and
+// 8 bits and the sampler.
 #pragma once
-#include "sd_kvq.hpp"
+#include "sd_kv8.hpp"
 #include "sd_sample.hpp"
 
 namespace sd {
@@ -13,6 +13,7 @@ struct KvPoolCfg {
     int interleaved = 0;
     float rope_theta = 10000.f;
     int device = 0;
+    int bits = 4;  // or 8
 };
 
 // Makes a device current and the previous one current again at the end.
@@ -46,10 +47,11 @@ class KvPool {
     int64_t layer_bytes = 0;
     int cus = 0;
 
-    KvqLayer layer(int l) const;
+    KvqLayer layer(int l) const;  // (of an 8-bit pool: what Kv8Layer is made of)
     void check_layer(int l) const;
-    // the plan of a call (ArgError for sizes that no call can have)
-    KvqPlan plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max_len) const;
+    int64_t page_bytes() const;
+    // the plan of a call (ArgError for sizes that no call can have); with 8 bits perhaps through a window
+    KvqPlan plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max_len, int window = 0, int sinks = 0) const;
 
   private:
     uint8_t *mem = nullptr;

@@ -6,27 +6,7 @@
 
 namespace sd {
 
-// Where row r of a call lives: its page id, or -1 where the row is left out.
-__device__ __forceinline__ int kvq_row_page(const KvqRows &t, const KvqLayer &L, int r, int &slot) {
-    const int s = t.seq ? t.seq[r] : 0;
-    slot = t.slot ? t.slot[r] : t.slot0 + r;
-    if (s < 0 || s >= t.n_seqs || slot < 0) return -1;
-    const int at = slot >> L.page_shift;
-    if (at >= t.table_ld) return -1;
-    const int page = t.table[(int64_t)s * t.table_ld + at];
-    return page >= 0 && page < L.n_pages ? page : -1;
-}
-
 // ---- append --------------------------------------------------------------------
-// The value of another lane of the same four (XOR 1 or 2) without LDS.
-template <int X> __device__ __forceinline__ uint32_t quad_xor(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, X == 1 ? 0xB1 : 0x4E, 0xf, 0xf, true);
-}
-template <int X> __device__ __forceinline__ double quad_xor(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)quad_xor<X>((uint32_t)b) | ((uint64_t)quad_xor<X>((uint32_t)(b >> 32)) << 32));
-}
-
 // c + 8 of clamp(rint(x / d), -8, 7).  The product with 1 / d is within 2^-49
 // of the quotient, so only a value that close to a half needs the division.
 __device__ __forceinline__ uint32_t group_code(double x, double d, double rd) {
@@ -34,46 +14,6 @@ __device__ __forceinline__ uint32_t group_code(double x, double d, double rd) {
     double r = rint(y);
     if (fabs(y - r) > 0.5 - 1e-9) r = rint(x / d);
     return (uint32_t)((int)fmin(fmax(r, -8.0), 7.0) + 8);
-}
-
-template <bool F32> __device__ __forceinline__ void load8(const void *base, int64_t at, float (&x)[8]) {
-    if constexpr (F32) {
-        const float4 a = *(const float4 *)((const float *)base + at), b = *(const float4 *)((const float *)base + at + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const half8 h = *(const half8 *)((const _Float16 *)base + at);
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)h[i];
-    }
-}
-
-// x[0..7] (channels 8 w ..) rotated in T: with neighbouring pairs inside the
-// thread, with halves against channels 8 w +- hd / 2 (y).
-template <typename T, int HD>
-__device__ __forceinline__ void rotate8(const float (&x)[8], const float (&y)[8], const float *cos_r, const float *sin_r,
-                                        int w, bool pairs, T (&out)[8]) {
-    if (pairs) {
-        const float4 c = *(const float4 *)(cos_r + 4 * w), s = *(const float4 *)(sin_r + 4 * w);
-        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const T a = x[2 * i], b = x[2 * i + 1], C = cc[i], S = ss[i];
-            out[2 * i] = a * C - b * S;
-            out[2 * i + 1] = b * C + a * S;
-        }
-    } else {
-        const bool upper = w >= HD / 16;
-        const int at = (8 * w) & (HD / 2 - 1);
-        const float4 c0 = *(const float4 *)(cos_r + at), c1 = *(const float4 *)(cos_r + at + 4);
-        const float4 s0 = *(const float4 *)(sin_r + at), s1 = *(const float4 *)(sin_r + at + 4);
-        const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const T a = x[i], b = y[i], C = cc[i], S = upper ? ss[i] : -ss[i];
-            out[i] = a * C + b * S;
-        }
-    }
 }
 
 __global__ __launch_bounds__(256) void k_kvq_tables(float *cos_t, float *sin_t, int64_t n, int half, double base) {

@@ -386,8 +386,8 @@ void Model::synthesize(int mix, uint64_t seed, float stdv) {
 }
 
 void Model::set_kv_format(int fmt) {
-    if (fmt != KV_F16 && fmt != KV_Q4) throw UnsupportedError("kv format must be F16 or Q4");
-    if ((fmt == KV_Q4) == (kvq != nullptr)) return;
+    if (fmt != KV_F16 && fmt != KV_Q4 && fmt != KV_Q8) throw UnsupportedError("kv format must be F16, Q4 or Q8");
+    if (fmt == (!kvq ? KV_F16 : kv8() ? KV_Q8 : KV_Q4)) return;
     SD_HIP_CHECK(hipSetDevice(cfg.device));
     sync();
     if (fmt == KV_F16) {
@@ -403,6 +403,7 @@ void Model::set_kv_format(int fmt) {
         c.n_pages = (int)((cap + kKvqPage - 1) / kKvqPage);
         c.interleaved = cfg.arch == 0;
         c.device = cfg.device;
+        c.bits = fmt == KV_Q8 ? 8 : 4;
         auto pool = std::make_unique<KvPool>(c);
         if (!kvq_table) {
             std::vector<int> ids(c.n_pages);
@@ -410,15 +411,17 @@ void Model::set_kv_format(int fmt) {
             kvq_table = dalloc<int>(ids.size());
             SD_HIP_CHECK(hipMemcpy(kvq_table, ids.data(), ids.size() * sizeof(int), hipMemcpyHostToDevice));
         }
-        if (!kvq_ws) {
-            // (a shorter context never needs more)
-            size_t most = 16;
-            for (int M = 1; M <= std::max(prompt_rows, cfg.max_batch); M++)
-                most = std::max(most, pool->plan(M, 1, M, cfg.ctx_len).ws_bytes);
-            kvq_ws = dalloc<uint8_t>(most);
+        // (a shorter context never needs more)
+        size_t most = 16;
+        for (int M = 1; M <= std::max(prompt_rows, cfg.max_batch); M++)
+            most = std::max(most, pool->plan(M, 1, M, cfg.ctx_len).ws_bytes);
+        if (most > kvq_ws_bytes) {
+            void *ws = dalloc<uint8_t>(most);
+            if (kvq_ws) (void)hipFree(kvq_ws);
+            kvq_ws = ws;
             kvq_ws_bytes = most;
         }
-        SD_HIP_CHECK(hipFree(kv));
+        if (kv) SD_HIP_CHECK(hipFree(kv));
         kv = nullptr;
         kvq = std::move(pool);
     }
@@ -435,7 +438,9 @@ void Model::read_kv_rows(int layer, int which, int head, size_t pos0, size_t n, 
         std::vector<uint16_t> all(n * cfg.n_kv_heads * hd);
         std::unique_ptr<uint16_t, void (*)(uint16_t *)> rows(dalloc<uint16_t>(all.size()), [](uint16_t *p) { (void)hipFree(p); });
         const KvqRows r{(int)n, nullptr, nullptr, (int)pos0, kvq_table, 1, kvq->cfg.n_pages};
-        launch_kvq_read(kvq->layer(layer), r, which ? nullptr : rows.get(), which ? rows.get() : nullptr, st);
+        uint16_t *k = which ? nullptr : rows.get(), *v = which ? rows.get() : nullptr;
+        if (kv8()) launch_kv8_read(Kv8Layer(kvq->layer(layer)), r, k, v, st);
+        else launch_kvq_read(kvq->layer(layer), r, k, v, st);
         SD_HIP_CHECK(hipMemcpyAsync(all.data(), rows.get(), all.size() * 2, hipMemcpyDeviceToHost, st));
         sync();
         for (size_t j = 0; j < n; j++) std::memcpy(out + j * hd, all.data() + (j * cfg.n_kv_heads + head) * hd, hd * 2);
@@ -504,6 +509,22 @@ void Model::fill_kv_synthetic(int P, uint64_t seed) {
             for (int p0 = 0; p0 < P; p0 += chunk) {
                 const int n = std::min(chunk, P - p0);
                 launch_synth_kv_rows(k, v, l, cfg.n_kv_heads, cfg.head_dim, p0, n, seed, mult, st);
+                if (kv8()) {
+                    Kv8Append b{};
+                    b.L = Kv8Layer(kvq->layer(l));
+                    b.seqs = {n, 1, n, nullptr, nullptr, p0 + n, kvq_table, kvq->cfg.n_pages};
+                    b.pos = a.pos;
+                    b.cos_t = cos_t;
+                    b.sin_t = sin_t;
+                    b.max_pos = 1;
+                    b.interleaved = 1;
+                    b.n_heads = cfg.n_heads;
+                    b.k = k;
+                    b.v = v;
+                    b.k_ld = b.v_ld = (int64_t)row;
+                    launch_kv8_append(b, st);
+                    continue;
+                }
                 a.L = kvq->layer(l);
                 a.rows = KvqRows{n, nullptr, nullptr, p0, kvq_table, 1, kvq->cfg.n_pages};
                 launch_kvq_append(a, st);
@@ -796,10 +817,10 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
     const bool spread = !fused && M > 16 && M <= 64;
     const int sp_parts = resid_u_parts(H);
     // K and V rows read once per layer by the attention: [0, P + M) of every KV head
-    const double kv_bytes = 2.0 * c.n_kv_heads * (double)(P + M) * (kvq ? kvq_block_bytes(c.head_dim) / 64.0 : c.head_dim * 2.0);
+    const double kv_bytes = 2.0 * c.n_kv_heads * (double)(P + M) * (kv8() ? c.head_dim : kvq ? kvq_block_bytes(c.head_dim) / 64.0 : c.head_dim * 2.0);
     KvqPlan kvq_plan{};
     if (kvq) kvq_plan = kvq->plan(M, 1, M, P + M);
-    if (kvq_plan.ws_bytes > kvq_ws_bytes) throw BackendError("the 4-bit attention's workspace is too small");
+    if (kvq_plan.ws_bytes > kvq_ws_bytes) throw BackendError("the attention's workspace is too small");
     // up to 16 rows, with the epilogues fused, the attention's workgroups join
     // the Q/K/V launch where its shape allows (qkv_attention_fits)
     auto qa_fits = [&](const GemmParams &g, const AttnParams &at) {
@@ -852,7 +873,7 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
             p.K = H;
             p.M = M;
             p.mode = GM_STORE;
-            p.allow_split = kvq ? 0 : split_ok;  // the 4-bit append reads whole sums
+            p.allow_split = kvq ? 0 : split_ok;  // the append to blocks reads whole sums
             if (spread) {
                 p.norm_ssq = ssq;
                 p.norm_parts = sp_parts;
@@ -936,8 +957,30 @@ void Model::forward(const int *ids, const int *pos, const uint64_t *mask, int ma
             kt.n_rep = c.n_heads / c.n_kv_heads;
             kt.scale = a.scale;
             const int ev = prof_on ? prof_begin() : 0;
-            launch_kvq_append(ka, st);
-            launch_kvq_attention(kt, kvq_plan, kvq_ws, st);
+            if (kv8()) {
+                Kv8Append k8{};
+                k8.L = Kv8Layer(ka.L);
+                k8.seqs = {M, 1, M, nullptr, nullptr, P + M, kvq_table, kvq->cfg.n_pages};
+                k8.pos = ka.pos;
+                k8.cos_t = ka.cos_t;
+                k8.sin_t = ka.sin_t;
+                k8.max_pos = ka.max_pos;
+                k8.interleaved = ka.interleaved;
+                k8.n_heads = ka.n_heads;
+                k8.f32 = 1;
+                k8.q = ka.q;
+                k8.k = ka.k;
+                k8.v = ka.v;
+                k8.q_ld = k8.k_ld = k8.v_ld = QKVD;
+                k8.q_out = q16;
+                launch_kv8_append(k8, st);
+                Kv8Attn k8t{};
+                static_cast<KvqAttn &>(k8t) = kt;
+                launch_kv8_attention(k8t, kvq_plan, kvq_ws, st);
+            } else {
+                launch_kvq_append(ka, st);
+                launch_kvq_attention(kt, kvq_plan, kvq_ws, st);
+            }
             if (prof_on) prof_end(ev, PC_ATTN, kv_bytes);
         } else {
             RopeKvParams r{};
@@ -1169,6 +1212,10 @@ void Model::compact_tail(int P, const std::vector<int> &src) {
     std::memcpy(h_stage, src.data(), n * sizeof(int));
     SD_HIP_CHECK(hipMemcpyAsync(d_src, h_stage, n * sizeof(int), hipMemcpyHostToDevice, st));
     stage_done();
+    if (kv8()) {
+        launch_kv8_keep_tail(Kv8Layer(kvq->layer(0)), kvq->layer_bytes, cfg.n_layers, kvq_table, P, d_src, n, st);
+        return;
+    }
     if (kvq) {
         launch_kvq_keep_tail(kvq->layer(0), kvq->layer_bytes, cfg.n_layers, kvq_table, P, d_src, n, st);
         return;

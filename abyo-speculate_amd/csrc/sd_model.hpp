@@ -142,15 +142,16 @@ class Model {
     static constexpr int kPromptRows = 2048;
     int prompt_rows = 0;
 
-    // The cache's format: fp16 in `kv`, or 4 bits in the pages of `kvq` (whose
-    // table names them in order, so that a position's place is its own).  Either
-    // one is allocated.  Changing it drops what is cached.
-    enum { KV_F16 = 1, KV_Q4 = 2 };
+    // The cache's format: fp16 in `kv`, or 4 or 8 bits in the pages of `kvq` (whose
+    // table names them in order, so that a position's place is its own).  One of
+    // them is allocated.  Changing it drops what is cached.
+    enum { KV_F16 = 1, KV_Q4 = 2, KV_Q8 = 3 };
     static constexpr int kKvqPage = 256;
     void set_kv_format(int fmt);
     // cache rows [pos0, pos0 + n) of one (layer, K or V, KV head) as fp16 [n][hd]
     void read_kv_rows(int layer, int which, int head, size_t pos0, size_t n, uint16_t *out);
     std::unique_ptr<KvPool> kvq;
+    bool kv8() const { return kvq && kvq->cfg.bits == 8; }
     int *kvq_table = nullptr;
     void *kvq_ws = nullptr;
     size_t kvq_ws_bytes = 0;

@@ -35,7 +35,7 @@ SD_OK, SD_ERR_SAMPLING, SD_ERR_ROLLBACK, SD_ERR_BACKEND, SD_ERR_ARG, SD_ERR_UNSU
 # formats (GGML type ids)
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
 F16 = 1  # rows of the operators on device memory
-KV_F16, KV_Q4 = 1, 2  # formats of a decoder's cache
+KV_F16, KV_Q4, KV_Q8 = 1, 2, 3  # formats of a decoder's cache
 # tensor kinds
 (TOK_EMBD, OUTPUT, OUTPUT_NORM, ATTN_Q, ATTN_K, ATTN_V, ATTN_OUTPUT, FFN_GATE, FFN_UP, FFN_DOWN,
  ATTN_NORM, FFN_NORM, ATTN_Q_BIAS, ATTN_K_BIAS, ATTN_V_BIAS) = range(15)
@@ -97,7 +97,7 @@ class Config:
     max_batch: int = 128
     tied_output: int = 0
     device: int = 0
-    kv_format: int = KV_F16  # KV_Q4: the cache in 4 bits (sd_model_set_kv_format)
+    kv_format: int = KV_F16  # KV_Q4, KV_Q8: the cache in 4 or 8 bits (sd_model_set_kv_format)
 
     def to_c(self) -> SdConfig:
         return SdConfig(**{k: getattr(self, k) for k, _ in SdConfig._fields_})
@@ -139,6 +139,32 @@ class KvQuery(ctypes.Structure):
                 ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p), ("n_seqs", ctypes.c_int32),
                 ("table_ld", ctypes.c_int32), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int32),
                 ("max_rows", ctypes.c_size_t), ("max_len", ctypes.c_size_t), ("scale", ctypes.c_float)]
+
+
+class KvSeqs(ctypes.Structure):
+    """sd_kv_seqs"""
+    _fields_ = [("rows", ctypes.c_size_t), ("row_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("n_seqs", ctypes.c_int32), ("table_ld", ctypes.c_int32),
+                ("max_rows", ctypes.c_size_t)]
+
+
+class KvWindow(ctypes.Structure):
+    """sd_kv_window"""
+    _fields_ = [("window", ctypes.c_size_t), ("sinks", ctypes.c_size_t)]
+
+
+class KvScores(ctypes.Structure):
+    """sd_kv_scores"""
+    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ld", ctypes.c_size_t), ("decay", ctypes.c_float)]
+
+
+class KvEvict(ctypes.Structure):
+    """sd_kv_evict"""
+    _fields_ = [("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p), ("new_table", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int32), ("table_ld", ctypes.c_int32), ("new_table_ld", ctypes.c_int32),
+                ("scores", ctypes.c_void_p), ("scores_ld", ctypes.c_size_t), ("scores_out", ctypes.c_void_p),
+                ("scores_out_ld", ctypes.c_size_t), ("budget", ctypes.c_size_t), ("sinks", ctypes.c_size_t),
+                ("recent", ctypes.c_size_t), ("kept", ctypes.c_void_p), ("new_len", ctypes.c_void_p)]
 
 
 class Sampling(ctypes.Structure):
@@ -247,6 +273,16 @@ def load_library(path: str = LIB_PATH):
         "sd_kvpool_read": ([P, I32, ctypes.POINTER(KvRows), P, P, P], I32),
         "sd_kvpool_attend_workspace": ([P, SZ, SZ, SZ, SZ], SZ),
         "sd_kvpool_attend": ([P, I32, ctypes.POINTER(KvQuery), P, SZ, P], I32),
+        "sd_kv8_create": ([ctypes.POINTER(KvPoolConfig), ctypes.POINTER(P)], I32),
+        "sd_kv8_destroy": ([P], None),
+        "sd_kv8_page_bytes": ([P], SZ),
+        "sd_kv8_append": ([P, I32, ctypes.POINTER(KvSeqs), I32, P, SZ, P, SZ, P, SZ, P, P, P], I32),
+        "sd_kv8_read": ([P, I32, ctypes.POINTER(KvRows), P, P, P], I32),
+        "sd_kv8_attend_workspace": ([P, SZ, SZ, SZ, SZ, ctypes.POINTER(KvWindow)], SZ),
+        "sd_kv8_attend": ([P, I32, ctypes.POINTER(KvQuery), ctypes.POINTER(KvWindow), P, P, SZ, P], I32),
+        "sd_kv8_weights": ([P, I32, ctypes.POINTER(KvQuery), ctypes.POINTER(KvWindow), P, ctypes.POINTER(KvScores), P], I32),
+        "sd_kv8_evict_workspace": ([P, SZ, SZ], SZ),
+        "sd_kv8_evict": ([P, I32, ctypes.POINTER(KvEvict), P, SZ, P], I32),
         "sd_sampler_create": ([I32, I32, I32, ctypes.POINTER(P)], I32),
         "sd_sampler_destroy": ([P], None),
         "sd_sampler_run": ([P, P, SZ, SZ, ctypes.POINTER(Sampling), P, P, P, P], I32),
@@ -669,7 +705,7 @@ class HipQuantDecoder:
             pass
 
     def set_kv_format(self, fmt: int):
-        """KV_F16 or KV_Q4, while the cache is empty."""
+        """KV_F16, KV_Q4 or KV_Q8, while the cache is empty."""
         _check(_lib.sd_model_set_kv_format(self._h, fmt))
 
     # ---- weights ----
@@ -1197,6 +1233,89 @@ class HipKvPool:
         a = KvQuery(q, q_ld, out, out_ld, rows, row_start, kv_len, table, n_seqs, table_ld, mask, mask_words, max_rows,
                     max_len, scale)
         _check(_lib.sd_kvpool_attend(self._h, layer, ctypes.byref(a), ws, ws_bytes, stream))
+
+
+class HipKv8Pool:
+    """A paged KV cache in 8 bits on one GPU with the attention over it, its
+    positions' attention weights and their eviction (sd_kv8_*).  Arguments
+    that are arrays are device addresses (int; 0 for an optional one that is
+    absent) of memory on the pool's GPU, `stream` a hipStream_t (0: the default
+    stream); calls enqueue and return."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_pages: int, page_tokens: int = 64,
+                 max_pos: int = 8192, rope_theta: float = 10000.0, interleaved: bool = True, device: int = 0):
+        load_library()
+        c = KvPoolConfig(n_layers, n_heads, n_kv_heads, head_dim, n_pages, page_tokens, max_pos, int(interleaved),
+                         rope_theta, device)
+        self._h = ctypes.c_void_p()
+        _check(_lib.sd_kv8_create(ctypes.byref(c), ctypes.byref(self._h)))
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value:
+            _lib.sd_kv8_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def page_bytes(self) -> int:
+        """Bytes of one page of one layer."""
+        return int(_lib.sd_kv8_page_bytes(self._h))
+
+    def append(self, layer: int, rows: int, row_start: int, kv_len: int, table: int, n_seqs: int, table_ld: int,
+               max_rows: int, k: int, v: int, dtype: int = F16, pos: int = 0, q: int = 0, q_out: int = 0, q_ld: int = 0,
+               k_ld: int = 0, v_ld: int = 0, stream: int = 0):
+        """The sequences' last rows k, v [rows][n_kv_heads][head_dim] (dtype F16
+        or F32) rotated, quantised and written; the rotated q rows go to q_out (fp16)."""
+        r = KvSeqs(rows, row_start, kv_len, table, n_seqs, table_ld, max_rows)
+        _check(_lib.sd_kv8_append(self._h, layer, ctypes.byref(r), dtype, q, q_ld, k, k_ld, v, v_ld, pos, q_out, stream))
+
+    def read(self, layer: int, n: int, slots: int, table: int, n_seqs: int, table_ld: int, k_out: int, v_out: int,
+             seqs: int = 0, stream: int = 0):
+        """The rows' keys and values as fp16 [n][n_kv_heads][head_dim]."""
+        r = KvRows(n, seqs, slots, table, n_seqs, table_ld)
+        _check(_lib.sd_kv8_read(self._h, layer, ctypes.byref(r), k_out, v_out, stream))
+
+    def attend_workspace(self, rows: int, n_seqs: int, max_rows: int, max_len: int, window: int = 0, sinks: int = 0) -> int:
+        """Bytes of device memory attend() needs for these sizes; one workspace per call in flight."""
+        w = KvWindow(window, sinks)
+        return int(_lib.sd_kv8_attend_workspace(self._h, rows, n_seqs, max_rows, max_len, ctypes.byref(w)))
+
+    def attend(self, layer: int, q: int, out: int, row_start: int, kv_len: int, table: int, n_seqs: int, table_ld: int,
+               rows: int, max_rows: int, max_len: int, ws: int = 0, ws_bytes: int = 0, mask: int = 0, mask_words: int = 0,
+               scale: float = 0.0, q_ld: int = 0, out_ld: int = 0, window: int = 0, sinks: int = 0, lse: int = 0,
+               stream: int = 0):
+        """Attention of the sequences' last rows over their positions (sd_kv_query), with a
+        window over the last `window` of them and the first `sinks`; lse: the rows' log-sum-exps."""
+        a = KvQuery(q, q_ld, out, out_ld, rows, row_start, kv_len, table, n_seqs, table_ld, mask, mask_words, max_rows,
+                    max_len, scale)
+        w = KvWindow(window, sinks)
+        _check(_lib.sd_kv8_attend(self._h, layer, ctypes.byref(a), ctypes.byref(w), lse, ws, ws_bytes, stream))
+
+    def weights(self, layer: int, q: int, lse: int, scores: int, ld: int, row_start: int, kv_len: int, table: int, n_seqs: int,
+                table_ld: int, rows: int, max_rows: int, max_len: int, previous: int = 0, decay: float = 1.0, mask: int = 0,
+                mask_words: int = 0, scale: float = 0.0, q_ld: int = 0, window: int = 0, sinks: int = 0, stream: int = 0):
+        """scores [n_seqs][n_kv_heads][ld] = decay * previous + each position's attention weight from the rows."""
+        a = KvQuery(q, q_ld, 0, 0, rows, row_start, kv_len, table, n_seqs, table_ld, mask, mask_words, max_rows, max_len,
+                    scale)
+        w, s = KvWindow(window, sinks), KvScores(previous, scores, ld, decay)
+        _check(_lib.sd_kv8_weights(self._h, layer, ctypes.byref(a), ctypes.byref(w), lse, ctypes.byref(s), stream))
+
+    def evict_workspace(self, n_seqs: int, budget: int) -> int:
+        """Bytes of device memory an eviction in place needs."""
+        return int(_lib.sd_kv8_evict_workspace(self._h, n_seqs, budget))
+
+    def evict(self, layer: int, kv_len: int, table: int, n_seqs: int, table_ld: int, scores: int, scores_ld: int, budget: int,
+              kept: int, new_len: int, sinks: int = 0, recent: int = 0, scores_out: int = 0, scores_out_ld: int = 0,
+              new_table: int = 0, new_table_ld: int = 0, ws: int = 0, ws_bytes: int = 0, stream: int = 0):
+        """Every sequence's heads keep their `budget` positions of the largest scores, the
+        first `sinks` and the last `recent` among them, in place or in new_table's pages."""
+        e = KvEvict(kv_len, table, new_table, n_seqs, table_ld, new_table_ld, scores, scores_ld, scores_out, scores_out_ld,
+                    budget, sinks, recent, kept, new_len)
+        _check(_lib.sd_kv8_evict(self._h, layer, ctypes.byref(e), ws, ws_bytes, stream))
 
 
 class HipSampler:

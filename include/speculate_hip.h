@@ -107,14 +107,16 @@ sd_status sd_model_create(const sd_config *cfg, sd_model **out);
 void sd_model_destroy(sd_model *m);
 
 /* The KV cache's format, while it is empty (after creation or sd_reset;
- * SD_ERR_ARG otherwise): fp16 as created, or the 4-bit blocks of sd_kvpool_*
- * below, 4.5 bits a value, which every entry point of the handle then appends
- * to and attends over.  Rows are rotated with the handle's own RoPE tables.
- * A handle of the 4-bit format does not keep row i of an M-row call equal
- * to the one-row call bit for bit.  On failure the format stays.  A handle is
- * created with the fp16 cache, and both exist while the format changes: the
- * context has to fit both. */
-enum { SD_KV_F16 = 1, SD_KV_Q4 = 2 };
+ * SD_ERR_ARG otherwise): fp16 as created, the 4-bit blocks of sd_kvpool_*
+ * below, 4.5 bits a value, or the 8-bit ones of sd_kv8_*, 8.02 bits a value of
+ * heads of 128, which every entry point of the handle then appends to and
+ * attends over.  Rows are rotated with the handle's own RoPE tables.  A handle
+ * of a 4-bit or 8-bit format does not keep row i of an M-row call equal to the
+ * one-row call bit for bit; in 8 bits the rows of one call share their block's
+ * scale.  On failure the format stays.  A handle is created with the fp16
+ * cache, and both caches exist while the format changes: the context has to
+ * fit both. */
+enum { SD_KV_F16 = 1, SD_KV_Q4 = 2, SD_KV_Q8 = 3 };
 sd_status sd_model_set_kv_format(sd_model *m, int32_t format);
 
 /* Uploads one tensor given in its GGUF byte layout (`layer` = -1 for the
@@ -491,6 +493,134 @@ size_t sd_kvpool_attend_workspace(const sd_kvpool *c, size_t rows, size_t n_seqs
  * bytes of ws that the call needs do not overlap (SD_ERR_ARG). */
 sd_status sd_kvpool_attend(sd_kvpool *c, int32_t layer, const sd_kv_query *query, void *ws, size_t ws_bytes,
                            void *stream);
+
+/* ---- a paged KV cache in 8 bits that can be kept short (device memory) ---------- */
+/* Next to the 4-bit one: closer to the fp16 values, with attention through a
+ * sliding window, the attention weight of each position, and eviction by it.
+ * 32 positions of a KV head, from a multiple of 32 on, are a block, whose keys
+ * and whose values have one scale each: the smallest 2^E, E in [-15, 8], with
+ * A <= 448 * 2^E, A the largest magnitude of what the block holds.  A value x
+ * is stored as the 8-bit float nearest to x / 2^E (4 exponent bits, 3 of
+ * mantissa, halves to even) and stands for that times 2^E, an fp16 number (what
+ * would be 2^16 is 61440).  A
+ * row (a position's keys or values of one head) with a value that is not
+ * finite or above 65504 stands for NaN in all its channels and does not count
+ * for the scale.  8.02 bits a value of heads of 128 channels, 8.03 of 64.
+ *
+ * Pointers, streams, captures and ordering are as for sd_kvpool_*: device
+ * memory of the pool's GPU; calls enqueue on `stream`, allocate nothing, can be
+ * captured and leave the current device as it was; calls that touch the same
+ * pages or workspace are ordered by the caller. */
+typedef struct sd_kv8 sd_kv8;
+/* Pages are zeroed.  The config's limits are sd_kvpool_create's. */
+sd_status sd_kv8_create(const sd_kvpool_config *cfg, sd_kv8 **out);
+void sd_kv8_destroy(sd_kv8 *c);
+/* bytes of one page of one layer */
+size_t sd_kv8_page_bytes(const sd_kv8 *c);
+
+/* The rows of a call: rows row_start[s] .. row_start[s + 1) are the last
+ * positions of sequence s, which holds kv_len[s] (up to 2^31 - 64) with them.
+ * Rows outside every sequence, rows past max_rows of one, and rows that fall on
+ * a negative position are left out: nothing is written for them.  Position p
+ * lives in page table[s * table_ld + p / page_tokens]; keys and values of
+ * positions past the table, or in pages whose id is outside the pool, are not
+ * written. */
+typedef struct sd_kv_seqs {
+    size_t rows;                /* rows of the inputs */
+    const int32_t *row_start;   /* [n_seqs + 1] */
+    const int32_t *kv_len;      /* [n_seqs] */
+    const int32_t *table;       /* [n_seqs][table_ld] */
+    int32_t n_seqs, table_ld;
+    size_t max_rows;            /* most rows of one sequence (host bound of row_start) */
+} sd_kv_seqs;
+/* Appends k and v [rows][n_kv_heads][head_dim] (fmt SD_F16 or SD_F32, row
+ * strides k_ld and v_ld elements, 0: dense) to a layer: k rotated to pos[r]
+ * (the row's own position with pos NULL; after an eviction the two differ),
+ * both quantised.  What a block holds in front of the rows stays, in the scale
+ * that the block has now; what it held behind them is gone: the rows are the
+ * sequence's end.  No block is written by two sequences of a call.  With q
+ * [rows][n_heads][head_dim], the rotated queries go to q_out [rows][n_heads]
+ * [head_dim] fp16, which overlaps none of the rows of q, k and v (SD_ERR_ARG);
+ * q NULL: keys and values only.  A row whose rotation position is outside
+ * [0, max_pos) is NaN in all three.  Rows must start at multiples of 16
+ * bytes. */
+sd_status sd_kv8_append(sd_kv8 *c, int32_t layer, const sd_kv_seqs *seqs, int32_t fmt, const void *q, size_t q_ld,
+                        const void *k, size_t k_ld, const void *v, size_t v_ld, const int32_t *pos, uint16_t *q_out,
+                        void *stream);
+/* As sd_kvpool_read (any positions, in any order); the outputs do not overlap. */
+sd_status sd_kv8_read(sd_kv8 *c, int32_t layer, const sd_kv_rows *rows, uint16_t *k_out, uint16_t *v_out, void *stream);
+
+/* As sd_kvpool_attend, and: with a window, a row at position p sees of what its
+ * mask shows the positions below `sinks` and those above p - window (its own
+ * and window - 1 before it; of a tree's rows too the positions count, not the
+ * depths).  window NULL or of 0: all.  lse, f32 [rows][n_heads] or NULL: the
+ * logarithm of the sum of exp(scale q k) over what the row sees, -inf where
+ * that is nothing; like out it is left as it was for rows that have no
+ * sequence.  Work is cut by the sequences' own lengths: max_len only bounds the
+ * number of ranges (from 64 positions a range on its size hardly matters), and
+ * larger kv_len stay correct.  lse overlaps neither q, out nor the workspace
+ * (SD_ERR_ARG). */
+typedef struct sd_kv_window {
+    size_t window, sinks;
+} sd_kv_window;
+size_t sd_kv8_attend_workspace(const sd_kv8 *c, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len,
+                               const sd_kv_window *window);
+sd_status sd_kv8_attend(sd_kv8 *c, int32_t layer, const sd_kv_query *query, const sd_kv_window *window, float *lse, void *ws,
+                        size_t ws_bytes, void *stream);
+
+/* What each position gets of the rows' attention, added to what it had: for
+ * every sequence s that has rows, KV head h and position j < min(kv_len[s], ld)
+ *   out[s][h][j] = decay * in[s][h][j] + the sum over the sequence's rows and
+ *                  the query heads of h, where they see j, of
+ *                  exp(scale q k_j - lse)
+ * with the query, mask, window and lse of an sd_kv8_attend over the same cache
+ * (query->out is not used; max_len bounds the grid, larger kv_len stay
+ * correct).  in may be out, or NULL or decay 0: `in` is not read.  Otherwise
+ * out overlaps neither in, q nor lse (SD_ERR_ARG).  Entries past the length
+ * stay as they were.  Sums are fp32 and always added in the same order. */
+typedef struct sd_kv_scores {
+    const float *in;
+    float *out;                 /* [n_seqs][n_kv_heads][ld] */
+    size_t ld;
+    float decay;
+} sd_kv_scores;
+sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *query, const sd_kv_window *window, const float *lse,
+                         const sd_kv_scores *scores, void *stream);
+
+/* Cuts sequences down to `budget` positions, each KV head by its own scores:
+ * the first `sinks` and the last `recent` stay, and of the others those with the
+ * largest scores (of equal ones the first; NaN counts as less than everything)
+ * until the budget is reached.  What stays keeps its order and moves to
+ * positions 0, 1, ..., in place (new_table NULL), or in the pages of new_table,
+ * which are none of the table's; blocks get the scales of what they hold now.
+ * A sequence of at most `budget` positions stays as it is, in new pages as a
+ * copy.  kv_len counts up to the table's and scores_ld's end.
+ *   kept        [n_seqs][n_kv_heads][budget]: the position each one had, -1
+ *               past the new length
+ *   new_len     [n_seqs]: min(kv_len, budget)
+ *   scores_out  [n_seqs][n_kv_heads][scores_out_ld] (0: budget) or NULL: the
+ *               scores of what stays; may be `scores` with its stride; entries
+ *               past the new length are left as they were
+ * Keys keep the rotation of the positions they had: later rows are appended
+ * with `pos`.  Outputs and the workspace overlap neither the inputs (but for
+ * scores_out) nor each other (SD_ERR_ARG).  Positions of absent pages stand
+ * for zeros, and what goes to one is dropped. */
+typedef struct sd_kv_evict {
+    const int32_t *kv_len;      /* [n_seqs] */
+    const int32_t *table;       /* [n_seqs][table_ld] */
+    const int32_t *new_table;   /* [n_seqs][new_table_ld] or NULL: in place */
+    int32_t n_seqs, table_ld, new_table_ld;
+    const float *scores;        /* [n_seqs][n_kv_heads][scores_ld] */
+    size_t scores_ld;
+    float *scores_out;
+    size_t scores_out_ld;
+    size_t budget, sinks, recent;
+    int32_t *kept, *new_len;
+} sd_kv_evict;
+/* Bytes of workspace for an eviction in place (none is needed into new pages). */
+size_t sd_kv8_evict_workspace(const sd_kv8 *c, size_t n_seqs, size_t budget);
+/* ws: 16-byte aligned device memory, whatever it holds; each call in flight needs its own. */
+sd_status sd_kv8_evict(sd_kv8 *c, int32_t layer, const sd_kv_evict *evict, void *ws, size_t ws_bytes, void *stream);
 
 /* ---- sampling (device memory) ----------------------------------------------------- */
 /* One token per row of logits from a given random number, with the filters
