@@ -119,11 +119,25 @@ template <int HD> __device__ __forceinline__ void kv8_codes_in(Kv8Sh &sh, const 
     if constexpr (HD == 128) *(uintx4 *)(sh.codes + threadIdx.x * 16) = *(const uintx4 *)(at + threadIdx.x * 16);
     else *(uintx2 *)(sh.codes + threadIdx.x * 8) = *(const uintx2 *)(at + threadIdx.x * 8);
 }
-// the C channels from c0 of position k of a block's codes
+// the values of 4 codes
+template <typename T> __device__ __forceinline__ void kv8_values(uint32_t w, float scale, T *x) {
+    const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = (T)(a.x * scale), x[1] = (T)(a.y * scale), x[2] = (T)(b.x * scale), x[3] = (T)(b.y * scale);
+}
+// the HD / 8 channels from c0 of position k of a block's codes
 template <int HD, bool V, typename T>
 __device__ __forceinline__ void kv8_row(const uint8_t *codes, int k, int c0, float scale, T (&x)[HD / 8]) {
+    if constexpr (V) {
 #pragma unroll
-    for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[V ? kv8_v_at(k, c0 + i, HD) : kv8_k_at(k, c0 + i, HD)], scale);
+        for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[kv8_v_at(k, c0 + i, HD)], scale);
+    } else {
+#pragma unroll
+        for (int i = 0; i < HD / 8; i += 8) {
+            const uintx2 w = *(const uintx2 *)(codes + kv8_k_at(k, c0 + i, HD));
+            kv8_values(w.x, scale, x + i);
+            kv8_values(w.y, scale, x + i + 4);
+        }
+    }
 }
 
 }  // namespace sd
