@@ -36,13 +36,15 @@ template <int HD> struct Kv8Step {
     uintx4 k[2][HD / 64];  // [kt][16 channels each]
     uintx4 v[HD / 32];     // [two channels each]
 };
-template <int HD> __device__ __forceinline__ void kv8_load(Kv8Step<HD> &b, const uint8_t *codes, int lane) {
+// (nothing is read where bytes is 0)
+template <int HD> __device__ __forceinline__ void kv8_load(Kv8Step<HD> &b, const uint8_t *codes, uint32_t bytes, int lane) {
+    const rsrc_t r = make_rsrc(codes, bytes);
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-        for (int i = 0; i < HD / 64; i++) b.k[kt][i] = *(const uintx4 *)(codes + (kt * (HD / 64) + i) * 1024 + lane * 16);
+        for (int i = 0; i < HD / 64; i++) b.k[kt][i] = bld16(r, lane * 16, (kt * (HD / 64) + i) * 1024);
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) b.v[i] = *(const uintx4 *)(codes + 32 * HD + i * 1024 + lane * 16);
+    for (int i = 0; i < HD / 32; i++) b.v[i] = bld16(r, lane * 16, 32 * HD + i * 1024);
 }
 
 // ---- up to 64 queries, 16 or 32 to a workgroup ------------------------------------
@@ -79,60 +81,51 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
     const float sl2 = p.scale * 1.4426950408889634f;  // scores in base-2 units
     const int steps = (b1 - b0 - wave + kKvqWaves - 1) / kKvqWaves;  // blocks b0 + wave + 4 i
     auto block = [&](int i) { return kv8_nth(W, b0 + wave + i * kKvqWaves); };
-    // lane i holds the page (-1: holds no positions) and the header of step i of 64
+    // Lane k holds the page (-1: holds no positions) and the header of the step whose number modulo 64 is k, 32 of them asked for
+    // at a time: those of the steps before are still needed.
     int pg = -1;
     uintx4 heads = {0, 0, 0, 0};
     auto pages = [&](int i0) {
-        const int i = i0 + lane, b = i < steps ? block(i) : 0;
-        pg = i < steps ? kvq_page(p, at.s, b) : -1;
+        const int i = i0 + (lane & 31);
+        if ((lane ^ i0) & 32) return;
+        pg = i < steps ? kvq_page(p, at.s, block(i)) : -1;
         if (pg < 0 || pg >= p.L.n_pages) pg = -1;
-        else heads = *(const uintx4 *)L.head(pg, h, b * 32);
+        else heads = *(const uintx4 *)L.head(pg, h, block(i) * 32);
     };
-    Kv8Step<HD> next{};
-    int page = -1;
-    auto fetch = [&](int i) {
-        if ((i & 63) == 0) pages(i);
-        page = __builtin_amdgcn_readlane(pg, i & 63);
-        if (page >= 0) kv8_load<HD>(next, L.codes(page, h, block(i) * 32), lane);
+    // The loads of a step past the end, or without a page, are issued all the same and read nothing: how many are in flight is
+    // always known.
+    auto fetch = [&](Kv8Step<HD> &b, int i) __attribute__((always_inline)) {
+        const int page = i < steps ? __builtin_amdgcn_readlane(pg, i & 63) : -1;
+        kv8_load<HD>(b, L.codes(max(page, 0), h, block(min(i, steps - 1)) * 32), page >= 0 ? 64 * HD : 0, lane);
     };
-    if (steps > 0) fetch(0);
-    for (int i = 0; i < steps; i++) {
-        Kv8Step<HD> k = next;
-        const bool have = page >= 0;
+    const float hidden = sl2 < 0.f ? INFINITY : -INFINITY;  // a masked score before it is scaled
+    // No maximum is looked for: a query keeps the reference of its first block until eight of its weights add up to more than
+    // 2^15 (below fp16's range); then the reference is raised and they are taken again.  A fused weight is of the unrounded
+    // score, which beyond 2^28 may lie more than 16 from the rounded one that the reference came from, past fp16's end on
+    // either side: where the reference is beyond 2^24, weights are always taken again, of the rounded scores.
+    constexpr float kMost = 32768.f, kFused = 16777216.f;
+    auto process = [&](const Kv8Step<HD> &k, int i) __attribute__((always_inline)) {
+        if (__builtin_amdgcn_readlane(pg, i & 63) < 0) return;
         uint32_t hd[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) hd[j] = (uint32_t)__builtin_amdgcn_readlane((int)heads[j], i & 63);
-        if (i + 1 < steps) fetch(i + 1);
-        if (!have) continue;
         const float ks = __uint_as_float(hd[0]), vs = __uint_as_float(hd[1]);
         const int base = block(i) * 32, key0 = base + 8 * g;
         const bool clean = (hd[2] | hd[3]) == 0, full = clean && kv8_full(p, W, base, 32);
-        float st[QT][8];
-        {
-            floatx4 acc[QT][2];
+        floatx4 acc[QT][2];
 #pragma unroll
-            for (int t = 0; t < QT; t++) acc[t][0] = acc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < QT; t++) acc[t][0] = acc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int dc = 0; dc < NDC; dc++) {
-                half8 a[2];
+        for (int dc = 0; dc < NDC; dc++) {
+            half8 a[2];
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-                    a[kt] = __builtin_bit_cast(half8, kv8_expand(k.k[kt][dc >> 1][2 * (dc & 1)], k.k[kt][dc >> 1][2 * (dc & 1) + 1], ks));
-#pragma unroll
-                for (int t = 0; t < QT; t++)
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++)
-                        acc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kt], __builtin_bit_cast(half8, qf[t][dc]), acc[t][kt], 0, 0, 0);
-            }
+            for (int kt = 0; kt < 2; kt++)
+                a[kt] = __builtin_bit_cast(half8, kv8_expand(k.k[kt][dc >> 1][2 * (dc & 1)], k.k[kt][dc >> 1][2 * (dc & 1) + 1], ks));
 #pragma unroll
             for (int t = 0; t < QT; t++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    // rounded here, not inside the weight: beyond 2^28 the rounding is more than fp16 has room for, so what is
-                    // weighed must be what the maximum is taken of
-#pragma clang fp contract(off)
-                    st[t][j] = acc[t][j >> 2][j & 3] * sl2;
-                }
+                for (int kt = 0; kt < 2; kt++)
+                    acc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kt], __builtin_bit_cast(half8, qf[t][dc]), acc[t][kt], 0, 0, 0);
         }
         uint32_t vis[QT];
         if (!full) {
@@ -142,31 +135,53 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
                 vis[t] = kv8_visible<8>(p, W, min(W.q0 + t * 16 + r16, W.nq - 1) / p.n_rep, key0);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    if (!clean && (kn >> j & 1)) st[t][j] = NAN;
-                    st[t][j] = (vis[t] >> j) & 1 ? st[t][j] : -INFINITY;
+                    float &s = ((float *)&acc[t][j >> 2])[j & 3];
+                    if (!clean && (kn >> j & 1)) s = NAN;
+                    s = (vis[t] >> j) & 1 ? s : hidden;
                 }
             }
         }
         uintx4 pk[QT];
+        float sum[QT];
+        bool again = false;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-            float top = st[t][0];
+            const float mu = m[t] == -INFINITY ? 0.f : m[t];
+            sum[t] = 0.f;
 #pragma unroll
-            for (int j = 1; j < 8; j++) top = fmaxf(top, st[t][j]);
-            // The reference moves only for a score that would weigh more than 2^15.  By the difference, which is exact for
-            // neighbouring scores: beyond 2^27 the reference and 15 add up to the score that is 16 above it.
-            if (__builtin_amdgcn_ballot_w64(top - m[t] > 15.f) != 0) {
-                const float tm = xmax4(top);
-                if (tm - m[t] > 15.f) {
-                    const float cm = tm - kKvqHead, alpha = __builtin_amdgcn_exp2f(m[t] - cm);
+            for (int j = 0; j < 4; j++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][j >> 1][(2 * j) & 3], sl2, -mu));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][j >> 1][(2 * j + 1) & 3], sl2, -mu));
+                sum[t] += x + y;
+                pk[t][j] = h2bits(half2v{(_Float16)x, (_Float16)y});
+            }
+            again |= sum[t] > kMost || !(fabsf(m[t]) < kFused);
+        }
+        if (__builtin_amdgcn_ballot_w64(again) != 0) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float st[8], top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    // rounded here, not inside the weight: what is weighed is what the maximum is taken of
+#pragma clang fp contract(off)
+                    st[j] = acc[t][j >> 2][j & 3] * sl2;
+                    top = fmaxf(top, st[j]);
+                }
+                const float cm = xmax4(top) - kKvqHead;
+                if (cm > m[t]) {
+                    const float alpha = __builtin_amdgcn_exp2f(m[t] - cm);
                     m[t] = cm;
                     l[t] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < NDT; dt++) o[t][dt] *= alpha;
                 }
+                sum[t] = 0.f;
+                pk[t] = kvq_weights(st, m[t] == -INFINITY ? 0.f : m[t], sum[t]);
             }
-            pk[t] = kvq_weights(st[t], m[t] == -INFINITY ? 0.f : m[t], l[t]);
         }
+#pragma unroll
+        for (int t = 0; t < QT; t++) l[t] += sum[t];
 #pragma unroll
         for (int dt = 0; dt < NDT; dt++) {
             const half8 a = __builtin_bit_cast(half8, kv8_expand(k.v[dt >> 1][2 * (dt & 1)], k.v[dt >> 1][2 * (dt & 1) + 1], vs));
@@ -186,6 +201,19 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
                     for (int dt = 0; dt < NDT; dt++) o[t][dt] = floatx4{NAN, NAN, NAN, NAN};
                 }
             }
+        }
+    };
+    if (steps > 0) {
+        Kv8Step<HD> even, odd;
+        pages(0);
+        fetch(even, 0);
+        fetch(odd, 1);
+        for (int i = 0; i < steps; i += 2) {
+            process(even, i);
+            if (((i + 2) & 31) == 0) pages(i + 2);
+            fetch(even, i + 2);
+            if (i + 1 < steps) process(odd, i + 1);
+            fetch(odd, i + 3);
         }
     }
     // the four waves' states, one query tile at a time
