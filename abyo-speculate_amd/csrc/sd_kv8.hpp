@@ -104,11 +104,25 @@ void launch_kv8_read(const Kv8Layer &L, const KvqRows &rows, uint16_t *k_out, ui
 void launch_kv8_keep_tail(const Kv8Layer &L0, int64_t layer_bytes, int n_layers, const int *table, int P, const int *src,
                           int n, hipStream_t st);
 
+// Division by a number that the host knows, of n < 2^31: with 2^L >= d, m = floor(2^(31 + L) / d) + 1
+// is at most 2^L / 2^(31 + L) of a quotient's unit too large for each unit of n.
+struct Kv8Div {
+    uint32_t d, m;
+    int shift;
+    static Kv8Div by(uint32_t d) {
+        int l = 0;
+        while ((1ull << l) < d) l++;
+        return {d, (uint32_t)((1ull << (31 + l)) / d + 1), 31 + l};
+    }
+    __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> shift); }
+};
+
 // Attention: the 4-bit one's parameters (L the 8-bit layer's), and
 struct Kv8Attn : KvqAttn {
     int window, sinks;  // 0: no window; else row p sees of what its mask shows the positions below sinks and above p - window
     float *lse;         // [rows][n_heads] ln of the sum of exp(score), or null
     int min_blocks;     // of a key range, from the plan
+    Kv8Div by_rep, by_kv, by_tiles, by_groups;  // n_rep, KV heads, tiles, groups
 };
 KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int window, int sinks,
                       int cus);

@@ -56,7 +56,8 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
     __shared__ float sh_o[kKvqWaves][16][HD];
     __shared__ float sh_ml[kKvqWaves][16][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
-    const KvqPlace at = kvq_place(p);
+    warm_kernargs<sizeof(Kv8Attn)>();
+    const KvqPlace at = kv8_place(p);
     const int split = at.split, h = at.h;
     Kv8Work W;
     if (!kv8_work(p, at.s, at.tile, QT * 16, W)) return;
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
     float m[QT], l[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        const uint16_t *qr = kvq_query(p, W, h, W.q0 + t * 16 + r16);
+        const uint16_t *qr = kv8_query(p, W, h, W.q0 + t * 16 + r16);
 #pragma unroll
         for (int dc = 0; dc < NDC; dc++) qf[t][dc] = *(const uintx4 *)(qr + 8 * (g * NDC + dc));
 #pragma unroll
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
             const uint32_t kn = hd[2] >> (8 * g) & 0xffu;
 #pragma unroll
             for (int t = 0; t < QT; t++) {
-                vis[t] = kv8_visible<8>(p, W, min(W.q0 + t * 16 + r16, W.nq - 1) / p.n_rep, key0);
+                vis[t] = kv8_visible<8>(p, W, p.by_rep.quot(min(W.q0 + t * 16 + r16, W.nq - 1)), key0);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     float &s = ((float *)&acc[t][j >> 2])[j & 3];
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
             for (int c = 0; c < HD / 16; c++) oc[c] += sh_o[w][tq][tc + c] * f;
         }
         if (q < W.nq) {
-            const int row = W.r0 + q / p.n_rep, head = h * p.n_rep + q % p.n_rep;
+            const int m = p.by_rep.quot(q), row = W.r0 + m, head = h * p.n_rep + q - m * p.n_rep;
             kvq_emit<HD / 16>(p, split, row, head, tc, oc, M, lw, tc == 0);
             if (p.nsplit == 1 && p.lse && tc == 0) p.lse[(int64_t)row * p.n_heads + head] = kv8_lse(M, lw);
         }
@@ -265,9 +266,12 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
     constexpr int LS = HD / 4, N = 256 / LS, U = 4;  // lanes of a split, splits of a round, rounds in flight
     __shared__ __align__(16) float sh[N][HD];
     const int s = blockIdx.y, lane = threadIdx.x & 63, mine = threadIdx.x / LS, c = threadIdx.x % LS * 4;
-    const int mr = blockIdx.x / p.n_heads, head = blockIdx.x % p.n_heads;
+    warm_kernargs<sizeof(Kv8Attn)>();
+    // (heads are n_rep to each of the KV heads)
+    const int mh = p.by_rep.quot(blockIdx.x), mr = p.by_kv.quot(mh), r = blockIdx.x - mh * p.n_rep;
+    const int head = (mh - mr * p.L.n_kv) * p.n_rep + r, tile = (mr * p.n_rep + r) >> (31 - __builtin_clz((unsigned)p.tile_q));
     Kv8Work W;
-    if (!kv8_work(p, s, (mr * p.n_rep + head % p.n_rep) / p.tile_q, p.tile_q, W)) return;
+    if (!kv8_work(p, s, tile, p.tile_q, W)) return;
     if (mr >= min(W.n, p.max_rows)) return;
     const int row = W.r0 + mr, ns = kv8_cut(p, W.total).n;
     const int64_t at = (int64_t)row * p.n_heads + head, step = (int64_t)p.rows * p.n_heads;
@@ -309,9 +313,12 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
     if (p.lse && d == 0) p.lse[at] = kv8_lse(M, l);
 }
 
-// Tiles of 16 or 32 queries; ranges as many as give every CU two workgroups (four
-// times as many in a batch, whose lengths differ), each of at least a block for each
-// wave.  A sequence's own length decides how many of them it has and how long they are.
+// Tiles of 16 or 32 queries.  Ranges: as many as give every CU two workgroups, one where
+// there is a single tile in a single sequence (5 rows of 32 heads over 8 and 8192 positions
+// 14.1 us, with two 16.9; a batch of 16 sequences with two 17.2 us, with one 19.5, with
+// eight 20; 60 rows over 8192 positions with two 28.2, with four 33.6), each of at least a
+// block for each wave.  A sequence's own length decides how many of them it has and how
+// long they are.
 KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int window, int sinks,
                       int cus) {
     KvqPlan r{};
@@ -321,7 +328,7 @@ KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
     // most blocks that a tile sees
     int64_t blocks = (max_len + 31) / 32;
     if (window > 0) blocks = std::min(blocks, ((int64_t)window + r.tile_q + 62) / 32 + ((int64_t)sinks + 31) / 32);
-    const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, fill = n_seqs > 1 ? 8 * cus : 2 * cus;
+    const int64_t groups = (int64_t)r.tiles * n_kv * n_seqs, fill = groups > n_kv ? 2 * cus : cus;
     const int64_t want = (fill + groups - 1) / groups, most = std::max<int64_t>(1, blocks / 4);
     r.nsplit = (int)std::max<int64_t>(1, std::min({want, most, (int64_t)64}));
     return r;
@@ -345,6 +352,10 @@ void launch_kv8_attention(const Kv8Attn &in, const KvqPlan &plan, void *ws, hipS
     p.tiles = plan.tiles;
     p.min_blocks = 4;
     p.groups = p.tiles * p.L.n_kv * p.n_seqs;
+    p.by_rep = Kv8Div::by((uint32_t)p.n_rep);
+    p.by_kv = Kv8Div::by((uint32_t)p.L.n_kv);
+    p.by_tiles = Kv8Div::by((uint32_t)p.tiles);
+    p.by_groups = Kv8Div::by((uint32_t)p.groups);
     p.part_o = (float *)ws;
     p.part_ml = p.part_o + (int64_t)p.nsplit * p.rows * p.n_heads * p.L.hd;
     if (p.L.hd == 128) launch_attn<128>(p, st);

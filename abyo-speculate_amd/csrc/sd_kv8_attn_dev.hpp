@@ -6,6 +6,20 @@
 
 namespace sd {
 
+// kvq_place and kvq_query without divisions
+__device__ __forceinline__ KvqPlace kv8_place(const Kv8Attn &p) {
+    KvqPlace r;
+    const uint32_t id = blockIdx.x, n = (uint32_t)p.groups;
+    r.split = (int)p.by_groups.quot(id);
+    uint32_t i = id - r.split * n + (uint32_t)r.split;
+    i -= p.by_groups.quot(i) * n;
+    const uint32_t a = p.by_kv.quot(i);
+    r.h = (int)(i - a * (uint32_t)p.L.n_kv);
+    r.s = (int)p.by_tiles.quot(a);
+    r.tile = (int)(a - r.s * (uint32_t)p.tiles);
+    return r;
+}
+
 // Rows and positions of a workgroup's sequence, its queries and their blocks.
 struct Kv8Work {
     int r0, n, T, P;   // row i of n is row r0 + i of the call and position P + i
@@ -27,7 +41,7 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &p, int s, int tile, int 
     if (w.q0 >= w.nq) return false;
     w.T = min(w.T, kKv8MaxLen);
     w.P = w.T - w.n;
-    const int m_first = w.q0 / p.n_rep, m_last = (min(w.q0 + tile_q, w.nq) - 1) / p.n_rep;
+    const int m_first = p.by_rep.quot(w.q0), m_last = p.by_rep.quot(min(w.q0 + tile_q, w.nq) - 1);
     w.t_end = p.mask ? w.T : min(w.T, w.P + m_last + 1);
     w.t_all = p.mask ? w.P : w.P + m_first + 1;
     // blocks that hold positions the table has pages for
@@ -41,6 +55,11 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &p, int s, int tile, int 
     }
     w.total = w.nsink + nblk - w.b_win;
     return true;
+}
+__device__ __forceinline__ const uint16_t *kv8_query(const Kv8Attn &p, const Kv8Work &w, int h, int q) {
+    q = min(q, w.nq - 1);
+    const int m = p.by_rep.quot(q);
+    return p.q + (int64_t)(w.r0 + m) * p.q_row + (int64_t)(h * p.n_rep + q - m * p.n_rep) * p.q_head;
 }
 // whether every row of the tile sees all of positions [a, a + n)
 __device__ __forceinline__ bool kv8_full(const Kv8Attn &p, const Kv8Work &w, int a, int n) {

@@ -40,6 +40,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
     // in base 2, read a tile later than the queries
     __shared__ __align__(16) float sh_lse[4][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
+    warm_kernargs<sizeof(Kv8Weights)>();
     const int s = blockIdx.z, h = blockIdx.y;
     const Kv8Layer L(p.a.L);
     Kv8Work W;
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
         float lse[2];
         // The thread's query of the tile that is asked for next, and how far the next tile's is; past the last one it is the
         // sequence's first.
-        const int rows = W.nq / n_rep, step_row = 32 / n_rep, step_rep = 32 % n_rep;
+        const int rows = p.a.by_rep.quot(W.nq), step_row = p.a.by_rep.quot(32), step_rep = 32 - step_row * n_rep;
         const int64_t q_step = step_row * p.a.q_row + step_rep * p.a.q_head, q_wrap = p.a.q_row - n_rep * p.a.q_head;
         const int64_t s_step = step_row * (int64_t)p.a.n_heads + step_rep, s_wrap = p.a.n_heads - n_rep;
         const uint16_t *q_first = p.a.q + (int64_t)W.r0 * p.a.q_row + (int64_t)h * n_rep * p.a.q_head + 16 * wave + 8 * hh;
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
         const float *s_at = s_first;
         auto start = [&](int t) __attribute__((always_inline)) {
             const int q = t * 32 + r32;
-            row = q / n_rep, rep = q % n_rep;
+            row = p.a.by_rep.quot(q), rep = q - row * n_rep;
             q_at = q_first + row * p.a.q_row + rep * p.a.q_head;
             s_at = s_first + row * (int64_t)p.a.n_heads + rep;
         };
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
                     for (int j = 0; j < 16; j++) {
                         const int q = q0 + 8 * (j >> 2) + (j & 3);
                         if (own && known && q < W.nq)
-                            vis |= (uint32_t)(p.a.mask[(int64_t)(W.r0 + q / n_rep) * p.a.mask_words + (x >> 6)] >> (x & 63) & 1) << j;
+                            vis |= (uint32_t)(p.a.mask[(int64_t)(W.r0 + p.a.by_rep.quot(q)) * p.a.mask_words + (x >> 6)] >> (x & 63) & 1) << j;
                     }
                 }
 #pragma unroll
@@ -242,6 +243,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
 // 64 positions a wave where that still gives every CU a workgroup
 void launch_kv8_weights(const Kv8Weights &in, hipStream_t st) {
     Kv8Weights p = in;
+    p.a.by_rep = Kv8Div::by((uint32_t)p.a.n_rep);
     int dev = 0, cus = 0;
     SD_HIP_CHECK(hipGetDevice(&dev));
     SD_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
