@@ -5,21 +5,44 @@
 
 namespace sd {
 
-// C channels from c0 of a head's row, rotated in T by the pairs' or halves' angles
+// The channels kv8_ch(c0, .) of a head's row, rotated in T by the pairs' or halves' angles (from f64: as kv8_odd leaves them)
 template <typename T, int HD, bool F32>
 __device__ __forceinline__ void kv8_rotated(const void *src, int64_t at, int c0, const float *cos_r, const float *sin_r,
-                                            bool pairs, T (&x)[HD / 8]) {
-    constexpr int W = HD / 8;
+                                            bool pairs, float (&x)[HD / 8]) {
+    constexpr int N = HD / 64;
+    float a[2][8] = {};  // with 64 channels the second eight are those that the first rotate with
+    load8<F32>(src, at + c0, a[0]);
+    if (N == 2 || !pairs) load8<F32>(src, at + (c0 + HD / 2) % HD, a[1]);
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        const int w = c0 / 8 + i;
-        float a[8], b[8] = {};
-        load8<F32>(src, at + 8 * w, a);
-        if (!pairs) load8<F32>(src, at + 8 * ((w + W / 2) % W), b);
+    for (int i = 0; i < N; i++) {
         T o[8];
-        rotate8<T, HD>(a, b, cos_r, sin_r, w, pairs, o);
+        rotate8<T, HD>(a[i], a[i ^ 1], cos_r, sin_r, c0 / 8 + 8 * i, pairs, o);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[8 * i + j] = o[j];
+        for (int j = 0; j < 8; j++) x[8 * i + j] = kv8_odd(o[j]);
+    }
+}
+
+// The channels kv8_ch(c0, .) of query head h of the row at position pos (row pos + shift), if it is one before hi
+template <int HD, bool F32>
+__device__ __forceinline__ void kv8_turn_q(const Kv8Append &p, int pos, int hi, int shift, int h, int c0) {
+    constexpr int C = HD / 8;
+    if (pos >= hi) return;
+    const int row = pos + shift, at = p.pos ? p.pos[row] : pos;
+    float x[C];
+    if (at >= 0 && at < p.max_pos) {
+        kv8_rotated<float, HD, F32>(p.q, (int64_t)row * p.q_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
+                                    p.sin_t + (int64_t)at * (HD / 2), p.interleaved != 0, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i++) x[i] = NAN;
+    }
+    uint16_t *out = p.q_out + ((int64_t)row * p.n_heads + h) * HD;
+#pragma unroll
+    for (int i = 0; i < C; i += 8) {
+        uintx4 v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = (uint32_t)f2h(x[i + 2 * j]) | (uint32_t)f2h(x[i + 2 * j + 1]) << 16;
+        *(uintx4 *)(out + kv8_ch<HD>(c0, i)) = v;
     }
 }
 
@@ -44,25 +67,8 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
     for (int b = (first >> 5) + (int)blockIdx.x; (int64_t)b * 32 < last; b += gridDim.x) {
         const int lo = max(first, b * 32), hi = min(last, b * 32 + 32);
         if (unit >= 2 * n_kv) {
-            const int u = (unit - 2 * n_kv) * 32 + (tid >> 3), pos = lo + u / p.n_heads, h = u % p.n_heads, c0 = (tid & 7) * C;
-            if (pos >= hi) continue;
-            const int row = r0 + pos - P, at = p.pos ? p.pos[row] : pos;
-            float x[C];
-            if (at >= 0 && at < p.max_pos) {
-                kv8_rotated<float, HD, F32>(p.q, (int64_t)row * p.q_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
-                                            p.sin_t + (int64_t)at * (HD / 2), pairs, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < C; i++) x[i] = NAN;
-            }
-            uint16_t *out = p.q_out + ((int64_t)row * p.n_heads + h) * HD + c0;
-#pragma unroll
-            for (int i = 0; i < C; i += 8) {
-                uintx4 v;
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[j] = (uint32_t)f2h(x[i + 2 * j]) | (uint32_t)f2h(x[i + 2 * j + 1]) << 16;
-                *(uintx4 *)(out + i) = v;
-            }
+            kv8_turn_q<HD, F32>(p, lo + ((unit - 2 * n_kv) * 32 + (tid >> 3)) / p.n_heads, hi, r0 - P,
+                                ((unit - 2 * n_kv) * 32 + (tid >> 3)) % p.n_heads, (tid & 7) * 8);
             continue;
         }
         const bool is_v = unit >= n_kv;
@@ -71,7 +77,7 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
         if (page < 0 || page >= p.L.n_pages) continue;
         uint8_t *codes = p.L.codes(page, h, b * 32) + (is_v ? 32 * HD : 0);
         Kv8Head *head = p.L.head(page, h, b * 32);
-        const int k = tid >> 3, c0 = (tid & 7) * C, pos = b * 32 + k;
+        const int k = tid >> 3, c0 = (tid & 7) * 8, pos = b * 32 + k;
         const bool live = pos < hi, held = pos < lo;
         float scale = 1.f;
         uint32_t nans = 0;
@@ -87,11 +93,11 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
             if (held) {
                 kv8_row<HD, true>(sh.codes, k, c0, scale, x);
             } else if (live) {
-                const int64_t at = (int64_t)row * p.v_ld + (int64_t)h * HD + c0;
+                const int64_t at = (int64_t)row * p.v_ld + (int64_t)h * HD;
 #pragma unroll
                 for (int i = 0; i < C; i += 8) {
                     float a[8];
-                    load8<F32>(p.v, at + i, a);
+                    load8<F32>(p.v, at + kv8_ch<HD>(c0, i), a);
 #pragma unroll
                     for (int j = 0; j < 8; j++) x[i + j] = a[j];
                 }
@@ -101,7 +107,7 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
             const bool past = live && !held && !p.pos && pos >= p.max_pos;
             kv8_build<HD, true>(sh, x, live, lost || past || (held && (nans >> k & 1)), scale, nans);
         } else {
-            double x[C] = {};
+            float x[C] = {};
             bool lost = held && (nans >> k & 1);
             if (held) {
                 kv8_row<HD, false>(sh.codes, k, c0, scale, x);
@@ -123,16 +129,50 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
     }
 }
 
-void launch_kv8_append(const Kv8Append &p, hipStream_t st) {
-    if (p.seqs.rows < 1) return;
+constexpr int64_t kApart = 1 << 16;
+// The queries by themselves: a thread's registers are then few enough for a CU's whole complement of waves.
+template <int HD, bool F32>
+__global__ __launch_bounds__(kKv8T) void k_kv8_queries(const Kv8Append p) {
+    const int s = blockIdx.z, tid = threadIdx.x;
+    const int r0 = p.seqs.row_start ? p.seqs.row_start[s] : 0;
+    const int end = p.seqs.row_start ? p.seqs.row_start[s + 1] : p.seqs.rows;
+    const int T = p.seqs.row_start ? p.seqs.kv_len[s] : p.seqs.len0;
+    if (r0 < 0 || end <= r0 || end > p.seqs.rows || T < 1 || T > kKv8MaxLen) return;
+    const int n = end - r0, P = T - n, first = max(P, 0), last = P + min(n, p.seqs.max_rows);
+    for (int64_t a = (int64_t)first + blockIdx.x * 32; a < last; a += (int64_t)gridDim.x * 32) {
+        const int u = blockIdx.y * 32 + (tid >> 3), m = u / p.n_heads;
+        kv8_turn_q<HD, F32>(p, (int)a + m, min(last, (int)a + 32), r0 - P, u - m * p.n_heads, (tid & 7) * 8);
+    }
+}
+
+void launch_kv8_append(const Kv8Append &in, hipStream_t st) {
+    if (in.seqs.rows < 1) return;
+    Kv8Append p = in;
+    const int seqs = p.seqs.n_seqs, kv = 2 * p.L.n_kv;
     // blocks that max_rows rows can touch; a sequence's are dealt round as many workgroups as even ragged lengths need
-    const int64_t blocks = (p.seqs.max_rows + 30) / 32 + 1;
-    const int64_t mean = (p.seqs.rows / 32 + 2 * (int64_t)p.seqs.n_seqs + p.seqs.n_seqs - 1) / p.seqs.n_seqs;
+    const int64_t blocks = (p.seqs.max_rows + 30) / 32 + 1, mean = (p.seqs.rows / 32 + 3 * (int64_t)seqs - 1) / seqs;
     const int q = p.q ? (int)(((int64_t)std::min(32, p.seqs.max_rows) * p.n_heads + 31) / 32) : 0;
     // (a grid holds fewer than 2^32 threads)
-    const int64_t units = 2 * p.L.n_kv + q, most = ((int64_t)1 << 23) / (units * p.seqs.n_seqs);
-    if (most < 1) throw BackendError("append: too many sequences and heads in one call");
-    const dim3 g((unsigned)std::min({blocks, 4 * mean, most}), (unsigned)units, (unsigned)p.seqs.n_seqs), b(kKv8T);
+    auto grid = [&](int64_t units) {
+        const int64_t most = ((int64_t)1 << 23) / (units * seqs);
+        if (most < 1) throw BackendError("append: too many sequences and heads in one call");
+        return dim3((unsigned)std::min({blocks, 4 * mean, most}), (unsigned)units, (unsigned)seqs);
+    };
+    // many queries in a launch of their own
+    const bool apart = q && (int64_t)p.seqs.rows * p.n_heads >= kApart;
+    const dim3 b(kKv8T);
+    if (apart) {
+        const dim3 g = grid(q);
+        if (p.L.hd == 128) {
+            if (p.f32) k_kv8_queries<128, true><<<g, b, 0, st>>>(p);
+            else k_kv8_queries<128, false><<<g, b, 0, st>>>(p);
+        } else {
+            if (p.f32) k_kv8_queries<64, true><<<g, b, 0, st>>>(p);
+            else k_kv8_queries<64, false><<<g, b, 0, st>>>(p);
+        }
+        SD_HIP_CHECK(hipGetLastError());
+    }
+    const dim3 g = grid(kv + (apart ? 0 : q));
     if (p.L.hd == 128) {
         if (p.f32) k_kv8_append<128, true><<<g, b, 0, st>>>(p);
         else k_kv8_append<128, false><<<g, b, 0, st>>>(p);
@@ -193,10 +233,13 @@ __device__ void kv8_keep(Kv8Sh &sh, uint8_t (&code)[kKeepMax][HD], float (&scale
     constexpr int C = HD / 8;
     const int tid = threadIdx.x;
     for (int i = tid; i < n * 8; i += kKv8T) {
-        const int j = i >> 3, c0 = (i & 7) * C, pos = P + src[j], page = table[pos >> L.page_shift];
+        const int j = i >> 3, c0 = (i & 7) * 8, pos = P + src[j], page = table[pos >> L.page_shift];
         const uint8_t *b = L.codes(page, h, pos) + (V ? 32 * HD : 0);
 #pragma unroll
-        for (int c = 0; c < C; c++) code[j][c0 + c] = b[V ? kv8_v_at(pos & 31, c0 + c, HD) : kv8_k_at(pos & 31, c0 + c, HD)];
+        for (int n = 0; n < C; n++) {
+            const int c = kv8_ch<HD>(c0, n);
+            code[j][c] = b[V ? kv8_v_at(pos & 31, c, HD) : kv8_k_at(pos & 31, c, HD)];
+        }
         if ((i & 7) == 0) {
             const Kv8Head *head = L.head(page, h, pos);
             scales[j] = head->scale[V];
@@ -204,7 +247,7 @@ __device__ void kv8_keep(Kv8Sh &sh, uint8_t (&code)[kKeepMax][HD], float (&scale
         }
     }
     __syncthreads();
-    const int k = tid >> 3, c0 = (tid & 7) * C;
+    const int k = tid >> 3, c0 = (tid & 7) * 8;
     for (int b = P >> 5; b * 32 < P + n; b++) {
         const int page = table[b * 32 >> L.page_shift], pos = b * 32 + k, j = pos - P;
         uint8_t *codes = L.codes(page, h, b * 32) + (V ? 32 * HD : 0);
@@ -218,7 +261,7 @@ __device__ void kv8_keep(Kv8Sh &sh, uint8_t (&code)[kKeepMax][HD], float (&scale
             lost = nans >> k & 1;
         } else if (j < n) {
 #pragma unroll
-            for (int c = 0; c < C; c++) x[c] = kv8_value(code[j][c0 + c], scales[j]);
+            for (int c = 0; c < C; c++) x[c] = kv8_value(code[j][kv8_ch<HD>(c0, c)], scales[j]);
             lost = bad[j] != 0;
         }
         kv8_build<HD, V>(sh, x, j < n, lost, scale, nans);  // (its first barrier: the block has been read)

@@ -8,23 +8,22 @@ namespace sd {
 typedef float float2v __attribute__((ext_vector_type(2)));
 
 constexpr int kKv8T = 256;  // threads that build a block: 8 to a position
+// Channel of the i-th of a thread's HD / 8 values: 8 from c0 = 8 (thread % 8) and, with 128
+// channels, the 8 that lie half a head away (which halves rotate with).
+template <int HD> __host__ __device__ constexpr int kv8_ch(int c0, int i) { return c0 + (i & 7) + (i >> 3) * 64; }
 
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float kv8_two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// The smallest e with a <= 448 * 2^e = 1.75 * 2^(8 + e), for a finite a >= 0.
-__device__ __forceinline__ int kv8_exp(double a) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, a);
-    return (int)(b >> 52) - 1023 - 8 + ((b & 0xfffffffffffffull) > 0xc000000000000ull);
-}
+// The smallest e with a <= 448 * 2^e = 1.75 * 2^(8 + e), for a finite a >= 0 (a
+// subnormal's result is wrong, but below the least scale in any case).
 __device__ __forceinline__ int kv8_exp(float a) {
     const uint32_t b = __float_as_uint(a);
     return (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u);
 }
-// (a subnormal's result is wrong, but below the least scale in any case)
 
-// x in 32 bits such that a later rounding to fewer bits gives what rounding x
-// itself would: what does not fit goes into the last bit
+// x in 32 bits such that comparing it with a number of fewer bits, or rounding it to
+// fewer, gives what x itself would: what does not fit goes into the last bit
 __device__ __forceinline__ float kv8_odd(double x) {
     const float f = (float)x;
     const double d = (double)f;
@@ -51,8 +50,9 @@ __device__ __forceinline__ uintx4 kv8_expand(uint32_t a, uint32_t b, float scale
                   h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true)))};
 }
 
-// A block's keys or values from the values of its positions: thread t has the
-// channels (HD / 8) (t & 7) .. of position t >> 3 in x (live: the position holds
+// A block's keys or values from the values of its positions (keys that were rotated in
+// f64 as kv8_odd leaves them): thread t has the
+// channels kv8_ch(8 (t & 7), .) of position t >> 3 in x (live: the position holds
 // something), in LDS `codes` come the block's 32 HD bytes of codes.  Returns the
 // scale and the NaN bits.  All 256 threads call it; what they read of `codes`
 // before, they have read when the first barrier is passed.
@@ -61,21 +61,21 @@ struct Kv8Sh {
     int exp[4];
     uint32_t nan[4];
 };
-template <int HD, bool V, typename T>
-__device__ __forceinline__ void kv8_build(Kv8Sh &sh, const T (&x)[HD / 8], bool live, bool nan, float &scale, uint32_t &nans) {
+template <int HD, bool V>
+__device__ __forceinline__ void kv8_build(Kv8Sh &sh, const float (&x)[HD / 8], bool live, bool nan, float &scale, uint32_t &nans) {
     constexpr int C = HD / 8;
-    const int tid = threadIdx.x, k = tid >> 3, c0 = (tid & 7) * C, lane = tid & 63;
-    T top = fabs(x[0]);
-    bool bad = !(top <= (T)65504);
+    const int tid = threadIdx.x, k = tid >> 3, c0 = (tid & 7) * 8, lane = tid & 63;
+    float top = fabsf(x[0]);
+    bool bad = !(top <= 65504.f);
 #pragma unroll
     for (int i = 1; i < C; i++) {
-        const T a = fabs(x[i]);
-        bad |= !(a <= (T)65504);
-        top = fmax(top, a);
+        const float a = fabsf(x[i]);
+        bad |= !(a <= 65504.f);
+        top = fmaxf(top, a);
     }
     const uint64_t wave_bad = __builtin_amdgcn_ballot_w64(live && (bad || nan));
     const bool row_bad = (wave_bad >> (lane & 56) & 0xff) != 0;
-    int e = live && !row_bad && top > (T)0 ? min(max(kv8_exp(top), kKv8MinExp), kKv8MaxExp) : kKv8MinExp;
+    int e = live && !row_bad && top > 0.f ? min(max(kv8_exp(top), kKv8MinExp), kKv8MaxExp) : kKv8MinExp;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o));
     if (lane == 0) {
@@ -96,17 +96,17 @@ __device__ __forceinline__ void kv8_build(Kv8Sh &sh, const T (&x)[HD / 8], bool 
         float y[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            y[j] = r == 0.f ? 0.f : kv8_odd(x[i + j]) * r;  // (not NaN or infinity times 0)
+            y[j] = r == 0.f ? 0.f : x[i + j] * r;  // (not NaN or infinity times 0)
             if (e == kKv8MaxExp) y[j] = fminf(fmaxf(y[j], -240.f), 240.f);  // 256 of it are more than fp16 holds
         }
         w[i / 4] = kv8_pack(y[0], y[1], y[2], y[3]);
     }
     if constexpr (!V) {
 #pragma unroll
-        for (int i = 0; i < C / 4; i += 2) *(uintx2 *)(sh.codes + kv8_k_at(k, c0 + 4 * i, HD)) = uintx2{w[i], w[i + 1]};
+        for (int i = 0; i < C / 4; i += 2) *(uintx2 *)(sh.codes + kv8_k_at(k, kv8_ch<HD>(c0, 4 * i), HD)) = uintx2{w[i], w[i + 1]};
     } else {
 #pragma unroll
-        for (int i = 0; i < C; i++) sh.codes[kv8_v_at(k, c0 + i, HD)] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+        for (int i = 0; i < C; i++) sh.codes[kv8_v_at(k, kv8_ch<HD>(c0, i), HD)] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
     }
     __syncthreads();
 }
@@ -124,16 +124,16 @@ template <typename T> __device__ __forceinline__ void kv8_values(uint32_t w, flo
     const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     x[0] = (T)(a.x * scale), x[1] = (T)(a.y * scale), x[2] = (T)(b.x * scale), x[3] = (T)(b.y * scale);
 }
-// the HD / 8 channels from c0 of position k of a block's codes
+// the channels kv8_ch(c0, .) of position k of a block's codes
 template <int HD, bool V, typename T>
 __device__ __forceinline__ void kv8_row(const uint8_t *codes, int k, int c0, float scale, T (&x)[HD / 8]) {
     if constexpr (V) {
 #pragma unroll
-        for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[kv8_v_at(k, c0 + i, HD)], scale);
+        for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[kv8_v_at(k, kv8_ch<HD>(c0, i), HD)], scale);
     } else {
 #pragma unroll
         for (int i = 0; i < HD / 8; i += 8) {
-            const uintx2 w = *(const uintx2 *)(codes + kv8_k_at(k, c0 + i, HD));
+            const uintx2 w = *(const uintx2 *)(codes + kv8_k_at(k, kv8_ch<HD>(c0, i), HD));
             kv8_values(w.x, scale, x + i);
             kv8_values(w.y, scale, x + i + 4);
         }

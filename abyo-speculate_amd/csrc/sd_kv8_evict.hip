@@ -186,9 +186,8 @@ template <int HD> __device__ __forceinline__ Kv8Spot kv8_to(const Kv8Evict &p, v
 // Keys: 8 threads to a position, whose codes are 16 (8) bytes next to each other.
 template <int HD>
 __device__ __forceinline__ void kv8_gather_k(const Kv8Evict &p, void *ws, Kv8Sh &sh, int s, int h, int d, int n) {
-    constexpr int C = HD / 8;
-    const int k = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * C, i = d * 32 + k;
-    float x[C] = {};
+    const int k = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 8, i = d * 32 + k;
+    float x[HD / 8] = {};
     bool nan = false;
     if (i < n) {
         const int64_t head = (int64_t)s * p.L.n_kv + h;
