@@ -1250,6 +1250,7 @@ sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *qy, const 
         w.ld = (int64_t)scores->ld;
         w.decay = scores->decay;
         w.max_len = (int64_t)qy->max_len;
+        w.cus = P.cus;
         need_aligned(lse, 4, 4, "lse");
         need_aligned(w.in, 4, 4, "scores");
         need_aligned(w.out, 4, 4, "scores");

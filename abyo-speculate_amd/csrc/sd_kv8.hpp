@@ -137,6 +137,7 @@ struct Kv8Weights {
     int64_t ld;
     float decay;
     int64_t max_len;
+    int cus;
 };
 void launch_kv8_weights(const Kv8Weights &p, hipStream_t st);
 
@@ -155,6 +156,8 @@ struct Kv8Evict {
     int *kept;             // [n_seqs][n_kv][budget]
     int *new_len;          // [n_seqs]
 };
+// allows the kernels their LDS on the current device; once before the first call there
+void kv8_prepare();
 size_t kv8_evict_ws_bytes(int n_seqs, int n_kv, int hd, int budget);
 void launch_kv8_evict(const Kv8Evict &p, void *ws, hipStream_t st);
 

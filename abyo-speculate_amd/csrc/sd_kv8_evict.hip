@@ -1,7 +1,5 @@
 // Eviction from the 8-bit cache by the positions' accumulated weights: which ones of
 // every sequence and KV head stay, and moving them together.
-#include <atomic>
-
 #include "sd_kv8_dev.hpp"
 
 namespace sd {
@@ -332,6 +330,10 @@ template <int HD> __global__ __launch_bounds__(kKv8T) void k_kv8_place(const Kv8
     if (threadIdx.x == 0) *to.head = *from.head;
 }
 
+void kv8_prepare() {
+    SD_HIP_CHECK(hipFuncSetAttribute((const void *)k_kv8_select, hipFuncAttributeMaxDynamicSharedMemorySize, kSelChunk * 4));
+}
+
 size_t kv8_evict_ws_bytes(int n_seqs, int n_kv, int hd, int budget) {
     return (size_t)n_seqs * n_kv * ((budget + 31) / 32) * (kv8_block_bytes(hd) + sizeof(Kv8Head));
 }
@@ -340,16 +342,6 @@ void launch_kv8_evict(const Kv8Evict &p, void *ws, hipStream_t st) {
     const unsigned kv = (unsigned)p.L.n_kv, seqs = (unsigned)p.n_seqs, nblk = (unsigned)((p.budget + 31) / 32);
     const int64_t most = std::min<int64_t>(((int64_t)p.table_ld << p.L.page_shift), p.scores_ld);
     const int lds = (int)std::min<int64_t>((most + kSelT - 1) / kSelT * kSelT, kSelChunk) * 4;
-    if (lds > 32 * 1024) {
-        static std::atomic<uint64_t> done{0};  // bit per device
-        int dev = 0;
-        SD_HIP_CHECK(hipGetDevice(&dev));
-        const uint64_t bit = 1ull << (dev & 63);
-        if (!(done.load(std::memory_order_acquire) & bit) || dev > 63) {
-            SD_HIP_CHECK(hipFuncSetAttribute((const void *)k_kv8_select, hipFuncAttributeMaxDynamicSharedMemorySize, kSelChunk * 4));
-            done.fetch_or(bit, std::memory_order_release);
-        }
-    }
     k_kv8_select<<<dim3(kv, seqs), dim3(kSelT), lds, st>>>(p);
     SD_HIP_CHECK(hipGetLastError());
     if (nblk == 0) return;

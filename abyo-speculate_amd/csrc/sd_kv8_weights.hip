@@ -244,11 +244,8 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
 void launch_kv8_weights(const Kv8Weights &in, hipStream_t st) {
     Kv8Weights p = in;
     p.a.by_rep = Kv8Div::by((uint32_t)p.a.n_rep);
-    int dev = 0, cus = 0;
-    SD_HIP_CHECK(hipGetDevice(&dev));
-    SD_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t groups = (int64_t)p.a.L.n_kv * p.a.n_seqs, len = std::max<int64_t>(1, std::min(p.max_len, p.ld));
-    const bool two = (len + 255) / 256 * groups >= cus;
+    const bool two = (len + 255) / 256 * groups >= p.cus;
     const int64_t chunk = two ? 256 : 128, most = std::max<int64_t>(1, ((int64_t)1 << 23) / groups);
     const dim3 g((unsigned)std::min((len + chunk - 1) / chunk, most), (unsigned)p.a.L.n_kv, (unsigned)p.a.n_seqs), b(64 * kWgtWaves);
     if (p.a.L.hd == 128) {

@@ -44,6 +44,7 @@ KvPool::KvPool(const KvPoolCfg &c) : cfg(c) {
     DeviceScope dev(c.device);
     SD_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, c.device));
     layer_bytes = c.n_pages * page_bytes();
+    if (c.bits == 8) kv8_prepare();
     try {
         SD_HIP_CHECK(hipMalloc(&mem, (size_t)layer_bytes * c.n_layers + 256));
         SD_HIP_CHECK(hipMemset(mem, 0, (size_t)layer_bytes * c.n_layers + 256));

@@ -857,3 +857,119 @@ def test_refused_calls_leave_no_error_behind(hip):
         p.pool.append(0, 1, 0, 0, 0, 1, 1, max_rows=1, k=0, v=0)
     p.fill([40])
     p.check_held()
+
+
+# ---- sizes that take other paths ---------------------------------------------------
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("hd,dt", [(128, np.float16), (64, np.float32)])
+def test_append_of_many_queries(hip, hd, dt, inter):
+    """Above 65536 pairs of rows and query heads these have a launch of their own."""
+    counts = [2500, 3, 700]
+    p = Pool(hip, hd, 32, 2, hd, [c + 45 for c in counts], page=64, interleaved=inter)
+    p.append([45] * 3, [45] * 3, p.rows(135, 2), p.rows(135, 2))
+    n = sum(counts)
+    k, v, q = p.rows(n, 2, dt), p.rows(n, 2, dt), p.rows(n, 32, dt)
+    pos = p.rng.integers(0, MAX_POS, n)
+    qo = p.append(counts, [c + 45 for c in counts], k, v, pos=pos, q=q)
+    p.check_held()
+    want = p.turned(q, pos)
+    assert np.all(np.abs(qo.astype(np.float64) - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * np.abs(q).max() + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("hd,window", [(128, 0), (64, 0), (128, 4800)])
+def test_attention_of_many_steps_a_wave(hip, hd, window):
+    """Enough rows that a key range is the whole sequence: a wave's pages and headers are asked for more than once; one page in
+    between is absent."""
+    T, rows = 6000, 620
+    p = Pool(hip, 61, 32, 8, hd, [T], page=64)
+    p.fill([T])
+    q = p.rows(rows, 32)
+    t = p.table.copy()
+    t[0, 70] = -1
+    out, lse = p.attend(q, [rows], [T], table=dev(t), window=window, sinks=3 if window else 0)
+    seen = _kv8.visible(rows, T, window=window, sinks=3 if window else 0)
+    seen[:, 70 * 64:71 * 64] = False
+    pick = p.rng.permutation(rows)[:60]  # (the oracle takes its time)
+    _kv8.Attention(q[pick], *p.held[0], seen[pick], hd ** -0.5).check(out[pick], lse[pick])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window,sinks,tree", [(0, 0, False), (300, 70, False), (0, 0, True), (100, 5, True)])
+def test_weights_of_many_positions(hip, hd, window, sinks, tree):
+    """Enough positions for 64 of them a wave, ends inside both of its blocks, NaN rows and an absent page."""
+    lens = [2100, 2047, 33, 2100, 1999, 2080, 2100, 1900]
+    counts = [70, 1, 33, 40, 5, 64, 3, 90]
+    p = Pool(hip, hd + window, 8, 4, hd, lens, page=64)
+
+    def edit(k, v):
+        k[5, 0, 1] = np.nan  # of sequence 0
+        k[sum(lens) - 10, 2, 3] = np.inf  # and of the last's own rows
+    p.fill(lens, edit)
+    q = p.rows(sum(counts), 8)
+    bits = [np.tril(p.rng.random((n, n)) < 0.5) | np.eye(n, dtype=bool) for n in counts] if tree else [None] * len(counts)
+    mask = None
+    if tree:
+        mask = np.zeros((sum(counts), 2), np.uint64)
+        at = 0
+        for n, b in zip(counts, bits):
+            w = _kv8.words(b)
+            mask[at:at + n, :w.shape[1]] = w
+            at += n
+    t = p.table.copy()
+    t[3, 20] = p.n_pages + 1
+    dt = dev(t)
+    more = dict(table=dt, window=window, sinks=sinks)
+    _, lse = p.attend(q, counts, lens, mask=mask, **more)
+    before = p.rng.random((len(lens), 4, 2100)).astype(np.float32)
+    w = p.weights(q, lse, counts, lens, 2100, previous=before, mask=mask, **more)
+    at = 0
+    for s, n in enumerate(counts):
+        seen = _kv8.visible(n, lens[s], bits[s], window, sinks)
+        if s == 3:
+            seen[:, 20 * 64:21 * 64] = False
+        a = _kv8.Attention(q[at:at + n], *p.held[s], seen, hd ** -0.5)
+        a.check_weights(lse[at:at + n], w[s, :, :lens[s]], before[s, :, :lens[s]])
+        assert (w[s, :, lens[s]:] == 3.0).all()
+        at += n
+
+
+def test_pages_past_32_bits(hip):
+    """Page ids whose bytes lie past 2^33 in the pool, for every call."""
+    p = Pool(hip, 81, 8, 8, 128, [600, 64], page=256, spare=17000)
+    assert p.pool.page_bytes() * p.n_pages > 2 ** 33
+    p.table[0, :3] = [p.n_pages - 1, 5, p.n_pages - 3]
+    p.table[1, 0] = 8200  # around 2^32 bytes
+    p.dtable = dev(p.table)
+    p.fill([600, 64])
+    p.check_held()
+    q = p.rows(3, 8)
+    out, lse = p.attend(q, [2, 1], [600, 64])
+    w = p.weights(q, lse, [2, 1], [600, 64], 600)
+    for s, (r, T) in enumerate(((slice(0, 2), 600), (slice(2, 3), 64))):
+        a = _kv8.Attention(q[r], *p.held[s], _kv8.visible(r.stop - r.start, T), 128 ** -0.5)
+        a.check(out[r], lse[r])
+        a.check_weights(lse[r], w[s, :, :T])
+    check_evict(p, [600, 64], w, 300, 4, 100, run_evict(p, [600, 64], w, 300, 4, 100, True, "same"))
+
+
+def test_eviction_in_place_captured_and_replayed(hip):
+    """A long sequence (its ranks need more LDS than a kernel has by default) cut down in a graph, filled again in between."""
+    T, budget = 20000, 700
+    p = Pool(hip, 82, 2, 2, 64, [T], page=64)
+    x = scores_of(p.rng, (1, 2, T), "plain")
+    ds, dl, kept, new_len = dev(x), dev(np.array([T], np.int32)), zeros((1, 2, budget), np.int32), zeros((1,), np.int32)
+    ws = zeros(p.pool.evict_workspace(1, budget), np.uint8)
+
+    def step(st):
+        p.pool.evict(0, ptr(dl), ptr(p.dtable), *p.table.shape, scores=ptr(ds), scores_ld=T, budget=budget, sinks=4, recent=100,
+                     kept=ptr(kept), new_len=ptr(new_len), scores_out=ptr(ds), scores_out_ld=T, ws=ptr(ws), ws_bytes=ws.nbytes, stream=st)
+    graph = Graph(step)
+    for i in range(3):
+        p.held[0] = [np.zeros((0, 2, 64))] * 2
+        for a in range(0, T, 5000):
+            p.append([5000], [a + 5000], p.rows(5000, 2), p.rows(5000, 2), pos=np.arange(a, a + 5000) % MAX_POS)
+        x = scores_of(p.rng, (1, 2, T), ("plain", "ties", "all equal")[i])
+        ds.put(x)
+        synchronize()
+        graph.launch()
+        check_evict(p, [T], x, budget, 4, 100, (kept.get(), new_len.get(), ds.get(), None))
