@@ -47,7 +47,7 @@ template <int HD> __device__ __forceinline__ void kv8_load(Kv8Step<HD> &b, const
     for (int i = 0; i < HD / 32; i++) b.v[i] = bld16(r, lane * 16, 32 * HD + i * 1024);
 }
 
-// ---- up to 64 queries, 16 or 32 to a workgroup ------------------------------------
+// ---- 16 or 32 queries to a workgroup ------------------------------------------------
 // Four waves take the blocks of a key range in turn, codes straight from memory
 // into registers.
 template <int HD, int QT>
@@ -313,9 +313,12 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
     if (p.lse && d == 0) p.lse[at] = kv8_lse(M, l);
 }
 
-// Tiles of 16 or 32 queries.  Ranges: as many as give every CU two workgroups, one where
-// there is a single tile in a single sequence (5 rows of 32 heads over 8 and 8192 positions
-// 14.1 us, with two 16.9; a batch of 16 sequences with two 17.2 us, with one 19.5, with
+// Tiles: of 16 queries up to 64 of them, which expand every value for each tile but
+// leave registers for more waves (5 rows of 32 heads over 8 and 32768 positions 19.8 us,
+// with one tile of 32 21.1; 16 rows 25.3 and 26.5), of 32 above (60 rows over 8192
+// positions 28.5 us, with 16 29.5; 2048 rows over 8191 267 and 324).  Ranges: as many as give every CU two workgroups, one where
+// there is a single tile in a single sequence (5 rows over 8192 positions in one tile 14.1 us,
+// with two 16.9; a batch of 16 sequences with two 17.2 us, with one 19.5, with
 // eight 20; 60 rows over 8192 positions with two 28.2, with four 33.6), each of at least a
 // block for each wave.  A sequence's own length decides how many of them it has and how
 // long they are.
@@ -323,7 +326,7 @@ KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
                       int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
-    r.tile_q = nq <= 16 ? 16 : 32;
+    r.tile_q = nq <= 64 ? 16 : 32;
     r.tiles = (int)((nq + r.tile_q - 1) / r.tile_q);
     // most blocks that a tile sees
     int64_t blocks = (max_len + 31) / 32;
