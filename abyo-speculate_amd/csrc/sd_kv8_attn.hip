@@ -7,6 +7,21 @@
 // become fp16 values (exactly what they stand for) in one conversion per two of them,
 // which takes the block's scale.  No code is ever NaN or infinite, so what a
 // probability of 0 meets is finite; the rows that are NaN are bits in the header.
+//
+// A value costs half a VALU operation, so no value is expanded for more than the wave
+// that needs it: codes go from memory straight into registers, two buffers of a block
+// each, and nothing waits for LDS before the waves' states are joined.  A block of 8.2 KB
+// is some 190 VALU operations and 512 cycles of matrix instructions for 32 queries.
+// 2048 rows of 32 heads over 8191 positions: 268 us, 900 TFLOP/s (a large product of
+// fp16 matrices reaches 1196); VALU instructions are issued in 64 % of the CUs' busy
+// cycles, matrix instructions take 39 %, and the two waves of a SIMD overlap them in
+// part.  5 rows over 32768 positions, 67 MB of blocks: 16.6 us, 11.2 at the rate of a
+// large read; the chain to the first block (arguments, lengths, page, block) is some
+// 3 us, joining the waves 1.5.
+// Tried and dropped: the values of a block multiplied beside the weights of the next
+// (2048 rows 435 us: the registers do not hold it), tiles of 64 queries with one wave a
+// SIMD (410), wave priorities around the products (no difference), a separate maximum
+// for each block (300).
 #include <atomic>
 #include <type_traits>
 
@@ -316,12 +331,12 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
 // Tiles: of 16 queries up to 64 of them, which expand every value for each tile but
 // leave registers for more waves (5 rows of 32 heads over 8 and 32768 positions 19.8 us,
 // with one tile of 32 21.1; 16 rows 25.3 and 26.5), of 32 above (60 rows over 8192
-// positions 28.5 us, with 16 29.5; 2048 rows over 8191 267 and 324).  Ranges: as many as give every CU two workgroups, one where
-// there is a single tile in a single sequence (5 rows over 8192 positions in one tile 14.1 us,
-// with two 16.9; a batch of 16 sequences with two 17.2 us, with one 19.5, with
-// eight 20; 60 rows over 8192 positions with two 28.2, with four 33.6), each of at least a
-// block for each wave.  A sequence's own length decides how many of them it has and how
-// long they are.
+// positions 28.5 us, with 16 29.5; 2048 rows over 8191 267 and 324).  Ranges: as many as
+// give every CU two workgroups, one where there is a single tile in a single sequence
+// (5 rows over 8192 positions in one tile 14.1 us, with two 16.9; a batch of 16
+// sequences with two 17.2 us, with one 19.5, with eight 20; 60 rows over 8192 positions
+// with two 28.2, with four 33.6), each of at least a block for each wave.  A sequence's
+// own length decides how many of them it has and how long they are.
 KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int window, int sinks,
                       int cus) {
     KvqPlan r{};

@@ -22,7 +22,9 @@ __device__ __forceinline__ uint32_t kv8_rank(float x) {
 // with the bits found so far; then every wave counts what it keeps of its part of the
 // positions, in order, and writes it.  Equal scores stay from the lowest position on.
 // Ranks are held in LDS, 32768 at a time: a sequence up to that length is read once, a
-// longer one once for each of the four rounds.
+// longer one once for each of the four rounds.  32768 positions: 26 us on the one CU that
+// a head has, of which reading takes 5, the first histogram 5 (positions of like scores
+// meet in a bin), the others 2 each, counting 2 and writing 4; 2176 positions 9.
 constexpr int kSelT = 1024, kSelWaves = kSelT / 64, kSelBins = 2048, kSelChunk = 32768;
 constexpr uint32_t kSelForced = ~0u;  // the rank of a first or last position
 struct Kv8Select {
@@ -299,6 +301,9 @@ __device__ __forceinline__ void kv8_gather_v(const Kv8Evict &p, void *ws, Kv8Gro
         to.head->nan[1] = G.nan;
     }
 }
+// 8 sequences of some 2200 positions cut to 2048, 4 heads of 128 channels, 31 MB moved:
+// 16 us; 32768 positions of 8 heads cut to 4096, 17 MB: 14 us, in which 43 MB are fetched,
+// since a position's values lie in one byte of eight of its group's.
 template <int HD> __global__ __launch_bounds__(kKv8T) void k_kv8_gather(const Kv8Evict p, void *ws) {
     __shared__ union Sh {
         Kv8Sh k;

@@ -32,7 +32,13 @@ struct Kv8Range {
 };
 
 // A tile of queries is multiplied while the weights of the one before are taken, is in
-// LDS one tile ahead and on its way from memory two ahead.
+// LDS one tile ahead and on its way from memory two ahead.  512 rows of 32 heads over 8
+// and 16384 positions: 97 us, 700 TFLOP/s; without that overlap and with a division for
+// each query's address 157.  Matrix instructions take 38 % of the CUs' busy cycles, VALU
+// instructions (of which 32 exponentials for each 64 positions and 32 queries) are issued
+// in 50 %, waves wait for 38 % of theirs: four of them meet at each tile.  A batch of
+// single rows (4 sequences, 15273 positions): 8 us, of which the keys' bytes are 1.3; the
+// rest is the chain of lengths, page, keys, and the queries behind them.
 template <int HD, int NB>
 __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_kv8_weights(const Kv8Weights p) {
     constexpr int NC = HD / 16, NQ = HD / 64;  // chunks; 16-byte pieces of a tile of queries to a thread

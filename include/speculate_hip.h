@@ -556,10 +556,9 @@ sd_status sd_kv8_read(sd_kv8 *c, int32_t layer, const sd_kv_rows *rows, uint16_t
  * depths).  window NULL or of 0: all.  lse, f32 [rows][n_heads] or NULL: the
  * logarithm of the sum of exp(scale q k) over what the row sees, -inf where
  * that is nothing; like out it is left as it was for rows that have no
- * sequence.  Work is cut by the sequences' own lengths: max_len only bounds the
- * number of ranges (from 64 positions a range on its size hardly matters), and
- * larger kv_len stay correct.  lse overlaps neither q, out nor the workspace
- * (SD_ERR_ARG). */
+ * sequence.  Work is cut by the sequences' own lengths, so a max_len far above
+ * them costs nothing but workspace, and larger kv_len stay correct.  lse
+ * overlaps neither q, out nor the workspace (SD_ERR_ARG). */
 typedef struct sd_kv_window {
     size_t window, sinks;
 } sd_kv_window;
@@ -591,8 +590,9 @@ sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *query, con
  * the first `sinks` and the last `recent` stay, and of the others those with the
  * largest scores (of equal ones the first; NaN counts as less than everything)
  * until the budget is reached.  What stays keeps its order and moves to
- * positions 0, 1, ..., in place (new_table NULL), or in the pages of new_table,
- * which are none of the table's; blocks get the scales of what they hold now.
+ * positions 0, 1, ..., in place (new_table NULL; no page is then in two rows of
+ * the table), or in the pages of new_table, each of them there once and none of
+ * the table's; blocks get the scales of what they hold now.
  * A sequence of at most `budget` positions stays as it is, in new pages as a
  * copy.  kv_len counts up to the table's and scores_ld's end.
  *   kept        [n_seqs][n_kv_heads][budget]: the position each one had, -1
