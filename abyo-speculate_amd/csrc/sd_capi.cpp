@@ -113,6 +113,15 @@ static std::unique_ptr<sd::KvPool> make_pool(const sd_kvpool_config &cfg, int bi
     if (c.max_pos < 1) throw sd::ArgError("kvpool: max_pos must be positive");
     return std::make_unique<sd::KvPool>(c);
 }
+// A window of as many positions as a sequence can have is none; the kernels' sums of
+// positions and windows are of 32 bits.
+static void kv8_window(const sd_kv_window *win, int &window, int &sinks) {
+    window = sinks = 0;
+    if (!win || win->window >= (size_t)sd::kKv8MaxLen) return;
+    if (win->window > ((size_t)1 << 30)) throw sd::ArgError("window must be at most 2^30, or from 2^31 - 64 on none");
+    window = (int)win->window;
+    sinks = (int)std::min(win->sinks, (size_t)sd::kKv8MaxLen);
+}
 // What an attention call and a call for its weights have in common: the rows, the
 // sequences, the mask and the window of a query over an 8-bit pool.
 static sd::Kv8Attn kv8_query(const sd::KvPool &P, int32_t layer, const sd_kv_query *qy, const sd_kv_window *win) {
@@ -141,18 +150,16 @@ static sd::Kv8Attn kv8_query(const sd::KvPool &P, int32_t layer, const sd_kv_que
     a.n_heads = P.cfg.n_heads;
     a.n_rep = P.cfg.n_heads / P.cfg.n_kv_heads;
     a.scale = qy->scale == 0.f ? (float)(1.0 / std::sqrt((double)hd)) : qy->scale;
-    if (win) {
-        a.window = (int)std::min(win->window, most);
-        a.sinks = (int)std::min(win->sinks, most);
-    }
+    kv8_window(win, a.window, a.sinks);
     return a;
 }
 static sd::KvqPlan kv8_plan(const sd::KvPool &P, size_t rows, size_t n_seqs, size_t max_rows, size_t max_len,
                             const sd_kv_window *win) {
-    const size_t most = (size_t)1 << 40, wide = (size_t)1 << 30;
+    const size_t most = (size_t)1 << 40;
+    int window, sinks;
+    kv8_window(win, window, sinks);
     return P.plan((int64_t)std::min(rows, most), (int64_t)std::min(n_seqs, most), (int64_t)std::min(max_rows, most),
-                  (int64_t)std::min(max_len, most), win ? (int)std::min(win->window, wide) : 0,
-                  win ? (int)std::min(win->sinks, wide) : 0);
+                  (int64_t)std::min(max_len, most), window, sinks);
 }
 // one range of memory
 static sd::RowBytes bytes_at(const void *p, int64_t bytes) { return {p, 0, bytes, 1}; }

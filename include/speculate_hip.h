@@ -553,7 +553,8 @@ sd_status sd_kv8_read(sd_kv8 *c, int32_t layer, const sd_kv_rows *rows, uint16_t
 /* As sd_kvpool_attend, and: with a window, a row at position p sees of what its
  * mask shows the positions below `sinks` and those above p - window (its own
  * and window - 1 before it; of a tree's rows too the positions count, not the
- * depths).  window NULL or of 0: all.  lse, f32 [rows][n_heads] or NULL: the
+ * depths).  window NULL or of 0, or of 2^31 - 64 or more: all; others are at most
+ * 2^30 (SD_ERR_ARG).  lse, f32 [rows][n_heads] or NULL: the
  * logarithm of the sum of exp(scale q k) over what the row sees, -inf where
  * that is nothing; like out it is left as it was for rows that have no
  * sequence.  Work is cut by the sequences' own lengths, so a max_len far above

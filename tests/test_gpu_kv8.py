@@ -973,3 +973,51 @@ def test_eviction_in_place_captured_and_replayed(hip):
         synchronize()
         graph.launch()
         check_evict(p, [T], x, budget, 4, 100, (kept.get(), new_len.get(), ds.get(), None))
+
+
+def test_windows_that_no_sequence_fills(hip):
+    # from 2^31 - 64 on a window is none, whatever `sinks` is; between that and 2^30 it is refused
+    p = Pool(hip, 90, 4, 2, 64, [300], page=32)
+    p.fill([300])
+    q = p.rows(3, 4)
+    want, lse = p.attend(q, [3], [300])
+    for window in (1 << 30, 2 ** 31 - 64, 2 ** 31, 2 ** 63):
+        for sinks in (0, 5, 2 ** 63):
+            out, stat = p.attend(q, [3], [300], window=window, sinks=sinks)
+            assert np.array_equal(out, want) and np.array_equal(stat, lse)
+            got = p.weights(q, lse, [3], [300], 300, window=window, sinks=sinks)
+            assert np.array_equal(got, p.weights(q, lse, [3], [300], 300))
+    for window in (2 ** 30 + 1, 2 ** 31 - 65):
+        assert p.pool.attend_workspace(3, 1, 3, 300, window) == 0
+        with pytest.raises(hip.ArgError):
+            p.attend(q, [3], [300], window=window)
+        with pytest.raises(hip.ArgError):
+            p.weights(q, lse, [3], [300], 300, window=window)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("rows", [1, 5, 70])
+def test_the_longest_sequence_through_a_window(hip, rows, tree):
+    # 2^31 - 64 positions of which the first and the last page exist: what a window sees is what it sees of two pages
+    page, T, short = 2048, 2 ** 31 - 64, 2 * 2048 - 64
+    p = Pool(hip, 91 + rows, 8, 2, 128, [short], page=page)
+    p.fill([short])
+    table = np.full((1, (T - 1) // page + 1), -1, np.int32)
+    table[0, 0], table[0, -1] = p.table[0, :2]
+    big = dev(table)
+    q, k, v = p.rows(rows, 8), p.rows(rows, 2), p.rows(rows, 2)
+    pos = dev((short - rows + np.arange(rows)).astype(np.int32))
+    start, lens, dk, dv = dev(np.array([0, rows], np.int32)), dev(np.array([T], np.int32)), dev(k), dev(v)
+    p.pool.append(0, rows, ptr(start), ptr(lens), ptr(big), 1, table.shape[1], rows, ptr(dk), ptr(dv), pos=ptr(pos))
+    for i, x in enumerate((p.turned(k, short - rows + np.arange(rows)), v.astype(np.float64))):
+        p.held[0][i] = _kv8.append(p.held[0][i], short - rows, x)
+    p.check_held()
+    rng = np.random.default_rng(rows)
+    bits = np.tril(rng.random((rows, rows)) < 0.5) | np.eye(rows, dtype=bool)
+    mask = _kv8.words(bits) if tree else None
+    for window, sinks in ((100, 5), (1500, 0), (1900, 40)):
+        see = _kv8.visible(rows, short, bits if tree else None, window, sinks)
+        out, lse = p.attend(q, [rows], [T], mask=mask, table=big, window=window, sinks=sinks)
+        _kv8.Attention(q, *p.held[0], see, 128 ** -0.5).check(out, lse)
+        shared = dict(mask=mask, window=window, sinks=sinks)
+        assert np.array_equal(p.weights(q, lse, [rows], [T], page, table=big, **shared), p.weights(q, lse, [rows], [short], page, **shared))
