@@ -129,7 +129,7 @@ static sd::Kv8Attn kv8_query(const sd::KvPool &P, int32_t layer, const sd_kv_que
     if (!qy->q || !qy->row_start || !qy->kv_len || !qy->table) throw sd::ArgError("null argument");
     if (qy->n_seqs < 1 || qy->table_ld < 1) throw sd::ArgError("n_seqs and table_ld must be positive");
     if (qy->mask && qy->mask_words < 1) throw sd::ArgError("mask_words must be positive");
-    if (!std::isfinite(qy->scale)) throw sd::ArgError("scale must be finite");
+    if (!std::isfinite(qy->scale * 1.4426950408889634f)) throw sd::ArgError("scale must be finite, in base 2 too");
     const int hd = P.cfg.head_dim;
     const size_t most = (size_t)1 << 30;
     sd::Kv8Attn a{};

@@ -1021,3 +1021,33 @@ def test_the_longest_sequence_through_a_window(hip, rows, tree):
         _kv8.Attention(q, *p.held[0], see, 128 ** -0.5).check(out, lse)
         shared = dict(mask=mask, window=window, sinks=sinks)
         assert np.array_equal(p.weights(q, lse, [rows], [T], page, table=big, **shared), p.weights(q, lse, [rows], [short], page, **shared))
+
+
+def test_scales_that_base_2_cannot_hold(hip):
+    p = Pool(hip, 95, 4, 2, 64, [40], page=32)
+    p.fill([40])
+    q = p.rows(1, 4)
+    for scale in (3e38, -3e38, float("inf"), float("nan")):
+        with pytest.raises(hip.ArgError):
+            p.attend(q, [1], [40], scale=scale)
+        with pytest.raises(hip.ArgError):
+            p.weights(q, np.zeros((1, 4), np.float32), [1], [40], 40, scale=scale)
+
+
+@pytest.mark.parametrize("hd,KV,page", [(128, 2, 32), (64, 3, 128)])
+def test_reading_any_positions_in_any_order(hip, hd, KV, page):
+    # runs that start inside a group of 8, go backwards, change their sequence or pass a page's end, positions that are not there
+    p = Pool(hip, 96, KV, KV, hd, [300, 77], page=page)
+    p.fill([300, 77], edit=lambda k, v: (k.__setitem__((50, 1, 3), np.nan), v.__setitem__((305, 0, 7), np.inf)))
+    rng = np.random.default_rng(5)
+    cases = [([0] * 300, range(300)), ([0] * 64, range(3, 67)), ([0] * 40, range(40, 80)), ([1] * 77, range(76, -1, -1)),
+             ([0] * 8 + [1] * 8, [*range(8, 16)] * 2), ([0] * 12 + [1] * 12, [*range(16, 28)] * 2), ([0], [5]), ([0] * 16, [9] * 16),
+             ([0, 1] * 30, rng.integers(0, 77, 60)), ([0] * 8 + [5] + [0] * 7 + [-1] * 8, [*range(24, 32), 0, *range(33, 40), *range(8)]),
+             ([0] * 10 + [1] * 6, [*range(8), -1, 1 << 20, *range(8, 14)]), (rng.integers(0, 2, 3000), rng.integers(0, 77, 3000))]
+    for seq, slot in cases:
+        k, v = p.read(seq, slot)
+        for i, (s, at) in enumerate(zip(seq, slot)):
+            there = 0 <= s < 2 and 0 <= at < p.table.shape[1] * page and p.table[s, at // page] >= 0
+            for got, held in ((k[i], p.held[s][0]), (v[i], p.held[s][1])) if there else ():
+                assert np.array_equal(got.astype(np.float64), held[at], equal_nan=True), (s, at)
+            assert there or ((k[i] == 5).all() and (v[i] == 5).all())
