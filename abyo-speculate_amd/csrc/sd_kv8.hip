@@ -191,43 +191,82 @@ void launch_kv8_append(const Kv8Append &in, hipStream_t st) {
 }
 
 // ---- read ----------------------------------------------------------------------
-// 16 rows of one KV head's keys or values to a workgroup, 16 or 8 threads to a row:
-// rows next to each other share the lines that their values' bytes lie in.  16384 rows
-// of 8 heads, 34 MB of blocks and 67 MB of rows: 31 us, 21 at the rate of a large copy;
-// the waves wait for 71 % of their time (a value row is 8 one-byte loads a thread).
-constexpr int kReadRows = 16;
+// 8 x 8 bytes of eight lanes next to each other: lane x has byte k of lane k's in place of its own byte k, for all k
+__device__ __forceinline__ uintx2 kv8_transpose(uintx2 w, int lane) {
+    const uint32_t give = lane & 4 ? w.x : w.y;
+    uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0x141, 0xf, 0xf, true);  // 7 - lane of each 8
+    got = (uint32_t)__builtin_amdgcn_mov_dpp((int)got, 0x1B, 0xf, 0xf, true);             // 3 - lane of each 4: lane ^ 4 in all
+    w = lane & 4 ? uintx2{got, w.y} : uintx2{w.x, got};
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t of = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[i], 0x4E, 0xf, 0xf, true);  // lane ^ 2
+        w[i] = lane & 2 ? __builtin_amdgcn_perm(w[i], of, 0x07060302u) : __builtin_amdgcn_perm(of, w[i], 0x05040100u);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t of = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[i], 0xB1, 0xf, 0xf, true);  // lane ^ 1
+        w[i] = lane & 1 ? __builtin_amdgcn_perm(w[i], of, 0x07030501u) : __builtin_amdgcn_perm(of, w[i], 0x06020400u);
+    }
+    return w;
+}
+
+// A wave has 8 rows of 64 channels of one KV head's keys or values, kReadU times: lane
+// 8 j + k the channels 8 j .. of row k.  Rows that are 8 positions of one group of a
+// block share the bytes that their values lie in: then lane 8 j + x loads the 8
+// positions of channel 8 j + x and the eight lanes exchange them; otherwise a lane
+// picks its 8 bytes.
+constexpr int kReadU = 2;
 template <int HD>
-__global__ __launch_bounds__(2 * HD) void k_kv8_read(const Kv8Layer L, const KvqRows rows, uint16_t *k_out, uint16_t *v_out) {
-    constexpr int W = HD / 8;
-    const int r = blockIdx.x * kReadRows + threadIdx.x / W, c0 = threadIdx.x % W * 8;
+__global__ __launch_bounds__(256) void k_kv8_read(const Kv8Layer L, const KvqRows rows, uint16_t *k_out, uint16_t *v_out) {
+    constexpr int PARTS = HD / 64, GROUPS = 4 / PARTS;  // of 64 channels, of 8 rows
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool is_v = (int)blockIdx.y >= L.n_kv;
     const int h = is_v ? (int)blockIdx.y - L.n_kv : (int)blockIdx.y;
     uint16_t *out = is_v ? v_out : k_out;
-    if (!out || r >= rows.n) return;
-    int slot;
-    const int page = kvq_row_page(rows, L, r, slot);
-    if (page < 0) return;
-    const int k = slot & 31;
-    const uint8_t *codes = L.codes(page, h, slot) + (is_v ? 32 * HD : 0);
-    const Kv8Head *head = L.head(page, h, slot);
-    const float scale = head->scale[is_v];
-    uintx2 w = {0, 0};
-    if (is_v) {
+    if (!out) return;
+    const int r0 = ((int)blockIdx.x * GROUPS + wave / PARTS) * 8 * kReadU + (lane & 7), c0 = wave % PARTS * 64 + (lane >> 3) * 8;
+    int slot[kReadU], page[kReadU];
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)codes[kv8_v_at(k, c0 + i, HD)] << (8 * (i & 3));
-    } else {
-        w = *(const uintx2 *)(codes + kv8_k_at(k, c0, HD));
+    for (int u = 0; u < kReadU; u++) {
+        const int r = r0 + 8 * u;
+        page[u] = r < rows.n ? kvq_row_page(rows, L, r, slot[u]) : -1;
+        if (page[u] < 0) slot[u] = 0;
     }
-    uintx4 v = kv8_expand(w.x, w.y, scale);
-    if (head->nan[is_v] >> k & 1) v = uintx4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
-    *(uintx4 *)(out + ((int64_t)r * L.n_kv + h) * HD + c0) = v;
+    uintx2 w[kReadU];
+    Kv8Head head[kReadU];
+    bool turn[kReadU];
+#pragma unroll
+    for (int u = 0; u < kReadU; u++) {
+        const int k = slot[u] & 31, at = max(page[u], 0);
+        const uint8_t *codes = L.codes(at, h, slot[u]) + (is_v ? 32 * HD : 0);
+        head[u] = *L.head(at, h, slot[u]);
+        const int first = __shfl(slot[u], lane & 56), of = __shfl(page[u], lane & 56);
+        turn[u] = is_v && __builtin_amdgcn_ballot_w64(page[u] < 0 || of != page[u] || (first & 7) != 0 || slot[u] != first + (lane & 7)) == 0;
+        if (turn[u]) {
+            w[u] = *(const uintx2 *)(codes + kv8_v_at(k & 24, c0 + (lane & 7), HD));
+        } else if (is_v) {
+            w[u] = uintx2{0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[u][i >> 2] |= (uint32_t)codes[kv8_v_at(k, c0 + i, HD)] << (8 * (i & 3));
+        } else {
+            w[u] = *(const uintx2 *)(codes + kv8_k_at(k, c0, HD));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadU; u++) {
+        if (turn[u]) w[u] = kv8_transpose(w[u], lane);
+        uintx4 v = kv8_expand(w[u].x, w[u].y, head[u].scale[is_v]);
+        if (head[u].nan[is_v] >> (slot[u] & 31) & 1) v = uintx4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+        if (page[u] >= 0) *(uintx4 *)(out + ((int64_t)(r0 + 8 * u) * L.n_kv + h) * HD + c0) = v;
+    }
 }
 
 void launch_kv8_read(const Kv8Layer &L, const KvqRows &rows, uint16_t *k_out, uint16_t *v_out, hipStream_t st) {
     if (rows.n < 1) return;
-    const dim3 g((unsigned)((rows.n + kReadRows - 1) / kReadRows), (unsigned)(2 * L.n_kv));
-    if (L.hd == 128) k_kv8_read<128><<<g, dim3(256), 0, st>>>(L, rows, k_out, v_out);
-    else k_kv8_read<64><<<g, dim3(128), 0, st>>>(L, rows, k_out, v_out);
+    const int each = 8 * kReadU * (4 / (L.hd / 64));
+    const dim3 g((unsigned)((rows.n + each - 1) / each), (unsigned)(2 * L.n_kv)), b(256);
+    if (L.hd == 128) k_kv8_read<128><<<g, b, 0, st>>>(L, rows, k_out, v_out);
+    else k_kv8_read<64><<<g, b, 0, st>>>(L, rows, k_out, v_out);
     SD_HIP_CHECK(hipGetLastError());
 }
 
