@@ -6,32 +6,45 @@
 namespace sd {
 
 // The channels kv8_ch(c0, .) of a head's row, rotated in T by the pairs' or halves' angles (from f64: as kv8_odd leaves them)
-template <typename T, int HD, bool F32>
+template <typename T, int HD, bool F32, bool PAIRS>
 __device__ __forceinline__ void kv8_rotated(const void *src, int64_t at, int c0, const float *cos_r, const float *sin_r,
-                                            bool pairs, float (&x)[HD / 8]) {
+                                            float (&x)[HD / 8]) {
     constexpr int N = HD / 64;
     float a[2][8] = {};  // with 64 channels the second eight are those that the first rotate with
     load8<F32>(src, at + c0, a[0]);
-    if (N == 2 || !pairs) load8<F32>(src, at + (c0 + HD / 2) % HD, a[1]);
+    if (N == 2 || !PAIRS) load8<F32>(src, at + (c0 + HD / 2) % HD, a[1]);
+    if constexpr (N == 2 && !PAIRS) {
+        // both halves' channels at once, which need the same numbers
+        float c[8], s[8];
+        load8<true>(cos_r, c0, c);
+        load8<true>(sin_r, c0, s);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        T o[8];
-        rotate8<T, HD>(a[i], a[i ^ 1], cos_r, sin_r, c0 / 8 + 8 * i, pairs, o);
+        for (int j = 0; j < 8; j++) {
+            const T A = a[0][j], B = a[1][j], C = c[j], S = s[j];
+            x[j] = kv8_odd(A * C + B * -S);
+            x[8 + j] = kv8_odd(B * C + A * S);
+        }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[8 * i + j] = kv8_odd(o[j]);
+        for (int i = 0; i < N; i++) {
+            T o[8];
+            rotate8<T, HD>(a[i], a[i ^ 1], cos_r, sin_r, c0 / 8 + 8 * i, PAIRS, o);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[8 * i + j] = kv8_odd(o[j]);
+        }
     }
 }
 
 // The channels kv8_ch(c0, .) of query head h of the row at position pos (row pos + shift), if it is one before hi
-template <int HD, bool F32>
+template <int HD, bool F32, bool PAIRS>
 __device__ __forceinline__ void kv8_turn_q(const Kv8Append &p, int pos, int hi, int shift, int h, int c0) {
     constexpr int C = HD / 8;
     if (pos >= hi) return;
     const int row = pos + shift, at = p.pos ? p.pos[row] : pos;
     float x[C];
     if (at >= 0 && at < p.max_pos) {
-        kv8_rotated<float, HD, F32>(p.q, (int64_t)row * p.q_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
-                                    p.sin_t + (int64_t)at * (HD / 2), p.interleaved != 0, x);
+        kv8_rotated<float, HD, F32, PAIRS>(p.q, (int64_t)row * p.q_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
+                                           p.sin_t + (int64_t)at * (HD / 2), x);
     } else {
 #pragma unroll
         for (int i = 0; i < C; i++) x[i] = NAN;
@@ -55,8 +68,8 @@ __device__ __forceinline__ void kv8_turn_q(const Kv8Append &p, int pos, int hi, 
 // large copy; VALU instructions are issued in 60 % of the CUs' busy cycles, and the f64
 // rotation's registers leave four waves a SIMD.  (8 channels a thread, 16 threads to a
 // position: 193 us for rows and queries, 107 so.)
-template <int HD, bool F32>
-__global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
+template <int HD, bool F32, bool PAIRS>
+__global__ __launch_bounds__(kKv8T) __attribute__((amdgpu_waves_per_eu(5))) void k_kv8_append(const Kv8Append p) {
     constexpr int C = HD / 8;
     __shared__ Kv8Sh sh;
     const int s = blockIdx.z, n_kv = p.L.n_kv, tid = threadIdx.x;
@@ -66,13 +79,12 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
     if (r0 < 0 || end <= r0 || end > p.seqs.rows || T < 1 || T > kKv8MaxLen) return;
     // row i is position P + i; of the positions [first, last)
     const int n = end - r0, P = T - n, first = max(P, 0), last = P + min(n, p.seqs.max_rows);
-    const bool pairs = p.interleaved != 0;
     const int unit = blockIdx.y;
     for (int b = (first >> 5) + (int)blockIdx.x; (int64_t)b * 32 < last; b += gridDim.x) {
         const int lo = max(first, b * 32), hi = min(last, b * 32 + 32);
         if (unit >= 2 * n_kv) {
-            kv8_turn_q<HD, F32>(p, lo + ((unit - 2 * n_kv) * 32 + (tid >> 3)) / p.n_heads, hi, r0 - P,
-                                ((unit - 2 * n_kv) * 32 + (tid >> 3)) % p.n_heads, (tid & 7) * 8);
+            kv8_turn_q<HD, F32, PAIRS>(p, lo + ((unit - 2 * n_kv) * 32 + (tid >> 3)) / p.n_heads, hi, r0 - P,
+                                       ((unit - 2 * n_kv) * 32 + (tid >> 3)) % p.n_heads, (tid & 7) * 8);
             continue;
         }
         const bool is_v = unit >= n_kv;
@@ -85,18 +97,16 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
         const bool live = pos < hi, held = pos < lo;
         float scale = 1.f;
         uint32_t nans = 0;
+        const int row = r0 + pos - P;
         if (lo > b * 32) {
             scale = head->scale[is_v];
             nans = head->nan[is_v];
-            kv8_codes_in<HD>(sh, codes);
-            __syncthreads();
         }
-        const int row = r0 + pos - P;
+        // (the barriers of kv8_build are behind all reads of the block)
+        float x[C] = {};
         if (is_v) {
-            float x[C] = {};
-            if (held) {
-                kv8_row<HD, true>(sh.codes, k, c0, scale, x);
-            } else if (live) {
+            if (lo > b * 32) kv8_held<HD, true>(codes, scale, x);
+            if (live && !held) {
                 const int64_t at = (int64_t)row * p.v_ld + (int64_t)h * HD;
 #pragma unroll
                 for (int i = 0; i < C; i += 8) {
@@ -111,16 +121,15 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
             const bool past = live && !held && !p.pos && pos >= p.max_pos;
             kv8_build<HD, true>(sh, x, live, lost || past || (held && (nans >> k & 1)), scale, nans);
         } else {
-            float x[C] = {};
             bool lost = held && (nans >> k & 1);
             if (held) {
-                kv8_row<HD, false>(sh.codes, k, c0, scale, x);
+                kv8_key<HD>(codes, k, c0, scale, x);
             } else if (live) {
                 const int at = p.pos ? p.pos[row] : pos;
                 lost = at < 0 || at >= p.max_pos;
                 if (!lost)
-                    kv8_rotated<double, HD, F32>(p.k, (int64_t)row * p.k_ld + (int64_t)h * HD, c0, p.cos_t + (int64_t)at * (HD / 2),
-                                                 p.sin_t + (int64_t)at * (HD / 2), pairs, x);
+                    kv8_rotated<double, HD, F32, PAIRS>(p.k, (int64_t)row * p.k_ld + (int64_t)h * HD, c0,
+                                                        p.cos_t + (int64_t)at * (HD / 2), p.sin_t + (int64_t)at * (HD / 2), x);
             }
             kv8_build<HD, false>(sh, x, live, lost, scale, nans);
         }
@@ -138,7 +147,7 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_append(const Kv8Append p) {
 // rate; a small call keeps them in the launch above, which saves a launch of 3 us: from
 // kApart pairs of a row and a head on the shorter kernel outweighs it.
 constexpr int64_t kApart = 1 << 16;
-template <int HD, bool F32>
+template <int HD, bool F32, bool PAIRS>
 __global__ __launch_bounds__(kKv8T) void k_kv8_queries(const Kv8Append p) {
     const int s = blockIdx.z, tid = threadIdx.x;
     const int r0 = p.seqs.row_start ? p.seqs.row_start[s] : 0;
@@ -148,10 +157,25 @@ __global__ __launch_bounds__(kKv8T) void k_kv8_queries(const Kv8Append p) {
     const int n = end - r0, P = T - n, first = max(P, 0), last = P + min(n, p.seqs.max_rows);
     for (int64_t a = (int64_t)first + blockIdx.x * 32; a < last; a += (int64_t)gridDim.x * 32) {
         const int u = blockIdx.y * 32 + (tid >> 3), m = u / p.n_heads;
-        kv8_turn_q<HD, F32>(p, (int)a + m, min(last, (int)a + 32), r0 - P, u - m * p.n_heads, (tid & 7) * 8);
+        kv8_turn_q<HD, F32, PAIRS>(p, (int)a + m, min(last, (int)a + 32), r0 - P, u - m * p.n_heads, (tid & 7) * 8);
     }
 }
 
+template <int HD, bool F32> static void launch_append(const Kv8Append &p, bool queries, dim3 g, hipStream_t st) {
+    const dim3 b(kKv8T);
+    if (queries) {
+        if (p.interleaved) k_kv8_queries<HD, F32, true><<<g, b, 0, st>>>(p);
+        else k_kv8_queries<HD, F32, false><<<g, b, 0, st>>>(p);
+    } else {
+        if (p.interleaved) k_kv8_append<HD, F32, true><<<g, b, 0, st>>>(p);
+        else k_kv8_append<HD, F32, false><<<g, b, 0, st>>>(p);
+    }
+    SD_HIP_CHECK(hipGetLastError());
+}
+static void launch_append(const Kv8Append &p, bool queries, dim3 g, hipStream_t st) {
+    if (p.L.hd == 128) p.f32 ? launch_append<128, true>(p, queries, g, st) : launch_append<128, false>(p, queries, g, st);
+    else p.f32 ? launch_append<64, true>(p, queries, g, st) : launch_append<64, false>(p, queries, g, st);
+}
 void launch_kv8_append(const Kv8Append &in, hipStream_t st) {
     if (in.seqs.rows < 1) return;
     Kv8Append p = in;
@@ -167,53 +191,15 @@ void launch_kv8_append(const Kv8Append &in, hipStream_t st) {
     };
     // many queries in a launch of their own
     const bool apart = q && (int64_t)p.seqs.rows * p.n_heads >= kApart;
-    const dim3 b(kKv8T);
-    if (apart) {
-        const dim3 g = grid(q);
-        if (p.L.hd == 128) {
-            if (p.f32) k_kv8_queries<128, true><<<g, b, 0, st>>>(p);
-            else k_kv8_queries<128, false><<<g, b, 0, st>>>(p);
-        } else {
-            if (p.f32) k_kv8_queries<64, true><<<g, b, 0, st>>>(p);
-            else k_kv8_queries<64, false><<<g, b, 0, st>>>(p);
-        }
-        SD_HIP_CHECK(hipGetLastError());
-    }
-    const dim3 g = grid(kv + (apart ? 0 : q));
-    if (p.L.hd == 128) {
-        if (p.f32) k_kv8_append<128, true><<<g, b, 0, st>>>(p);
-        else k_kv8_append<128, false><<<g, b, 0, st>>>(p);
-    } else {
-        if (p.f32) k_kv8_append<64, true><<<g, b, 0, st>>>(p);
-        else k_kv8_append<64, false><<<g, b, 0, st>>>(p);
-    }
-    SD_HIP_CHECK(hipGetLastError());
+    if (apart) launch_append(p, true, grid(q), st);
+    launch_append(p, false, grid(kv + (apart ? 0 : q)), st);
 }
 
 // ---- read ----------------------------------------------------------------------
-// 8 x 8 bytes of eight lanes next to each other: lane x has byte k of lane k's in place of its own byte k, for all k
-__device__ __forceinline__ uintx2 kv8_transpose(uintx2 w, int lane) {
-    const uint32_t give = lane & 4 ? w.x : w.y;
-    uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0x141, 0xf, 0xf, true);  // 7 - lane of each 8
-    got = (uint32_t)__builtin_amdgcn_mov_dpp((int)got, 0x1B, 0xf, 0xf, true);             // 3 - lane of each 4: lane ^ 4 in all
-    w = lane & 4 ? uintx2{got, w.y} : uintx2{w.x, got};
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t of = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[i], 0x4E, 0xf, 0xf, true);  // lane ^ 2
-        w[i] = lane & 2 ? __builtin_amdgcn_perm(w[i], of, 0x07060302u) : __builtin_amdgcn_perm(of, w[i], 0x05040100u);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t of = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[i], 0xB1, 0xf, 0xf, true);  // lane ^ 1
-        w[i] = lane & 1 ? __builtin_amdgcn_perm(w[i], of, 0x07030501u) : __builtin_amdgcn_perm(of, w[i], 0x06020400u);
-    }
-    return w;
-}
-
 // A wave has 8 rows of 64 channels of one KV head's keys or values, kReadU times: lane
-// 8 j + k the channels 8 j .. of row k.  Rows that are 8 positions of one group of a
-// block share the bytes that their values lie in: then lane 8 j + x loads the 8
-// positions of channel 8 j + x and the eight lanes exchange them; otherwise a lane
+// 8 k + j the channels 8 j .. of row k.  Rows that are 8 positions of one group of a
+// block share the bytes that their values lie in: then lane 8 k + j loads the 8
+// positions of channel 8 j + k and the eight lanes exchange them; otherwise a lane
 // picks its 8 bytes.
 constexpr int kReadU = 2;
 template <int HD>
@@ -224,7 +210,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(const Kv8Layer L, const KvqRow
     const int h = is_v ? (int)blockIdx.y - L.n_kv : (int)blockIdx.y;
     uint16_t *out = is_v ? v_out : k_out;
     if (!out) return;
-    const int r0 = ((int)blockIdx.x * GROUPS + wave / PARTS) * 8 * kReadU + (lane & 7), c0 = wave % PARTS * 64 + (lane >> 3) * 8;
+    const int r0 = ((int)blockIdx.x * GROUPS + wave / PARTS) * 8 * kReadU + (lane >> 3), c0 = wave % PARTS * 64 + (lane & 7) * 8;
     int slot[kReadU], page[kReadU];
 #pragma unroll
     for (int u = 0; u < kReadU; u++) {
@@ -240,10 +226,10 @@ __global__ __launch_bounds__(256) void k_kv8_read(const Kv8Layer L, const KvqRow
         const int k = slot[u] & 31, at = max(page[u], 0);
         const uint8_t *codes = L.codes(at, h, slot[u]) + (is_v ? 32 * HD : 0);
         head[u] = *L.head(at, h, slot[u]);
-        const int first = __shfl(slot[u], lane & 56), of = __shfl(page[u], lane & 56);
-        turn[u] = is_v && __builtin_amdgcn_ballot_w64(page[u] < 0 || of != page[u] || (first & 7) != 0 || slot[u] != first + (lane & 7)) == 0;
+        const int first = __builtin_amdgcn_readfirstlane(slot[u]), of = __builtin_amdgcn_readfirstlane(page[u]);
+        turn[u] = is_v && __builtin_amdgcn_ballot_w64(page[u] < 0 || of != page[u] || (first & 7) != 0 || slot[u] != first + (lane >> 3)) == 0;
         if (turn[u]) {
-            w[u] = *(const uintx2 *)(codes + kv8_v_at(k & 24, c0 + (lane & 7), HD));
+            w[u] = *(const uintx2 *)(codes + kv8_v_at(k & 24, c0 + (lane >> 3), HD));
         } else if (is_v) {
             w[u] = uintx2{0, 0};
 #pragma unroll
@@ -304,8 +290,8 @@ __device__ void kv8_keep(Kv8Sh &sh, uint8_t (&code)[kKeepMax][HD], float (&scale
         uint32_t nans = head->nan[V];
         float x[C] = {};
         bool lost = false;
+        kv8_held<HD, V>(codes, scale, x);
         if (j < 0) {
-            kv8_row<HD, V>(codes, k, c0, scale, x);
             lost = nans >> k & 1;
         } else if (j < n) {
 #pragma unroll

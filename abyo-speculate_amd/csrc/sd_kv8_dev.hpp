@@ -50,6 +50,22 @@ __device__ __forceinline__ uintx4 kv8_expand(uint32_t a, uint32_t b, float scale
                   h2bits(__builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true)))};
 }
 
+// 8 x 8 bytes of the eight lanes that are 8 apart, lane 8 k + j the k-th of them: it has byte
+// k of the i-th's at byte i afterwards
+__device__ __forceinline__ uintx2 kv8_transpose(uintx2 w, int lane) {
+    const auto far = __builtin_amdgcn_permlane32_swap(w.x, w.y, false, false);
+    const auto mid = __builtin_amdgcn_permlane16_swap(__builtin_amdgcn_perm(far[1], far[0], 0x05040100u),
+                                                      __builtin_amdgcn_perm(far[1], far[0], 0x07060302u), false, false);
+    w = uintx2{__builtin_amdgcn_perm(mid[1], mid[0], 0x05040100u), __builtin_amdgcn_perm(mid[1], mid[0], 0x07060302u)};
+    const uint32_t pick = lane & 8 ? 0x03070105u : 0x06020400u;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t of = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[i], 0x128, 0xf, 0xf, true);  // lane ^ 8
+        w[i] = __builtin_amdgcn_perm(of, w[i], pick);
+    }
+    return w;
+}
+
 // A block's keys or values from the values of its positions (keys that were rotated in
 // f64 as kv8_odd leaves them): thread t has the
 // channels kv8_ch(8 (t & 7), .) of position t >> 3 in x (live: the position holds
@@ -101,42 +117,44 @@ __device__ __forceinline__ void kv8_build(Kv8Sh &sh, const float (&x)[HD / 8], b
         }
         w[i / 4] = kv8_pack(y[0], y[1], y[2], y[3]);
     }
-    if constexpr (!V) {
 #pragma unroll
-        for (int i = 0; i < C / 4; i += 2) *(uintx2 *)(sh.codes + kv8_k_at(k, kv8_ch<HD>(c0, 4 * i), HD)) = uintx2{w[i], w[i + 1]};
-    } else {
-#pragma unroll
-        for (int i = 0; i < C; i++) sh.codes[kv8_v_at(k, kv8_ch<HD>(c0, i), HD)] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+    for (int i = 0; i < C / 4; i += 2) {
+        const uintx2 v{w[i], w[i + 1]};
+        const int c = kv8_ch<HD>(c0, 4 * i);
+        if constexpr (!V) *(uintx2 *)(sh.codes + kv8_k_at(k, c, HD)) = v;
+        else *(uintx2 *)(sh.codes + kv8_v_at(k & 24, c + (k & 7), HD)) = kv8_transpose(v, lane);
     }
     __syncthreads();
 }
-// the codes in LDS to or from a block's keys or values in memory
+// the codes in LDS to a block's keys or values in memory
 template <int HD> __device__ __forceinline__ void kv8_codes_out(const Kv8Sh &sh, uint8_t *at) {
     if constexpr (HD == 128) *(uintx4 *)(at + threadIdx.x * 16) = *(const uintx4 *)(sh.codes + threadIdx.x * 16);
     else *(uintx2 *)(at + threadIdx.x * 8) = *(const uintx2 *)(sh.codes + threadIdx.x * 8);
 }
-template <int HD> __device__ __forceinline__ void kv8_codes_in(Kv8Sh &sh, const uint8_t *at) {
-    if constexpr (HD == 128) *(uintx4 *)(sh.codes + threadIdx.x * 16) = *(const uintx4 *)(at + threadIdx.x * 16);
-    else *(uintx2 *)(sh.codes + threadIdx.x * 8) = *(const uintx2 *)(at + threadIdx.x * 8);
-}
 // the values of 4 codes
-template <typename T> __device__ __forceinline__ void kv8_values(uint32_t w, float scale, T *x) {
+__device__ __forceinline__ void kv8_values(uint32_t w, float scale, float *x) {
     const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    x[0] = (T)(a.x * scale), x[1] = (T)(a.y * scale), x[2] = (T)(b.x * scale), x[3] = (T)(b.y * scale);
+    x[0] = a.x * scale, x[1] = a.y * scale, x[2] = b.x * scale, x[3] = b.y * scale;
 }
-// the channels kv8_ch(c0, .) of position k of a block's codes
-template <int HD, bool V, typename T>
-__device__ __forceinline__ void kv8_row(const uint8_t *codes, int k, int c0, float scale, T (&x)[HD / 8]) {
-    if constexpr (V) {
+// as kv8_build takes them, a thread's channels of its position from a block's keys or values; all lanes of a wave call it
+template <int HD, bool V> __device__ __forceinline__ void kv8_held(const uint8_t *codes, float scale, float (&x)[HD / 8]) {
+    const int k = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 8, lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < HD / 8; i++) x[i] = (T)kv8_value(codes[kv8_v_at(k, kv8_ch<HD>(c0, i), HD)], scale);
-    } else {
+    for (int i = 0; i < HD / 8; i += 8) {
+        const int c = kv8_ch<HD>(c0, i);
+        const uintx2 w = V ? kv8_transpose(*(const uintx2 *)(codes + kv8_v_at(k & 24, c + (k & 7), HD)), lane)
+                           : *(const uintx2 *)(codes + kv8_k_at(k, c, HD));
+        kv8_values(w.x, scale, x + i);
+        kv8_values(w.y, scale, x + i + 4);
+    }
+}
+// the channels kv8_ch(c0, .) of position k of a block's keys
+template <int HD> __device__ __forceinline__ void kv8_key(const uint8_t *codes, int k, int c0, float scale, float (&x)[HD / 8]) {
 #pragma unroll
-        for (int i = 0; i < HD / 8; i += 8) {
-            const uintx2 w = *(const uintx2 *)(codes + kv8_k_at(k, kv8_ch<HD>(c0, i), HD));
-            kv8_values(w.x, scale, x + i);
-            kv8_values(w.y, scale, x + i + 4);
-        }
+    for (int i = 0; i < HD / 8; i += 8) {
+        const uintx2 w = *(const uintx2 *)(codes + kv8_k_at(k, kv8_ch<HD>(c0, i), HD));
+        kv8_values(w.x, scale, x + i);
+        kv8_values(w.y, scale, x + i + 4);
     }
 }
 

@@ -183,7 +183,7 @@ __device__ __forceinline__ Kv8Spot kv8_in_pool(const Kv8Evict &p, int s, int h, 
 template <int HD> __device__ __forceinline__ Kv8Spot kv8_to(const Kv8Evict &p, void *ws, int s, int h, int d) {
     return p.new_table ? kv8_in_pool(p, s, h, d) : kv8_in_ws<HD>(ws, p.n_seqs, p.L.n_kv, (p.budget + 31) / 32, s, h, d);
 }
-// Keys: 8 threads to a position, whose codes are 16 (8) bytes next to each other.
+// Keys: 8 threads to a position, whose codes are 8 bytes next to each other.
 template <int HD>
 __device__ __forceinline__ void kv8_gather_k(const Kv8Evict &p, void *ws, Kv8Sh &sh, int s, int h, int d, int n) {
     const int k = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 8, i = d * 32 + k;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void kv8_gather_k(const Kv8Evict &p, void *ws, Kv8Sh 
             p.scores_out[head * p.scores_out_ld + i] = p.scores[head * p.scores_ld + pos];
         if (page >= 0 && page < p.L.n_pages) {  // (a position without a page is zeros)
             const Kv8Head *of = p.L.head(page, h, pos);
-            kv8_row<HD, false>(p.L.codes(page, h, pos), pos & 31, c0, of->scale[0], x);
+            kv8_key<HD>(p.L.codes(page, h, pos), pos & 31, c0, of->scale[0], x);
             nan = of->nan[0] >> (pos & 31) & 1;
         }
     }
