@@ -64,10 +64,11 @@ __device__ __forceinline__ void kv8_turn_q(const Kv8Append &p, int pos, int hi, 
 // sequence are dealt round gridDim.x workgroups.  What a block holds in front of the
 // call's rows is read, and the whole block written: its scale may have changed.  Keys
 // are rotated and rounded in f64, so that no code depends on the order of roundings.
-// 16384 fp16 rows of 8 KV heads of 128 channels, 100 MB: 42 us, 21 at the rate of a
-// large copy; VALU instructions are issued in 60 % of the CUs' busy cycles, and the f64
-// rotation's registers leave four waves a SIMD.  (8 channels a thread, 16 threads to a
-// position: 193 us for rows and queries, 107 so.)
+// 16384 fp16 rows of 8 KV heads of 128 channels, 100 MB: 35 us, 21 at the rate of a
+// large copy; VALU instructions, most of them the f64 rotation's, are issued in 69 % of
+// the CUs' busy cycles and waves wait for 54 % of theirs.  Five waves a SIMD: with four
+// 6 us more, with six registers spill and it is 3 us more.  (8 channels a thread, 16
+// threads to a position: 193 us for rows and queries, 107 so.)
 template <int HD, bool F32, bool PAIRS>
 __global__ __launch_bounds__(kKv8T) __attribute__((amdgpu_waves_per_eu(5))) void k_kv8_append(const Kv8Append p) {
     constexpr int C = HD / 8;
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kKv8T) __attribute__((amdgpu_waves_per_eu(5))) void
 
 // The queries by themselves: a thread's registers are then few enough for a CU's whole
 // complement of waves.  16384 rows of 32 heads, 268 MB: 57 us, 4.7 TB/s, a large copy's
-// rate; a small call keeps them in the launch above, which saves a launch of 3 us: from
+// rate (54 to 57); a small call keeps them in the launch above, which saves a launch of 3 us: from
 // kApart pairs of a row and a head on the shorter kernel outweighs it.
 constexpr int64_t kApart = 1 << 16;
 template <int HD, bool F32, bool PAIRS>
@@ -200,7 +201,8 @@ void launch_kv8_append(const Kv8Append &in, hipStream_t st) {
 // 8 k + j the channels 8 j .. of row k.  Rows that are 8 positions of one group of a
 // block share the bytes that their values lie in: then lane 8 k + j loads the 8
 // positions of channel 8 j + k and the eight lanes exchange them; otherwise a lane
-// picks its 8 bytes.
+// picks its 8 bytes.  16384 rows of 8 heads, 34 MB of blocks and 67 MB of rows: 20 us,
+// a large copy's rate (31 where every lane picks).
 constexpr int kReadU = 2;
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv8_read(const Kv8Layer L, const KvqRows rows, uint16_t *k_out, uint16_t *v_out) {
