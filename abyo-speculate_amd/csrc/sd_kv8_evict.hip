@@ -1,5 +1,7 @@
 // Eviction from the 8-bit cache by the positions' accumulated weights: which ones of
 // every sequence and KV head stay, and moving them together.
+#include <type_traits>
+
 #include "sd_kv8_dev.hpp"
 
 namespace sd {
@@ -41,6 +43,10 @@ __device__ __forceinline__ uint32_t kv8_sum_first(const uint32_t *v, int n, int 
     x += __builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true);  // 15 - lane of each 16
     return (uint32_t)x;
 }
+// bits of m below the lane's own
+__device__ __forceinline__ uint32_t kv8_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
 __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
     extern __shared__ __align__(16) uint32_t sel_rank[];
     __shared__ Kv8Select sh;
@@ -57,24 +63,35 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
     }
     const int lo = p.sinks, hi = T - p.recent;  // candidates [lo, hi)
     const bool once = T <= kSelChunk;
-    // ranks of the positions from `at` on, eight loads in flight; zeros up to a multiple of a round
-    auto load = [&](int at) {
+    // ranks of the positions from `at` on, zeros up to a multiple of a round; the first time counted by their highest 11 bits
+    auto load = [&](int at, auto first) {
         const int m = min(kSelChunk, T - at), round = (m + kSelT - 1) / kSelT * kSelT;
-        __syncthreads();
-        for (int i0 = tid; i0 < round; i0 += 8 * kSelT) {
-            float v[8];
+        float v[8], w[8];
+        auto ask = [&](int i0) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = x[at + min(i0 + j * kSelT, m - 1)];
+        };
+        ask(tid);
+        __syncthreads();
+        for (int i0 = tid; i0 < round; i0 += 8 * kSelT) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = v[j];
+            if (i0 + 8 * kSelT < round) ask(i0 + 8 * kSelT);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int i = i0 + j * kSelT;
-                if (i < round) sel_rank[i] = i >= m ? 0 : at + i < lo || at + i >= hi ? kSelForced : kv8_rank(v[j]);
+                const bool open = i < m && at + i >= lo && at + i < hi;
+                const uint32_t r = i >= m ? 0 : open ? kv8_rank(w[j]) : kSelForced;
+                if (i < round) sel_rank[i] = r;
+                if (first && open) atomicAdd(&sh.bins[r >> 21][lane & 1], 1u);
             }
         }
         __syncthreads();
         return m;
     };
-    int m = load(0);
+    *(uintx4 *)&sh.bins[2 * tid][0] = uintx4{0, 0, 0, 0};
+    int m = 0;
+    for (int at = 0; at < T; at += kSelChunk) m = load(at, std::true_type{});
     uint32_t need = (uint32_t)(p.budget - p.sinks - p.recent);  // candidates that stay
     const bool any = need > 0;
     uint32_t prefix = any ? 0 : kSelForced - 1;  // the bits found of the last one's rank
@@ -82,17 +99,19 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
     for (int pass = 0; pass < 3 && any; pass++) {
         const int bits = pass < 2 ? 11 : 10, above = shift;  // bits of the prefix end at `above`
         shift -= bits;
-        *(uintx4 *)&sh.bins[2 * tid][0] = uintx4{0, 0, 0, 0};
-        __syncthreads();
-        for (int at = 0; at < T; at += kSelChunk) {
-            if (!once) m = load(at);
+        if (pass > 0) {
+            *(uintx4 *)&sh.bins[2 * tid][0] = uintx4{0, 0, 0, 0};
+            __syncthreads();
+        }
+        for (int at = 0; pass > 0 && at < T; at += kSelChunk) {
+            if (!once) m = load(at, std::false_type{});
             const uint32_t low = (1u << bits) - 1u;
 #pragma unroll 2
             for (int i = 4 * tid; i < m; i += 4 * kSelT) {
                 const uintx4 q = *(const uintx4 *)&sel_rank[i];  // (zeros past the end; forced ones are no number's rank)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (pass == 0 ? q[j] - 1u < kSelForced - 1u : q[j] >> above == prefix && q[j] - 1u < kSelForced - 1u)
+                    if (q[j] >> above == prefix && q[j] - 1u < kSelForced - 1u)
                         atomicAdd(&sh.bins[(q[j] >> shift) & low][lane & 1], 1u);
             }
         }
@@ -117,20 +136,20 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
     }
     // `prefix` is the last one's rank, `need` of its equals stay
     uint32_t at_chunk = 0, eq_chunk = 0;  // what is above it and what equals it in front of the chunk
-    const uint64_t below = (1ull << lane) - 1ull;
     for (int at = 0; at < T; at += kSelChunk) {
-        if (!once) m = load(at);
+        if (!once) m = load(at, std::false_type{});
         // wave w has the positions [first, last) of the chunk, whole rounds of 64
         const int seg = (m + kSelT - 1) / kSelT * 64, first = wave * seg, last = first + seg;
-        uint32_t count = 0, equals = 0;
-#pragma unroll 4
-        for (int i = first; i < last; i += 64) {
-            const uint32_t r = sel_rank[i + lane];
-            count += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(r > prefix));
-            equals += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(r == prefix));
+        uint32_t count = 0;  // of those above it, and 65536 times that of its equals
+        for (int i = first + 4 * lane; i < last; i += 256) {
+            const uintx4 q = *(const uintx4 *)&sel_rank[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) count += (q[j] > prefix ? 1u : 0u) + (q[j] == prefix ? 65536u : 0u);
         }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o);
         __syncthreads();  // the parts of the pass or chunk before have been read
-        if (lane == 0) sh.part[wave] = count, sh.eq_part[wave] = equals;
+        if (lane == 0) sh.part[wave] = count & 0xffffu, sh.eq_part[wave] = count >> 16;
         __syncthreads();
         uint32_t seen = eq_chunk + kv8_sum_first(sh.eq_part, wave, lane);
         uint32_t to = at_chunk + kv8_sum_first(sh.part, wave, lane) + min(seen, need);
@@ -139,11 +158,14 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
 #pragma unroll 4
         for (int i = first; i < last; i += 64) {
             const uint32_t r = sel_rank[i + lane];
+            bool stay = r > prefix;
             const uint64_t e = __builtin_amdgcn_ballot_w64(r == prefix);
-            const bool stay = r > prefix || (r == prefix && seen + (uint32_t)__popcll(e & below) < need);
-            seen += (uint32_t)__popcll(e);
+            if (e != 0) {
+                stay |= r == prefix && seen + kv8_below(e) < need;
+                seen += (uint32_t)__popcll(e);
+            }
             const uint64_t k = __builtin_amdgcn_ballot_w64(stay);
-            if (stay) kept[to + (uint32_t)__popcll(k & below)] = at + i + lane;
+            if (stay) kept[to + kv8_below(k)] = at + i + lane;
             to += (uint32_t)__popcll(k);
         }
     }
