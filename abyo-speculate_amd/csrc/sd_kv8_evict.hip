@@ -16,7 +16,7 @@ __device__ __forceinline__ int kv8_evict_len(const Kv8Evict &p, int s) {
 __device__ __forceinline__ uint32_t kv8_rank(float x) {
     if (x != x) return 1;
     const uint32_t b = __float_as_uint(x + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
 
 // One workgroup per (KV head, sequence).  The rank of the last position that stays is
@@ -24,10 +24,12 @@ __device__ __forceinline__ uint32_t kv8_rank(float x) {
 // with the bits found so far; then every wave counts what it keeps of its part of the
 // positions, in order, and writes it.  Equal scores stay from the lowest position on.
 // Ranks are held in LDS, 32768 at a time: a sequence up to that length is read once, a
-// longer one once for each of the four rounds.  32768 positions: 26 us on the one CU that
-// a head has, of which reading takes 5, the first histogram 5 (positions of like scores
-// meet in a bin), the others 2 each, counting 2 and writing 4; 2176 positions 9.
+// longer one once for each of the four rounds.  32768 positions: 20 us on the one CU that
+// a head has, where VALU instructions are issued in two thirds of its cycles; with the
+// first histogram behind the reading, bounds checked at every position and one position a
+// lane in the counts 28.  2176 positions: 9, most of them the rounds' barriers.
 constexpr int kSelT = 1024, kSelWaves = kSelT / 64, kSelBins = 2048, kSelChunk = 32768;
+static_assert(kSelChunk % (8 * kSelT) == 0, "a full chunk has no position past its end");
 constexpr uint32_t kSelForced = ~0u;  // the rank of a first or last position
 struct Kv8Select {
     __align__(16) uint32_t bins[kSelBins][2];  // of even and odd lanes: fewer meet in one
@@ -79,7 +81,13 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
             if (i0 + 8 * kSelT < round) ask(i0 + 8 * kSelT);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int i = i0 + j * kSelT;
+                const int i = i0 + j * kSelT, from = at + i - tid;
+                if (from >= lo && from + kSelT <= hi) {  // (i < m: hi is at most T, and a chunk whole strides)
+                    const uint32_t r = kv8_rank(w[j]);
+                    sel_rank[i] = r;
+                    if (first) atomicAdd(&sh.bins[r >> 21][lane & 1], 1u);
+                    continue;
+                }
                 const bool open = i < m && at + i >= lo && at + i < hi;
                 const uint32_t r = i >= m ? 0 : open ? kv8_rank(w[j]) : kSelForced;
                 if (i < round) sel_rank[i] = r;
@@ -108,10 +116,11 @@ __global__ __launch_bounds__(kSelT) void k_kv8_select(const Kv8Evict p) {
             const uint32_t low = (1u << bits) - 1u;
 #pragma unroll 2
             for (int i = 4 * tid; i < m; i += 4 * kSelT) {
-                const uintx4 q = *(const uintx4 *)&sel_rank[i];  // (zeros past the end; forced ones are no number's rank)
+                // (forced ones' highest bits are no number's; the zeros past the end come behind all that can be looked for)
+                const uintx4 q = *(const uintx4 *)&sel_rank[i];
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (q[j] >> above == prefix && q[j] - 1u < kSelForced - 1u)
+                    if (q[j] >> above == prefix)
                         atomicAdd(&sh.bins[(q[j] >> shift) & low][lane & 1], 1u);
             }
         }
