@@ -1051,3 +1051,22 @@ def test_reading_any_positions_in_any_order(hip, hd, KV, page):
             for got, held in ((k[i], p.held[s][0]), (v[i], p.held[s][1])) if there else ():
                 assert np.array_equal(got.astype(np.float64), held[at], equal_nan=True), (s, at)
             assert there or ((k[i] == 5).all() and (v[i] == 5).all())
+
+
+@pytest.mark.parametrize("hd,KV", [(128, 2), (64, 3)])
+@pytest.mark.parametrize("budget,sinks,recent", [(100, 4, 20), (1, 0, 1), (1500, 3, 200)])
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("scores_out", ["own", "same", "none"])
+def test_scores_move_with_their_positions(hip, hd, KV, budget, sinks, recent, in_place, scores_out):
+    """In place and into new pages, into the scores themselves and elsewhere: of sequences above and under the budget, and no
+    entry past the new length is written."""
+    lens = [1700, budget, budget + 1, 5, 0, 3100]
+    p = Pool(hip, 3 * hd + budget, 2 * KV, KV, hd, [max(n, 1) for n in lens], page=64, spare=len(lens) * 25)
+    p.fill(lens)
+    x = scores_of(p.rng, (len(lens), KV, 3200), "plain")
+    got = run_evict(p, lens, x, budget, sinks, recent, in_place, scores_out)
+    check_evict(p, lens, x, budget, sinks, recent, got)
+    if scores_out != "none":
+        for s, n in enumerate(min(n, budget) for n in lens):
+            past = got[2][s, :, n:]
+            assert np.array_equal(past, np.full_like(past, 4.0) if scores_out == "own" else x[s, :, n:])
