@@ -1256,6 +1256,7 @@ sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *qy, const 
         if (!std::isfinite(scores->decay)) throw sd::ArgError("weights: decay must be finite");
         w.ld = (int64_t)scores->ld;
         w.decay = scores->decay;
+        w.anew = scores->own_rows_anew != 0;
         w.max_len = (int64_t)qy->max_len;
         w.cus = P.cus;
         need_aligned(lse, 4, 4, "lse");

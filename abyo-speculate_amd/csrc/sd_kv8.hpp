@@ -129,13 +129,15 @@ KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, i
 void launch_kv8_attention(const Kv8Attn &p, const KvqPlan &plan, void *ws, hipStream_t st);
 
 // out[s][h][j] = decay * in[s][h][j] + what position j of sequence s gets from its
-// rows' weights in the query heads of KV head h (p.lse is read)
+// rows' weights in the query heads of KV head h (p.lse is read); anew: the first
+// term is 0 for the positions of the rows themselves
 struct Kv8Weights {
     Kv8Attn a;
     const float *in;  // or null: zeros
     float *out;
     int64_t ld;
     float decay;
+    int anew;
     int64_t max_len;
     int cus;
 };

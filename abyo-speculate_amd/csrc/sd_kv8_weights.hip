@@ -239,7 +239,8 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
             const int pos = base + 32 * b + r32;
             if (hh == 0 && pos < T) {
                 const int64_t at = ((int64_t)s * p.a.L.n_kv + h) * p.ld + pos;
-                p.out[at] = p.in && p.decay != 0.f ? p.decay * p.in[at] + total : total;
+                const bool had = p.decay != 0.f && !(p.anew && pos >= W.P);
+                p.out[at] = had ? p.decay * p.in[at] + total : total;
             }
         }
         __syncthreads();
@@ -249,6 +250,7 @@ __global__ __launch_bounds__(64 * kWgtWaves) __attribute__((amdgpu_waves_per_eu(
 // 64 positions a wave where that still gives every CU a workgroup
 void launch_kv8_weights(const Kv8Weights &in, hipStream_t st) {
     Kv8Weights p = in;
+    if (!p.in) p.decay = 0.f;  // nothing is read then
     p.a.by_rep = Kv8Div::by((uint32_t)p.a.n_rep);
     const int64_t groups = (int64_t)p.a.L.n_kv * p.a.n_seqs, len = std::max<int64_t>(1, std::min(p.max_len, p.ld));
     const bool two = (len + 255) / 256 * groups >= p.cus;

@@ -155,7 +155,8 @@ class KvWindow(ctypes.Structure):
 
 class KvScores(ctypes.Structure):
     """sd_kv_scores"""
-    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ld", ctypes.c_size_t), ("decay", ctypes.c_float)]
+    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ld", ctypes.c_size_t), ("decay", ctypes.c_float),
+                ("own_rows_anew", ctypes.c_int32)]
 
 
 class KvEvict(ctypes.Structure):
@@ -1297,11 +1298,14 @@ class HipKv8Pool:
 
     def weights(self, layer: int, q: int, lse: int, scores: int, ld: int, row_start: int, kv_len: int, table: int, n_seqs: int,
                 table_ld: int, rows: int, max_rows: int, max_len: int, previous: int = 0, decay: float = 1.0, mask: int = 0,
-                mask_words: int = 0, scale: float = 0.0, q_ld: int = 0, window: int = 0, sinks: int = 0, stream: int = 0):
-        """scores [n_seqs][n_kv_heads][ld] = decay * previous + each position's attention weight from the rows."""
+                mask_words: int = 0, scale: float = 0.0, q_ld: int = 0, window: int = 0, sinks: int = 0, stream: int = 0,
+                own_rows_anew: bool = False):
+        """scores [n_seqs][n_kv_heads][ld] = decay * previous + each position's attention weight from the rows;
+        own_rows_anew: at the rows' own positions `previous` is not read and counts as 0 (what an evicted or
+        rolled-back position left there is no sum of theirs)."""
         a = KvQuery(q, q_ld, 0, 0, rows, row_start, kv_len, table, n_seqs, table_ld, mask, mask_words, max_rows, max_len,
                     scale)
-        w, s = KvWindow(window, sinks), KvScores(previous, scores, ld, decay)
+        w, s = KvWindow(window, sinks), KvScores(previous, scores, ld, decay, int(own_rows_anew))
         _check(_lib.sd_kv8_weights(self._h, layer, ctypes.byref(a), ctypes.byref(w), lse, ctypes.byref(s), stream))
 
     def evict_workspace(self, n_seqs: int, budget: int) -> int:
@@ -1312,7 +1316,8 @@ class HipKv8Pool:
               kept: int, new_len: int, sinks: int = 0, recent: int = 0, scores_out: int = 0, scores_out_ld: int = 0,
               new_table: int = 0, new_table_ld: int = 0, ws: int = 0, ws_bytes: int = 0, stream: int = 0):
         """Every sequence's heads keep their `budget` positions of the largest scores, the
-        first `sinks` and the last `recent` among them, in place or in new_table's pages."""
+        first `sinks` and the last `recent` among them, in place or in new_table's pages.  Scores that are
+        summed on move too: scores_out=scores, scores_out_ld=scores_ld (0: none move)."""
         e = KvEvict(kv_len, table, new_table, n_seqs, table_ld, new_table_ld, scores, scores_ld, scores_out, scores_out_ld,
                     budget, sinks, recent, kept, new_len)
         _check(_lib.sd_kv8_evict(self._h, layer, ctypes.byref(e), ws, ws_bytes, stream))

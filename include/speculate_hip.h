@@ -577,12 +577,21 @@ sd_status sd_kv8_attend(sd_kv8 *c, int32_t layer, const sd_kv_query *query, cons
  * (query->out is not used; max_len bounds the grid, larger kv_len stay
  * correct).  in may be out, or NULL or decay 0: `in` is not read.  Otherwise
  * out overlaps neither in, q nor lse (SD_ERR_ARG).  Entries past the length
- * stay as they were.  Sums are fp32 and always added in the same order. */
+ * stay as they were.  Sums are fp32 and always added in the same order.
+ *
+ * An entry belongs to a place, not to what lies there: after an eviction or a
+ * rollback, entries past the new length still have the sums of what has gone.
+ * With own_rows_anew, positions of the call's own rows, those from kv_len[s]
+ * minus the sequence's rows on, have nothing yet: `in` is not read there and
+ * counts as 0.  That is right for the first call after the rows' append; with
+ * 0, and for rows that get no such call, the host clears the entries of
+ * positions that are new to their sequence. */
 typedef struct sd_kv_scores {
     const float *in;
     float *out;                 /* [n_seqs][n_kv_heads][ld] */
     size_t ld;
     float decay;
+    int32_t own_rows_anew;      /* 0: `in` counts for every position */
 } sd_kv_scores;
 sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *query, const sd_kv_window *window, const float *lse,
                          const sd_kv_scores *scores, void *stream);
@@ -600,8 +609,9 @@ sd_status sd_kv8_weights(sd_kv8 *c, int32_t layer, const sd_kv_query *query, con
  *               past the new length
  *   new_len     [n_seqs]: min(kv_len, budget)
  *   scores_out  [n_seqs][n_kv_heads][scores_out_ld] (0: budget) or NULL: the
- *               scores of what stays; may be `scores` with its stride; entries
- *               past the new length are left as they were
+ *               scores of what stays; may be `scores` with its stride (without
+ *               it those keep the order from before); entries past the new
+ *               length are left as they were (own_rows_anew of sd_kv_scores)
  * Keys keep the rotation of the positions they had: later rows are appended
  * with `pos`.  Outputs and the workspace overlap neither the inputs (but for
  * scores_out) nor each other (SD_ERR_ARG).  Positions of absent pages stand

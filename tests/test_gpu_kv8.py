@@ -1070,3 +1070,69 @@ def test_scores_move_with_their_positions(hip, hd, KV, budget, sinks, recent, in
         for s, n in enumerate(min(n, budget) for n in lens):
             past = got[2][s, :, n:]
             assert np.array_equal(past, np.full_like(past, 4.0) if scores_out == "own" else x[s, :, n:])
+
+
+@pytest.mark.parametrize("hd,KV,H", [(128, 2, 8), (64, 4, 4), (128, 1, 7)])
+def test_own_rows_start_anew(hip, hd, KV, H):
+    """What is summed over steps of a batch, none of it cleared by hand: rows come, are scored, some of them are rolled back and
+    others come in their places, sequences are cut down.  The array starts as NaN: nothing is read that no call has written."""
+    budget, sinks, recent, ld, decay = 96, 4, 16, 200, 0.75
+    counts, lens, true_len = [150, 60, 1], [150, 60, 1], [150, 60, 1]
+    p = Pool(hip, 101 + hd, H, KV, hd, [ld] * 3, page=32)
+    scores = full((3, KV, ld), np.nan)
+    want = np.full((3, KV, ld), np.nan)  # what the array held before the call, with zeros where rows are new
+    for step in range(10):
+        n = sum(counts)
+        pos = np.concatenate([np.arange(t - c, t) for t, c in zip(true_len, counts)])
+        turned = p.append(counts, lens, p.rows(n, KV), p.rows(n, KV), pos=pos, q=p.rows(n, H))
+        window = dict(window=50, sinks=3) if step % 3 == 2 else {}
+        mask = None
+        if step % 4 == 3:
+            mask = np.ascontiguousarray(np.concatenate([_kv8.words(np.tril(np.ones((c, c), bool)))[:, :1] for c in counts if c]))
+        _, lse = p.attend(turned, counts, lens, mask=mask, **window)
+        call, keep = p.call(turned, counts, lens, mask=mask, **window)
+        dl = dev(lse)
+        synchronize()
+        p.pool.weights(0, lse=ptr(dl), scores=ptr(scores), ld=ld, previous=ptr(scores), decay=decay, own_rows_anew=True, **call)
+        new, at = scores.get(), 0
+        for s, c in enumerate(counts):
+            T = lens[s]
+            if c:
+                want[s, :, T - c:T] = 0
+                a = _kv8.Attention(turned[at:at + c], *p.held[s], _kv8.visible(c, T, **window), hd ** -0.5)
+                a.check_weights(lse[at:at + c], new[s, :, :T], want[s, :, :T], decay)
+            assert np.array_equal(new[s, :, T if c else 0:], want[s, :, T if c else 0:].astype(np.float32), equal_nan=True)
+            at += c
+        # some of the last rows go again
+        for s in range(3):
+            back = min(counts[s], step % 3)
+            lens[s], true_len[s] = lens[s] - back, true_len[s] - back
+            p.held[s] = [a[:lens[s]] for a in p.held[s]]
+        if step % 2 == 0:
+            got = run_evict(p, lens, new, budget, sinks, recent, True, "same")
+            check_evict(p, lens, new, budget, sinks, recent, got)
+            lens, new = got[1].tolist(), got[2]
+            scores = dev(new)
+        want = new.astype(np.float64)
+        counts = [1 + step % 3, 20 if step == 4 else 1, 0 if step == 5 else 5]
+        lens, true_len = ([a + c for a, c in zip(x, counts)] for x in (lens, true_len))
+
+
+@pytest.mark.parametrize("rows,T,most", [(1, 1, 1), (3, 40, 3), (40, 30, 40), (700, 1400, 700), (40, 300, 20)])
+def test_own_rows_and_no_others_start_anew(hip, rows, T, most):
+    """The sums of a call with own_rows_anew are those of one whose `in` is 0 at the rows' positions, bit for bit; more rows than
+    positions, and rows past max_rows, are the sequence's own as well."""
+    p = Pool(hip, rows + T, 4, 2, 64, [T], page=64)
+    p.fill([T])
+    q = p.rows(rows, 4)
+    _, lse = p.attend(q, [rows], [T], max_rows=most)
+    lse[most:] = 0
+    before = p.rng.random((1, 2, T + 3)).astype(np.float32)
+    cleared = before.copy()
+    cleared[:, :, max(T - rows, 0):] = 0
+    stale = before.copy()
+    stale[:, :, max(T - rows, 0):] = np.nan
+    got = p.weights(q, lse, [rows], [T], T + 3, previous=stale, decay=0.75, own_rows_anew=True, max_rows=most)
+    assert np.array_equal(got, p.weights(q, lse, [rows], [T], T + 3, previous=cleared, decay=0.75, max_rows=most))
+    assert np.array_equal(p.weights(q, lse, [rows], [T], T + 3, own_rows_anew=True, max_rows=most),
+                          p.weights(q, lse, [rows], [T], T + 3, max_rows=most))
