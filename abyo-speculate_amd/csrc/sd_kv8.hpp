@@ -124,8 +124,7 @@ struct Kv8Attn : KvqAttn {
     int min_blocks;     // of a key range, from the plan
     Kv8Div by_rep, by_kv, by_tiles, by_groups;  // n_rep, KV heads, tiles, groups
 };
-KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int window, int sinks,
-                      int cus);
+KvqPlan kv8_attn_plan(int n_heads, int n_kv, int n_seqs, int max_rows, int64_t max_len, int window, int sinks, int cus);
 void launch_kv8_attention(const Kv8Attn &p, const KvqPlan &plan, void *ws, hipStream_t st);
 
 // out[s][h][j] = decay * in[s][h][j] + what position j of sequence s gets from its

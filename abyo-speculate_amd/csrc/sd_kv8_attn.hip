@@ -7,6 +7,9 @@
 // become fp16 values (exactly what they stand for) in one conversion per two of them,
 // which takes the block's scale.  No code is ever NaN or infinite, so what a
 // probability of 0 meets is finite; the rows that are NaN are bits in the header.
+// Probabilities are rounded to fp16 (2^-11 of each, see kKvqHead) since the matrix
+// instruction takes both its operands in 16 bits, and the values fill fp16's; sums,
+// references and results stay in f32.
 //
 // A value costs half a VALU operation, so no value is expanded for more than the wave
 // that needs it: codes go from memory straight into registers, two buffers of a block
@@ -22,16 +25,11 @@
 // (2048 rows 435 us: the registers do not hold it), tiles of 64 queries with one wave a
 // SIMD (410), wave priorities around the products (no difference), a separate maximum
 // for each block (300).
-#include <atomic>
-#include <type_traits>
-
 #include "sd_kv8_attn_dev.hpp"
 
 #pragma clang fp contract(fast)
 
 namespace sd {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 // What a tile's blocks are cut into: ranges of `chunk` blocks, none shorter than min_blocks unless it is the only one.
 struct Kv8Cut {
@@ -148,7 +146,7 @@ __global__ __launch_bounds__(kKvqT) __attribute__((amdgpu_waves_per_eu(2))) void
             const uint32_t kn = hd[2] >> (8 * g) & 0xffu;
 #pragma unroll
             for (int t = 0; t < QT; t++) {
-                vis[t] = kv8_visible<8>(p, W, p.by_rep.quot(min(W.q0 + t * 16 + r16, W.nq - 1)), key0);
+                vis[t] = kv8_visible(p, W, p.by_rep.quot(min(W.q0 + t * 16 + r16, W.nq - 1)), key0);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     float &s = ((float *)&acc[t][j >> 2])[j & 3];
@@ -328,6 +326,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
     if (p.lse && d == 0) p.lse[at] = kv8_lse(M, l);
 }
 
+// Measured with heads of 128 channels; those of 64 follow the same rules.
 // Tiles: of 16 queries up to 64 of them, which expand every value for each tile but
 // leave registers for more waves (5 rows of 32 heads over 8 and 32768 positions 19.8 us,
 // with one tile of 32 21.1; 16 rows 25.3 and 26.5), of 32 above (60 rows over 8192
@@ -337,8 +336,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv8_combine(const Kv8
 // sequences with two 17.2 us, with one 19.5, with eight 20; 60 rows over 8192 positions
 // with two 28.2, with four 33.6), each of at least a block for each wave.  A sequence's
 // own length decides how many of them it has and how long they are.
-KvqPlan kv8_attn_plan(int n_heads, int n_kv, int hd, int n_seqs, int max_rows, int64_t max_len, int window, int sinks,
-                      int cus) {
+KvqPlan kv8_attn_plan(int n_heads, int n_kv, int n_seqs, int max_rows, int64_t max_len, int window, int sinks, int cus) {
     KvqPlan r{};
     const int64_t nq = (int64_t)max_rows * (n_heads / n_kv);
     r.tile_q = nq <= 64 ? 16 : 32;

@@ -66,25 +66,23 @@ __device__ __forceinline__ bool kv8_full(const Kv8Attn &p, const Kv8Work &w, int
     return a + n <= w.t_all && a + n <= w.T && (p.window <= 0 || a >= w.w_all || a + n <= p.sinks);
 }
 
-// the lowest n of N bits
-template <int N> __device__ __forceinline__ uint32_t kv8_low(int n) {
-    return n >= N ? (N == 32 ? ~0u : (1u << (N & 31)) - 1u) : (1u << max(n, 0)) - 1u;
-}
-// bit j: row m sees position key0 + j, j < N (8 or 32); key0 a multiple of N
-template <int N> __device__ __forceinline__ uint32_t kv8_visible(const Kv8Attn &p, const Kv8Work &w, int m, int key0) {
+// the lowest n of 8 bits
+__device__ __forceinline__ uint32_t kv8_low(int n) { return n >= 8 ? 0xffu : (1u << max(n, 0)) - 1u; }
+// bit j: row m sees position key0 + j, j < 8; key0 a multiple of 8
+__device__ __forceinline__ uint32_t kv8_visible(const Kv8Attn &p, const Kv8Work &w, int m, int key0) {
     uint32_t vis;
     if (!p.mask) {
-        vis = kv8_low<N>(w.P + m + 1 - key0);
+        vis = kv8_low(w.P + m + 1 - key0);
     } else {
-        // N bits from x0 of the row's words: both words they can lie in are loaded at once, whatever x0 is
+        // 8 bits from x0 of the row's words: both words they can lie in are loaded at once, whatever x0 is
         const uint64_t *mk = p.mask + (int64_t)(w.r0 + m) * p.mask_words;
         const int x0 = key0 - w.P, a = x0 >> 6, s = x0 & 63;
         const uint64_t w0 = mk[min(max(a, 0), p.mask_words - 1)], w1 = mk[min(max(a + 1, 0), p.mask_words - 1)];
         const uint64_t lo = a >= 0 && a < p.mask_words ? w0 : 0, hi = a + 1 >= 0 && a + 1 < p.mask_words ? w1 : 0;
-        vis = (uint32_t)(lo >> s | (hi << 1) << (63 - s)) & kv8_low<N>(w.n - x0);
-        if (x0 < 0) vis |= kv8_low<N>(-x0);  // the prefix
+        vis = (uint32_t)(lo >> s | (hi << 1) << (63 - s)) & kv8_low(w.n - x0);
+        if (x0 < 0) vis |= kv8_low(-x0);  // the prefix
     }
-    if (p.window > 0) vis &= kv8_low<N>(p.sinks - key0) | ~kv8_low<N>(w.P + m - p.window + 1 - key0);
+    if (p.window > 0) vis &= kv8_low(p.sinks - key0) | ~kv8_low(w.P + m - p.window + 1 - key0);
     return vis;
 }
 
