@@ -96,6 +96,8 @@ KvqPlan KvPool::plan(int64_t rows, int64_t n_seqs, int64_t max_rows, int64_t max
     if (n_seqs < 1 || n_seqs > 65535) throw ArgError("kvpool: n_seqs must be in [1, 65535]");
     if (max_rows < 1 || max_rows > rows) throw ArgError("kvpool: max_rows must be in [1, rows]");
     if (max_len < 0 || max_len > 0x7fffffc0) throw ArgError("kvpool: max_len out of range");
+    // (before the plan's numbers are of 32 bits; below, tiles are fewer than that)
+    if (max_rows * (cfg.n_heads / cfg.n_kv_heads) > (1 << 30)) throw UnsupportedError("kvpool: too many rows in one call");
     KvqPlan p = cfg.bits == 8 ? kv8_attn_plan(cfg.n_heads, cfg.n_kv_heads, (int)n_seqs, (int)max_rows, max_len, window, sinks, cus)
                               : kvq_attn_plan(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, (int)n_seqs, (int)max_rows, max_len, cus);
     // a grid holds fewer than 2^32 threads, at up to 512 a workgroup

@@ -1136,3 +1136,19 @@ def test_own_rows_and_no_others_start_anew(hip, rows, T, most):
     assert np.array_equal(got, p.weights(q, lse, [rows], [T], T + 3, previous=cleared, decay=0.75, max_rows=most))
     assert np.array_equal(p.weights(q, lse, [rows], [T], T + 3, own_rows_anew=True, max_rows=most),
                           p.weights(q, lse, [rows], [T], T + 3, max_rows=most))
+
+
+def test_more_queries_of_a_head_than_32_bits_number(hip):
+    """2^24 rows of 4096 query heads over one KV head: 2^31 tiles of 32, refused before anything is launched."""
+    pools = [kind(n_layers=1, n_heads=4096, n_kv_heads=1, head_dim=64, n_pages=1, page_tokens=32, max_pos=64)
+             for kind in (hip.HipKv8Pool, hip.HipKvPool)]
+    buf, ints = zeros((1 << 12,)), zeros((8,), np.int32)
+    a = dict(row_start=ptr(ints), kv_len=ptr(ints), table=ptr(ints), n_seqs=1, table_ld=1, rows=1 << 24, max_rows=1 << 24, max_len=32)
+    far = ptr(buf) + (1 << 44)  # (never read: a result that does not meet the queries)
+    for pool in pools:
+        assert pool.attend_workspace(1 << 24, 1, 1 << 24, 32) == 0
+        with pytest.raises(hip.UnsupportedMethod):
+            pool.attend(0, q=ptr(buf), out=far, **a)
+    with pytest.raises(hip.UnsupportedMethod):
+        pools[0].weights(0, q=ptr(buf), lse=ptr(buf), scores=far, ld=32, **a)
+    assert pools[0].attend_workspace(1 << 10, 1, 1 << 10, 32) == pools[1].attend_workspace(1 << 10, 1, 1 << 10, 32) == 0
