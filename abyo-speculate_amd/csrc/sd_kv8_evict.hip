@@ -24,8 +24,9 @@ __device__ __forceinline__ uint32_t kv8_rank(float x) {
 // with the bits found so far; then every wave counts what it keeps of its part of the
 // positions, in order, and writes it.  Equal scores stay from the lowest position on.
 // Ranks are held in LDS, 32768 at a time: a sequence up to that length is read once, a
-// longer one once for each of the four rounds.  32768 positions: 20 us on the one CU that
-// a head has, where VALU instructions are issued in two thirds of its cycles; with the
+// longer one once for each of the four rounds (32769 positions 41 us, 131072 112).  32768
+// positions: 20 us on the one CU that a head has, where VALU instructions are issued in
+// more than half of its cycles (equal scores meet in one bin: 53 us); with the
 // first histogram behind the reading, bounds checked at every position and one position a
 // lane in the counts 28.  2176 positions: 9, most of them the rounds' barriers.
 constexpr int kSelT = 1024, kSelWaves = kSelT / 64, kSelBins = 2048, kSelChunk = 32768;
